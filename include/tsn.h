@@ -319,6 +319,104 @@ double tsn_encoder_weight_bytes(tsn_encoder * e);
 int tsn_encoder_profile_ops(tsn_encoder * e, char * out, size_t cap);
 int tsn_encoder_free(tsn_encoder * e);
 
+/* ------------------------------------------------------------------ transformer-block operators */
+/* Three operators of a transformer block, without counterpart in the reference. They follow one another
+ * inside a block: norms around a branch (tsn_block_norm), rotary positions of its queries and keys
+ * (tsn_rope_axes), differential attention (tsn_diff_attn). Each issues one kernel on the device's
+ * stream and returns without synchronising; a size of zero rows is no work and no error. Inputs and
+ * results are device memory that the caller owns; results may not overlap inputs except where a call
+ * says so. All sums, softmax statistics and norms are held in 32 bits; a result is rounded once. */
+enum { TSN_F32 = 0, TSN_F16 = 1, TSN_BF16 = 2 };
+enum { TSN_NORM_NONE = 0, TSN_NORM_RMS = 1, TSN_NORM_LAYER = 2 };
+
+/* Rows of C consecutive elements: row t of batch b starts at element b * sb + t * st of p. A stride of
+ * 0 repeats the row (inputs only), so one row per batch has st = 0. p null: the term is absent. */
+typedef struct tsn_rows { void * p; int64_t sb, st; } tsn_rows;
+/* Head rows of consecutive elements: token s, head h of batch b starts at element b*sb + s*ss + h*sh. */
+typedef struct tsn_heads { void * p; int64_t sb, ss, sh; } tsn_heads;
+
+/* Norms before and after a block, fused with the block's gate and residual scale. Per row of C:
+ *   x_out = r * x + act(gate) * Npost(y)          h = Npre(x_out) * (1 + scale) + shift
+ * RMS: N(u) = u / sqrt(mean(u^2) + eps) * w (+ b); LAYER: N(u) = (u - mean) / sqrt(var + eps) * w (+ b);
+ * NONE: N(u) = u. r is res_vec [C] where given, else res_scale; act is tanh if gate_tanh. Npre sees
+ * x_out before it is rounded to xtype. Absent terms: y (then x_out = r * x), gate (1), scale (0), shift
+ * (0), weights (1), biases (0); x_out or h may be absent, not both. x and x_out are of xtype, which
+ * is `type` or TSN_F32; y, h, gate, shift and scale are of `type`; weights, biases and res_vec are f32.
+ * x_out may be x, and h may be y, at the same strides. C 1..16384; any strides and alignment (rows that
+ * all start at 16-byte boundaries are read 16 bytes at a time). */
+typedef struct tsn_block_norm_args {
+    uint32_t B, T, C;
+    int32_t xtype, type, post, pre, gate_tanh;
+    float post_eps, pre_eps, res_scale;
+    tsn_rows x, y, x_out, h, gate, shift, scale;
+    const float * post_w, * post_b, * pre_w, * pre_b, * res_vec;
+} tsn_block_norm_args;
+int tsn_block_norm(tsn_device * dev, const tsn_block_norm_args * a);
+
+/* Rotary positions with 1 to 4 axes (time, height, width, ...), after an optional RMSNorm of each head.
+ * A head of D elements has P = sum(pairs) rotated pairs, pairs[0] of the first axis, then pairs[1] of
+ * the second, and so on; elements from 2 P on pass through. Pair i of the n pairs of axis a turns by
+ * pos[a] * scale[a] * theta[a]^(-i / n): (u, v) -> (u cos - v sin, u sin + v cos). The pair's
+ * elements are 2 j, 2 j + 1 (TSN_ROPE_INTERLEAVED) or j, j + P (TSN_ROPE_HALF), j counting over all axes.
+ * tsn_rope_plan fills the plan (host only, no device): each pair's turns per position as a 64-bit
+ * fraction, so that an angle keeps its full precision at any 32-bit position. */
+enum { TSN_ROPE_INTERLEAVED = 0, TSN_ROPE_HALF = 1 };
+enum { TSN_ROPE_MAX_PAIRS = 128, TSN_ROPE_MAX_AXES = 4 };
+typedef struct tsn_rope_plan_t {
+    uint32_t D, axes, P;
+    int32_t layout;
+    uint64_t turn[TSN_ROPE_MAX_PAIRS];
+    uint8_t axis[TSN_ROPE_MAX_PAIRS];
+} tsn_rope_plan_t;
+/* D even, 2..256, 2 P <= D; theta > 0, scale finite. */
+int tsn_rope_plan(uint32_t D, uint32_t axes, const uint32_t * pairs, const double * theta, const double * scale,
+                  int layout, tsn_rope_plan_t * out);
+/* q [B, S, Hq, D] and k [B, S, Hk, D] of `type` into q_out and k_out (the inputs themselves, at the same
+ * strides, or other memory, e.g. a cache). Either pair may be absent (p null). pos: int32, axis a of
+ * token s of batch b at pos[b * pos_sb + s * pos_ss + a] (pos_sb 0: shared by the batch). q_norm, k_norm:
+ * f32 [D] weights of the heads' RMSNorm, or null for none. */
+typedef struct tsn_rope_args {
+    uint32_t B, S, Hq, Hk;
+    int32_t type;
+    float eps;
+    tsn_heads q, k, q_out, k_out;
+    const int32_t * pos;
+    int64_t pos_sb, pos_ss;
+    const float * q_norm, * k_norm;
+} tsn_rope_args;
+int tsn_rope_axes(tsn_device * dev, const tsn_rope_plan_t * plan, const tsn_rope_args * a);
+
+/* Differential attention: the difference of two softmax maps over shared values, then an RMSNorm of each
+ * head. A query or key head is [q1 | q2] of d elements each, a value head has 2 d:
+ *   A_m = softmax(scale * q_m k_m^T) over the visible keys,  o = (A_1 - lambda A_2) v
+ *   lambda = exp(lq1 . lk1) - exp(lq2 . lk2) + lambda_init
+ *   out = o / sqrt(mean(o^2) + eps) * norm_w * (1 - lambda_init)
+ * q [B, Sq, H, 2 d], k and v [B, Sk, Hk, 2 d] (query head h reads kv head h / (H / Hk)), out as q, all of
+ * `type` TSN_F16 or TSN_BF16; d is 32 or 64, H / Hk at most 128. Base addresses and strides of q, k, v and
+ * out are multiples of 16 bytes. scale 0 means 1 / sqrt(d).
+ * Visible keys of query i in batch b, with n = key_len[b] (int32, clamped to 0..Sk; null: Sk): j < n; and
+ * key_mask[b * mask_sb + j] != 0 (bytes; null: all); and with causal j <= i + n - Sq, so the last query
+ * sees the last key. A row that sees no key is zero. What masked keys and values hold has no effect, NaN
+ * and infinities included; a row that sees a non-finite value is NaN.
+ * lq1 .. lk2: f32 vectors of d, one per query head lam_sh elements apart (0: shared). norm_w: f32 [2 d] or
+ * null for ones.
+ * The probabilities are rounded to `type` before the product with v, as the tensor cores take them.
+ * Few query rows over many keys split the keys over several CTAs through a workspace that the device handle
+ * allocates at its first such call and keeps: make one such call before capturing it in a CUDA graph. */
+typedef struct tsn_diff_attn_args {
+    uint32_t B, Sq, Sk, H, Hk, d;
+    int32_t type, causal;
+    float scale, lambda_init, eps;
+    tsn_heads q, k, v, out;
+    const int32_t * key_len;
+    const uint8_t * key_mask;
+    int64_t mask_sb;
+    const float * lq1, * lk1, * lq2, * lk2;
+    int64_t lam_sh;
+    const float * norm_w;
+} tsn_diff_attn_args;
+int tsn_diff_attn(tsn_device * dev, const tsn_diff_attn_args * a);
+
 /* ------------------------------------------------------------------ fixtures */
 /* Write the seeded synthetic DiT GGUF (with_prep adds the conditioning-prep tensors). Host only. */
 int tsn_gguf_write_synthetic(const char * path, const tsn_dit_geom * g, uint64_t seed, int with_prep);

@@ -6,6 +6,7 @@
 #include <memory>
 #include <unistd.h>
 
+#include "block_ops.h"
 #include "compat.h"
 #include "gguf_io.h"
 #include "runtime.h"
@@ -284,6 +285,44 @@ int tsn_cfg_euler(tsn_device * dev, const void * fc, const void * fu, void * x, 
 }
 int tsn_mean_cols(tsn_device * dev, const void * x, void * y, uint32_t S, uint32_t H) {
     RT_BEGIN return compat_mean_cols(c, x, y, S, H);
+}
+
+// ------------------------------------------------------------------- transformer-block operators
+// No exception crosses the C boundary: what the host side throws (a failed allocation of a message or a
+// lock) becomes a status.
+}   // extern "C"
+
+template <class F>
+static int guarded(tsn_device * dev, const void * args, F && f) {
+    try {
+        if (!dev || !args) return fail(TSN_ERR_ARG, "null argument");
+        RT_BEGIN
+        return f(c);
+    } catch (const std::bad_alloc &) {
+        return TSN_ERR_OOM;
+    } catch (...) {
+        return TSN_ERR_STATE;
+    }
+}
+
+extern "C" {
+
+int tsn_block_norm(tsn_device * dev, const tsn_block_norm_args * a) {
+    return guarded(dev, a, [&](DeviceCtx & c) { return block_norm(c, *a); });
+}
+int tsn_rope_plan(uint32_t D, uint32_t axes, const uint32_t * pairs, const double * theta, const double * scale,
+                  int layout, tsn_rope_plan_t * out) {
+    try {
+        return rope_plan(D, axes, pairs, theta, scale, layout, out);
+    } catch (...) {
+        return TSN_ERR_OOM;
+    }
+}
+int tsn_rope_axes(tsn_device * dev, const tsn_rope_plan_t * plan, const tsn_rope_args * a) {
+    return guarded(dev, plan ? (const void *) a : nullptr, [&](DeviceCtx & c) { return rope_axes(c, *plan, *a); });
+}
+int tsn_diff_attn(tsn_device * dev, const tsn_diff_attn_args * a) {
+    return guarded(dev, a, [&](DeviceCtx & c) { return diff_attn(c, *a); });
 }
 
 // ------------------------------------------------------------------------------- model face

@@ -42,6 +42,46 @@ def geom(H=1024, NH=16, F=4096, depth=21, fused_depth=14, latent_dim=64, rope_th
     return Geom(H, NH, F, depth, fused_depth, latent_dim, rope_theta, t_max_period)
 
 
+class Rows(C.Structure):
+    """tsn_rows: rows of consecutive elements, by batch and row stride (0 repeats the row)."""
+    _fields_ = [("p", C.c_void_p), ("sb", C.c_int64), ("st", C.c_int64)]
+
+
+class Heads(C.Structure):
+    """tsn_heads: head rows of consecutive elements, by batch, token and head stride."""
+    _fields_ = [("p", C.c_void_p), ("sb", C.c_int64), ("ss", C.c_int64), ("sh", C.c_int64)]
+
+
+class BlockNormArgs(C.Structure):
+    _fields_ = ([(n, C.c_uint32) for n in ("B", "T", "C")]
+                + [(n, C.c_int32) for n in ("xtype", "type", "post", "pre", "gate_tanh")]
+                + [(n, C.c_float) for n in ("post_eps", "pre_eps", "res_scale")]
+                + [(n, Rows) for n in ("x", "y", "x_out", "h", "gate", "shift", "scale")]
+                + [(n, C.c_void_p) for n in ("post_w", "post_b", "pre_w", "pre_b", "res_vec")])
+
+
+class RopePlan(C.Structure):
+    _fields_ = [("D", C.c_uint32), ("axes", C.c_uint32), ("P", C.c_uint32), ("layout", C.c_int32),
+                ("turn", C.c_uint64 * 128), ("axis", C.c_uint8 * 128)]
+
+
+class RopeArgs(C.Structure):
+    _fields_ = ([(n, C.c_uint32) for n in ("B", "S", "Hq", "Hk")] + [("type", C.c_int32), ("eps", C.c_float)]
+                + [(n, Heads) for n in ("q", "k", "q_out", "k_out")]
+                + [("pos", C.c_void_p), ("pos_sb", C.c_int64), ("pos_ss", C.c_int64), ("q_norm", C.c_void_p),
+                   ("k_norm", C.c_void_p)])
+
+
+class DiffAttnArgs(C.Structure):
+    _fields_ = ([(n, C.c_uint32) for n in ("B", "Sq", "Sk", "H", "Hk", "d")]
+                + [(n, C.c_int32) for n in ("type", "causal")]
+                + [(n, C.c_float) for n in ("scale", "lambda_init", "eps")]
+                + [(n, Heads) for n in ("q", "k", "v", "out")]
+                + [("key_len", C.c_void_p), ("key_mask", C.c_void_p), ("mask_sb", C.c_int64)]
+                + [(n, C.c_void_p) for n in ("lq1", "lk1", "lq2", "lk2")]
+                + [("lam_sh", C.c_int64), ("norm_w", C.c_void_p)])
+
+
 _lib = None
 
 # (name, restype, argtypes)
@@ -136,6 +176,11 @@ _SIGS = [
     ("tsn_dit_autotune", C.c_int, [C.c_void_p, C.c_char_p, C.c_size_t]),
     ("tsn_dit_get_tiles", C.c_int, [C.c_void_p, C.c_void_p, C.c_int, C.POINTER(C.c_int)]),
     ("tsn_dit_set_tiles", C.c_int, [C.c_void_p, C.c_void_p, C.c_int]),
+    ("tsn_block_norm", C.c_int, [C.c_void_p, C.POINTER(BlockNormArgs)]),
+    ("tsn_rope_plan", C.c_int, [C.c_uint32, C.c_uint32, C.POINTER(C.c_uint32), C.POINTER(C.c_double),
+                                C.POINTER(C.c_double), C.c_int, C.POINTER(RopePlan)]),
+    ("tsn_rope_axes", C.c_int, [C.c_void_p, C.POINTER(RopePlan), C.POINTER(RopeArgs)]),
+    ("tsn_diff_attn", C.c_int, [C.c_void_p, C.POINTER(DiffAttnArgs)]),
     ("tsn_gguf_write_synthetic", C.c_int, [C.c_char_p, C.POINTER(Geom), C.c_uint64, C.c_int]),
     ("tsn_gguf_write_synthetic_vae", C.c_int, [C.c_char_p, C.c_uint32, C.c_uint32, C.c_uint32, C.c_uint64]),
 ]
@@ -551,3 +596,11 @@ def inspect(path: str):
 
 def write_synthetic_gguf(path: str, g: Geom, seed: int = 4242, with_prep: bool = False):
     check(lib().tsn_gguf_write_synthetic(path.encode(), C.byref(g), seed, int(with_prep)))
+
+
+def __getattr__(name):
+    """The operators on torch tensors, imported when first named: the rest of the binding needs no torch."""
+    if name in ("BlockNorm", "RopeAxes", "DiffAttention"):
+        from . import block_ops
+        return getattr(block_ops, name)
+    raise AttributeError(f"module {__name__!r} has no attribute {name!r}")
