@@ -393,7 +393,8 @@ int tsn_rope_axes(tsn_device * dev, const tsn_rope_plan_t * plan, const tsn_rope
  *   out = o / sqrt(mean(o^2) + eps) * norm_w * (1 - lambda_init)
  * q [B, Sq, H, 2 d], k and v [B, Sk, Hk, 2 d] (query head h reads kv head h / (H / Hk)), out as q, all of
  * `type` TSN_F16 or TSN_BF16; d is 32 or 64, H / Hk at most 128. Base addresses and strides of q, k, v and
- * out are multiples of 16 bytes. scale 0 means 1 / sqrt(d).
+ * out are multiples of 16 bytes; those of k and v are positive, or 0 for the batch in both (shared keys).
+ * scale 0 means 1 / sqrt(d).
  * Visible keys of query i in batch b, with n = key_len[b] (int32, clamped to 0..Sk; null: Sk): j < n; and
  * key_mask[b * mask_sb + j] != 0 (bytes; null: all); and with causal j <= i + n - Sq, so the last query
  * sees the last key. A row that sees no key is zero. What masked keys and values hold has no effect, NaN

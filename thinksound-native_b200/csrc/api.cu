@@ -60,6 +60,7 @@ int tsn_device_create(int ordinal, tsn_device ** out) {
     CKR(configure_attention_short());
     CKR(configure_gemv());
     CKR(configure_gemv_tc());
+    CKR(configure_diff_attn());
     *out = d.release();
     return TSN_OK;
 }
@@ -73,6 +74,9 @@ int tsn_device_destroy(tsn_device * dev) {
     for (auto & r : c.host_regs) cudaHostUnregister((void *) r.first);
     if (c.scratch) cudaFree(c.scratch);
     if (c.col) cudaFree(c.col);
+    if (c.split_used) cudaEventSynchronize(c.split_ev);
+    if (c.split_ws) cudaFree(c.split_ws);
+    if (c.split_ev) cudaEventDestroy(c.split_ev);
     if (c.d_err) cudaFree(c.d_err);
     if (c.ev0) cudaEventDestroy(c.ev0);
     if (c.ev1) cudaEventDestroy(c.ev1);

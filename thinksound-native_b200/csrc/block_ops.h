@@ -12,6 +12,7 @@ int block_norm(DeviceCtx & c, const tsn_block_norm_args & a);
 int rope_plan(uint32_t D, uint32_t axes, const uint32_t * pairs, const double * theta, const double * scale, int layout,
               tsn_rope_plan_t * out);
 int rope_axes(DeviceCtx & c, const tsn_rope_plan_t & p, const tsn_rope_args & a);
+cudaError_t configure_diff_attn();   // once per device, before the first launch
 int diff_attn(DeviceCtx & c, const tsn_diff_attn_args & a);
 
 inline bool known_type(int t) { return t == TSN_F32 || t == TSN_F16 || t == TSN_BF16; }

@@ -1,84 +1,563 @@
-// diff_attn.cu — differential attention (tsn_diff_attn).
+// diff_attn.cu — differential attention on the tcgen05 tensor cores (tsn_diff_attn).
 //
-// One pass over the keys with the running maximum and sum of both softmax maps: the unnormalised sums
-// O_m = sum_j 2^(s_mj - max_m) v_j are rescaled when a maximum grows, and o = O_1 / l_1 - lambda O_2 / l_2.
-// One warp per query row on the CUDA cores.
+//   o = O_1 / l_1 - lambda O_2 / l_2,   O_m = sum_j p_mj v_j,  l_m = sum_j p_mj,  p_mj = 2^(c q_m.k_mj - ref_m)
+// in one pass over the keys: ref_m follows the running maximum of the row, O_m and l_m are rescaled when it
+// moves. The two maps share every value tile, so K and V are read once for both.
+//
+// One CTA per 128 query rows of one kv head (rows are (token, query head of the group), so a group's heads
+// share the K and V tiles) and, where there are few rows, per part of the keys. 320 threads:
+//   warp 8      TMA: lane 0 streams 128-key K tiles, lane 1 V tiles, through a ring of stages
+//   warp 9      one thread issues S_m = Q_m K_m^T (M 128, N 128, K d) and O_m += P_m V (M 128, N 2 d, K 128; P_m from
+//               TMEM). The order PV_1, QK_1, PV_2, QK_2 keeps the tensor cores on one map while the other
+//               map's softmax runs
+//   warps 0-3   map 1, warps 4-7 map 2: one row per thread. S_m from TMEM, mask, maximum, exponentials, P_m over
+//               S_m's columns. O_m stays in TMEM; it is rescaled only when the maximum has grown by more than
+//               2^8, which f32 and both 16-bit types hold without loss
+// TMEM: S_1, S_2 (128 columns each), O_1, O_2 (2 d each): all 512 columns at d = 64.
+// What bounds it: 2 exponentials for 12 d operations. At d = 64 a 128 x 128 tile pair takes 2048 cycles of the
+// SFU (16 exponentials a cycle) and 1536 of the tensor cores.
+// P is rounded to 16 bits, as the tensor cores take it; scores, maxima, sums and O are f32.
+//
+// Values behind masked keys may be NaN, and 0 * NaN is NaN. So where a tile has masked keys, the map-1 threads
+// zero their V rows in shared memory, and where causal rows differ in what they see, non-finite values of
+// a V row become zero and each row that sees such a key is marked: its result is NaN.
+//
+// With splits, each CTA leaves its O_m, ref_m and l_m in the workspace and the CTA that arrives last adds them
+// up in the order of the splits, so the result does not depend on which one that is.
+// Every wait is bounded; barriers of the whole block are on paths that all threads take.
 #include "block_ops.h"
+#include "ptx.cuh"
+
+#include <cudaTypedefs.h>
+
+#include <algorithm>
+#include <mutex>
 
 namespace tsn {
 
 namespace {
 
-template <class T, int D>   // D = 2 d, the width of a head
-__global__ void diff_attn_kernel(const __grid_constant__ tsn_diff_attn_args a) {
-    constexpr int E = D / 32, d = D / 2;
-    const int lane = threadIdx.x & 31;
-    const long long row = (long long) blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5);
-    if (row >= (long long) a.B * a.Sq * a.H) return;
-    const int h = (int) (row % a.H);
-    const long long b = row / a.H / a.Sq, i = row / a.H % a.Sq;
-    const int hk = h / (int) (a.H / a.Hk);
-    const int n = a.key_len ? max(0, min(a.key_len[b], (int) a.Sk)) : (int) a.Sk;
-    const long long last = a.causal ? min((long long) n - 1, i + n - (long long) a.Sq) : n - 1;
-    // lane l holds elements E l .. E l + E - 1: the first half of the warp has map 1, the second map 2
-    const T * q = (const T *) a.q.p + b * a.q.sb + i * a.q.ss + h * a.q.sh + E * lane;
-    float qv[E], o1[E] = {}, o2[E] = {};
-    const float c = a.scale * 1.44269504088896341f;
-    for (int e = 0; e < E; ++e) qv[e] = to_f32(q[e]);
-    float m = -INFINITY, l = 0.0f;   // this half's map
-    bool bad = false;
-    for (long long j = 0; j <= last; ++j) {
-        if (a.key_mask && !a.key_mask[b * a.mask_sb + j]) continue;
-        const T * k = (const T *) a.k.p + b * a.k.sb + j * a.k.ss + hk * a.k.sh + E * lane;
-        const T * v = (const T *) a.v.p + b * a.v.sb + j * a.v.ss + hk * a.v.sh + E * lane;
-        float s = 0.0f;
-        for (int e = 0; e < E; ++e) s = fmaf(qv[e], to_f32(k[e]), s);
-        for (int x = 8; x; x >>= 1) s += __shfl_xor_sync(0xffffffffu, s, x);
-        s *= c;
-        const float mn = fmaxf(m, s);
-        const float ref = mn == -INFINITY ? 0.0f : mn;
-        const float f = exp2f(m - ref), p = to_f32(from_f32<T>(exp2f(s - ref)));
-        m = mn;
-        l = l * f + p;
-        const float f1 = __shfl_sync(0xffffffffu, f, 0), f2 = __shfl_sync(0xffffffffu, f, 16);
-        const float p1 = __shfl_sync(0xffffffffu, p, 0), p2 = __shfl_sync(0xffffffffu, p, 16);
-        for (int e = 0; e < E; ++e) {
-            const float vv = to_f32(v[e]);
-            bad |= !(fabsf(vv) < INFINITY);
-            o1[e] = fmaf(p1, vv, o1[e] * f1);
-            o2[e] = fmaf(p2, vv, o2[e] * f2);
-        }
-    }
-    bad = __any_sync(0xffffffffu, bad);
-    const float l1 = __shfl_sync(0xffffffffu, l, 0), l2 = __shfl_sync(0xffffffffu, l, 16);
-    float z1 = 0.0f, z2 = 0.0f;
-    for (int e = lane; e < d; e += 32) {
-        z1 += a.lq1[h * a.lam_sh + e] * a.lk1[h * a.lam_sh + e];
-        z2 += a.lq2[h * a.lam_sh + e] * a.lk2[h * a.lam_sh + e];
-    }
-    for (int x = 16; x; x >>= 1) { z1 += __shfl_xor_sync(0xffffffffu, z1, x); z2 += __shfl_xor_sync(0xffffffffu, z2, x); }
-    const float lam = expf(z1) - expf(z2) + a.lambda_init;
-    const float w1 = l1 == 0.0f ? 0.0f : 1.0f / l1, w2 = l2 == 0.0f ? 0.0f : lam / l2;
-    float ss = 0.0f;
-    for (int e = 0; e < E; ++e) {
-        o1[e] = bad ? NAN : o1[e] * w1 - o2[e] * w2;
-        ss += o1[e] * o1[e];
-    }
-    for (int x = 16; x; x >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, x);
-    const float g = rsqrtf(ss / (float) D + a.eps) * (1.0f - a.lambda_init);
-    T * out = (T *) a.out.p + b * a.out.sb + i * a.out.ss + h * a.out.sh + E * lane;
-    for (int e = 0; e < E; ++e) out[e] = from_f32<T>(o1[e] * g * (a.norm_w ? a.norm_w[E * lane + e] : 1.0f));
+constexpr int ROWS = 128, KEYS = 128;
+constexpr int THREADS = 320;
+constexpr float LOG2E = 1.44269504088896341f;
+constexpr float LAZY = 8.0f;   // log2 units that a maximum may grow before O is rescaled
+
+// shared memory of one CTA for heads of D = 2 d elements
+template <int D>
+struct Lay {
+    static constexpr int TILE = 128 * D * 2;             // Q, K or V tile: boxes of 128 rows x 64 elements
+    static constexpr int STAGES = D == 128 ? 3 : 4;
+    static constexpr int OFF_K = TILE, OFF_V = OFF_K + STAGES * TILE, OFF_LAM = OFF_V + STAGES * TILE;
+    static constexpr int OFF_W = OFF_LAM + 128 * 4, OFF_BAR = OFF_W + 128 * 4, TOTAL = OFF_BAR + 256;
+    static_assert(TOTAL <= 227 * 1024, "one CTA's shared memory");
+};
+
+struct Args {
+    tsn_diff_attn_args a;
+    float c;                    // scale * log2(e)
+    int G;                      // query heads per kv head
+    long long R;                // Sq * G rows of one kv head
+    int splits, kv_b;           // parts of the keys; 0: every batch reads the same keys
+    int wr;                     // rows of a partial result
+    float * part;
+    unsigned int * count;
+    int * err;
+};
+
+__device__ __forceinline__ float ex2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+__device__ __forceinline__ uint64_t f2_pack(float a, float b) {
+    uint64_t r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+    return r;
+}
+__device__ __forceinline__ void f2_unpack(uint64_t r, float & a, float & b) {
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(r));
+}
+__device__ __forceinline__ uint64_t ffma2(uint64_t a, uint64_t b, uint64_t c) {
+    uint64_t d;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+    return d;
+}
+__device__ __forceinline__ uint64_t fadd2(uint64_t a, uint64_t b) {
+    uint64_t d;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+    return d;
+}
+template <bool BF16>
+__device__ __forceinline__ uint32_t pack16(float a, float b) {
+    uint32_t r;
+    if (BF16) asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(b), "f"(a));
+    else asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(b), "f"(a));
+    return r;
+}
+// the low n bits of a word, n of any sign and size
+__device__ __forceinline__ uint32_t low_bits(int n) { return n >= 32 ? 0xffffffffu : n <= 0 ? 0u : (1u << n) - 1u; }
+// of two 16-bit values, the non-finite ones set to zero
+template <bool BF16>
+__device__ __forceinline__ uint32_t finite_only(uint32_t v) {
+    const uint32_t e = BF16 ? 0x7f80u : 0x7c00u;
+    if ((v & e) == e) v &= 0xffff0000u;
+    if ((v & (e << 16)) == (e << 16)) v &= 0x0000ffffu;
+    return v;
 }
 
-template <class T>
-cudaError_t launch(const tsn_diff_attn_args & a, cudaStream_t s) {
-    const long long rows = (long long) a.B * a.Sq * a.H;
-    if (a.d == 32) diff_attn_kernel<T, 64><<<(unsigned) ((rows + 3) / 4), 128, 0, s>>>(a);
-    else diff_attn_kernel<T, 128><<<(unsigned) ((rows + 3) / 4), 128, 0, s>>>(a);
+template <int D, bool BF16>
+__global__ void __launch_bounds__(THREADS, 1)
+diff_attn_tc(const __grid_constant__ CUtensorMap tk, const __grid_constant__ CUtensorMap tv, const __grid_constant__ Args p) {
+    using L = Lay<D>;
+    constexpr int d = D / 2, BOX = 128 * 128, ATOMS = D / 64, CH = D / 8;   // CH: 16-byte pieces of a head
+    extern __shared__ __align__(1024) uint8_t smem[];
+    const tsn_diff_attn_args & a = p.a;
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    if (smem_u32(smem) & 1023) {   // the swizzled tiles need 1024-byte alignment
+        if (tid == 0 && p.err) atomicCAS(p.err, 0, DEV_BAD_ARGS);
+        return;
+    }
+    float * lam = (float *) (smem + L::OFF_LAM), * nw = (float *) (smem + L::OFF_W);
+    uint64_t * bar = (uint64_t *) (smem + L::OFF_BAR);
+    uint64_t * q_full = bar, * k_full = bar + 1, * k_empty = k_full + L::STAGES, * v_full = k_empty + L::STAGES,
+             * v_empty = v_full + L::STAGES, * s_full = v_empty + L::STAGES, * p_full = s_full + 2, * o_full = p_full + 2,
+             * bad_bar = o_full + 1;
+    uint32_t * words = (uint32_t *) (bad_bar + 1);   // TMEM address, abort flag, last-to-arrive flag, bad keys [4]
+    volatile int * abort_flag = (volatile int *) (words + 1);
+
+    // this CTA's rows, keys and part of them; long rows of a causal call come first
+    const unsigned gid = blockIdx.x / p.splits, split = blockIdx.x % p.splits;
+    const int hk = (int) (gid % a.Hk), b = (int) (gid / a.Hk % a.B);
+    const long long qt = (p.R + ROWS - 1) / ROWS - 1 - gid / a.Hk / a.B, r0 = qt * ROWS;
+    const int rows = (int) min((long long) ROWS, p.R - r0);
+    const int i0 = (int) (r0 / p.G), rem0 = (int) (r0 % p.G);   // row t: token i0 + (rem0 + t) / G, head (rem0 + t) % G
+    const int n = a.key_len ? max(0, min(a.key_len[b], (int) a.Sk)) : (int) a.Sk;
+    auto limit = [&](int t) {   // keys before which row t sees
+        if (!a.causal) return n;
+        return (int) max(0ll, min((long long) n, (long long) (i0 + (rem0 + t) / p.G) + n - (long long) a.Sq + 1));
+    };
+    const int most = limit(rows - 1), least = limit(0);
+    const int all_tiles = (most + KEYS - 1) / KEYS, per = (all_tiles + p.splits - 1) / p.splits;
+    const int t0 = min(all_tiles, (int) split * per), nt = min(all_tiles, t0 + per) - t0;
+
+    if (tid == 0) {
+        mbar_init(q_full, 8);
+        for (int s = 0; s < L::STAGES; ++s) {
+            mbar_init(&k_full[s], 1); mbar_init(&k_empty[s], 1);
+            mbar_init(&v_full[s], 1); mbar_init(&v_empty[s], 1);
+        }
+        for (int m = 0; m < 2; ++m) { mbar_init(&s_full[m], 1); mbar_init(&p_full[m], 4); }
+        mbar_init(o_full, 1);
+        mbar_init(bad_bar, 4);
+        *abort_flag = 0;
+        fence_mbar_init();
+    }
+    if (warp == 8 && lane == 0) { tma_prefetch(&tk); tma_prefetch(&tv); }
+    if (warp == 9) tmem_alloc(words, 512);
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = words[0];
+    const uint32_t TM_O = tmem + 256;
+
+    // the row of a softmax thread
+    const int m = warp >> 2, t = tid & 127;
+    float l = 0.0f, ref = -INFINITY;
+    bool ok = true;
+
+    if (warp == 8) {
+        if (lane < 2) {
+            const CUtensorMap * tm = lane == 0 ? &tk : &tv;
+            uint64_t * full = lane == 0 ? k_full : v_full, * empty = lane == 0 ? k_empty : v_empty;
+            uint8_t * ring = smem + (lane == 0 ? L::OFF_K : L::OFF_V);
+            for (int j = 0; j < nt; ++j) {
+                const int s = j % L::STAGES;
+                if (j >= L::STAGES && !mbar_wait(&empty[s], (j / L::STAGES - 1) & 1, abort_flag, p.err, DEV_TIMEOUT_EMPTY)) break;
+                mbar_expect_tx(&full[s], L::TILE);
+                for (int x = 0; x < ATOMS; ++x)
+                    tma_load_4d(ring + s * L::TILE + x * BOX, tm, &full[s], 64 * x, (t0 + j) * KEYS, hk, b * p.kv_b);
+            }
+        }
+    } else if (warp == 9) {
+        if (lane == 0 && nt > 0) {
+            const uint32_t id_s = umma_idesc_f16(KEYS, BF16), id_pv = umma_idesc_f16(D, BF16, 1);
+            // map 2's halves of Q and K: the second box at d = 64, the second half of each 128-byte row at d = 32
+            constexpr int MAP2 = D == 128 ? BOX : 64;
+            auto qk = [&](int mm, int j) {
+                const int s = j % L::STAGES;
+                if (mm == 0 && !mbar_wait(&k_full[s], (j / L::STAGES) & 1, abort_flag, p.err, DEV_TIMEOUT_FULL)) return false;
+                tc_fence_after();
+                const uint64_t qd = umma_desc_sw128(smem + mm * MAP2), kd = umma_desc_sw128(smem + L::OFF_K + s * L::TILE + mm * MAP2);
+#pragma unroll
+                for (int kk = 0; kk < d / 16; ++kk) umma_f16(tmem + 128 * mm, qd + 2 * kk, kd + 2 * kk, id_s, kk != 0);
+                umma_commit(&s_full[mm]);
+                if (mm == 1) umma_commit(&k_empty[s]);
+                return true;
+            };
+            auto pv = [&](int mm, int j) {
+                const int s = j % L::STAGES;
+                if (!mbar_wait(&p_full[mm], j & 1, abort_flag, p.err, DEV_TIMEOUT_TMEM)) return false;
+                if (mm == 0 && !mbar_wait(&v_full[s], (j / L::STAGES) & 1, abort_flag, p.err, DEV_TIMEOUT_FULL)) return false;
+                tc_fence_after();
+                const uint8_t * v = smem + L::OFF_V + s * L::TILE;
+#pragma unroll
+                for (int kk = 0; kk < KEYS / 16; ++kk)
+                    umma_f16_ts(TM_O + D * mm, tmem + 128 * mm + 8 * kk, umma_desc_sw128_mn(v + kk * 2048, BOX), id_pv, j > 0 || kk > 0);
+                if (mm == 1) umma_commit(&v_empty[s]);
+                return true;
+            };
+            bool go = mbar_wait(q_full, 0, abort_flag, p.err, DEV_TIMEOUT_FULL) && qk(0, 0) && qk(1, 0);
+            for (int j = 0; j < nt && go; ++j) {
+                go = pv(0, j) && (j + 1 == nt || qk(0, j + 1)) && pv(1, j) && (j + 1 == nt || qk(1, j + 1));
+            }
+            if (go) umma_commit(o_full);
+        }
+    } else {
+        // Q into its swizzled boxes, rows past the last one as zeros; lambda of each head of the group; weights
+        for (int i = tid; i < ROWS * CH; i += 256) {
+            const int r = i / CH, ch = i % CH, u = rem0 + r;
+            uint4 x = make_uint4(0, 0, 0, 0);
+            if (r < rows)
+                x = *(const uint4 *) ((const uint16_t *) a.q.p + b * a.q.sb + (long long) (i0 + u / p.G) * a.q.ss +
+                                      (long long) (hk * p.G + u % p.G) * a.q.sh + ch * 8);
+            *(uint4 *) (smem + (ch >> 3) * BOX + r * 128 + (((ch & 7) ^ (r & 7)) << 4)) = x;
+        }
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(q_full);
+        for (int g = warp; g < p.G; g += 8) {
+            const long long h = (long long) (hk * p.G + g) * a.lam_sh;
+            float z1 = 0.0f, z2 = 0.0f;
+            for (int e = lane; e < d; e += 32) { z1 += a.lq1[h + e] * a.lk1[h + e]; z2 += a.lq2[h + e] * a.lk2[h + e]; }
+#pragma unroll
+            for (int x = 16; x; x >>= 1) { z1 += __shfl_xor_sync(~0u, z1, x); z2 += __shfl_xor_sync(~0u, z2, x); }
+            if (lane == 0) lam[g] = expf(z1) - expf(z2) + a.lambda_init;
+        }
+        if (tid < D) nw[tid] = (a.norm_w ? a.norm_w[tid] : 1.0f) * (1.0f - a.lambda_init);
+
+        const uint32_t lane0 = (uint32_t) ((warp & 3) * 32) << 16;
+        const uint32_t ts = tmem + 128 * m + lane0, to = TM_O + D * m + lane0;
+        const int lim = t < rows ? limit(t) : n;
+        const uint8_t * mask = a.key_mask ? a.key_mask + b * a.mask_sb : nullptr;
+        bool poison = false;
+        uint32_t mb[4] = {};   // mask bytes of the next tile
+        auto fetch_mask = [&](int j) {
+#pragma unroll
+            for (int w = 0; w < 4; ++w) {
+                const int key = (t0 + j) * KEYS + 32 * w + lane;
+                mb[w] = key < n ? mask[key] : 0u;
+            }
+        };
+        if (mask && nt > 0) fetch_mask(0);
+        for (int j = 0; j < nt; ++j) {
+            const int base = (t0 + j) * KEYS;
+            // the keys that exist, and those that this row sees
+            uint32_t kw[4], vis[4];
+#pragma unroll
+            for (int w = 0; w < 4; ++w) {
+                kw[w] = mask ? __ballot_sync(~0u, mb[w] != 0) : low_bits(n - base - 32 * w);
+                vis[w] = kw[w] & low_bits(lim - base - 32 * w);
+            }
+            if (mask && j + 1 < nt) fetch_mask(j + 1);
+            if (!mbar_wait(&s_full[m], j & 1, abort_flag, p.err, DEV_TIMEOUT_TMEM)) { ok = false; break; }
+            __syncwarp();
+            tc_fence_after();
+            float s[128];
+            tmem_ld128(ts, s);
+            if (__any_sync(~0u, (vis[0] & vis[1] & vis[2] & vis[3]) != ~0u)) {
+#pragma unroll
+                for (int e = 0; e < 128; ++e)
+                    if (!((vis[e >> 5] >> (e & 31)) & 1u)) s[e] = -INFINITY;
+            }
+            float mx[4] = {s[0], s[1], s[2], s[3]};
+#pragma unroll
+            for (int e = 4; e < 128; ++e) mx[e & 3] = fmaxf(mx[e & 3], s[e]);
+            const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * p.c;
+            // a row moves its reference by itself, so its result does not depend on its neighbours
+            const bool move = top > ref + (j ? LAZY : 0.0f);
+            if (__any_sync(~0u, move)) {
+                const float f = move ? ex2(ref - top) : 1.0f;
+                if (move) { ref = top; l *= f; }
+                if (j > 0) {   // S_j complete means that PV_(j-1) is
+#pragma unroll
+                    for (int x = 0; x < D; x += 32) {
+                        float o[32];
+                        tmem_ld32(to + x, o);
+#pragma unroll
+                        for (int e = 0; e < 32; ++e) o[e] *= f;
+                        tmem_st32(to + x, (const uint32_t *) o);
+                    }
+                }
+            }
+            const float neg = ref == -INFINITY ? 0.0f : -ref;
+            const uint64_t c2 = f2_pack(p.c, p.c), neg2 = f2_pack(neg, neg);
+            uint64_t sum[2] = {0ull, 0ull};
+            uint32_t pk[64];
+#pragma unroll
+            for (int e = 0; e < 64; ++e) {
+                float x, y;
+                f2_unpack(ffma2(f2_pack(s[2 * e], s[2 * e + 1]), c2, neg2), x, y);
+                x = ex2(x);
+                y = ex2(y);
+                sum[e & 1] = fadd2(sum[e & 1], f2_pack(x, y));
+                pk[e] = pack16<BF16>(x, y);
+            }
+            float x, y;
+            f2_unpack(fadd2(sum[0], sum[1]), x, y);
+            l += x + y;
+            tmem_st32(ts, pk);
+            tmem_st32(ts + 32, pk + 32);
+            tmem_st_wait();
+            if (m == 0) {
+                const bool gone = (kw[0] & kw[1] & kw[2] & kw[3]) != ~0u, mixed = a.causal && least < min(n, base + KEYS);
+                if (gone || mixed) {   // the same for every thread of the map
+                    if (!mbar_wait(&v_full[j % L::STAGES], (j / L::STAGES) & 1, abort_flag, p.err, DEV_TIMEOUT_FULL)) { ok = false; break; }
+                    __syncwarp();
+                    uint8_t * v = smem + L::OFF_V + (j % L::STAGES) * L::TILE + t * 128;
+                    const bool here = (kw[t >> 5] >> lane) & 1u;   // thread t has key t
+                    bool odd = false;
+                    if (!here || mixed) {
+#pragma unroll
+                        for (int ch = 0; ch < CH; ++ch) {
+                            uint4 * at = (uint4 *) (v + (ch >> 3) * BOX + (((ch & 7) ^ (t & 7)) << 4));
+                            if (!here) {
+                                *at = make_uint4(0, 0, 0, 0);
+                            } else {
+                                const uint4 o = *at;
+                                const uint4 f = make_uint4(finite_only<BF16>(o.x), finite_only<BF16>(o.y), finite_only<BF16>(o.z), finite_only<BF16>(o.w));
+                                if (o.x != f.x || o.y != f.y || o.z != f.z || o.w != f.w) { *at = f; odd = true; }
+                            }
+                        }
+                    }
+                    fence_proxy_async_smem();
+                    if (mixed) {
+                        const uint32_t w = __ballot_sync(~0u, odd);
+                        if (lane == 0) { words[3 + warp] = w; mbar_arrive(bad_bar); }
+                        int turn = (base - t0 * KEYS) / KEYS - max(0, (least - t0 * KEYS) / KEYS);   // mixed tiles before this one
+                        if (!mbar_wait(bad_bar, turn & 1, abort_flag, p.err, DEV_TIMEOUT_TMEM)) { ok = false; break; }
+                        __syncwarp();
+                        volatile uint32_t * bad = words + 3;
+#pragma unroll
+                        for (int x = 0; x < 4; ++x) poison |= (bad[x] & vis[x]) != 0;
+                    }
+                }
+            }
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&p_full[m]);
+        }
+        if (poison) l = NAN;
+        if (ok && nt > 0) ok = mbar_wait(o_full, 0, abort_flag, p.err, DEV_TIMEOUT_TMEM);
+        __syncwarp();
+        tc_fence_after();
+    }
+
+    // ---------------------------------------------------------------- results, every thread on the same path
+    // K's and V's stages are free now: row sums [2][128], sums of squares [2][128]
+    float * rl = (float *) (smem + L::OFF_K), * rss = rl + 256;
+    const uint32_t lane0 = (uint32_t) ((warp & 3) * 32) << 16;
+    const bool soft = warp < 8;
+    const int half = m;   // of the columns, in what follows
+    float o[d];
+    bool mine = soft && t < rows;
+    bool finish = true;
+    if (p.splits > 1) {
+        // partial: [2 maps][D / 4][wr][4] sums, then ref [2][wr], l [2][wr]
+        const size_t size = (size_t) p.wr * (2 * D + 4);
+        if (soft) {
+            float * out = p.part + ((size_t) gid * p.splits + split) * size;
+            if (nt > 0) {
+                for (int x = 0; x < D; x += 32) {
+                    float v[32];
+                    tmem_ld32(TM_O + D * m + lane0 + x, v);
+                    if (mine)
+#pragma unroll
+                        for (int e = 0; e < 32; e += 4)
+                            *(float4 *) (out + ((size_t) (m * (D / 4) + (x + e) / 4) * p.wr + t) * 4) = make_float4(v[e], v[e + 1], v[e + 2], v[e + 3]);
+                }
+            }
+            if (mine) {
+                float * st = out + (size_t) p.wr * 2 * D;
+                st[m * p.wr + t] = ref;
+                st[(2 + m) * p.wr + t] = l;
+            }
+            __threadfence();
+        }
+        __syncthreads();
+        if (tid == 0) {
+            const bool last = atomicAdd(&p.count[gid], 1u) + 1u == (unsigned) p.splits;
+            if (last) p.count[gid] = 0;   // for the next call
+            words[2] = last;
+            __threadfence();
+        }
+        __syncthreads();
+        finish = words[2] != 0;
+        if (finish && mine) {
+            const float * first = p.part + (size_t) gid * p.splits * size;
+            float top[2] = {-INFINITY, -INFINITY}, sum[2] = {0.0f, 0.0f};
+            for (int s = 0; s < p.splits; ++s) {
+                const float * st = first + s * size + (size_t) p.wr * 2 * D;
+                for (int x = 0; x < 2; ++x) top[x] = fmaxf(top[x], __ldcg(st + x * p.wr + t));
+            }
+            for (int x = 0; x < 2; ++x) if (top[x] == -INFINITY) top[x] = 0.0f;
+            for (int s = 0; s < p.splits; ++s) {
+                const float * st = first + s * size + (size_t) p.wr * 2 * D;
+                for (int x = 0; x < 2; ++x) sum[x] += ex2(__ldcg(st + x * p.wr + t) - top[x]) * __ldcg(st + (2 + x) * p.wr + t);
+            }
+            const float w1 = sum[0] == 0.0f ? 0.0f : 1.0f / sum[0];
+            const float w2 = sum[1] == 0.0f ? 0.0f : -lam[(rem0 + t) % p.G] / sum[1];
+#pragma unroll
+            for (int e = 0; e < d; ++e) o[e] = 0.0f;
+            for (int s = 0; s < p.splits; ++s) {
+                const float * at = first + s * size, * st = at + (size_t) p.wr * 2 * D;
+                for (int x = 0; x < 2; ++x) {
+                    const float r = __ldcg(st + x * p.wr + t), f = ex2(r - top[x]) * (x ? w2 : w1);
+                    if (r == -INFINITY) continue;   // nothing seen in this part: its sums may not be written
+#pragma unroll
+                    for (int e = 0; e < d; e += 4) {
+                        const float4 v = __ldcg((const float4 *) (at + ((size_t) (x * (D / 4) + (half * d + e) / 4) * p.wr + t) * 4));
+                        o[e] = fmaf(f, v.x, o[e]); o[e + 1] = fmaf(f, v.y, o[e + 1]);
+                        o[e + 2] = fmaf(f, v.z, o[e + 2]); o[e + 3] = fmaf(f, v.w, o[e + 3]);
+                    }
+                }
+            }
+            if (!(sum[0] >= 0.0f) || !(sum[1] >= 0.0f)) o[0] = NAN;
+        }
+    } else {
+        if (soft) rl[tid] = l;
+        __syncthreads();
+        if (soft) {
+            const float l1 = rl[t], l2 = rl[128 + t];
+            const float w1 = l1 == 0.0f ? 0.0f : 1.0f / l1;
+            const float w2 = l2 == 0.0f ? 0.0f : t < rows ? lam[(rem0 + t) % p.G] / l2 : 0.0f;
+            if (nt > 0) {
+#pragma unroll
+                for (int x = 0; x < d; x += 32) {
+                    float v[32];
+                    tmem_ld32(TM_O + lane0 + half * d + x, o + x);
+                    tmem_ld32(TM_O + D + lane0 + half * d + x, v);
+#pragma unroll
+                    for (int e = 0; e < 32; ++e) o[x + e] = o[x + e] * w1 - v[e] * w2;
+                }
+            } else {
+#pragma unroll
+                for (int e = 0; e < d; ++e) o[e] = 0.0f;
+            }
+        }
+    }
+    // RMSNorm over both halves; the result through Q's place, so that whole rows are written
+    if (finish) {
+        float ss = 0.0f;
+        if (mine) {
+#pragma unroll
+            for (int e = 0; e < d; ++e) ss += o[e] * o[e];
+            rss[tid] = ss;
+        }
+        __syncthreads();
+        if (mine) {
+            ss = rss[t] + rss[128 + t];
+            const float g = ss < INFINITY ? rsqrtf(ss * (1.0f / D) + a.eps) : NAN;
+#pragma unroll
+            for (int e = 0; e < d; e += 8) {
+                uint32_t x[4];
+#pragma unroll
+                for (int k = 0; k < 4; ++k)
+                    x[k] = pack16<BF16>(o[e + 2 * k] * g * nw[half * d + e + 2 * k], o[e + 2 * k + 1] * g * nw[half * d + e + 2 * k + 1]);
+                const int ch = half * (CH / 2) + e / 8;
+                *(uint4 *) (smem + t * (D * 2) + ((ch ^ (t & 7)) << 4)) = make_uint4(x[0], x[1], x[2], x[3]);
+            }
+        }
+        __syncthreads();
+        if (!*abort_flag)
+            for (int i = tid; i < rows * CH; i += THREADS) {
+                const int r = i / CH, ch = i % CH, u = rem0 + r;
+                *(uint4 *) ((uint16_t *) a.out.p + b * a.out.sb + (long long) (i0 + u / p.G) * a.out.ss +
+                            (long long) (hk * p.G + u % p.G) * a.out.sh + ch * 8) =
+                    *(const uint4 *) (smem + r * (D * 2) + ((ch ^ (r & 7)) << 4));
+            }
+    }
+    tc_fence_before();
+    __syncthreads();
+    if (warp == 9) {
+        tc_fence_after();
+        tmem_dealloc(tmem, 512);
+    }
+    if (*abort_flag && tid == 0) {
+        // let copies that were issued but never consumed land before the CTA's shared memory is reused
+        const uint64_t t1 = global_ns();
+        while (global_ns() - t1 < 20000ull) {}
+    }
+}
+
+// ---------------------------------------------------------------- host
+PFN_cuTensorMapEncodeTiled_v12000 encoder() {
+    static const PFN_cuTensorMapEncodeTiled_v12000 enc = [] {
+        cudaDriverEntryPointQueryResult q{};
+        void * fn = nullptr;
+        if (cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &fn, 12000, cudaEnableDefault, &q) != cudaSuccess ||
+            q != cudaDriverEntryPointSuccess)
+            fn = nullptr;
+        return (PFN_cuTensorMapEncodeTiled_v12000) fn;
+    }();
+    return enc;
+}
+
+// {2 d, Sk, Hk, B} view of keys or values with {64, box_keys, 1, 1} boxes. A dimension of one element has a
+// stride that is never taken: any valid one stands in.
+bool make_kv_map(CUtensorMap * m, const tsn_diff_attn_args & a, const tsn_heads & t, uint32_t B, uint32_t box_keys) {
+    const PFN_cuTensorMapEncodeTiled_v12000 enc = encoder();
+    if (!enc) return false;
+    const cuuint64_t row = 2 * a.d * 2;
+    const cuuint64_t dims[4] = {2 * a.d, a.Sk, a.Hk, B};
+    const cuuint64_t strides[3] = {a.Sk > 1 ? (cuuint64_t) t.ss * 2 : row, a.Hk > 1 ? (cuuint64_t) t.sh * 2 : row,
+                                   B > 1 ? (cuuint64_t) t.sb * 2 : row};
+    const cuuint32_t box[4] = {64, box_keys, 1, 1}, es[4] = {1, 1, 1, 1};
+    return enc(m, a.type == TSN_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4, t.p, dims, strides,
+               box, es, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+               CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+constexpr size_t COUNTERS = 4096, WORKSPACE = COUNTERS * 4 + ((size_t) 32 << 20);
+constexpr int SMS = 148;
+
+// The device's workspace, ordered after the last call that used it on another stream.
+int workspace(DeviceCtx & c, bool capturing) {
+    if (!c.split_ws) {
+        if (capturing) return fail(TSN_ERR_STATE, "tsn_diff_attn: a first call that splits its keys cannot be captured");
+        void * p = nullptr;
+        if (cudaMalloc(&p, WORKSPACE) != cudaSuccess) { cudaGetLastError(); return fail(TSN_ERR_OOM, "tsn_diff_attn: workspace"); }
+        cudaError_t e = cudaMemset(p, 0, COUNTERS * 4);
+        if (e == cudaSuccess) e = cudaDeviceSynchronize();
+        if (e == cudaSuccess && !c.split_ev) e = cudaEventCreateWithFlags(&c.split_ev, cudaEventDisableTiming);
+        if (e != cudaSuccess) { cudaFree(p); return fail(TSN_ERR_CUDA, std::string("tsn_diff_attn: ") + cudaGetErrorString(e)); }
+        c.split_ws = p;
+    }
+    if (!capturing && c.split_used && c.split_stream != c.stream) {
+        cudaError_t e = cudaStreamWaitEvent(c.stream, c.split_ev, 0);
+        if (e != cudaSuccess) return fail(TSN_ERR_CUDA, std::string("tsn_diff_attn: ") + cudaGetErrorString(e));
+    }
+    return TSN_OK;
+}
+
+template <int D, bool BF16>
+cudaError_t launch_tc(const CUtensorMap & tk, const CUtensorMap & tv, const Args & p, unsigned grid, cudaStream_t s) {
+    diff_attn_tc<D, BF16><<<grid, THREADS, Lay<D>::TOTAL, s>>>(tk, tv, p);
     return cudaGetLastError();
 }
 
 } // namespace
+
+cudaError_t configure_diff_attn() {
+    cudaError_t e = cudaSuccess;
+    auto set = [&](auto * k, int bytes) {
+        if (e == cudaSuccess) e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+    };
+    set(diff_attn_tc<64, false>, Lay<64>::TOTAL);
+    set(diff_attn_tc<64, true>, Lay<64>::TOTAL);
+    set(diff_attn_tc<128, false>, Lay<128>::TOTAL);
+    set(diff_attn_tc<128, true>, Lay<128>::TOTAL);
+    return e;
+}
 
 int diff_attn(DeviceCtx & c, const tsn_diff_attn_args & in) {
     tsn_diff_attn_args a = in;
@@ -90,7 +569,6 @@ int diff_attn(DeviceCtx & c, const tsn_diff_attn_args & in) {
         return fail(TSN_ERR_ARG, "tsn_diff_attn: at most 2^30 queries or keys, 65535 sequences or heads");
     if (!(a.scale >= 0.0f) || !(a.eps >= 0.0f)) return fail(TSN_ERR_ARG, "tsn_diff_attn: negative scale or eps");
     if (a.B == 0 || a.Sq == 0) return TSN_OK;
-    if ((long long) a.B * a.Sq * a.H > 0x7fffffffLL * 4) return fail(TSN_ERR_ARG, "tsn_diff_attn: too many query rows");
     if (!a.q.p || !a.out.p || (a.Sk && (!a.k.p || !a.v.p)) || !a.lq1 || !a.lk1 || !a.lq2 || !a.lk2)
         return fail(TSN_ERR_ARG, "tsn_diff_attn: null operand");
     auto aligned = [&](const tsn_heads & t, uint32_t S, uint32_t H) {   // a stride that is never taken does not count
@@ -101,7 +579,55 @@ int diff_attn(DeviceCtx & c, const tsn_diff_attn_args & in) {
     if ((a.B > 1 && !a.out.sb) || (a.Sq > 1 && !a.out.ss) || (a.H > 1 && !a.out.sh))
         return fail(TSN_ERR_ARG, "tsn_diff_attn: a result with a stride of 0");
     if (a.scale == 0.0f) a.scale = a.d == 32 ? 0.17677669529663687f : 0.125f;
-    cudaError_t e = a.type == TSN_F16 ? launch<__half>(a, c.stream) : launch<__nv_bfloat16>(a, c.stream);
+
+    // a batch stride of 0 in both K and V: one batch of keys. In one of them only, the map needs real strides.
+    Args p{};
+    p.kv_b = a.B > 1 && (a.k.sb || a.v.sb) ? 1 : 0;
+    const uint32_t KB = p.kv_b ? a.B : 1;
+    auto mappable = [&](const tsn_heads & t) {
+        auto fits = [](int64_t s) { return s > 0 && s < (1ll << 39); };
+        return (a.Sk <= 1 || fits(t.ss)) && (a.Hk == 1 || fits(t.sh)) && (KB == 1 || fits(t.sb));
+    };
+    if (a.Sk && (!mappable(a.k) || !mappable(a.v)))
+        return fail(TSN_ERR_ARG, "tsn_diff_attn: strides of k and v must be positive (0 only for the batch, in both)");
+    p.a = a;
+    p.c = a.scale * LOG2E;
+    p.G = (int) (a.H / a.Hk);
+    p.R = (long long) a.Sq * p.G;
+    p.err = c.d_err;
+    const long long groups = (p.R + ROWS - 1) / ROWS * a.B * a.Hk;
+    if (groups > 0x7fffffffLL) return fail(TSN_ERR_ARG, "tsn_diff_attn: too many query rows");
+    // Split the keys where whole tiles leave SMs without work: as many parts as fill one wave, of two key tiles at
+    // least (a part costs its CTA's start and a trip through the workspace, about what two tiles take).
+    const long long tiles = ((long long) a.Sk + KEYS - 1) / KEYS;
+    p.splits = (int) std::max(1ll, std::min(SMS / groups, tiles / 2));
+    p.wr = (int) std::min<long long>(ROWS, p.R);
+    if (p.splits > 1) {
+        cudaStreamCaptureStatus st = cudaStreamCaptureStatusNone;
+        cudaError_t e = cudaStreamIsCapturing(c.stream, &st);
+        if (e != cudaSuccess) return fail(TSN_ERR_CUDA, std::string("tsn_diff_attn: ") + cudaGetErrorString(e));
+        int rc = workspace(c, st != cudaStreamCaptureStatusNone);
+        if (rc) return rc;
+        p.count = (unsigned int *) c.split_ws;
+        p.part = (float *) ((char *) c.split_ws + COUNTERS * 4);
+    }
+    static_assert(SMS <= COUNTERS && (size_t) SMS * 128 * (2 * 128 + 4) * 4 <= ((size_t) 32 << 20), "one wave of partial results fits");
+    CUtensorMap tk{}, tv{};
+    if (a.Sk && (!make_kv_map(&tk, a, a.k, KB, KEYS) || !make_kv_map(&tv, a, a.v, KB, KEYS)))
+        return fail(TSN_ERR_ARG, "tsn_diff_attn: k or v cannot be described to the tensor memory accelerator");
+    const unsigned grid = (unsigned) (groups * p.splits);
+    const bool bf = a.type == TSN_BF16;
+    cudaError_t e = a.d == 32 ? (bf ? launch_tc<64, true>(tk, tv, p, grid, c.stream) : launch_tc<64, false>(tk, tv, p, grid, c.stream))
+                              : (bf ? launch_tc<128, true>(tk, tv, p, grid, c.stream) : launch_tc<128, false>(tk, tv, p, grid, c.stream));
+    if (e == cudaSuccess && p.splits > 1) {
+        cudaStreamCaptureStatus st = cudaStreamCaptureStatusNone;
+        e = cudaStreamIsCapturing(c.stream, &st);
+        if (e == cudaSuccess && st == cudaStreamCaptureStatusNone) {
+            e = cudaEventRecord(c.split_ev, c.stream);
+            c.split_used = true;
+            c.split_stream = c.stream;
+        }
+    }
     if (e != cudaSuccess) return fail(TSN_ERR_CUDA, std::string("tsn_diff_attn: ") + cudaGetErrorString(e));
     return TSN_OK;
 }

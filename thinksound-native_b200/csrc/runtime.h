@@ -38,6 +38,12 @@ struct DeviceCtx {
     // runtime-face conv: im2col scratch of one chunk of output rows (at most 16 M floats)
     void * col = nullptr;
     size_t col_bytes = 0;
+    // transformer-block operators: partial results of calls that split their keys, allocated once at
+    // its full size; split_ev follows the last call that used it, so calls on other streams wait for it
+    void * split_ws = nullptr;
+    cudaEvent_t split_ev = nullptr;
+    cudaStream_t split_stream = nullptr;
+    bool split_used = false;
     int activate();                  // cudaSetDevice(ordinal)
     int check_device_error();        // after a sync: TSN_ERR_TIMEOUT if a kernel gave up
     int sync();                      // stream sync + device error word
