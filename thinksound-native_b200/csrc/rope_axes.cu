@@ -3,7 +3,11 @@
 // Pair j of a head turns by pos[axis j] * turn[j] turns, turn[j] a 64-bit fraction of a turn per position:
 // the product of the two wraps at whole turns in 64-bit integer arithmetic, so the angle is as exact at
 // position 10^6 as at 0 (a 32-bit product of position and frequency is off by 10^6 * 2^-24 rad there).
-// One warp per head row.
+// Bound by HBM: every head is read and written once. A block takes a few whole tokens: it computes the tokens'
+// cosines and sines once for all their heads into shared memory (in 64-bit phases and sincospi, which
+// would cost more than the memory traffic if each head did it), then its warps run over the heads, 8 elements a
+// lane, with several heads of a token side by side in a warp and their RMSNorm by shuffles.
+#include <algorithm>
 #include <cmath>
 
 #include "block_ops.h"
@@ -18,53 +22,181 @@ __device__ __forceinline__ float phase(int pos, uint64_t turn) {
     return (float) (int) (p >> 32) * 0x1p-32f;
 }
 
+// The address of a head row: heads 0 .. Hq - 1 are the queries', the following the keys'.
 template <class T>
-__global__ void rope_kernel(const __grid_constant__ tsn_rope_plan_t p, const __grid_constant__ tsn_rope_args a) {
-    const int lane = threadIdx.x & 31, D = (int) p.D, P = (int) p.P, Hq = a.q.p ? (int) a.Hq : 0, Hk = a.k.p ? (int) a.Hk : 0;
-    const long long rows = (long long) a.B * a.S * (Hq + Hk);
-    const long long row = (long long) blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5);
-    if (row >= rows) return;
-    const int head = (int) (row % (Hq + Hk));
-    const long long tok = row / (Hq + Hk), b = tok / a.S, s = tok % a.S;
+struct Row {
+    const T * x;
+    T * y;
+};
+template <class T>
+__device__ __forceinline__ Row<T> row_of(const tsn_rope_args & a, int Hq, long long b, long long s, int head) {
     const bool is_q = head < Hq;
-    const tsn_heads & hi = is_q ? a.q : a.k, & ho = is_q ? a.q_out : a.k_out;
+    const tsn_heads & i = is_q ? a.q : a.k, & o = is_q ? a.q_out : a.k_out;
     const int h = is_q ? head : head - Hq;
-    const T * x = (const T *) hi.p + b * hi.sb + s * hi.ss + h * hi.sh;
-    T * y = (T *) ho.p + b * ho.sb + s * ho.ss + h * ho.sh;
-    const float * w = is_q ? a.q_norm : a.k_norm;
-    float v[8];   // element 2 i or 2 i + 1 of this lane's pairs of neighbours: e = 64 * i + 2 * lane
-    float ss = 0.0f;
-    for (int i = 0; i < 4; ++i)
-        for (int k = 0; k < 2; ++k) {
-            const int e = 64 * i + 2 * lane + k;
-            v[2 * i + k] = e < D ? to_f32(x[e]) : 0.0f;
-            ss += v[2 * i + k] * v[2 * i + k];
-        }
-    for (int o = 16; o; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
-    const float inv = w ? rsqrtf(ss / (float) D + a.eps) : 1.0f;
-    __shared__ float buf[8][256];
-    float * u = buf[threadIdx.x >> 5];
-    for (int i = 0; i < 4; ++i)
-        for (int k = 0; k < 2; ++k) {
-            const int e = 64 * i + 2 * lane + k;
-            if (e < D) u[e] = w ? v[2 * i + k] * inv * w[e] : v[2 * i + k];
-        }
-    __syncwarp();
-    const int32_t * pos = a.pos + b * a.pos_sb + s * a.pos_ss;
-    for (int j = lane; j < P; j += 32) {
-        float sn, cs;
-        sincospif(2.0f * phase(pos[p.axis[j]], p.turn[j]), &sn, &cs);
-        const int e0 = p.layout == TSN_ROPE_HALF ? j : 2 * j, e1 = p.layout == TSN_ROPE_HALF ? j + P : 2 * j + 1;
-        const float p0 = u[e0], p1 = u[e1];
-        y[e0] = from_f32<T>(p0 * cs - p1 * sn);
-        y[e1] = from_f32<T>(p0 * sn + p1 * cs);
+    return {(const T *) i.p + b * i.sb + s * i.ss + h * i.sh, (T *) o.p + b * o.sb + s * o.ss + h * o.sh};
+}
+
+__device__ __forceinline__ float2 turn_of(const tsn_rope_plan_t & p, const tsn_rope_args & a, long long b, long long s, int j) {
+    float sn, cs;
+    sincospif(2.0f * phase(a.pos[b * a.pos_sb + s * a.pos_ss + p.axis[j]], p.turn[j]), &sn, &cs);
+    return make_float2(cs, sn);
+}
+
+constexpr int WARPS = 8, MAX_TOK = 4;
+
+// Heads whose rows start at 16-byte boundaries, D a multiple of 8. lph: lanes of a head, the power of two from
+// D / 8 up; tok: tokens of a block.
+template <class T, bool HALF>
+__global__ void __launch_bounds__(32 * WARPS) rope_rows8(const __grid_constant__ tsn_rope_plan_t p, const __grid_constant__ tsn_rope_args a,
+                                                         int lph, int tok) {
+    __shared__ float2 turn[MAX_TOK * TSN_ROPE_MAX_PAIRS];
+    __shared__ __align__(16) float weight[2][2 * TSN_ROPE_MAX_PAIRS];
+    __shared__ float mate[HALF ? WARPS : 1][32 * 9];   // a lane's 8 elements, one word of padding between lanes
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int D = (int) p.D, P = (int) p.P, Hq = a.q.p ? (int) a.Hq : 0, H = Hq + (a.k.p ? (int) a.Hk : 0);
+    const long long tokens = (long long) a.B * a.S, first = (long long) blockIdx.x * tok;
+    const int n = (int) min((long long) tok, tokens - first);
+    const int side = 32 / lph, chunks = (H + side - 1) / side;   // heads side by side in a warp
+    const int at = (lane & (lph - 1)) * 8, sub = lane / lph;
+    const bool in = at < D;
+
+    auto fetch = [&](int item, Row<T> & r, T (&x)[8]) {
+        const int head = item % chunks * side + sub;
+        if (!in || head >= H) { r.y = nullptr; return; }
+        const long long t = first + item / chunks;
+        r = row_of<T>(a, Hq, t / a.S, t % a.S, head);
+#pragma unroll
+        for (int i = 0; i < (int) sizeof(T) / 2; ++i) ((uint4 *) x)[i] = ((const uint4 *) (r.x + at))[i];
+    };
+    alignas(16) T x[8];
+    Row<T> r;
+    if (warp < n * chunks) fetch(warp, r, x);   // before the table: the loads are on their way
+    for (int i = threadIdx.x; i < n * P; i += 32 * WARPS) {
+        const long long t = first + i / P;
+        turn[i] = turn_of(p, a, t / a.S, t % a.S, i % P);
     }
-    for (int e = 2 * P + lane; e < D; e += 32) y[e] = from_f32<T>(u[e]);
+    for (int i = threadIdx.x; i < D; i += 32 * WARPS) {
+        weight[0][i] = a.q_norm ? a.q_norm[i] : 1.0f;
+        weight[1][i] = a.k_norm ? a.k_norm[i] : 1.0f;
+    }
+    __syncthreads();
+    for (int item = warp; item < n * chunks; item += WARPS) {
+        const int head = item % chunks * side + sub;
+        const float2 * tr = turn + item / chunks * P;
+        const bool is_q = head < Hq, mine = r.y != nullptr;
+        T * y = r.y;
+        float u[8];
+        float ss = 0.0f;
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+            u[k] = mine ? to_f32(x[k]) : 0.0f;
+            ss = fmaf(u[k], u[k], ss);
+        }
+        if (item + WARPS < n * chunks) fetch(item + WARPS, r, x);
+        if (a.q_norm || a.k_norm) {
+            for (int o = lph >> 1; o; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+            if (is_q ? a.q_norm != nullptr : a.k_norm != nullptr) {
+                const float inv = rsqrtf(ss / (float) D + a.eps);
+                const float * w = weight[is_q ? 0 : 1] + (in ? at : 0);
+#pragma unroll
+                for (int k = 0; k < 8; ++k) u[k] *= inv * w[k];
+            }
+        }
+        float v[8];
+        if (HALF) {
+            float * m = mate[warp];
+#pragma unroll
+            for (int k = 0; k < 8; ++k) m[lane * 9 + k] = u[k];
+            __syncwarp();
+            const int base = lane - (lane & (lph - 1));   // the head's first lane
+#pragma unroll
+            for (int k = 0; k < 8; ++k) {
+                const int e = at + k;
+                v[k] = u[k];
+                if (e < 2 * P && mine) {
+                    const int o = e < P ? e + P : e - P;
+                    const float w = m[(base + (o >> 3)) * 9 + (o & 7)];
+                    const float2 cs = tr[e < P ? e : e - P];
+                    v[k] = e < P ? u[k] * cs.x - w * cs.y : w * cs.y + u[k] * cs.x;
+                }
+            }
+            __syncwarp();
+        } else {
+#pragma unroll
+            for (int k = 0; k < 8; k += 2) {
+                const int j = (at + k) >> 1;
+                v[k] = u[k];
+                v[k + 1] = u[k + 1];
+                if (j < P) {
+                    const float2 cs = tr[j];
+                    v[k] = u[k] * cs.x - u[k + 1] * cs.y;
+                    v[k + 1] = u[k] * cs.y + u[k + 1] * cs.x;
+                }
+            }
+        }
+        if (mine) {
+            alignas(16) T o[8];
+#pragma unroll
+            for (int k = 0; k < 8; ++k) o[k] = from_f32<T>(v[k]);
+#pragma unroll
+            for (int i = 0; i < (int) sizeof(T) / 2; ++i) ((uint4 *) (y + at))[i] = ((uint4 *) o)[i];
+        }
+    }
+}
+
+// Any D, strides and alignment: one warp per head row.
+template <class T>
+__global__ void __launch_bounds__(32 * WARPS) rope_rows1(const __grid_constant__ tsn_rope_plan_t p, const __grid_constant__ tsn_rope_args a) {
+    __shared__ float buf[WARPS][2 * TSN_ROPE_MAX_PAIRS];
+    const int lane = threadIdx.x & 31, D = (int) p.D, P = (int) p.P, Hq = a.q.p ? (int) a.Hq : 0, H = Hq + (a.k.p ? (int) a.Hk : 0);
+    const long long item = (long long) blockIdx.x * WARPS + (threadIdx.x >> 5);
+    if (item >= (long long) a.B * a.S * H) return;
+    const int head = (int) (item % H);
+    const long long t = item / H, b = t / a.S, s = t % a.S;
+    const Row<T> r = row_of<T>(a, Hq, b, s, head);
+    const float * w = head < Hq ? a.q_norm : a.k_norm;
+    float * u = buf[threadIdx.x >> 5];
+    float ss = 0.0f;
+    for (int e = lane; e < D; e += 32) {
+        const float v = to_f32(r.x[e]);
+        u[e] = v;
+        ss = fmaf(v, v, ss);
+    }
+    for (int o = 16; o; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+    __syncwarp();
+    const float inv = rsqrtf(ss / (float) D + a.eps);
+    auto normed = [&](int e) { return w ? u[e] * (inv * w[e]) : u[e]; };
+    for (int j = lane; j < P; j += 32) {
+        const float2 cs = turn_of(p, a, b, s, j);
+        const int e0 = p.layout == TSN_ROPE_HALF ? j : 2 * j, e1 = p.layout == TSN_ROPE_HALF ? j + P : 2 * j + 1;
+        const float p0 = normed(e0), p1 = normed(e1);
+        r.y[e0] = from_f32<T>(p0 * cs.x - p1 * cs.y);
+        r.y[e1] = from_f32<T>(p0 * cs.y + p1 * cs.x);
+    }
+    for (int e = 2 * P + lane; e < D; e += 32) r.y[e] = from_f32<T>(normed(e));
 }
 
 template <class T>
-cudaError_t launch(const tsn_rope_plan_t & p, const tsn_rope_args & a, long long rows, cudaStream_t s) {
-    rope_kernel<T><<<(unsigned) ((rows + 7) / 8), 256, 0, s>>>(p, a);
+cudaError_t launch(const tsn_rope_plan_t & p, const tsn_rope_args & a, cudaStream_t s) {
+    auto rows16 = [&](const tsn_heads & h, uint32_t H) {
+        return !h.p || !H || ((((uintptr_t) h.p) | (uintptr_t) (a.B > 1 ? h.sb : 0) * sizeof(T) | (uintptr_t) (a.S > 1 ? h.ss : 0) * sizeof(T) |
+                               (uintptr_t) (H > 1 ? h.sh : 0) * sizeof(T)) & 15) == 0;
+    };
+    const long long tokens = (long long) a.B * a.S;
+    const int H = (int) ((a.q.p ? a.Hq : 0) + (a.k.p ? a.Hk : 0));
+    if (p.D % 8 == 0 && rows16(a.q, a.Hq) && rows16(a.k, a.Hk) && (!a.q.p || rows16(a.q_out, a.Hq)) && (!a.k.p || rows16(a.k_out, a.Hk))) {
+        int lph = 1;
+        while (lph * 8 < (int) p.D) lph *= 2;
+        // Tokens of a block: as many as give each warp four rounds, fewer while blocks do not fill the SMs.
+        const int chunks = (H + 32 / lph - 1) / (32 / lph);
+        int tok = std::min(MAX_TOK, std::max(1, 4 * WARPS / chunks));
+        tok = (int) std::min<long long>(tok, std::max(1ll, tokens / (4 * 148)));
+        const unsigned blocks = (unsigned) ((tokens + tok - 1) / tok);
+        if (p.layout == TSN_ROPE_HALF) rope_rows8<T, true><<<blocks, 32 * WARPS, 0, s>>>(p, a, lph, tok);
+        else rope_rows8<T, false><<<blocks, 32 * WARPS, 0, s>>>(p, a, lph, tok);
+    } else {
+        rope_rows1<T><<<(unsigned) ((tokens * H + WARPS - 1) / WARPS), 32 * WARPS, 0, s>>>(p, a);
+    }
     return cudaGetLastError();
 }
 
@@ -102,7 +234,7 @@ int rope_axes(DeviceCtx & c, const tsn_rope_plan_t & p, const tsn_rope_args & a)
     const long long heads = (a.q.p ? (long long) a.Hq : 0) + (a.k.p ? (long long) a.Hk : 0);
     const long long tokens = (long long) a.B * a.S;
     if (tokens == 0 || heads == 0) return TSN_OK;
-    if (heads > 65536 || tokens > (0x7fffffffLL * 8) / heads) return fail(TSN_ERR_ARG, "tsn_rope_axes: too many rows");
+    if (heads > 65536 || tokens > 0x7fffffffLL || tokens > (0x7fffffffLL * WARPS) / heads) return fail(TSN_ERR_ARG, "tsn_rope_axes: too many rows");
     if ((a.q.p && a.Hq && !a.q_out.p) || (a.k.p && a.Hk && !a.k_out.p) || (p.P && !a.pos))
         return fail(TSN_ERR_ARG, "tsn_rope_axes: null result or positions");
     auto distinct = [&](const tsn_heads & o, uint32_t H) {
@@ -110,10 +242,12 @@ int rope_axes(DeviceCtx & c, const tsn_rope_plan_t & p, const tsn_rope_args & a)
     };
     if ((a.q.p && a.Hq && !distinct(a.q_out, a.Hq)) || (a.k.p && a.Hk && !distinct(a.k_out, a.Hk)))
         return fail(TSN_ERR_ARG, "tsn_rope_axes: a result with a stride of 0");
-    const long long rows = tokens * heads;
-    cudaError_t e = a.type == TSN_F32   ? launch<float>(p, a, rows, c.stream)
-                    : a.type == TSN_F16 ? launch<__half>(p, a, rows, c.stream)
-                                        : launch<__nv_bfloat16>(p, a, rows, c.stream);
+    const uintptr_t addresses = (uintptr_t) a.q.p | (uintptr_t) a.k.p | (uintptr_t) (a.q.p ? a.q_out.p : nullptr) | (uintptr_t) (a.k.p ? a.k_out.p : nullptr);
+    if ((addresses & (type_size(a.type) - 1)) || (((uintptr_t) a.pos | (uintptr_t) a.q_norm | (uintptr_t) a.k_norm) & 3))
+        return fail(TSN_ERR_ARG, "tsn_rope_axes: an address that is no multiple of its element's size");
+    cudaError_t e = a.type == TSN_F32   ? launch<float>(p, a, c.stream)
+                    : a.type == TSN_F16 ? launch<__half>(p, a, c.stream)
+                                        : launch<__nv_bfloat16>(p, a, c.stream);
     if (e != cudaSuccess) return fail(TSN_ERR_CUDA, std::string("tsn_rope_axes: ") + cudaGetErrorString(e));
     return TSN_OK;
 }
