@@ -10,6 +10,7 @@
 #include "block_ops.h"
 
 #include <algorithm>
+#include <type_traits>
 
 namespace tsn {
 
@@ -20,35 +21,52 @@ struct NormArgs {
     unsigned rows;
 };
 
-// V elements of type T, held as they lie in memory
+// V elements of type T: 16-byte words where a piece has some, else the elements themselves.
 template <class T, int V>
-struct alignas(sizeof(T) * V > 16 ? 16 : sizeof(T) * V) Piece {
-    T v[V];
+struct Piece {
+    static constexpr bool WIDE = sizeof(T) * V >= 16;
+    typename std::conditional<WIDE, Words<T, WIDE ? V : 16>, T>::type r;
+    __device__ __forceinline__ void load(const T * p) {
+        if constexpr (WIDE) r = load_words<T, V>(p);
+        else r = *p;
+    }
+    __device__ __forceinline__ void get(float * v) const {
+        if constexpr (WIDE) to_floats<T, V>(r, v);
+        else *v = to_f32(r);
+    }
 };
 template <class T, int V>
-__device__ __forceinline__ Piece<T, V> load(const T * p) {
-    Piece<T, V> r;
-    if constexpr (sizeof(T) * V >= 16) {
-#pragma unroll
-        for (int i = 0; i < (int) (sizeof(T) * V / 16); ++i) ((uint4 *) &r)[i] = ((const uint4 *) p)[i];
-    } else {
-#pragma unroll
-        for (int i = 0; i < V; ++i) r.v[i] = p[i];
-    }
-    return r;
-}
-template <class T, int V>
 __device__ __forceinline__ void store(T * p, const float * v) {
-    Piece<T, V> r;
-#pragma unroll
-    for (int i = 0; i < V; ++i) r.v[i] = from_f32<T>(v[i]);
-    if constexpr (sizeof(T) * V >= 16) {
-#pragma unroll
-        for (int i = 0; i < (int) (sizeof(T) * V / 16); ++i) ((uint4 *) p)[i] = ((uint4 *) &r)[i];
+    if constexpr (Piece<T, V>::WIDE) store_words<T, V>(p, v);
+    else *p = from_f32<T>(*v);
+}
+// v[k] = f(v[k], ...) over a piece, two at a time where it has two
+template <int V, class F2>
+__device__ __forceinline__ void each(float * v, F2 f2) {
+    if constexpr (V == 1) {
+        v[0] = f2(make_float2(v[0], 0.0f), 0).x;
     } else {
 #pragma unroll
-        for (int i = 0; i < V; ++i) p[i] = r.v[i];
+        for (int k = 0; k < V; k += 2) {
+            const float2 r = f2(make_float2(v[k], v[k + 1]), k);
+            v[k] = r.x;
+            v[k + 1] = r.y;
+        }
     }
+}
+template <int V>
+__device__ __forceinline__ float2 at2(const float * v, int k) { return make_float2(v[k], V == 1 ? 0.0f : v[k + (V > 1)]); }
+__device__ __forceinline__ float2 both(float v) { return make_float2(v, v); }
+
+// tanh(x) = 1 - 2 / (e^(2x) + 1). For 16-bit gates: off by 2^-22 at most, where the gate itself is known to 2^-12
+// of its value; the library's tanhf, exact to its last bits near 0 as well, would cost more than the row's traffic.
+template <class T>
+__device__ __forceinline__ float gate_tanh(float x) {
+    if (sizeof(T) == 4) return tanhf(x);
+    float e, r;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(x * 2.88539008177792681f));
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(e + 1.0f));
+    return fmaf(-2.0f, r, 1.0f);
 }
 
 // Sum over the row's threads: a warp, or the whole block (one barrier; red is another array for each sum).
@@ -57,53 +75,55 @@ __device__ __forceinline__ float row_sum(float v, float * red) {
 #pragma unroll
     for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
     if (!BLOCK) return v;
-    const int warps = (int) (blockDim.x >> 5);
-    if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = v;
+    const int warps = (int) (blockDim.x >> 5), lane = (int) (threadIdx.x & 31);
+    if (lane == 0) red[threadIdx.x >> 5] = v;
     __syncthreads();
-    float s = 0.0f;
-    if (warps <= 8) {
-        for (int w = 0; w < warps; ++w) s += red[w];
-        return s;
-    }
-    s = (int) (threadIdx.x & 31) < warps ? red[threadIdx.x & 31] : 0.0f;
-#pragma unroll
-    for (int o = 16; o; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
-    return s;
+    float s = lane < warps ? red[lane] : 0.0f;
+    for (int o = 1; o < warps; o <<= 1) s += __shfl_xor_sync(0xffffffffu, s, o);   // lane 0's power of two of lanes
+    return __shfl_sync(0xffffffffu, s, 0);
 }
 
 // u normalised in place. Elements past C are zero and stay so; at(i): whether piece i lies inside the row.
 template <int NV, int V, bool BLOCK, class At, class Col>
-__device__ __forceinline__ void norm(float (&u)[NV][V], int C, int kind, float eps, const float * w, const float * b, float * red,
+__device__ __forceinline__ void norm(float (&u)[NV][V], float inv_C, int kind, float eps, const float * w, const float * b, float * red,
                                      At at, Col col) {
     if (kind == TSN_NORM_NONE) return;
     float mean = 0.0f;
     if (kind == TSN_NORM_LAYER) {
-        float s = 0.0f;
+        float2 s = both(0.0f);
 #pragma unroll
         for (int i = 0; i < NV; ++i)
-#pragma unroll
-            for (int k = 0; k < V; ++k) s += u[i][k];
-        mean = row_sum<BLOCK>(s, red) / (float) C;
+            each<V>(u[i], [&](float2 v, int) { s = add2(s, v); return v; });
+        mean = row_sum<BLOCK>(s.x + s.y, red) * inv_C;
     }
-    float q = 0.0f;
+    float2 q = both(0.0f);
+    const float2 minus = both(-mean);
 #pragma unroll
     for (int i = 0; i < NV; ++i)
         if (at(i))
-#pragma unroll
-            for (int k = 0; k < V; ++k) { const float d = u[i][k] - mean; q = fmaf(d, d, q); }
-    const float inv = rsqrtf(row_sum<BLOCK>(q, red + 32) / (float) C + eps);
+            each<V>(u[i], [&](float2 v, int) {
+                v = add2(v, minus);
+                if (V == 1) v.y = 0.0f;
+                q = fma2(v, v, q);
+                return v;
+            });
+    const float2 inv = both(rsqrtf(fmaf(row_sum<BLOCK>(q.x + q.y, red + 32), inv_C, eps)));
 #pragma unroll
     for (int i = 0; i < NV; ++i)
         if (at(i)) {
-            Piece<float, V> wv, bv;
-            if (w) wv = load<float, V>(w + col(i));
-            if (b) bv = load<float, V>(b + col(i));
-#pragma unroll
-            for (int k = 0; k < V; ++k) {
-                float v = (u[i][k] - mean) * inv;
-                if (w) v *= wv.v[k];
-                if (b) v += bv.v[k];
-                u[i][k] = v;
+            each<V>(u[i], [&](float2 v, int) { return mul2(v, inv); });
+            float wv[V], bv[V];
+            if (w) {
+                Piece<float, V> r;
+                r.load(w + col(i));
+                r.get(wv);
+                each<V>(u[i], [&](float2 v, int k) { return mul2(v, at2<V>(wv, k)); });
+            }
+            if (b) {
+                Piece<float, V> r;
+                r.load(b + col(i));
+                r.get(bv);
+                each<V>(u[i], [&](float2 v, int k) { return add2(v, at2<V>(bv, k)); });
             }
         }
 }
@@ -117,29 +137,33 @@ __global__ void __launch_bounds__(most_threads(V, NV, BLOCK)) block_norm_kernel(
     __shared__ float red[BLOCK ? 128 : 1];
     const tsn_block_norm_args & a = n.a;
     const int C = (int) a.C;
+    const float inv_C = 1.0f / (float) C;
     const unsigned row = BLOCK ? blockIdx.x : blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5);
     if (!BLOCK && row >= n.rows) return;
     const int first = (BLOCK ? (int) threadIdx.x : (int) (threadIdx.x & 31)) * V, step = (BLOCK ? (int) blockDim.x : 32) * V;
     auto col = [&](int i) { return first + i * step; };
     auto at = [&](int i) { return col(i) < C; };
-    const long long b = row / a.T, t = row % a.T;
+    const unsigned b = row / a.T, t = row % a.T;
     auto in = [&](const tsn_rows & r) { return b * r.sb + t * r.st; };
 
-    Piece<TX, V> x[NV];
     constexpr bool EARLY = NV <= 2;
+    Piece<TX, V> x[NV];
     Piece<T, V> y[NV], g[EARLY ? NV : 1], sc[EARLY ? NV : 1], sh[EARLY ? NV : 1];
-    auto modulation = [&](Piece<T, V> & r, const tsn_rows & m, int i) { r = load<T, V>((const T *) m.p + in(m) + col(i)); };
+    auto modulation = [&](Piece<T, V> & r, const tsn_rows & m, int i) { r.load((const T *) m.p + in(m) + col(i)); };
 #pragma unroll
     for (int i = 0; i < NV; ++i)
         if (at(i)) {
-            if (a.y.p) y[i] = load<T, V>((const T *) a.y.p + in(a.y) + col(i));
-            x[i] = load<TX, V>((const TX *) a.x.p + in(a.x) + col(i));
-            if (EARLY) {
-                if (a.gate.p) modulation(g[i], a.gate, i);
+            if (a.y.p) y[i].load((const T *) a.y.p + in(a.y) + col(i));
+            x[i].load((const TX *) a.x.p + in(a.x) + col(i));
+            if (EARLY && a.gate.p) modulation(g[i], a.gate, i);
+        }
+    if (EARLY)
+#pragma unroll
+        for (int i = 0; i < NV; ++i)
+            if (at(i)) {
                 if (a.scale.p) modulation(sc[i], a.scale, i);
                 if (a.shift.p) modulation(sh[i], a.shift, i);
             }
-        }
     float u[NV][V];
 #pragma unroll
     for (int i = 0; i < NV; ++i)
@@ -148,46 +172,54 @@ __global__ void __launch_bounds__(most_threads(V, NV, BLOCK)) block_norm_kernel(
     if (a.y.p) {
 #pragma unroll
         for (int i = 0; i < NV; ++i)
-            if (at(i))
-#pragma unroll
-                for (int k = 0; k < V; ++k) u[i][k] = to_f32(y[i].v[k]);
-        norm<NV, V, BLOCK>(u, C, a.post, a.post_eps, a.post_w, a.post_b, red, at, col);
+            if (at(i)) y[i].get(u[i]);
+        norm<NV, V, BLOCK>(u, inv_C, a.post, a.post_eps, a.post_w, a.post_b, red, at, col);
         if (a.gate.p)
 #pragma unroll
             for (int i = 0; i < NV; ++i)
                 if (at(i)) {
                     Piece<T, V> & gi = g[EARLY ? i : 0];
                     if (!EARLY) modulation(gi, a.gate, i);
+                    float gv[V];
+                    gi.get(gv);
+                    if (a.gate_tanh)
 #pragma unroll
-                    for (int k = 0; k < V; ++k) {
-                        const float v = to_f32(gi.v[k]);
-                        u[i][k] *= a.gate_tanh ? tanhf(v) : v;
-                    }
+                        for (int k = 0; k < V; ++k) gv[k] = gate_tanh<T>(gv[k]);
+                    each<V>(u[i], [&](float2 v, int k) { return mul2(v, at2<V>(gv, k)); });
                 }
     }
 #pragma unroll
     for (int i = 0; i < NV; ++i)
         if (at(i)) {
-            Piece<float, V> r;
-            if (a.res_vec) r = load<float, V>(a.res_vec + col(i));
-#pragma unroll
-            for (int k = 0; k < V; ++k) u[i][k] = fmaf(to_f32(x[i].v[k]), a.res_vec ? r.v[k] : a.res_scale, u[i][k]);
+            float xv[V], rv[V];
+            x[i].get(xv);
+            if (a.res_vec) {
+                Piece<float, V> r;
+                r.load(a.res_vec + col(i));
+                r.get(rv);
+                each<V>(u[i], [&](float2 v, int k) { return fma2(at2<V>(xv, k), at2<V>(rv, k), v); });
+            } else {
+                each<V>(u[i], [&](float2 v, int k) { return fma2(at2<V>(xv, k), both(a.res_scale), v); });
+            }
             if (a.x_out.p) store<TX, V>((TX *) a.x_out.p + in(a.x_out) + col(i), u[i]);
         }
     if (!a.h.p) return;
-    norm<NV, V, BLOCK>(u, C, a.pre, a.pre_eps, a.pre_w, a.pre_b, red + (BLOCK ? 64 : 0), at, col);
+    norm<NV, V, BLOCK>(u, inv_C, a.pre, a.pre_eps, a.pre_w, a.pre_b, red + (BLOCK ? 64 : 0), at, col);
 #pragma unroll
     for (int i = 0; i < NV; ++i)
         if (at(i)) {
-            Piece<T, V> & si = sc[EARLY ? i : 0], & hi = sh[EARLY ? i : 0];
-            if (!EARLY) {
-                if (a.scale.p) modulation(si, a.scale, i);
-                if (a.shift.p) modulation(hi, a.shift, i);
+            float mv[V];
+            if (a.scale.p) {
+                Piece<T, V> & si = sc[EARLY ? i : 0];
+                if (!EARLY) modulation(si, a.scale, i);
+                si.get(mv);
+                each<V>(u[i], [&](float2 v, int k) { return mul2(v, add2(at2<V>(mv, k), both(1.0f))); });
             }
-#pragma unroll
-            for (int k = 0; k < V; ++k) {
-                if (a.scale.p) u[i][k] *= 1.0f + to_f32(si.v[k]);
-                if (a.shift.p) u[i][k] += to_f32(hi.v[k]);
+            if (a.shift.p) {
+                Piece<T, V> & hi = sh[EARLY ? i : 0];
+                if (!EARLY) modulation(hi, a.shift, i);
+                hi.get(mv);
+                each<V>(u[i], [&](float2 v, int k) { return add2(v, at2<V>(mv, k)); });
             }
             store<T, V>((T *) a.h.p + in(a.h) + col(i), u[i]);
         }
@@ -203,9 +235,10 @@ cudaError_t launch(const NormArgs & n, cudaStream_t s) {
         if (pieces <= 4 * threads) block_norm_kernel<TX, T, V, 4, true><<<n.rows, threads, 0, s>>>(n);
         else block_norm_kernel<TX, T, V, 16, true><<<n.rows, threads, 0, s>>>(n);
     } else {
-        // Two pieces a thread where the rows fill the GPU, one where there are few and their latency counts.
-        const bool few = n.rows <= 2 * 148;
-        const int per = pieces > 2048 ? 8 : pieces > 1024 ? 4 : few ? 1 : 2;
+        // One piece a thread while a block of 512 holds the row: the least latency where there are few rows (658
+        // rows of 1024: 4.2 us, 4.8 with two pieces, 8.6 with four), and no slower where rows fill the GPU (32 500 of
+        // 2048: 174, 175 and 233 us).
+        const int per = pieces > 2048 ? 8 : pieces > 1024 ? 4 : pieces > 512 ? 2 : 1;
         const int threads = (pieces + 32 * per - 1) / (32 * per) * 32;
         if (per == 1) block_norm_kernel<TX, T, V, 1, true><<<n.rows, threads, 0, s>>>(n);
         else if (per == 2) block_norm_kernel<TX, T, V, 2, true><<<n.rows, threads, 0, s>>>(n);

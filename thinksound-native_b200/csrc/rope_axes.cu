@@ -45,34 +45,30 @@ __device__ __forceinline__ float2 turn_of(const tsn_rope_plan_t & p, const tsn_r
 constexpr int WARPS = 8, MAX_TOK = 4;
 
 // Heads whose rows start at 16-byte boundaries, D a multiple of 8. lph: lanes of a head, the power of two from
-// D / 8 up; tok: tokens of a block.
+// D / 8 up; tok: tokens of a block. A warp's item is a chunk of 32 / lph heads of one token, queries' or keys'.
 template <class T, bool HALF>
 __global__ void __launch_bounds__(32 * WARPS) rope_rows8(const __grid_constant__ tsn_rope_plan_t p, const __grid_constant__ tsn_rope_args a,
                                                          int lph, int tok) {
     __shared__ float2 turn[MAX_TOK * TSN_ROPE_MAX_PAIRS];
     __shared__ __align__(16) float weight[2][2 * TSN_ROPE_MAX_PAIRS];
+    __shared__ T * start[MAX_TOK][4];                  // a token's first head: q, k, q_out, k_out
     __shared__ float mate[HALF ? WARPS : 1][32 * 9];   // a lane's 8 elements, one word of padding between lanes
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const int D = (int) p.D, P = (int) p.P, Hq = a.q.p ? (int) a.Hq : 0, H = Hq + (a.k.p ? (int) a.Hk : 0);
-    const long long tokens = (long long) a.B * a.S, first = (long long) blockIdx.x * tok;
-    const int n = (int) min((long long) tok, tokens - first);
-    const int side = 32 / lph, chunks = (H + side - 1) / side;   // heads side by side in a warp
-    const int at = (lane & (lph - 1)) * 8, sub = lane / lph;
+    const int D = (int) p.D, P = (int) p.P, Hq = a.q.p ? (int) a.Hq : 0, Hk = a.k.p ? (int) a.Hk : 0;
+    const unsigned first = blockIdx.x * (unsigned) tok;
+    const int n = (int) min((unsigned) tok, a.B * a.S - first);
+    const int side = 32 / lph, sub = lane / lph, at = (lane & (lph - 1)) * 8;
+    const int q_chunks = (Hq + side - 1) / side, chunks = q_chunks + (Hk + side - 1) / side;
     const bool in = at < D;
+    const float inv_D = 1.0f / (float) D;
 
-    auto fetch = [&](int item, Row<T> & r, T (&x)[8]) {
-        const int head = item % chunks * side + sub;
-        if (!in || head >= H) { r.y = nullptr; return; }
-        const long long t = first + item / chunks;
-        r = row_of<T>(a, Hq, t / a.S, t % a.S, head);
-#pragma unroll
-        for (int i = 0; i < (int) sizeof(T) / 2; ++i) ((uint4 *) x)[i] = ((const uint4 *) (r.x + at))[i];
-    };
-    alignas(16) T x[8];
-    Row<T> r;
-    if (warp < n * chunks) fetch(warp, r, x);   // before the table: the loads are on their way
+    if (threadIdx.x < 4 * n) {
+        const unsigned t = first + (threadIdx.x >> 2), b = t / a.S, s = t % a.S;
+        const tsn_heads & h = (threadIdx.x & 3) == 0 ? a.q : (threadIdx.x & 3) == 1 ? a.k : (threadIdx.x & 3) == 2 ? a.q_out : a.k_out;
+        start[threadIdx.x >> 2][threadIdx.x & 3] = (T *) h.p + b * h.sb + s * h.ss;
+    }
     for (int i = threadIdx.x; i < n * P; i += 32 * WARPS) {
-        const long long t = first + i / P;
+        const unsigned t = first + i / P;
         turn[i] = turn_of(p, a, t / a.S, t % a.S, i % P);
     }
     for (int i = threadIdx.x; i < D; i += 32 * WARPS) {
@@ -80,67 +76,74 @@ __global__ void __launch_bounds__(32 * WARPS) rope_rows8(const __grid_constant__
         weight[1][i] = a.k_norm ? a.k_norm[i] : 1.0f;
     }
     __syncthreads();
-    for (int item = warp; item < n * chunks; item += WARPS) {
-        const int head = item % chunks * side + sub;
-        const float2 * tr = turn + item / chunks * P;
-        const bool is_q = head < Hq, mine = r.y != nullptr;
-        T * y = r.y;
+
+    int k = warp / chunks, chunk = warp % chunks;
+    Words<T, 8> x;
+    T * y = nullptr;
+    auto fetch = [&]() {
+        y = nullptr;
+        if (k >= n) return;
+        const bool is_q = chunk < q_chunks;
+        const int head = (is_q ? chunk : chunk - q_chunks) * side + sub;
+        if (!in || head >= (is_q ? Hq : Hk)) return;
+        x = load_words<T, 8>(start[k][is_q ? 0 : 1] + head * (is_q ? a.q.sh : a.k.sh) + at);
+        y = start[k][is_q ? 2 : 3] + head * (is_q ? a.q_out.sh : a.k_out.sh) + at;
+    };
+    fetch();
+    while (k < n) {
+        const float2 * tr = turn + k * P;
+        const bool is_q = chunk < q_chunks;
+        T * const to = y;
         float u[8];
-        float ss = 0.0f;
+        if (to) {
+            to_floats<T, 8>(x, u);
+        } else {
 #pragma unroll
-        for (int k = 0; k < 8; ++k) {
-            u[k] = mine ? to_f32(x[k]) : 0.0f;
-            ss = fmaf(u[k], u[k], ss);
+            for (int i = 0; i < 8; ++i) u[i] = 0.0f;
         }
-        if (item + WARPS < n * chunks) fetch(item + WARPS, r, x);
-        if (a.q_norm || a.k_norm) {
+        for (chunk += WARPS; chunk >= chunks; chunk -= chunks) ++k;
+        fetch();   // the next item's heads, while this one is turned
+        if (is_q ? a.q_norm != nullptr : a.k_norm != nullptr) {
+            float ss = 0.0f;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) ss = fmaf(u[i], u[i], ss);
             for (int o = lph >> 1; o; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
-            if (is_q ? a.q_norm != nullptr : a.k_norm != nullptr) {
-                const float inv = rsqrtf(ss / (float) D + a.eps);
-                const float * w = weight[is_q ? 0 : 1] + (in ? at : 0);
-#pragma unroll
-                for (int k = 0; k < 8; ++k) u[k] *= inv * w[k];
-            }
+            const float inv = rsqrtf(fmaf(ss, inv_D, a.eps));
+            const float4 * w = (const float4 *) (weight[is_q ? 0 : 1] + (in ? at : 0));
+            const float4 w0 = w[0], w1 = w[1];
+            u[0] *= inv * w0.x; u[1] *= inv * w0.y; u[2] *= inv * w0.z; u[3] *= inv * w0.w;
+            u[4] *= inv * w1.x; u[5] *= inv * w1.y; u[6] *= inv * w1.z; u[7] *= inv * w1.w;
         }
-        float v[8];
         if (HALF) {
             float * m = mate[warp];
 #pragma unroll
-            for (int k = 0; k < 8; ++k) m[lane * 9 + k] = u[k];
+            for (int i = 0; i < 8; ++i) m[lane * 9 + i] = u[i];
             __syncwarp();
             const int base = lane - (lane & (lph - 1));   // the head's first lane
 #pragma unroll
-            for (int k = 0; k < 8; ++k) {
-                const int e = at + k;
-                v[k] = u[k];
-                if (e < 2 * P && mine) {
+            for (int i = 0; i < 8; ++i) {
+                const int e = at + i;
+                if (e < 2 * P && in) {
                     const int o = e < P ? e + P : e - P;
                     const float w = m[(base + (o >> 3)) * 9 + (o & 7)];
                     const float2 cs = tr[e < P ? e : e - P];
-                    v[k] = e < P ? u[k] * cs.x - w * cs.y : w * cs.y + u[k] * cs.x;
+                    u[i] = fmaf(u[i], cs.x, e < P ? -w * cs.y : w * cs.y);
                 }
             }
             __syncwarp();
         } else {
 #pragma unroll
-            for (int k = 0; k < 8; k += 2) {
-                const int j = (at + k) >> 1;
-                v[k] = u[k];
-                v[k + 1] = u[k + 1];
+            for (int i = 0; i < 8; i += 2) {
+                const int j = (at + i) >> 1;
                 if (j < P) {
                     const float2 cs = tr[j];
-                    v[k] = u[k] * cs.x - u[k + 1] * cs.y;
-                    v[k + 1] = u[k] * cs.y + u[k + 1] * cs.x;
+                    const float v = u[i];
+                    u[i] = v * cs.x - u[i + 1] * cs.y;
+                    u[i + 1] = v * cs.y + u[i + 1] * cs.x;
                 }
             }
         }
-        if (mine) {
-            alignas(16) T o[8];
-#pragma unroll
-            for (int k = 0; k < 8; ++k) o[k] = from_f32<T>(v[k]);
-#pragma unroll
-            for (int i = 0; i < (int) sizeof(T) / 2; ++i) ((uint4 *) (y + at))[i] = ((uint4 *) o)[i];
-        }
+        if (to) store_words<T, 8>(to, u);
     }
 }
 
@@ -187,9 +190,9 @@ cudaError_t launch(const tsn_rope_plan_t & p, const tsn_rope_args & a, cudaStrea
     if (p.D % 8 == 0 && rows16(a.q, a.Hq) && rows16(a.k, a.Hk) && (!a.q.p || rows16(a.q_out, a.Hq)) && (!a.k.p || rows16(a.k_out, a.Hk))) {
         int lph = 1;
         while (lph * 8 < (int) p.D) lph *= 2;
-        // Tokens of a block: as many as give each warp four rounds, fewer while blocks do not fill the SMs.
-        const int chunks = (H + 32 / lph - 1) / (32 / lph);
-        int tok = std::min(MAX_TOK, std::max(1, 4 * WARPS / chunks));
+        // Tokens of a block: as many as give each warp eight rounds, fewer while blocks do not fill the SMs.
+        const int chunks = std::max(1, H / (32 / lph));
+        int tok = std::min(MAX_TOK, std::max(1, 8 * WARPS / chunks));
         tok = (int) std::min<long long>(tok, std::max(1ll, tokens / (4 * 148)));
         const unsigned blocks = (unsigned) ((tokens + tok - 1) / tok);
         if (p.layout == TSN_ROPE_HALF) rope_rows8<T, true><<<blocks, 32 * WARPS, 0, s>>>(p, a, lph, tok);
