@@ -9,6 +9,7 @@
 // lane, with several heads of a token side by side in a warp and their RMSNorm by shuffles.
 #include <algorithm>
 #include <cmath>
+#include <type_traits>
 
 #include "block_ops.h"
 
@@ -42,108 +43,133 @@ __device__ __forceinline__ float2 turn_of(const tsn_rope_plan_t & p, const tsn_r
     return make_float2(cs, sn);
 }
 
-constexpr int WARPS = 8, MAX_TOK = 4;
+constexpr int WARPS = 8, MAX_TOK = 8;
 
-// Heads whose rows start at 16-byte boundaries, D a multiple of 8. lph: lanes of a head, the power of two from
-// D / 8 up; tok: tokens of a block. A warp's item is a chunk of 32 / lph heads of one token, queries' or keys'.
-template <class T, bool HALF>
-__global__ void __launch_bounds__(32 * WARPS) rope_rows8(const __grid_constant__ tsn_rope_plan_t p, const __grid_constant__ tsn_rope_args a,
-                                                         int lph, int tok) {
-    __shared__ float2 turn[MAX_TOK * TSN_ROPE_MAX_PAIRS];
-    __shared__ __align__(16) float weight[2][2 * TSN_ROPE_MAX_PAIRS];
-    __shared__ T * start[MAX_TOK][4];                  // a token's first head: q, k, q_out, k_out
-    __shared__ float mate[HALF ? WARPS : 1][32 * 9];   // a lane's 8 elements, one word of padding between lanes
+// How a lane finds the other element of its pairs.
+enum { NEXT, LANES, SHARED };   // interleaved: its own; halves: another lane's (P a multiple of 8), or shared memory
+
+// Heads whose rows start at 16-byte boundaries, D a multiple of 8. LPH: lanes of a head, the power of two from
+// D / 8 up. Block (x, b, z): tokens x * tok .. of sequence b, chunks 8 z .. of 32 / LPH heads. A warp takes one chunk,
+// queries' or keys', through the block's tokens, so that a token costs its lanes a load, a store and the
+// arithmetic; with fewer chunks than warps, several warps share a chunk's tokens.
+// Loads run one round ahead of the arithmetic: 32 500 tokens x 64 heads of 64, bf16, written head-major, take 102 us
+// (5.2 TB/s, 0.80 of the measured copy) with two tokens a round at four blocks per SM; 110 with one, 108 with four at
+// fewer blocks, 113 without the round ahead. With 16 tokens a block 104, with 32 113.
+template <class T, int LPH, int PAIR>
+__global__ void __launch_bounds__(32 * WARPS, 4) rope_rows8(const __grid_constant__ tsn_rope_plan_t p, const __grid_constant__ tsn_rope_args a, int tok) {
+    constexpr int SIDE = 32 / LPH, AHEAD = sizeof(T) == 4 ? 1 : 2;   // tokens of a round: 16 or 32 bytes a lane each
+    __shared__ __align__(16) float2 turn[MAX_TOK * TSN_ROPE_MAX_PAIRS + 8];
+    __shared__ float mate[PAIR == SHARED ? WARPS : 1][32 * 9];   // a lane's 8 elements, one word of padding between lanes
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int D = (int) p.D, P = (int) p.P, Hq = a.q.p ? (int) a.Hq : 0, Hk = a.k.p ? (int) a.Hk : 0;
-    const unsigned first = blockIdx.x * (unsigned) tok;
-    const int n = (int) min((unsigned) tok, a.B * a.S - first);
-    const int side = 32 / lph, sub = lane / lph, at = (lane & (lph - 1)) * 8;
-    const int q_chunks = (Hq + side - 1) / side, chunks = q_chunks + (Hk + side - 1) / side;
-    const bool in = at < D;
+    const long long b = blockIdx.y, s0 = (long long) blockIdx.x * tok;
+    const int n = (int) min((long long) tok, a.S - s0);
+    const int sub = lane / LPH, at = (lane & (LPH - 1)) * 8;
+    const int q_chunks = (Hq + SIDE - 1) / SIDE, chunks = q_chunks + (Hk + SIDE - 1) / SIDE;
+    const int sharing = chunks < WARPS ? WARPS / chunks : 1;   // warps of a chunk
     const float inv_D = 1.0f / (float) D;
+    const int row = (P + 1) & ~1;   // a token's pairs in the table, from a 16-byte boundary on
 
-    if (threadIdx.x < 4 * n) {
-        const unsigned t = first + (threadIdx.x >> 2), b = t / a.S, s = t % a.S;
-        const tsn_heads & h = (threadIdx.x & 3) == 0 ? a.q : (threadIdx.x & 3) == 1 ? a.k : (threadIdx.x & 3) == 2 ? a.q_out : a.k_out;
-        start[threadIdx.x >> 2][threadIdx.x & 3] = (T *) h.p + b * h.sb + s * h.ss;
-    }
-    for (int i = threadIdx.x; i < n * P; i += 32 * WARPS) {
-        const unsigned t = first + i / P;
-        turn[i] = turn_of(p, a, t / a.S, t % a.S, i % P);
-    }
-    for (int i = threadIdx.x; i < D; i += 32 * WARPS) {
-        weight[0][i] = a.q_norm ? a.q_norm[i] : 1.0f;
-        weight[1][i] = a.k_norm ? a.k_norm[i] : 1.0f;
-    }
-    __syncthreads();
-
-    int k = warp / chunks, chunk = warp % chunks;
-    Words<T, 8> x;
-    T * y = nullptr;
-    auto fetch = [&]() {
-        y = nullptr;
-        if (k >= n) return;
-        const bool is_q = chunk < q_chunks;
-        const int head = (is_q ? chunk : chunk - q_chunks) * side + sub;
-        if (!in || head >= (is_q ? Hq : Hk)) return;
-        x = load_words<T, 8>(start[k][is_q ? 0 : 1] + head * (is_q ? a.q.sh : a.k.sh) + at);
-        y = start[k][is_q ? 2 : 3] + head * (is_q ? a.q_out.sh : a.k_out.sh) + at;
+    const int chunk = sharing > 1 ? (warp < sharing * chunks ? warp % chunks : chunks) : (int) blockIdx.z * WARPS + warp;
+    const bool is_q = chunk < q_chunks;
+    const tsn_heads & hi = is_q ? a.q : a.k, & ho = is_q ? a.q_out : a.k_out;
+    const float * wp = is_q ? a.q_norm : a.k_norm;
+    const int head = (is_q ? chunk : chunk - q_chunks) * SIDE + sub, from = sharing > 1 ? warp / chunks : 0;
+    const bool mine = chunk < chunks && at < D && head < (is_q ? Hq : Hk);
+    const T * x = (const T *) hi.p + b * hi.sb + (s0 + from) * hi.ss + head * hi.sh + at;
+    T * y = (T *) ho.p + b * ho.sb + (s0 + from) * ho.ss + head * ho.sh + at;
+    const long long dx = sharing * hi.ss, dy = sharing * ho.ss;
+    Words<T, 8> raw[AHEAD], next[AHEAD];
+    auto fetch = [&](int k0) {
+#pragma unroll
+        for (int c = 0; c < AHEAD; ++c)
+            if (mine && k0 + c * sharing < n) next[c] = load_words<T, 8>(x + c * dx);
+        x += AHEAD * dx;
     };
-    fetch();
-    while (k < n) {
-        const float2 * tr = turn + k * P;
-        const bool is_q = chunk < q_chunks;
-        T * const to = y;
-        float u[8];
-        if (to) {
-            to_floats<T, 8>(x, u);
-        } else {
+    fetch(from);   // before the table: the loads are on their way
+    float2 w[4];
+    if (wp)
 #pragma unroll
-            for (int i = 0; i < 8; ++i) u[i] = 0.0f;
-        }
-        for (chunk += WARPS; chunk >= chunks; chunk -= chunks) ++k;
-        fetch();   // the next item's heads, while this one is turned
-        if (is_q ? a.q_norm != nullptr : a.k_norm != nullptr) {
-            float ss = 0.0f;
+        for (int i = 0; i < 4; ++i) w[i] = mine ? make_float2(wp[at + 2 * i], wp[at + 2 * i + 1]) : make_float2(0.0f, 0.0f);
+    for (int i = threadIdx.x; i < n * P; i += 32 * WARPS) turn[i / P * row + i % P] = turn_of(p, a, b, s0 + i / P, i % P);
+    __syncthreads();
+    if (chunk >= chunks) return;
+
+    for (int k0 = from; k0 < n; k0 += AHEAD * sharing) {
 #pragma unroll
-            for (int i = 0; i < 8; ++i) ss = fmaf(u[i], u[i], ss);
-            for (int o = lph >> 1; o; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
-            const float inv = rsqrtf(fmaf(ss, inv_D, a.eps));
-            const float4 * w = (const float4 *) (weight[is_q ? 0 : 1] + (in ? at : 0));
-            const float4 w0 = w[0], w1 = w[1];
-            u[0] *= inv * w0.x; u[1] *= inv * w0.y; u[2] *= inv * w0.z; u[3] *= inv * w0.w;
-            u[4] *= inv * w1.x; u[5] *= inv * w1.y; u[6] *= inv * w1.z; u[7] *= inv * w1.w;
-        }
-        if (HALF) {
-            float * m = mate[warp];
+        for (int c = 0; c < AHEAD; ++c) raw[c] = next[c];
+        fetch(k0 + AHEAD * sharing);
 #pragma unroll
-            for (int i = 0; i < 8; ++i) m[lane * 9 + i] = u[i];
-            __syncwarp();
-            const int base = lane - (lane & (lph - 1));   // the head's first lane
+        for (int c = 0; c < AHEAD; ++c) {
+            const int k = k0 + c * sharing;
+            if (k >= n) break;
+            float u[8];
+            to_floats<T, 8>(raw[c], u);
+            if (wp) {
+                float2 q = make_float2(0.0f, 0.0f);
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                const int e = at + i;
-                if (e < 2 * P && in) {
-                    const int o = e < P ? e + P : e - P;
-                    const float w = m[(base + (o >> 3)) * 9 + (o & 7)];
-                    const float2 cs = tr[e < P ? e : e - P];
-                    u[i] = fmaf(u[i], cs.x, e < P ? -w * cs.y : w * cs.y);
+                for (int i = 0; i < 8; i += 2) q = fma2(make_float2(u[i], u[i + 1]), make_float2(u[i], u[i + 1]), q);
+                float ss = mine ? q.x + q.y : 0.0f;
+#pragma unroll
+                for (int o = LPH >> 1; o; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+                const float inv = rsqrtf(fmaf(ss, inv_D, a.eps));
+#pragma unroll
+                for (int i = 0; i < 8; i += 2) {
+                    const float2 r = mul2(make_float2(u[i], u[i + 1]), mul2(w[i / 2], make_float2(inv, inv)));
+                    u[i] = r.x;
+                    u[i + 1] = r.y;
                 }
             }
-            __syncwarp();
-        } else {
+            const float2 * tr = turn + k * row;
+            if (PAIR == NEXT) {
 #pragma unroll
-            for (int i = 0; i < 8; i += 2) {
-                const int j = (at + i) >> 1;
-                if (j < P) {
-                    const float2 cs = tr[j];
-                    const float v = u[i];
-                    u[i] = v * cs.x - u[i + 1] * cs.y;
-                    u[i + 1] = v * cs.y + u[i + 1] * cs.x;
+                for (int i = 0; i < 8; i += 4) {
+                    const int j = (at + i) >> 1;
+                    const float4 cs = *(const float4 *) (tr + (j < row ? j : 0));
+                    const float2 v = make_float2(u[i], u[i + 2]);
+                    if (j < P) {
+                        u[i] = v.x * cs.x - u[i + 1] * cs.y;
+                        u[i + 1] = v.x * cs.y + u[i + 1] * cs.x;
+                    }
+                    if (j + 1 < P) {
+                        u[i + 2] = v.y * cs.z - u[i + 3] * cs.w;
+                        u[i + 3] = v.y * cs.w + u[i + 3] * cs.z;
+                    }
                 }
+            } else if (PAIR == LANES) {
+                const bool low = at < P, turned = at < 2 * P;
+                const int other = turned ? (low ? lane + P / 8 : lane - P / 8) : lane;
+                const float4 * cs = (const float4 *) (tr + (turned ? (low ? at : at - P) : 0));
+#pragma unroll
+                for (int i = 0; i < 8; i += 2) {
+                    const float4 c2 = cs[i / 2];
+                    const float m0 = __shfl_sync(0xffffffffu, u[i], other), m1 = __shfl_sync(0xffffffffu, u[i + 1], other);
+                    if (turned) {
+                        u[i] = fmaf(u[i], c2.x, low ? -m0 * c2.y : m0 * c2.y);
+                        u[i + 1] = fmaf(u[i + 1], c2.z, low ? -m1 * c2.w : m1 * c2.w);
+                    }
+                }
+            } else {
+                float * m = mate[warp];
+#pragma unroll
+                for (int i = 0; i < 8; ++i) m[lane * 9 + i] = u[i];
+                __syncwarp();
+                const int base = lane & ~(LPH - 1);   // the head's first lane
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    const int e = at + i;
+                    if (e < 2 * P) {
+                        const int o = e < P ? e + P : e - P;
+                        const float v = m[(base + (o >> 3)) * 9 + (o & 7)];
+                        const float2 cs = tr[e < P ? e : e - P];
+                        u[i] = fmaf(u[i], cs.x, e < P ? -v * cs.y : v * cs.y);
+                    }
+                }
+                __syncwarp();
             }
+            if (mine) store_words<T, 8>(y + c * dy, u);
         }
-        if (to) store_words<T, 8>(to, u);
+        y += AHEAD * dy;
     }
 }
 
@@ -187,16 +213,26 @@ cudaError_t launch(const tsn_rope_plan_t & p, const tsn_rope_args & a, cudaStrea
     };
     const long long tokens = (long long) a.B * a.S;
     const int H = (int) ((a.q.p ? a.Hq : 0) + (a.k.p ? a.Hk : 0));
-    if (p.D % 8 == 0 && rows16(a.q, a.Hq) && rows16(a.k, a.Hk) && (!a.q.p || rows16(a.q_out, a.Hq)) && (!a.k.p || rows16(a.k_out, a.Hk))) {
+    if (p.D % 8 == 0 && a.B <= 65535 && rows16(a.q, a.Hq) && rows16(a.k, a.Hk) && (!a.q.p || rows16(a.q_out, a.Hq)) && (!a.k.p || rows16(a.k_out, a.Hk))) {
         int lph = 1;
         while (lph * 8 < (int) p.D) lph *= 2;
-        // Tokens of a block: as many as give each warp eight rounds, fewer while blocks do not fill the SMs.
-        const int chunks = std::max(1, H / (32 / lph));
-        int tok = std::min(MAX_TOK, std::max(1, 8 * WARPS / chunks));
-        tok = (int) std::min<long long>(tok, std::max(1ll, tokens / (4 * 148)));
-        const unsigned blocks = (unsigned) ((tokens + tok - 1) / tok);
-        if (p.layout == TSN_ROPE_HALF) rope_rows8<T, true><<<blocks, 32 * WARPS, 0, s>>>(p, a, lph, tok);
-        else rope_rows8<T, false><<<blocks, 32 * WARPS, 0, s>>>(p, a, lph, tok);
+        // Tokens of a block: 8 share its start; fewer while blocks would not fill the SMs.
+        const int tok = (int) std::min<long long>(MAX_TOK, std::max(1ll, tokens / (4 * 148)));
+        const int side = 32 / lph, chunks = (int) ((a.q.p ? a.Hq : 0) + side - 1) / side + (int) ((a.k.p ? a.Hk : 0) + side - 1) / side;
+        const dim3 blocks((a.S + tok - 1) / tok, a.B, (chunks + WARPS - 1) / WARPS);
+        const int pair = p.layout == TSN_ROPE_INTERLEAVED ? NEXT : p.P % 8 == 0 ? LANES : SHARED;
+        auto go = [&](auto L) {
+            constexpr int LPH = decltype(L)::value;
+            if (pair == NEXT) rope_rows8<T, LPH, NEXT><<<blocks, 32 * WARPS, 0, s>>>(p, a, tok);
+            else if (pair == LANES) rope_rows8<T, LPH, LANES><<<blocks, 32 * WARPS, 0, s>>>(p, a, tok);
+            else rope_rows8<T, LPH, SHARED><<<blocks, 32 * WARPS, 0, s>>>(p, a, tok);
+        };
+        if (lph == 1) go(std::integral_constant<int, 1>());
+        else if (lph == 2) go(std::integral_constant<int, 2>());
+        else if (lph == 4) go(std::integral_constant<int, 4>());
+        else if (lph == 8) go(std::integral_constant<int, 8>());
+        else if (lph == 16) go(std::integral_constant<int, 16>());
+        else go(std::integral_constant<int, 32>());
     } else {
         rope_rows1<T><<<(unsigned) ((tokens * H + WARPS - 1) / WARPS), 32 * WARPS, 0, s>>>(p, a);
     }
