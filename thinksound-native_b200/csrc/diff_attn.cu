@@ -1,4 +1,5 @@
-// diff_attn.cu — differential attention on the tcgen05 tensor cores (tsn_diff_attn).
+// diff_attn.cu — differential attention (tsn_diff_attn): diff_attn_tc on the tcgen05 tensor cores, and
+// diff_attn_rows for at most 16 query rows.
 //
 //   o = O_1 / l_1 - lambda O_2 / l_2,   O_m = sum_j p_mj v_j,  l_m = sum_j p_mj,  p_mj = 2^(c q_m.k_mj - ref_m)
 // in one pass over the keys: ref_m follows the running maximum of the row, O_m and l_m are rescaled when it
@@ -59,6 +60,7 @@ struct Args {
     long long R;                // Sq * G rows of one kv head
     int splits, kv_b;           // parts of the keys; 0: every batch reads the same keys
     int wr;                     // rows of a partial result
+    int chunk;                  // few rows: slabs of a part
     float * part;
     unsigned int * count;
     int * err;
@@ -152,7 +154,7 @@ diff_attn_tc(const __grid_constant__ CUtensorMap tk, const __grid_constant__ CUt
         *abort_flag = 0;
         fence_mbar_init();
     }
-    if (warp == 8 && lane == 0) { tma_prefetch(&tk); tma_prefetch(&tv); }
+    if (warp == 8 && lane == 0 && nt > 0) { tma_prefetch(&tk); tma_prefetch(&tv); }
     if (warp == 9) tmem_alloc(words, 512);
     tc_fence_before();
     __syncthreads();
@@ -489,6 +491,381 @@ diff_attn_tc(const __grid_constant__ CUtensorMap tk, const __grid_constant__ CUt
     }
 }
 
+// ================================================================ few rows
+// diff_attn_rows: at most 16 rows of a kv head (one token with its group's heads, or a few), bound by reading K and V.
+// A 128-row tile would spend its time on rows that do not exist; here mma.sync takes 16 rows (m16n8k16), which
+// is far from being the limit: 48 products for 16 keys of 8 KB.
+// Each warp streams its own 16-key slabs (slab w, w + W, ...) by TMA through a ring of its own, so warps never wait
+// for one another: scores, online softmax and O of both maps stay in the warp's registers. The warps' sums
+// are added up in shared memory at the end, the parts of split keys through the workspace.
+constexpr int SLAB = 16, RING = 3;
+
+template <int D, int W>
+struct RowLay {
+    static constexpr int BOX = SLAB * 128, HALF = SLAB * D * 2, STAGE = 2 * HALF;   // a slab's keys, then its values
+    static constexpr int OFF_LAM = W * RING * STAGE, OFF_W = OFF_LAM + 16 * 4, OFF_BAR = OFF_W + D * 4;
+    static constexpr int TOTAL = OFF_BAR + W * RING * 8 + 16;
+    // after the last slab: each warp's O [16][2][D] and its ref and l [2 maps][16] each
+    static constexpr int SUMS = 16 * 2 * D + 64;
+    static_assert(W * SUMS * 4 <= W * RING * STAGE, "the warps' sums fit in their rings");
+};
+
+template <bool BF16>
+__device__ __forceinline__ void mma16816(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    if (BF16)
+        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                     : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+    else
+        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                     : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+template <bool TRANS>
+__device__ __forceinline__ void ldmatrix4(uint32_t (&r)[4], uint32_t at) {
+    if (TRANS)
+        asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(at) : "memory");
+    else
+        asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(at) : "memory");
+}
+
+// Adds up `count` sets of sums for one row, one warp: set i has O [2][D] of the row at o + i * stride, and ref and l of
+// map m at st + i * stride + m * rows and + (2 + m) * rows. Returns O (this lane's D / 32 columns), ref and l.
+template <int D, bool GLOBAL>
+__device__ __forceinline__ void add_up(const float * o, const float * st, size_t stride, int rows, int count, int lane,
+                                       float (&sum)[2][D / 32], float (&top)[2], float (&l)[2]) {
+    constexpr int E = D / 32;
+    auto rd = [&](const float * p) { return GLOBAL ? __ldcg(p) : *p; };
+#pragma unroll
+    for (int m = 0; m < 2; ++m) {
+        top[m] = -INFINITY;
+        l[m] = 0.0f;
+        for (int i = lane; i < count; i += 32) top[m] = fmaxf(top[m], rd(st + i * stride + m * rows));
+#pragma unroll
+        for (int x = 16; x; x >>= 1) top[m] = fmaxf(top[m], __shfl_xor_sync(~0u, top[m], x));
+        const float ref = top[m] == -INFINITY ? 0.0f : top[m];
+        for (int i = lane; i < count; i += 32) l[m] += ex2(rd(st + i * stride + m * rows) - ref) * rd(st + i * stride + (2 + m) * rows);
+#pragma unroll
+        for (int x = 16; x; x >>= 1) l[m] += __shfl_xor_sync(~0u, l[m], x);
+#pragma unroll
+        for (int e = 0; e < E; ++e) sum[m][e] = 0.0f;
+#pragma unroll 8
+        for (int i = 0; i < count; ++i) {
+            const float f = ex2(rd(st + i * stride + m * rows) - ref);
+            const float * at = o + i * stride + m * D + E * lane;
+            float v[E];
+            if constexpr (E == 4) {
+                const float4 x = GLOBAL ? __ldcg((const float4 *) at) : *(const float4 *) at;
+                v[0] = x.x; v[1] = x.y; v[2] = x.z; v[3] = x.w;
+            } else {
+                const float2 x = GLOBAL ? __ldcg((const float2 *) at) : *(const float2 *) at;
+                v[0] = x.x; v[1] = x.y;
+            }
+#pragma unroll
+            for (int e = 0; e < E; ++e) sum[m][e] = fmaf(f, v[e], sum[m][e]);
+        }
+    }
+}
+
+template <int D, bool BF16, int W>
+__global__ void __launch_bounds__(32 * W, W == 8 ? 1 : 2)
+diff_attn_rows(const __grid_constant__ CUtensorMap tk, const __grid_constant__ CUtensorMap tv, const __grid_constant__ Args p) {
+    using L = RowLay<D, W>;
+    constexpr int d = D / 2, E = D / 32;
+    extern __shared__ __align__(1024) uint8_t smem[];
+    const tsn_diff_attn_args & a = p.a;
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    if (smem_u32(smem) & 1023) {
+        if (tid == 0 && p.err) atomicCAS(p.err, 0, DEV_BAD_ARGS);
+        return;
+    }
+    float * lam = (float *) (smem + L::OFF_LAM), * nw = (float *) (smem + L::OFF_W);
+    uint64_t * full = (uint64_t *) (smem + L::OFF_BAR) + warp * RING;
+    volatile int * flags = (volatile int *) (smem + L::OFF_BAR + W * RING * 8);   // abort, last to arrive
+
+    const unsigned gid = blockIdx.x / p.splits, split = blockIdx.x % p.splits;
+    const int hk = (int) (gid % a.Hk), b = (int) (gid / a.Hk), R = (int) p.R;
+    const int n = a.key_len ? max(0, min(a.key_len[b], (int) a.Sk)) : (int) a.Sk;
+    auto limit = [&](int r) {   // keys before which row r sees; rows past the last one see all
+        if (!a.causal || r >= R) return n;
+        return (int) max(0ll, min((long long) n, (long long) (r / p.G) + n - (long long) a.Sq + 1));
+    };
+    const int least = limit(0);
+    // this CTA's slabs, and this warp's
+    const int s0 = (int) min((long long) (n + SLAB - 1) / SLAB, (long long) split * p.chunk);
+    const int s1 = min((n + SLAB - 1) / SLAB, s0 + p.chunk);
+    const int mine = s1 - s0 > warp ? (s1 - s0 - warp + W - 1) / W : 0;
+
+    if (tid == 0) flags[0] = 0;
+    if (lane == 0) {
+        if (mine > 0) { tma_prefetch(&tk); tma_prefetch(&tv); }
+        for (int s = 0; s < RING; ++s) mbar_init(&full[s], 1);
+        fence_mbar_init();
+    }
+    __syncwarp();
+    uint8_t * ring = smem + warp * RING * L::STAGE;
+    auto request = [&](int i) {   // slab i of this warp, one lane
+        uint8_t * at = ring + (i % RING) * L::STAGE;
+        const int key = (s0 + warp + i * W) * SLAB;
+        mbar_expect_tx(&full[i % RING], L::STAGE);
+#pragma unroll
+        for (int x = 0; x < D / 64; ++x) {
+            tma_load_4d(at + x * L::BOX, &tk, &full[i % RING], 64 * x, key, hk, b * p.kv_b);
+            tma_load_4d(at + L::HALF + x * L::BOX, &tv, &full[i % RING], 64 * x, key, hk, b * p.kv_b);
+        }
+    };
+    if (lane == 0)
+        for (int i = 0; i < RING && i < mine; ++i) request(i);
+
+    // lambda of each head of the group, the norm's weights
+    for (int g = warp; g < p.G; g += W) {
+        const long long h = (long long) (hk * p.G + g) * a.lam_sh;
+        float z1 = 0.0f, z2 = 0.0f;
+        for (int e = lane; e < d; e += 32) { z1 += a.lq1[h + e] * a.lk1[h + e]; z2 += a.lq2[h + e] * a.lk2[h + e]; }
+#pragma unroll
+        for (int x = 16; x; x >>= 1) { z1 += __shfl_xor_sync(~0u, z1, x); z2 += __shfl_xor_sync(~0u, z2, x); }
+        if (lane == 0) lam[g] = expf(z1) - expf(z2) + a.lambda_init;
+    }
+    for (int e = tid; e < D; e += 32 * W) nw[e] = (a.norm_w ? a.norm_w[e] : 1.0f) * (1.0f - a.lambda_init);
+
+    // Q as A operands: rows lane / 4 and lane / 4 + 8, rows past the last one as zeros
+    const int r0 = lane >> 2, c0 = (lane & 3) * 2;
+    uint32_t qa[2][d / 16][4];
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+        const int r = r0 + 8 * h;
+        const uint16_t * q = (const uint16_t *) a.q.p + b * a.q.sb + (long long) (r / p.G) * a.q.ss + (long long) (hk * p.G + r % p.G) * a.q.sh;
+#pragma unroll
+        for (int m = 0; m < 2; ++m)
+#pragma unroll
+            for (int k = 0; k < d / 16; ++k) {
+                qa[m][k][h] = r < R ? *(const uint32_t *) (q + m * d + 16 * k + c0) : 0u;
+                qa[m][k][2 + h] = r < R ? *(const uint32_t *) (q + m * d + 16 * k + c0 + 8) : 0u;
+            }
+    }
+    const int lim[2] = {limit(r0), limit(r0 + 8)};
+    const uint8_t * mask = a.key_mask ? a.key_mask + b * a.mask_sb : nullptr;
+    __syncthreads();   // the abort flag, lambda and the weights are set
+
+    float o[2][D / 8][4], l[2][2] = {}, ref[2][2];
+#pragma unroll
+    for (int m = 0; m < 2; ++m) {
+        ref[m][0] = ref[m][1] = -INFINITY;
+#pragma unroll
+        for (int x = 0; x < D / 8; ++x)
+#pragma unroll
+            for (int k = 0; k < 4; ++k) o[m][x][k] = 0.0f;
+    }
+    bool poison[2] = {false, false};
+    // addresses of ldmatrix: K rows (key) with the two 8-element halves of a k step side by side, V rows (key)
+    // with two groups of 8 columns
+    const int krow = (lane & 7) + ((lane >> 4) << 3), kch = (lane >> 3) & 1;
+    const int vrow = (lane & 7) + (((lane >> 3) & 1) << 3), vch = lane >> 4;
+    for (int i = 0; i < mine; ++i) {
+        const int base = (s0 + warp + i * W) * SLAB;
+        uint32_t there = low_bits(n - base) & 0xffffu;   // the keys that exist
+        if (mask) there = __ballot_sync(~0u, lane < SLAB && base + lane < n && mask[base + lane] != 0);
+        if (!mbar_wait(&full[i % RING], (i / RING) & 1, flags, p.err, DEV_TIMEOUT_FULL)) break;
+        __syncwarp();
+        const uint32_t kt = smem_u32(ring + (i % RING) * L::STAGE), vt = kt + L::HALF;
+        float s[2][2][4];
+#pragma unroll
+        for (int m = 0; m < 2; ++m) {
+#pragma unroll
+            for (int x = 0; x < 2; ++x)
+#pragma unroll
+                for (int k = 0; k < 4; ++k) s[m][x][k] = 0.0f;
+#pragma unroll
+            for (int k = 0; k < d / 16; ++k) {
+                const int col = m * d + 16 * k;
+                uint32_t f[4];
+                ldmatrix4<false>(f, kt + (col / 64) * L::BOX + krow * 128 + ((((col % 64) / 8 + kch) ^ (krow & 7)) << 4));
+                mma16816<BF16>(s[m][0], qa[m][k], f[0], f[1]);
+                mma16816<BF16>(s[m][1], qa[m][k], f[2], f[3]);
+            }
+        }
+        const bool gone = there != 0xffffu, mixed = a.causal && least < min(n, base + SLAB);
+        uint32_t vis[2];
+#pragma unroll
+        for (int h = 0; h < 2; ++h) vis[h] = there & low_bits(lim[h] - base);
+        if (gone || mixed) {
+#pragma unroll
+            for (int m = 0; m < 2; ++m)
+#pragma unroll
+                for (int x = 0; x < 2; ++x)
+#pragma unroll
+                    for (int k = 0; k < 4; ++k)
+                        if (!((vis[k >> 1] >> (8 * x + c0 + (k & 1))) & 1u)) s[m][x][k] = -INFINITY;
+        }
+        bool move = false;
+        float top[2][2];
+#pragma unroll
+        for (int m = 0; m < 2; ++m)
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                top[m][h] = fmaxf(fmaxf(s[m][0][2 * h], s[m][0][2 * h + 1]), fmaxf(s[m][1][2 * h], s[m][1][2 * h + 1])) * p.c;
+                move |= top[m][h] > ref[m][h] + LAZY;
+            }
+        if (__any_sync(~0u, move)) {
+#pragma unroll
+            for (int m = 0; m < 2; ++m)
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    float t = fmaxf(top[m][h], __shfl_xor_sync(~0u, top[m][h], 1));
+                    t = fmaxf(t, __shfl_xor_sync(~0u, t, 2));
+                    if (t > ref[m][h] + LAZY) {   // a row moves its reference by itself
+                        const float f = ex2(ref[m][h] - t);
+                        ref[m][h] = t;
+                        l[m][h] *= f;
+#pragma unroll
+                        for (int x = 0; x < D / 8; ++x) { o[m][x][2 * h] *= f; o[m][x][2 * h + 1] *= f; }
+                    }
+                }
+        }
+        uint32_t pa[2][4];
+#pragma unroll
+        for (int m = 0; m < 2; ++m) {
+            const float n0 = ref[m][0] == -INFINITY ? 0.0f : -ref[m][0], n1 = ref[m][1] == -INFINITY ? 0.0f : -ref[m][1];
+#pragma unroll
+            for (int x = 0; x < 2; ++x) {
+                const float e0 = ex2(fmaf(s[m][x][0], p.c, n0)), e1 = ex2(fmaf(s[m][x][1], p.c, n0));
+                const float e2 = ex2(fmaf(s[m][x][2], p.c, n1)), e3 = ex2(fmaf(s[m][x][3], p.c, n1));
+                l[m][0] += e0 + e1;
+                l[m][1] += e2 + e3;
+                pa[m][2 * x] = pack16<BF16>(e0, e1);
+                pa[m][2 * x + 1] = pack16<BF16>(e2, e3);
+            }
+        }
+        if (!gone && !mixed) {
+#pragma unroll
+            for (int x = 0; x < D / 16; ++x) {
+                uint32_t f[4];
+                ldmatrix4<true>(f, vt + (x / 4) * L::BOX + vrow * 128 + (((2 * (x % 4) + vch) ^ (vrow & 7)) << 4));
+#pragma unroll
+                for (int m = 0; m < 2; ++m) {
+                    mma16816<BF16>(o[m][2 * x], pa[m], f[0], f[1]);
+                    mma16816<BF16>(o[m][2 * x + 1], pa[m], f[2], f[3]);
+                }
+            }
+        } else {
+            // values behind masked keys count as zero; where rows differ, so do non-finite ones, and rows that see one are marked
+            const auto word = [](uint32_t two) { return (two & 1u ? 0xffffu : 0u) | (two & 2u ? 0xffff0000u : 0u); };
+            const uint32_t keep0 = word(there >> c0), keep1 = word(there >> (c0 + 8));
+            uint32_t bad = 0;
+#pragma unroll
+            for (int x = 0; x < D / 16; ++x) {
+                uint32_t f[4];
+                ldmatrix4<true>(f, vt + (x / 4) * L::BOX + vrow * 128 + (((2 * (x % 4) + vch) ^ (vrow & 7)) << 4));
+                f[0] &= keep0; f[1] &= keep1; f[2] &= keep0; f[3] &= keep1;
+                if (mixed) {
+#pragma unroll
+                    for (int y = 0; y < 4; ++y) {
+                        const uint32_t g = finite_only<BF16>(f[y]), diff = f[y] ^ g;
+                        if (diff & 0xffffu) bad |= 1u << (c0 + 8 * (y & 1));
+                        if (diff >> 16) bad |= 2u << (c0 + 8 * (y & 1));
+                        f[y] = g;
+                    }
+                }
+#pragma unroll
+                for (int m = 0; m < 2; ++m) {
+                    mma16816<BF16>(o[m][2 * x], pa[m], f[0], f[1]);
+                    mma16816<BF16>(o[m][2 * x + 1], pa[m], f[2], f[3]);
+                }
+            }
+            bad = __reduce_or_sync(~0u, bad);
+            poison[0] |= (bad & vis[0]) != 0;
+            poison[1] |= (bad & vis[1]) != 0;
+        }
+        __syncwarp();   // every lane has its operands: the stage may be loaded again
+        if (lane == 0 && i + RING < mine) request(i + RING);
+    }
+
+    // the warp's sums in its ring, then warp w adds up rows w, w + W, ... of all warps
+    float * sums = (float *) ring;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+        const int r = r0 + 8 * h;
+#pragma unroll
+        for (int m = 0; m < 2; ++m) {
+            float t = l[m][h];
+            t += __shfl_xor_sync(~0u, t, 1);
+            t += __shfl_xor_sync(~0u, t, 2);
+            if ((lane & 3) == 0) {
+                sums[16 * 2 * D + m * 16 + r] = ref[m][h];
+                sums[16 * 2 * D + (2 + m) * 16 + r] = poison[h] ? NAN : t;
+            }
+            if (r < R)
+#pragma unroll
+                for (int x = 0; x < D / 8; ++x)
+                    *(float2 *) (sums + (r * 2 + m) * D + 8 * x + c0) = make_float2(o[m][x][2 * h], o[m][x][2 * h + 1]);
+        }
+    }
+    __syncthreads();
+    auto finish = [&](int r, float (&sum)[2][E], float (&rl)[2]) {
+        const int g = r % p.G;
+        const float w1 = rl[0] == 0.0f ? 0.0f : 1.0f / rl[0], w2 = rl[1] == 0.0f ? 0.0f : lam[g] / rl[1];
+        float ss = 0.0f, v[E];
+#pragma unroll
+        for (int e = 0; e < E; ++e) {
+            v[e] = sum[0][e] * w1 - sum[1][e] * w2;
+            ss += v[e] * v[e];
+        }
+#pragma unroll
+        for (int x = 16; x; x >>= 1) ss += __shfl_xor_sync(~0u, ss, x);
+        const float f = ss < INFINITY ? rsqrtf(ss * (1.0f / D) + a.eps) : NAN;
+        uint32_t x[E / 2];
+#pragma unroll
+        for (int e = 0; e < E; e += 2) x[e / 2] = pack16<BF16>(v[e] * f * nw[E * lane + e], v[e + 1] * f * nw[E * lane + e + 1]);
+        uint16_t * out = (uint16_t *) a.out.p + b * a.out.sb + (long long) (r / p.G) * a.out.ss + (long long) (hk * p.G + g) * a.out.sh + E * lane;
+        if (flags[0]) return;
+        if constexpr (E == 4) *(uint2 *) out = make_uint2(x[0], x[1]);
+        else *(uint32_t *) out = x[0];
+    };
+    const float * all = (const float *) smem;
+    constexpr size_t STRIDE = (size_t) RING * L::STAGE / 4;
+    const size_t size = (size_t) R * (2 * D + 4);
+    float * part = p.part + (size_t) gid * p.splits * size;
+    for (int r = warp; r < R; r += W) {
+        float sum[2][E], top[2], rl[2];
+        add_up<D, false>(all + r * 2 * D, all + 16 * 2 * D + r, STRIDE, 16, W, lane, sum, top, rl);
+        if (p.splits == 1) {
+            finish(r, sum, rl);
+        } else {
+            float * at = part + split * size;
+#pragma unroll
+            for (int m = 0; m < 2; ++m) {
+                float * to = at + (size_t) (r * 2 + m) * D + E * lane;
+                if constexpr (E == 4) *(float4 *) to = make_float4(sum[m][0], sum[m][1], sum[m][2], sum[m][3]);
+                else *(float2 *) to = make_float2(sum[m][0], sum[m][1]);
+                if (lane == 0) {
+                    at[(size_t) R * 2 * D + m * R + r] = top[m];
+                    at[(size_t) R * 2 * D + (2 + m) * R + r] = rl[m];
+                }
+            }
+        }
+    }
+    if (p.splits > 1) {
+        __threadfence();
+        __syncthreads();
+        if (tid == 0) {
+            const bool last = atomicAdd(&p.count[gid], 1u) + 1u == (unsigned) p.splits;
+            if (last) p.count[gid] = 0;   // for the next call
+            __threadfence();
+            flags[1] = last;
+        }
+        __syncthreads();
+        if (flags[1])
+            for (int r = warp; r < R; r += W) {
+                float sum[2][E], top[2], rl[2];
+                add_up<D, true>(part + (size_t) r * 2 * D, part + (size_t) R * 2 * D + r, size, R, p.splits, lane, sum, top, rl);
+                finish(r, sum, rl);
+            }
+    }
+    if (flags[0] && tid == 0) {
+        // let copies that were issued but never consumed land before the CTA's shared memory is reused
+        const uint64_t t1 = global_ns();
+        while (global_ns() - t1 < 20000ull) {}
+    }
+}
+
 // ---------------------------------------------------------------- host
 PFN_cuTensorMapEncodeTiled_v12000 encoder() {
     static const PFN_cuTensorMapEncodeTiled_v12000 enc = [] {
@@ -544,6 +921,12 @@ cudaError_t launch_tc(const CUtensorMap & tk, const CUtensorMap & tv, const Args
     diff_attn_tc<D, BF16><<<grid, THREADS, Lay<D>::TOTAL, s>>>(tk, tv, p);
     return cudaGetLastError();
 }
+template <int D, bool BF16>
+cudaError_t launch_rows(const CUtensorMap & tk, const CUtensorMap & tv, const Args & p, unsigned grid, int warps, cudaStream_t s) {
+    if (warps == 8) diff_attn_rows<D, BF16, 8><<<grid, 256, RowLay<D, 8>::TOTAL, s>>>(tk, tv, p);
+    else diff_attn_rows<D, BF16, 4><<<grid, 128, RowLay<D, 4>::TOTAL, s>>>(tk, tv, p);
+    return cudaGetLastError();
+}
 
 } // namespace
 
@@ -552,6 +935,14 @@ cudaError_t configure_diff_attn() {
     auto set = [&](auto * k, int bytes) {
         if (e == cudaSuccess) e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
     };
+    set(diff_attn_rows<64, false, 4>, RowLay<64, 4>::TOTAL);
+    set(diff_attn_rows<64, true, 4>, RowLay<64, 4>::TOTAL);
+    set(diff_attn_rows<128, false, 4>, RowLay<128, 4>::TOTAL);
+    set(diff_attn_rows<128, true, 4>, RowLay<128, 4>::TOTAL);
+    set(diff_attn_rows<64, false, 8>, RowLay<64, 8>::TOTAL);
+    set(diff_attn_rows<64, true, 8>, RowLay<64, 8>::TOTAL);
+    set(diff_attn_rows<128, false, 8>, RowLay<128, 8>::TOTAL);
+    set(diff_attn_rows<128, true, 8>, RowLay<128, 8>::TOTAL);
     set(diff_attn_tc<64, false>, Lay<64>::TOTAL);
     set(diff_attn_tc<64, true>, Lay<64>::TOTAL);
     set(diff_attn_tc<128, false>, Lay<128>::TOTAL);
@@ -595,13 +986,33 @@ int diff_attn(DeviceCtx & c, const tsn_diff_attn_args & in) {
     p.G = (int) (a.H / a.Hk);
     p.R = (long long) a.Sq * p.G;
     p.err = c.d_err;
+    const bool rows = p.R <= 16;
     const long long groups = (p.R + ROWS - 1) / ROWS * a.B * a.Hk;
     if (groups > 0x7fffffffLL) return fail(TSN_ERR_ARG, "tsn_diff_attn: too many query rows");
-    // Split the keys where whole tiles leave SMs without work: as many parts as fill one wave, of two key tiles at
-    // least (a part costs its CTA's start and a trip through the workspace, about what two tiles take).
-    const long long tiles = ((long long) a.Sk + KEYS - 1) / KEYS;
-    p.splits = (int) std::max(1ll, std::min(SMS / groups, tiles / 2));
-    p.wr = (int) std::min<long long>(ROWS, p.R);
+    int warps = 8;
+    if (rows) {
+        // Parts of 512 keys (four slabs for each of eight warps) while that is at most one CTA per SM, and none up to
+        // 1024 keys, where the trip through the workspace costs more than the keys. Beyond, CTAs of four warps, two
+        // per SM, in about four rounds, so that sequences of unequal length even out; at most 64 parts, as one CTA
+        // adds them up, and no more than the workspace holds.
+        const long long slabs = ((long long) a.Sk + SLAB - 1) / SLAB;
+        long long parts = slabs <= 64 ? 1 : (slabs + 31) / 32;
+        if (groups * parts > SMS) {
+            warps = 4;
+            parts = std::min(parts, std::max(1ll, 8 * SMS / groups));
+        }
+        const long long size = p.R * (4 * a.d + 4) * 4;
+        parts = std::min({parts, 64ll, std::max(1ll, (long long) (WORKSPACE - COUNTERS * 4) / (groups * size))});
+        if (groups > (long long) COUNTERS) parts = 1;
+        p.chunk = (int) std::max(1ll, (slabs + parts - 1) / parts);
+        p.splits = (int) std::max(1ll, (slabs + p.chunk - 1) / p.chunk);
+    } else {
+        // Split the keys where whole tiles leave SMs without work: as many parts as fill one wave, of two key tiles at
+        // least (a part costs its CTA's start and a trip through the workspace, about what two tiles take).
+        const long long tiles = ((long long) a.Sk + KEYS - 1) / KEYS;
+        p.splits = (int) std::max(1ll, std::min(SMS / groups, tiles / 2));
+        p.wr = (int) std::min<long long>(ROWS, p.R);
+    }
     if (p.splits > 1) {
         cudaStreamCaptureStatus st = cudaStreamCaptureStatusNone;
         cudaError_t e = cudaStreamIsCapturing(c.stream, &st);
@@ -613,12 +1024,17 @@ int diff_attn(DeviceCtx & c, const tsn_diff_attn_args & in) {
     }
     static_assert(SMS <= COUNTERS && (size_t) SMS * 128 * (2 * 128 + 4) * 4 <= ((size_t) 32 << 20), "one wave of partial results fits");
     CUtensorMap tk{}, tv{};
-    if (a.Sk && (!make_kv_map(&tk, a, a.k, KB, KEYS) || !make_kv_map(&tv, a, a.v, KB, KEYS)))
+    if (a.Sk && (!make_kv_map(&tk, a, a.k, KB, rows ? SLAB : KEYS) || !make_kv_map(&tv, a, a.v, KB, rows ? SLAB : KEYS)))
         return fail(TSN_ERR_ARG, "tsn_diff_attn: k or v cannot be described to the tensor memory accelerator");
     const unsigned grid = (unsigned) (groups * p.splits);
     const bool bf = a.type == TSN_BF16;
-    cudaError_t e = a.d == 32 ? (bf ? launch_tc<64, true>(tk, tv, p, grid, c.stream) : launch_tc<64, false>(tk, tv, p, grid, c.stream))
-                              : (bf ? launch_tc<128, true>(tk, tv, p, grid, c.stream) : launch_tc<128, false>(tk, tv, p, grid, c.stream));
+    cudaError_t e;
+    if (rows)
+        e = a.d == 32 ? (bf ? launch_rows<64, true>(tk, tv, p, grid, warps, c.stream) : launch_rows<64, false>(tk, tv, p, grid, warps, c.stream))
+                      : (bf ? launch_rows<128, true>(tk, tv, p, grid, warps, c.stream) : launch_rows<128, false>(tk, tv, p, grid, warps, c.stream));
+    else
+        e = a.d == 32 ? (bf ? launch_tc<64, true>(tk, tv, p, grid, c.stream) : launch_tc<64, false>(tk, tv, p, grid, c.stream))
+                      : (bf ? launch_tc<128, true>(tk, tv, p, grid, c.stream) : launch_tc<128, false>(tk, tv, p, grid, c.stream));
     if (e == cudaSuccess && p.splits > 1) {
         cudaStreamCaptureStatus st = cudaStreamCaptureStatusNone;
         e = cudaStreamIsCapturing(c.stream, &st);
