@@ -3,29 +3,14 @@
 //
 //   o = O_1 / l_1 - lambda O_2 / l_2,   O_m = sum_j p_mj v_j,  l_m = sum_j p_mj,  p_mj = 2^(c q_m.k_mj - ref_m)
 // in one pass over the keys: ref_m follows the running maximum of the row, O_m and l_m are rescaled when it
-// moves. The two maps share every value tile, so K and V are read once for both.
-//
-// One CTA per 128 query rows of one kv head (rows are (token, query head of the group), so a group's heads
-// share the K and V tiles) and, where there are few rows, per part of the keys. 320 threads:
-//   warp 8      TMA: lane 0 streams 128-key K tiles, lane 1 V tiles, through a ring of stages
-//   warp 9      one thread issues S_m = Q_m K_m^T (M 128, N 128, K d) and O_m += P_m V (M 128, N 2 d, K 128; P_m from
-//               TMEM). The order PV_1, QK_1, PV_2, QK_2 keeps the tensor cores on one map while the other
-//               map's softmax runs
-//   warps 0-3   map 1, warps 4-7 map 2: one row per thread. S_m from TMEM, mask, maximum, exponentials, P_m over
-//               S_m's columns. O_m stays in TMEM; it is rescaled only when the maximum has grown by more than
-//               2^8, which f32 and both 16-bit types hold without loss
-// TMEM: S_1, S_2 (128 columns each), O_1, O_2 (2 d each): all 512 columns at d = 64.
-// What bounds it: 2 exponentials for 12 d operations. At d = 64 a 128 x 128 tile pair takes 2048 cycles of the
-// SFU (16 exponentials a cycle) and 1536 of the tensor cores.
+// moves, which is only when the maximum has grown by more than 2^8 (f32 and both 16-bit types hold that without
+// loss). The two maps share every value tile, so K and V are read once for both.
 // P is rounded to 16 bits, as the tensor cores take it; scores, maxima, sums and O are f32.
 //
-// Values behind masked keys may be NaN, and 0 * NaN is NaN. So where a tile has masked keys, the map-1 threads
-// zero their V rows in shared memory, and where causal rows differ in what they see, non-finite values of
-// a V row become zero and each row that sees such a key is marked: its result is NaN.
-//
-// With splits, each CTA leaves its O_m, ref_m and l_m in the workspace and the CTA that arrives last adds them
-// up in the order of the splits, so the result does not depend on which one that is.
-// Every wait is bounded; barriers of the whole block are on paths that all threads take.
+// Values behind masked keys may be NaN, and 0 * NaN is NaN. So V rows of masked keys count as zero, and where
+// causal rows differ in what they see, non-finite values of a V row become zero and each row that sees such a
+// key is marked: its result is NaN.
+// Every wait is bounded; barriers of a whole block or cluster are on paths that all threads take.
 #include "block_ops.h"
 #include "ptx.cuh"
 
@@ -38,20 +23,10 @@ namespace tsn {
 
 namespace {
 
-constexpr int ROWS = 128, KEYS = 128;
-constexpr int THREADS = 320;
+constexpr int ROWS = 128, KEYS = 64;
+constexpr int THREADS = 384;
 constexpr float LOG2E = 1.44269504088896341f;
 constexpr float LAZY = 8.0f;   // log2 units that a maximum may grow before O is rescaled
-
-// shared memory of one CTA for heads of D = 2 d elements
-template <int D>
-struct Lay {
-    static constexpr int TILE = 128 * D * 2;             // Q, K or V tile: boxes of 128 rows x 64 elements
-    static constexpr int STAGES = D == 128 ? 3 : 4;
-    static constexpr int OFF_K = TILE, OFF_V = OFF_K + STAGES * TILE, OFF_LAM = OFF_V + STAGES * TILE;
-    static constexpr int OFF_W = OFF_LAM + 128 * 4, OFF_BAR = OFF_W + 128 * 4, TOTAL = OFF_BAR + 256;
-    static_assert(TOTAL <= 227 * 1024, "one CTA's shared memory");
-};
 
 struct Args {
     tsn_diff_attn_args a;
@@ -59,7 +34,6 @@ struct Args {
     int G;                      // query heads per kv head
     long long R;                // Sq * G rows of one kv head
     int splits, kv_b;           // parts of the keys; 0: every batch reads the same keys
-    int wr;                     // rows of a partial result
     int chunk;                  // few rows: slabs of a part
     float * part;
     unsigned int * count;
@@ -107,25 +81,122 @@ __device__ __forceinline__ uint32_t finite_only(uint32_t v) {
     return v;
 }
 
+// A row's sums as they are added up over warps, CTAs or parts of the keys: O [2 maps][D], then ref and l of both maps.
+constexpr int row_words(int D) { return 2 * D + 4; }
+
+// E (2 or 4) words of shared or, past the L1 cache, global memory
+template <int E, bool GLOBAL>
+__device__ __forceinline__ void read_words(const float * at, float * v) {
+    if (E == 4) {
+        const float4 x = GLOBAL ? __ldcg((const float4 *) at) : *(const float4 *) at;
+        v[0] = x.x; v[1] = x.y; v[2] = x.z; v[3] = x.w;
+    } else {
+        const float2 x = GLOBAL ? __ldcg((const float2 *) at) : *(const float2 *) at;
+        v[0] = x.x; v[1] = x.y;
+    }
+}
+
+// Adds up `count` sets of a row's sums, one warp: rd(i, k) is word k of set i, rdv(i, k, v) D / 32 words from k on.
+// Returns O (this lane's D / 32 columns), ref and l. The order is that of the sets.
+template <int D, class Rd, class RdV>
+__device__ __forceinline__ void add_up(int count, int lane, float (&sum)[2][D / 32], float (&top)[2], float (&l)[2], Rd rd, RdV rdv) {
+    constexpr int E = D / 32;
+#pragma unroll
+    for (int m = 0; m < 2; ++m) {
+        top[m] = -INFINITY;
+        l[m] = 0.0f;
+        for (int i = lane; i < count; i += 32) top[m] = fmaxf(top[m], rd(i, 2 * D + m));
+#pragma unroll
+        for (int x = 16; x; x >>= 1) top[m] = fmaxf(top[m], __shfl_xor_sync(~0u, top[m], x));
+        const float ref = top[m] == -INFINITY ? 0.0f : top[m];
+        for (int i = lane; i < count; i += 32) l[m] += ex2(rd(i, 2 * D + m) - ref) * rd(i, 2 * D + 2 + m);
+#pragma unroll
+        for (int x = 16; x; x >>= 1) l[m] += __shfl_xor_sync(~0u, l[m], x);
+#pragma unroll
+        for (int e = 0; e < E; ++e) sum[m][e] = 0.0f;
+#pragma unroll 8
+        for (int i = 0; i < count; ++i) {
+            const float f = ex2(rd(i, 2 * D + m) - ref);
+            float v[4];
+            rdv(i, m * D + E * lane, v);
+#pragma unroll
+            for (int e = 0; e < E; ++e) sum[m][e] = fmaf(f, v[e], sum[m][e]);
+        }
+    }
+}
+
+// The result of one row from its sums, one warp: lam lambda of its head, nw the norm's weights.
+template <int D, bool BF16>
+__device__ __forceinline__ void write_row(const Args & p, int b, int hk, int i, int g, float lam, const float * nw, int lane,
+                                          const float (&sum)[2][D / 32], const float (&l)[2]) {
+    constexpr int E = D / 32;
+    const tsn_diff_attn_args & a = p.a;
+    const float w1 = l[0] == 0.0f ? 0.0f : 1.0f / l[0], w2 = l[1] == 0.0f ? 0.0f : lam / l[1];
+    float ss = 0.0f, v[E];
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+        v[e] = sum[0][e] * w1 - sum[1][e] * w2;
+        ss += v[e] * v[e];
+    }
+#pragma unroll
+    for (int x = 16; x; x >>= 1) ss += __shfl_xor_sync(~0u, ss, x);
+    const float f = ss < INFINITY ? rsqrtf(ss * (1.0f / D) + a.eps) : NAN;
+    uint32_t x[E / 2];
+#pragma unroll
+    for (int e = 0; e < E; e += 2) x[e / 2] = pack16<BF16>(v[e] * f * nw[E * lane + e], v[e + 1] * f * nw[E * lane + e + 1]);
+    uint16_t * out = (uint16_t *) a.out.p + b * a.out.sb + (long long) i * a.out.ss + (long long) (hk * p.G + g) * a.out.sh + E * lane;
+    if constexpr (E == 4) *(uint2 *) out = make_uint2(x[0], x[1]);
+    else *(uint32_t *) out = x[0];
+}
+
+// ================================================================ tensor cores
+// diff_attn_tc: one CTA per 128 query rows of one kv head (rows are (token, query head of the group), so a group's
+// heads share the K and V tiles) and, where there are few rows, per part of the keys; a cluster holds the parts.
+// 384 threads:
+//   warp 8      TMA: streams 64-key K and V tiles through a ring of stages
+//   warps 9-10  one for each map m issue O_m += P_m V (M 128, N 2 d, K 64; P_m from TMEM) of tile j and then
+//               S_m = Q_m K_m^T (M 128, N 64, K d) of tile j + BUF. (One thread for both maps, under a branch of its
+//               own, took 1100 cycles for a map's eight products, commits and waits: twice what they run.)
+//   warp 11     where some keys are masked: makes the tiles' V rows fit for the product (see above)
+//   warps 0-3   map 1, warps 4-7 map 2: one row per thread. S_m from TMEM, mask, maximum, exponentials, P_m over
+//               S_m's columns; O_m stays in TMEM
+// TMEM at d = 64: S in two buffers per map (4 x 64 columns), so that a map's next scores are there when its
+// softmax is done, and O_1, O_2 (128 each): all 512 columns.
+// What bounds it: 2 exponentials for 12 d operations. At d = 64 a 128 x 64 tile pair takes 1024 cycles of the SFU
+// (16 exponentials a cycle) and 896 of the tensor cores (the products with N 64 wait for shared memory).
+// Parts of the keys: each CTA leaves its rows' sums in its shared memory and, after a cluster barrier, adds up its
+// share of the rows over the cluster, in the order of the parts.
+template <int D>
+struct Lay {
+    static constexpr int BUF = D == 128 ? 2 : 2;
+    static constexpr int Q = ROWS * D * 2, BOX = KEYS * 128, TILE = KEYS * D * 2;   // boxes of 64 keys x 64 elements
+    static constexpr int STAGES = 6;
+    static constexpr int OFF_K = Q, OFF_V = OFF_K + STAGES * TILE, OFF_LAM = OFF_V + STAGES * TILE;
+    static constexpr int OFF_W = OFF_LAM + 128 * 4, OFF_BAR = OFF_W + 128 * 4, TOTAL = OFF_BAR + 320;
+    static constexpr uint32_t TM_O = 2 * BUF * KEYS, TM = 512;
+    static_assert(TOTAL <= 227 * 1024, "one CTA's shared memory");
+    static_assert(ROWS * row_words(D) * 4 <= 2 * STAGES * TILE, "the rows' sums fit in the ring");
+    static_assert(TM_O + 2 * D <= TM, "tensor memory");
+};
+
 template <int D, bool BF16>
 __global__ void __launch_bounds__(THREADS, 1)
 diff_attn_tc(const __grid_constant__ CUtensorMap tk, const __grid_constant__ CUtensorMap tv, const __grid_constant__ Args p) {
     using L = Lay<D>;
-    constexpr int d = D / 2, BOX = 128 * 128, ATOMS = D / 64, CH = D / 8;   // CH: 16-byte pieces of a head
+    constexpr int d = D / 2, ATOMS = D / 64, CH = D / 8, BUF = L::BUF;   // CH: 16-byte pieces of a head
+    constexpr int QBOX = ROWS * 128;
     extern __shared__ __align__(1024) uint8_t smem[];
     const tsn_diff_attn_args & a = p.a;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-    if (smem_u32(smem) & 1023) {   // the swizzled tiles need 1024-byte alignment
-        if (tid == 0 && p.err) atomicCAS(p.err, 0, DEV_BAD_ARGS);
-        return;
-    }
+    const bool fits = (smem_u32(smem) & 1023) == 0;   // the swizzled tiles need 1024-byte alignment
+    if (!fits && tid == 0 && p.err) atomicCAS(p.err, 0, DEV_BAD_ARGS);
     float * lam = (float *) (smem + L::OFF_LAM), * nw = (float *) (smem + L::OFF_W);
     uint64_t * bar = (uint64_t *) (smem + L::OFF_BAR);
-    uint64_t * q_full = bar, * k_full = bar + 1, * k_empty = k_full + L::STAGES, * v_full = k_empty + L::STAGES,
-             * v_empty = v_full + L::STAGES, * s_full = v_empty + L::STAGES, * p_full = s_full + 2, * o_full = p_full + 2,
-             * bad_bar = o_full + 1;
-    uint32_t * words = (uint32_t *) (bad_bar + 1);   // TMEM address, abort flag, last-to-arrive flag, bad keys [4]
+    uint64_t * q_full = bar, * full = bar + 1, * empty = full + L::STAGES, * s_full = empty + L::STAGES, * p_full = s_full + 2 * BUF,
+             * o_full = p_full + 2 * BUF, * v_ready = o_full + 2 * BUF;
+    uint32_t * words = (uint32_t *) (v_ready + L::STAGES);   // TMEM address, abort flag, keys of each stage with non-finite values [2]
     volatile int * abort_flag = (volatile int *) (words + 1);
+    static_assert((1 + 3 * L::STAGES + 6 * BUF) * 8 + (2 + 2 * L::STAGES) * 4 <= 320, "barriers");
 
     // this CTA's rows, keys and part of them; long rows of a causal call come first
     const unsigned gid = blockIdx.x / p.splits, split = blockIdx.x % p.splits;
@@ -140,349 +211,366 @@ diff_attn_tc(const __grid_constant__ CUtensorMap tk, const __grid_constant__ CUt
     };
     const int most = limit(rows - 1), least = limit(0);
     const int all_tiles = (most + KEYS - 1) / KEYS, per = (all_tiles + p.splits - 1) / p.splits;
-    const int t0 = min(all_tiles, (int) split * per), nt = min(all_tiles, t0 + per) - t0;
+    const int t0 = min(all_tiles, (int) split * per), nt = fits ? min(all_tiles, t0 + per) - t0 : 0;
+    const uint8_t * mask = a.key_mask ? a.key_mask + b * a.mask_sb : nullptr;
+    auto mixed = [&](int base) { return a.causal && least < min(n, base + KEYS); };   // rows see different keys of the tile
+    const bool mend = nt > 0 && (mask || (t0 + nt) * KEYS > n || mixed((t0 + nt - 1) * KEYS));
 
     if (tid == 0) {
         mbar_init(q_full, 8);
-        for (int s = 0; s < L::STAGES; ++s) {
-            mbar_init(&k_full[s], 1); mbar_init(&k_empty[s], 1);
-            mbar_init(&v_full[s], 1); mbar_init(&v_empty[s], 1);
-        }
-        for (int m = 0; m < 2; ++m) { mbar_init(&s_full[m], 1); mbar_init(&p_full[m], 4); }
-        mbar_init(o_full, 1);
-        mbar_init(bad_bar, 4);
+        for (int s = 0; s < L::STAGES; ++s) { mbar_init(&full[s], 1); mbar_init(&empty[s], 2); mbar_init(&v_ready[s], 1); }
+        for (int x = 0; x < 2 * BUF; ++x) { mbar_init(&s_full[x], 1); mbar_init(&p_full[x], 4); mbar_init(&o_full[x], 1); }
         *abort_flag = 0;
         fence_mbar_init();
     }
     if (warp == 8 && lane == 0 && nt > 0) { tma_prefetch(&tk); tma_prefetch(&tv); }
-    if (warp == 9) tmem_alloc(words, 512);
+    if (warp == 9) tmem_alloc(words, L::TM);
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
-    const uint32_t tmem = words[0];
-    const uint32_t TM_O = tmem + 256;
+    const uint32_t tmem = __shfl_sync(~0u, words[0], 0), TM_O = tmem + L::TM_O;
 
     // the row of a softmax thread
     const int m = warp >> 2, t = tid & 127;
+    const uint32_t lane0 = (uint32_t) ((warp & 3) * 32) << 16;
     float l = 0.0f, ref = -INFINITY;
     bool ok = true;
 
-    if (warp == 8) {
-        if (lane < 2) {
-            const CUtensorMap * tm = lane == 0 ? &tk : &tv;
-            uint64_t * full = lane == 0 ? k_full : v_full, * empty = lane == 0 ? k_empty : v_empty;
-            uint8_t * ring = smem + (lane == 0 ? L::OFF_K : L::OFF_V);
-            for (int j = 0; j < nt; ++j) {
-                const int s = j % L::STAGES;
-                if (j >= L::STAGES && !mbar_wait(&empty[s], (j / L::STAGES - 1) & 1, abort_flag, p.err, DEV_TIMEOUT_EMPTY)) break;
-                mbar_expect_tx(&full[s], L::TILE);
-                for (int x = 0; x < ATOMS; ++x)
-                    tma_load_4d(ring + s * L::TILE + x * BOX, tm, &full[s], 64 * x, (t0 + j) * KEYS, hk, b * p.kv_b);
-            }
-        }
-    } else if (warp == 9) {
-        if (lane == 0 && nt > 0) {
-            const uint32_t id_s = umma_idesc_f16(KEYS, BF16), id_pv = umma_idesc_f16(D, BF16, 1);
-            // map 2's halves of Q and K: the second box at d = 64, the second half of each 128-byte row at d = 32
-            constexpr int MAP2 = D == 128 ? BOX : 64;
-            auto qk = [&](int mm, int j) {
-                const int s = j % L::STAGES;
-                if (mm == 0 && !mbar_wait(&k_full[s], (j / L::STAGES) & 1, abort_flag, p.err, DEV_TIMEOUT_FULL)) return false;
-                tc_fence_after();
-                const uint64_t qd = umma_desc_sw128(smem + mm * MAP2), kd = umma_desc_sw128(smem + L::OFF_K + s * L::TILE + mm * MAP2);
-#pragma unroll
-                for (int kk = 0; kk < d / 16; ++kk) umma_f16(tmem + 128 * mm, qd + 2 * kk, kd + 2 * kk, id_s, kk != 0);
-                umma_commit(&s_full[mm]);
-                if (mm == 1) umma_commit(&k_empty[s]);
-                return true;
-            };
-            auto pv = [&](int mm, int j) {
-                const int s = j % L::STAGES;
-                if (!mbar_wait(&p_full[mm], j & 1, abort_flag, p.err, DEV_TIMEOUT_TMEM)) return false;
-                if (mm == 0 && !mbar_wait(&v_full[s], (j / L::STAGES) & 1, abort_flag, p.err, DEV_TIMEOUT_FULL)) return false;
-                tc_fence_after();
-                const uint8_t * v = smem + L::OFF_V + s * L::TILE;
-#pragma unroll
-                for (int kk = 0; kk < KEYS / 16; ++kk)
-                    umma_f16_ts(TM_O + D * mm, tmem + 128 * mm + 8 * kk, umma_desc_sw128_mn(v + kk * 2048, BOX), id_pv, j > 0 || kk > 0);
-                if (mm == 1) umma_commit(&v_empty[s]);
-                return true;
-            };
-            bool go = mbar_wait(q_full, 0, abort_flag, p.err, DEV_TIMEOUT_FULL) && qk(0, 0) && qk(1, 0);
-            for (int j = 0; j < nt && go; ++j) {
-                go = pv(0, j) && (j + 1 == nt || qk(0, j + 1)) && pv(1, j) && (j + 1 == nt || qk(1, j + 1));
-            }
-            if (go) umma_commit(o_full);
-        }
-    } else {
-        // Q into its swizzled boxes, rows past the last one as zeros; lambda of each head of the group; weights
-        for (int i = tid; i < ROWS * CH; i += 256) {
-            const int r = i / CH, ch = i % CH, u = rem0 + r;
-            uint4 x = make_uint4(0, 0, 0, 0);
-            if (r < rows)
-                x = *(const uint4 *) ((const uint16_t *) a.q.p + b * a.q.sb + (long long) (i0 + u / p.G) * a.q.ss +
-                                      (long long) (hk * p.G + u % p.G) * a.q.sh + ch * 8);
-            *(uint4 *) (smem + (ch >> 3) * BOX + r * 128 + (((ch & 7) ^ (r & 7)) << 4)) = x;
-        }
-        fence_proxy_async_smem();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(q_full);
-        for (int g = warp; g < p.G; g += 8) {
-            const long long h = (long long) (hk * p.G + g) * a.lam_sh;
-            float z1 = 0.0f, z2 = 0.0f;
-            for (int e = lane; e < d; e += 32) { z1 += a.lq1[h + e] * a.lk1[h + e]; z2 += a.lq2[h + e] * a.lk2[h + e]; }
-#pragma unroll
-            for (int x = 16; x; x >>= 1) { z1 += __shfl_xor_sync(~0u, z1, x); z2 += __shfl_xor_sync(~0u, z2, x); }
-            if (lane == 0) lam[g] = expf(z1) - expf(z2) + a.lambda_init;
-        }
-        if (tid < D) nw[tid] = (a.norm_w ? a.norm_w[tid] : 1.0f) * (1.0f - a.lambda_init);
-
-        const uint32_t lane0 = (uint32_t) ((warp & 3) * 32) << 16;
-        const uint32_t ts = tmem + 128 * m + lane0, to = TM_O + D * m + lane0;
-        const int lim = t < rows ? limit(t) : n;
-        const uint8_t * mask = a.key_mask ? a.key_mask + b * a.mask_sb : nullptr;
-        bool poison = false;
-        uint32_t mb[4] = {};   // mask bytes of the next tile
-        auto fetch_mask = [&](int j) {
-#pragma unroll
-            for (int w = 0; w < 4; ++w) {
-                const int key = (t0 + j) * KEYS + 32 * w + lane;
-                mb[w] = key < n ? mask[key] : 0u;
-            }
-        };
-        if (mask && nt > 0) fetch_mask(0);
-        for (int j = 0; j < nt; ++j) {
-            const int base = (t0 + j) * KEYS;
-            // the keys that exist, and those that this row sees
-            uint32_t kw[4], vis[4];
-#pragma unroll
-            for (int w = 0; w < 4; ++w) {
-                kw[w] = mask ? __ballot_sync(~0u, mb[w] != 0) : low_bits(n - base - 32 * w);
-                vis[w] = kw[w] & low_bits(lim - base - 32 * w);
-            }
-            if (mask && j + 1 < nt) fetch_mask(j + 1);
-            if (!mbar_wait(&s_full[m], j & 1, abort_flag, p.err, DEV_TIMEOUT_TMEM)) { ok = false; break; }
-            __syncwarp();
-            tc_fence_after();
-            float s[128];
-            tmem_ld128(ts, s);
-            if (__any_sync(~0u, (vis[0] & vis[1] & vis[2] & vis[3]) != ~0u)) {
-#pragma unroll
-                for (int e = 0; e < 128; ++e)
-                    if (!((vis[e >> 5] >> (e & 31)) & 1u)) s[e] = -INFINITY;
-            }
-            float mx[4] = {s[0], s[1], s[2], s[3]};
-#pragma unroll
-            for (int e = 4; e < 128; ++e) mx[e & 3] = fmaxf(mx[e & 3], s[e]);
-            const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * p.c;
-            // a row moves its reference by itself, so its result does not depend on its neighbours
-            const bool move = top > ref + (j ? LAZY : 0.0f);
-            if (__any_sync(~0u, move)) {
-                const float f = move ? ex2(ref - top) : 1.0f;
-                if (move) { ref = top; l *= f; }
-                if (j > 0) {   // S_j complete means that PV_(j-1) is
-#pragma unroll
-                    for (int x = 0; x < D; x += 32) {
-                        float o[32];
-                        tmem_ld32(to + x, o);
-#pragma unroll
-                        for (int e = 0; e < 32; ++e) o[e] *= f;
-                        tmem_st32(to + x, (const uint32_t *) o);
+    if (warp >= 8) {
+        if (warp == 8) {
+            if (lane == 0) {
+                for (int j = 0; j < nt; ++j) {
+                    const int s = j % L::STAGES;
+                    if (j >= L::STAGES && !mbar_wait(&empty[s], (j / L::STAGES - 1) & 1, abort_flag, p.err, DEV_TIMEOUT_EMPTY)) break;
+                    mbar_expect_tx(&full[s], 2 * L::TILE);
+                    for (int x = 0; x < ATOMS; ++x) {
+                        tma_load_4d(smem + L::OFF_K + s * L::TILE + x * L::BOX, &tk, &full[s], 64 * x, (t0 + j) * KEYS, hk, b * p.kv_b);
+                        tma_load_4d(smem + L::OFF_V + s * L::TILE + x * L::BOX, &tv, &full[s], 64 * x, (t0 + j) * KEYS, hk, b * p.kv_b);
                     }
                 }
             }
-            const float neg = ref == -INFINITY ? 0.0f : -ref;
-            const uint64_t c2 = f2_pack(p.c, p.c), neg2 = f2_pack(neg, neg);
-            uint64_t sum[2] = {0ull, 0ull};
-            uint32_t pk[64];
+        } else if (warp == 11) {
+            for (int j = 0; j < nt && mend; ++j) {
+                const int base = (t0 + j) * KEYS, s = j % L::STAGES;
+                uint32_t kw[2], bad[2] = {0, 0};
 #pragma unroll
-            for (int e = 0; e < 64; ++e) {
-                float x, y;
-                f2_unpack(ffma2(f2_pack(s[2 * e], s[2 * e + 1]), c2, neg2), x, y);
-                x = ex2(x);
-                y = ex2(y);
-                sum[e & 1] = fadd2(sum[e & 1], f2_pack(x, y));
-                pk[e] = pack16<BF16>(x, y);
-            }
-            float x, y;
-            f2_unpack(fadd2(sum[0], sum[1]), x, y);
-            l += x + y;
-            tmem_st32(ts, pk);
-            tmem_st32(ts + 32, pk + 32);
-            tmem_st_wait();
-            if (m == 0) {
-                const bool gone = (kw[0] & kw[1] & kw[2] & kw[3]) != ~0u, mixed = a.causal && least < min(n, base + KEYS);
-                if (gone || mixed) {   // the same for every thread of the map
-                    if (!mbar_wait(&v_full[j % L::STAGES], (j / L::STAGES) & 1, abort_flag, p.err, DEV_TIMEOUT_FULL)) { ok = false; break; }
-                    __syncwarp();
-                    uint8_t * v = smem + L::OFF_V + (j % L::STAGES) * L::TILE + t * 128;
-                    const bool here = (kw[t >> 5] >> lane) & 1u;   // thread t has key t
-                    bool odd = false;
-                    if (!here || mixed) {
+                for (int w = 0; w < 2; ++w) {
+                    const int key = base + 32 * w + lane;
+                    kw[w] = __ballot_sync(~0u, key < n && (!mask || mask[key] != 0));
+                }
+                if (!mbar_wait(&full[s], (j / L::STAGES) & 1, abort_flag, p.err, DEV_TIMEOUT_FULL)) break;
+                __syncwarp();
+                const bool differ = mixed(base);
+                if ((kw[0] & kw[1]) != ~0u || differ) {
+                    constexpr int AT_ONCE = 32 / CH, AHEAD = 4;   // rows of one step, steps whose loads run together
+                    for (int key0 = 0; key0 < KEYS; key0 += AT_ONCE * AHEAD) {
+                        uint4 o[AHEAD];
+                        auto at = [&](int y) {
+                            const int key = key0 + y * AT_ONCE + lane / CH, ch = lane % CH;
+                            return (uint4 *) (smem + L::OFF_V + s * L::TILE + (ch >> 3) * L::BOX + key * 128 + (((ch & 7) ^ (key & 7)) << 4));
+                        };
+                        const uint32_t here = kw[key0 >> 5] >> (key0 & 31);
+                        if (differ)
 #pragma unroll
-                        for (int ch = 0; ch < CH; ++ch) {
-                            uint4 * at = (uint4 *) (v + (ch >> 3) * BOX + (((ch & 7) ^ (t & 7)) << 4));
-                            if (!here) {
-                                *at = make_uint4(0, 0, 0, 0);
-                            } else {
-                                const uint4 o = *at;
-                                const uint4 f = make_uint4(finite_only<BF16>(o.x), finite_only<BF16>(o.y), finite_only<BF16>(o.z), finite_only<BF16>(o.w));
-                                if (o.x != f.x || o.y != f.y || o.z != f.z || o.w != f.w) { *at = f; odd = true; }
+                            for (int y = 0; y < AHEAD; ++y) o[y] = *at(y);
+#pragma unroll
+                        for (int y = 0; y < AHEAD; ++y) {
+                            if (!((here >> (y * AT_ONCE + lane / CH)) & 1u)) {
+                                *at(y) = make_uint4(0, 0, 0, 0);
+                            } else if (differ) {
+                                const uint4 f = make_uint4(finite_only<BF16>(o[y].x), finite_only<BF16>(o[y].y), finite_only<BF16>(o[y].z), finite_only<BF16>(o[y].w));
+                                if (o[y].x != f.x || o[y].y != f.y || o[y].z != f.z || o[y].w != f.w) {
+                                    *at(y) = f;
+                                    bad[key0 >> 5] |= 1u << ((key0 + y * AT_ONCE + lane / CH) & 31);
+                                }
                             }
                         }
                     }
                     fence_proxy_async_smem();
-                    if (mixed) {
-                        const uint32_t w = __ballot_sync(~0u, odd);
-                        if (lane == 0) { words[3 + warp] = w; mbar_arrive(bad_bar); }
-                        int turn = (base - t0 * KEYS) / KEYS - max(0, (least - t0 * KEYS) / KEYS);   // mixed tiles before this one
-                        if (!mbar_wait(bad_bar, turn & 1, abort_flag, p.err, DEV_TIMEOUT_TMEM)) { ok = false; break; }
-                        __syncwarp();
-                        volatile uint32_t * bad = words + 3;
-#pragma unroll
-                        for (int x = 0; x < 4; ++x) poison |= (bad[x] & vis[x]) != 0;
-                    }
+                }
+                bad[0] = __reduce_or_sync(~0u, bad[0]);
+                bad[1] = __reduce_or_sync(~0u, bad[1]);
+                if (lane == 0) {
+                    words[2 + 2 * s] = bad[0];
+                    words[3 + 2 * s] = bad[1];
+                    mbar_arrive(&v_ready[s]);
                 }
             }
-            tc_fence_before();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(&p_full[m]);
+        } else if (warp >= 9) {
+            const int mm = warp - 9;
+            const uint32_t lead = elect_lane(), id_s = umma_idesc_f16(KEYS, BF16), id_pv = umma_idesc_f16(D, BF16, 1);
+            // map 2's halves of Q and K: the second box at d = 64, the second half of each 128-byte row at d = 32
+            const uint64_t qd = umma_desc_sw128(smem + mm * (D == 128 ? QBOX : 64));
+            const uint64_t kd = umma_desc_sw128(smem + L::OFF_K + mm * (D == 128 ? L::BOX : 64)), vd = umma_desc_sw128_mn(smem + L::OFF_V, L::BOX);
+            const uint32_t to = TM_O + D * mm, ts = tmem + KEYS * BUF * mm;
+            auto qk = [&](int j) {
+                const int s = j % L::STAGES, x = j % BUF;
+                if (!mbar_wait(&full[s], (j / L::STAGES) & 1, abort_flag, p.err, DEV_TIMEOUT_FULL)) return false;
+                const uint64_t k = kd + (uint64_t) (s * (L::TILE >> 4));
+#pragma unroll
+                for (int kk = 0; kk < d / 16; ++kk) umma_f16_if(lead, ts + KEYS * x, qd + 2 * kk, k + 2 * kk, id_s, kk != 0);
+                umma_commit_if(lead, &s_full[mm * BUF + x]);
+                return true;
+            };
+            bool go = nt > 0 && mbar_wait(q_full, 0, abort_flag, p.err, DEV_TIMEOUT_FULL);
+            for (int j = 0; j < BUF && j < nt && go; ++j) go = qk(j);
+            for (int j = 0; j < nt && go; ++j) {
+                const int s = j % L::STAGES, x = j % BUF;
+                if (!mbar_wait(&p_full[mm * BUF + x], (j / BUF) & 1, abort_flag, p.err, DEV_TIMEOUT_TMEM)) break;
+                if (mend && !mbar_wait(&v_ready[s], (j / L::STAGES) & 1, abort_flag, p.err, DEV_TIMEOUT_FULL)) break;
+                tc_fence_after();
+                const uint64_t v = vd + (uint64_t) (s * (L::TILE >> 4));
+#pragma unroll
+                for (int kk = 0; kk < KEYS / 16; ++kk)
+                    umma_f16_ts_if(lead, to, ts + KEYS * x + 8 * kk, v + 128 * kk, id_pv, j > 0 || kk > 0);
+                umma_commit_if(lead, &empty[s]);
+                if (j + BUF < nt) go = qk(j + BUF);
+                else umma_commit_if(lead, &o_full[mm * BUF + nt - 1 - j]);   // the last BUF tiles, [0] the last
+            }
         }
-        if (poison) l = NAN;
-        if (ok && nt > 0) ok = mbar_wait(o_full, 0, abort_flag, p.err, DEV_TIMEOUT_TMEM);
+        // the barriers of the other warps' results
         __syncwarp();
-        tc_fence_after();
-    }
-
-    // ---------------------------------------------------------------- results, every thread on the same path
-    // K's and V's stages are free now: row sums [2][128], sums of squares [2][128]
-    float * rl = (float *) (smem + L::OFF_K), * rss = rl + 256;
-    const uint32_t lane0 = (uint32_t) ((warp & 3) * 32) << 16;
-    const bool soft = warp < 8;
-    const int half = m;   // of the columns, in what follows
-    float o[d];
-    bool mine = soft && t < rows;
-    bool finish = true;
-    if (p.splits > 1) {
-        // partial: [2 maps][D / 4][wr][4] sums, then ref [2][wr], l [2][wr]
-        const size_t size = (size_t) p.wr * (2 * D + 4);
-        if (soft) {
-            float * out = p.part + ((size_t) gid * p.splits + split) * size;
-            if (nt > 0) {
-                for (int x = 0; x < D; x += 32) {
-                    float v[32];
-                    tmem_ld32(TM_O + D * m + lane0 + x, v);
-                    if (mine)
-#pragma unroll
-                        for (int e = 0; e < 32; e += 4)
-                            *(float4 *) (out + ((size_t) (m * (D / 4) + (x + e) / 4) * p.wr + t) * 4) = make_float4(v[e], v[e + 1], v[e + 2], v[e + 3]);
-                }
-            }
-            if (mine) {
-                float * st = out + (size_t) p.wr * 2 * D;
-                st[m * p.wr + t] = ref;
-                st[(2 + m) * p.wr + t] = l;
-            }
-            __threadfence();
-        }
-        __syncthreads();
-        if (tid == 0) {
-            const bool last = atomicAdd(&p.count[gid], 1u) + 1u == (unsigned) p.splits;
-            if (last) p.count[gid] = 0;   // for the next call
-            words[2] = last;
-            __threadfence();
-        }
-        __syncthreads();
-        finish = words[2] != 0;
-        if (finish && mine) {
-            const float * first = p.part + (size_t) gid * p.splits * size;
-            float top[2] = {-INFINITY, -INFINITY}, sum[2] = {0.0f, 0.0f};
-            for (int s = 0; s < p.splits; ++s) {
-                const float * st = first + s * size + (size_t) p.wr * 2 * D;
-                for (int x = 0; x < 2; ++x) top[x] = fmaxf(top[x], __ldcg(st + x * p.wr + t));
-            }
-            for (int x = 0; x < 2; ++x) if (top[x] == -INFINITY) top[x] = 0.0f;
-            for (int s = 0; s < p.splits; ++s) {
-                const float * st = first + s * size + (size_t) p.wr * 2 * D;
-                for (int x = 0; x < 2; ++x) sum[x] += ex2(__ldcg(st + x * p.wr + t) - top[x]) * __ldcg(st + (2 + x) * p.wr + t);
-            }
-            const float w1 = sum[0] == 0.0f ? 0.0f : 1.0f / sum[0];
-            const float w2 = sum[1] == 0.0f ? 0.0f : -lam[(rem0 + t) % p.G] / sum[1];
-#pragma unroll
-            for (int e = 0; e < d; ++e) o[e] = 0.0f;
-            for (int s = 0; s < p.splits; ++s) {
-                const float * at = first + s * size, * st = at + (size_t) p.wr * 2 * D;
-                for (int x = 0; x < 2; ++x) {
-                    const float r = __ldcg(st + x * p.wr + t), f = ex2(r - top[x]) * (x ? w2 : w1);
-                    if (r == -INFINITY) continue;   // nothing seen in this part: its sums may not be written
-#pragma unroll
-                    for (int e = 0; e < d; e += 4) {
-                        const float4 v = __ldcg((const float4 *) (at + ((size_t) (x * (D / 4) + (half * d + e) / 4) * p.wr + t) * 4));
-                        o[e] = fmaf(f, v.x, o[e]); o[e + 1] = fmaf(f, v.y, o[e + 1]);
-                        o[e + 2] = fmaf(f, v.z, o[e + 2]); o[e + 3] = fmaf(f, v.w, o[e + 3]);
-                    }
-                }
-            }
-            if (!(sum[0] >= 0.0f) || !(sum[1] >= 0.0f)) o[0] = NAN;
+        if (p.splits > 1) {
+            __syncthreads();
+            cluster_sync_all();
+            cluster_sync_all();
+        } else {
+            for (int i = 0; i < 4; ++i) __syncthreads();
         }
     } else {
-        if (soft) rl[tid] = l;
-        __syncthreads();
-        if (soft) {
-            const float l1 = rl[t], l2 = rl[128 + t];
-            const float w1 = l1 == 0.0f ? 0.0f : 1.0f / l1;
-            const float w2 = l2 == 0.0f ? 0.0f : t < rows ? lam[(rem0 + t) % p.G] / l2 : 0.0f;
-            if (nt > 0) {
+        if (fits) {
+            // Q into its swizzled boxes, rows past the last one as zeros; lambda of each head of the group; weights
+            for (int i = tid; i < ROWS * CH; i += 256) {
+                const int r = i / CH, ch = i % CH, u = rem0 + r;
+                uint4 x = make_uint4(0, 0, 0, 0);
+                if (r < rows)
+                    x = *(const uint4 *) ((const uint16_t *) a.q.p + b * a.q.sb + (long long) (i0 + u / p.G) * a.q.ss +
+                                          (long long) (hk * p.G + u % p.G) * a.q.sh + ch * 8);
+                *(uint4 *) (smem + (ch >> 3) * QBOX + r * 128 + (((ch & 7) ^ (r & 7)) << 4)) = x;
+            }
+            fence_proxy_async_smem();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(q_full);
+            for (int g = warp; g < p.G; g += 8) {
+                const long long h = (long long) (hk * p.G + g) * a.lam_sh;
+                float z1 = 0.0f, z2 = 0.0f;
+                for (int e = lane; e < d; e += 32) { z1 += a.lq1[h + e] * a.lk1[h + e]; z2 += a.lq2[h + e] * a.lk2[h + e]; }
 #pragma unroll
-                for (int x = 0; x < d; x += 32) {
-                    float v[32];
-                    tmem_ld32(TM_O + lane0 + half * d + x, o + x);
-                    tmem_ld32(TM_O + D + lane0 + half * d + x, v);
+                for (int x = 16; x; x >>= 1) { z1 += __shfl_xor_sync(~0u, z1, x); z2 += __shfl_xor_sync(~0u, z2, x); }
+                if (lane == 0) lam[g] = expf(z1) - expf(z2) + a.lambda_init;
+            }
+            if (tid < D) nw[tid] = (a.norm_w ? a.norm_w[tid] : 1.0f) * (1.0f - a.lambda_init);
+
+            const uint32_t to = TM_O + D * m + lane0;
+            const int lim = t < rows ? limit(t) : n;
+            bool poison = false;
+            uint32_t mb[2] = {};   // mask bytes of the next tile
+            auto fetch_mask = [&](int j) {
 #pragma unroll
-                    for (int e = 0; e < 32; ++e) o[x + e] = o[x + e] * w1 - v[e] * w2;
+                for (int w = 0; w < 2; ++w) {
+                    const int key = (t0 + j) * KEYS + 32 * w + lane;
+                    mb[w] = key < n ? mask[key] : 0u;
                 }
-            } else {
+            };
+            // the keys of tile j that this row sees; clear: every row sees all of them
+            auto clear = [&](int j) { return !mask && (t0 + j + 1) * KEYS <= least; };
+            auto visible = [&](int j, uint32_t (&vis)[2]) {
+#pragma unroll
+                for (int w = 0; w < 2; ++w) {
+                    const int at = (t0 + j) * KEYS + 32 * w;
+                    vis[w] = (mask ? __ballot_sync(~0u, mb[w] != 0) : low_bits(n - at)) & low_bits(lim - at);
+                }
+            };
+            auto hide = [&](const uint32_t vis, uint32_t * s) {   // masks 32 keys
+                if (__any_sync(~0u, vis != ~0u))
+#pragma unroll
+                    for (int e = 0; e < 32; ++e)
+                        if (!((vis >> e) & 1u)) s[e] = 0xff800000u;   // -inf
+            };
+            if (mask && nt > 0) fetch_mask(0);
+            for (int j = 0; j < nt; ++j) {
+                const int x = m * BUF + j % BUF;
+                const uint32_t ts = tmem + KEYS * x + lane0;
+                uint32_t vis[2] = {~0u, ~0u};
+                if (!clear(j)) visible(j, vis);
+                if (mask && j + 1 < nt) fetch_mask(j + 1);
+                if (!mbar_wait(&s_full[x], (j / BUF) & 1, abort_flag, p.err, DEV_TIMEOUT_TMEM)) { ok = false; break; }
+                __syncwarp();
+                tc_fence_after();
+                uint32_t s[KEYS], pk[KEYS / 2];
+                tmem_request32(ts, s);
+                tmem_request32(ts + 32, s + 32);
+                tmem_landed32(s);
+                tmem_landed32(s + 32);
+                if (!clear(j)) {
+                    hide(vis[0], s);
+                    hide(vis[1], s + 32);
+                }
+                // The exponentials are taken against the reference of the tiles before, and the maximum beside them, so that
+                // the SFU need not wait for it; the few tiles whose maximum is too far above the reference are done again.
+                uint64_t sum[2];
+                while (true) {
+                    const float neg = ref == -INFINITY ? 0.0f : -ref;
+                    const uint64_t c2 = f2_pack(p.c, p.c), neg2 = f2_pack(neg, neg);
+                    float mx[2] = {-INFINITY, -INFINITY};
+                    sum[0] = sum[1] = 0ull;
+#pragma unroll
+                    for (int e = 0; e < KEYS / 2; ++e) {
+                        const float a0 = __uint_as_float(s[2 * e]), a1 = __uint_as_float(s[2 * e + 1]);
+                        float y, z;
+                        f2_unpack(ffma2(f2_pack(a0, a1), c2, neg2), y, z);
+                        y = ex2(y);
+                        z = ex2(z);
+                        sum[e & 1] = fadd2(sum[e & 1], f2_pack(y, z));
+                        pk[e] = pack16<BF16>(y, z);
+                        mx[e & 1] = fmaxf(mx[e & 1], fmaxf(a0, a1));
+                    }
+                    const float top = fmaxf(mx[0], mx[1]) * p.c;
+                    const bool move = top > ref + LAZY;
+                    if (!__any_sync(~0u, move)) break;
+                    // a row moves its reference by itself, so its result does not depend on its neighbours
+                    const float f = move ? ex2(ref - top) : 1.0f;
+                    if (move) { ref = top; l *= f; }
+                    if (j > 0) {
+                        // O is complete up to tile j - 1: the scores issued after that product are there, or its own commit
+                        const int i = j - 1 + BUF;
+                        uint64_t * done = i < nt ? &s_full[m * BUF + i % BUF] : &o_full[m * BUF + nt - j];
+                        if (!mbar_wait(done, i < nt ? (i / BUF) & 1 : 0, abort_flag, p.err, DEV_TIMEOUT_TMEM)) { ok = false; break; }
+                        __syncwarp();
+                        tc_fence_after();
+#pragma unroll 1
+                        for (int y = 0; y < D; y += 16) {
+                            float o[16];
+                            tmem_ld16(to + y, o);
+#pragma unroll
+                            for (int e = 0; e < 16; ++e) o[e] *= f;
+                            tmem_st16(to + y, (const uint32_t *) o);
+                        }
+                    }
+                }
+                if (!ok) break;
+                float y, z;
+                f2_unpack(fadd2(sum[0], sum[1]), y, z);
+                l += y + z;
+                tmem_st32(ts, pk);
+                tmem_st_wait();
+                if (m == 0 && mixed((t0 + j) * KEYS)) {
+                    if (!mbar_wait(&v_ready[j % L::STAGES], (j / L::STAGES) & 1, abort_flag, p.err, DEV_TIMEOUT_FULL)) { ok = false; break; }
+                    const volatile uint32_t * bad = words + 2 + 2 * (j % L::STAGES);
+                    poison |= (bad[0] & vis[0]) != 0 || (bad[1] & vis[1]) != 0;
+                }
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&p_full[x]);
+            }
+            if (poison) l = NAN;
+            if (ok && nt > 0) ok = mbar_wait(&o_full[m * BUF], 0, abort_flag, p.err, DEV_TIMEOUT_TMEM);
+            __syncwarp();
+            tc_fence_after();
+        }
+        // ------------------------------------------------------------ results
+        if (p.splits > 1) {
+            // this part's sums in place of K and V: [row][row_words], a row 16 bytes past a multiple of all banks
+            __syncthreads();   // both maps are done with the ring
+            float * sums = (float *) (smem + L::OFF_K);
+            if (fits) {
+                float * to = sums + t * row_words(D);
+#pragma unroll
+                for (int x = 0; x < D; x += 32) {
+                    float v[32];
+                    if (nt > 0) {
+                        tmem_ld32(TM_O + D * m + lane0 + x, v);
+                    } else {
+#pragma unroll
+                        for (int e = 0; e < 32; ++e) v[e] = 0.0f;
+                    }
+#pragma unroll
+                    for (int e = 0; e < 32; e += 4) *(float4 *) (to + m * D + x + e) = make_float4(v[e], v[e + 1], v[e + 2], v[e + 3]);
+                }
+                to[2 * D + m] = ref;
+                to[2 * D + 2 + m] = l;
+            }
+            cluster_sync_all();
+            const int share = (rows + p.splits - 1) / p.splits, last = min(rows, ((int) split + 1) * share);
+            const uint32_t here = smem_u32(sums);
+            for (int r = (int) split * share + warp; r < last && !*abort_flag; r += 8) {
+                constexpr int E = D / 32;
+                float sum[2][E], top[2], rl[2];
+                auto at = [&](int i, int k) { return dsmem_map(here, (uint32_t) i) + (uint32_t) (r * row_words(D) + k) * 4; };
+                add_up<D>(p.splits, lane, sum, top, rl, [&](int i, int k) { return dsmem_ld1(at(i, k)); },
+                          [&](int i, int k, float * v) {
+                              if (E == 4) {
+                                  const float4 x = dsmem_ld4(at(i, k));
+                                  v[0] = x.x; v[1] = x.y; v[2] = x.z; v[3] = x.w;
+                              } else {
+                                  v[0] = dsmem_ld1(at(i, k));
+                                  v[1] = dsmem_ld1(at(i, k + 1));
+                              }
+                          });
+                const int u = rem0 + r, g = u % p.G;
+                write_row<D, BF16>(p, b, hk, i0 + u / p.G, g, lam[g], nw, lane, sum, rl);
+            }
+            cluster_sync_all();   // nobody leaves while its sums are read
+        } else {
+            // o = O_1 / l_1 - lambda O_2 / l_2, thread (row t, half m of the columns); RMSNorm over both halves; the result
+            // through Q's place, so that whole rows are written. In place of K: row sums [2][128], sums of squares [2][128]
+            float * rl = (float *) (smem + L::OFF_K), * rss = rl + 256;
+            float o[d];
+            tc_fence_before();
+            __syncthreads();   // both maps are done with the ring, and their O is there
+            tc_fence_after();
+            rl[tid] = l;
+            __syncthreads();
+            {
+                const float l1 = rl[t], l2 = rl[128 + t];
+                const float w1 = l1 == 0.0f ? 0.0f : 1.0f / l1;
+                const float w2 = l2 == 0.0f ? 0.0f : t < rows ? lam[(rem0 + t) % p.G] / l2 : 0.0f;
 #pragma unroll
                 for (int e = 0; e < d; ++e) o[e] = 0.0f;
-            }
-        }
-    }
-    // RMSNorm over both halves; the result through Q's place, so that whole rows are written
-    if (finish) {
-        float ss = 0.0f;
-        if (mine) {
+                if (nt > 0) {
 #pragma unroll
-            for (int e = 0; e < d; ++e) ss += o[e] * o[e];
-            rss[tid] = ss;
-        }
-        __syncthreads();
-        if (mine) {
-            ss = rss[t] + rss[128 + t];
-            const float g = ss < INFINITY ? rsqrtf(ss * (1.0f / D) + a.eps) : NAN;
+                    for (int x = 0; x < d; x += 32) {
+                        float v[32];
+                        tmem_ld32(TM_O + lane0 + m * d + x, o + x);
+                        tmem_ld32(TM_O + D + lane0 + m * d + x, v);
 #pragma unroll
-            for (int e = 0; e < d; e += 8) {
-                uint32_t x[4];
+                        for (int e = 0; e < 32; ++e) o[x + e] = o[x + e] * w1 - v[e] * w2;
+                    }
+                }
+                float ss = 0.0f;
 #pragma unroll
-                for (int k = 0; k < 4; ++k)
-                    x[k] = pack16<BF16>(o[e + 2 * k] * g * nw[half * d + e + 2 * k], o[e + 2 * k + 1] * g * nw[half * d + e + 2 * k + 1]);
-                const int ch = half * (CH / 2) + e / 8;
-                *(uint4 *) (smem + t * (D * 2) + ((ch ^ (t & 7)) << 4)) = make_uint4(x[0], x[1], x[2], x[3]);
+                for (int e = 0; e < d; ++e) ss += o[e] * o[e];
+                rss[tid] = ss;
             }
+            __syncthreads();
+            {
+                const float ss = rss[t] + rss[128 + t];
+                const float g = ss < INFINITY ? rsqrtf(ss * (1.0f / D) + a.eps) : NAN;
+#pragma unroll
+                for (int e = 0; e < d; e += 8) {
+                    uint32_t x[4];
+#pragma unroll
+                    for (int k = 0; k < 4; ++k)
+                        x[k] = pack16<BF16>(o[e + 2 * k] * g * nw[m * d + e + 2 * k], o[e + 2 * k + 1] * g * nw[m * d + e + 2 * k + 1]);
+                    const int ch = m * (CH / 2) + e / 8;
+                    *(uint4 *) (smem + t * (D * 2) + ((ch ^ (t & 7)) << 4)) = make_uint4(x[0], x[1], x[2], x[3]);
+                }
+            }
+            __syncthreads();
+            if (!*abort_flag && fits)
+                for (int i = tid; i < rows * CH; i += 256) {
+                    const int r = i / CH, ch = i % CH, u = rem0 + r;
+                    *(uint4 *) ((uint16_t *) a.out.p + b * a.out.sb + (long long) (i0 + u / p.G) * a.out.ss +
+                                (long long) (hk * p.G + u % p.G) * a.out.sh + ch * 8) =
+                        *(const uint4 *) (smem + r * (D * 2) + ((ch ^ (r & 7)) << 4));
+                }
         }
-        __syncthreads();
-        if (!*abort_flag)
-            for (int i = tid; i < rows * CH; i += THREADS) {
-                const int r = i / CH, ch = i % CH, u = rem0 + r;
-                *(uint4 *) ((uint16_t *) a.out.p + b * a.out.sb + (long long) (i0 + u / p.G) * a.out.ss +
-                            (long long) (hk * p.G + u % p.G) * a.out.sh + ch * 8) =
-                    *(const uint4 *) (smem + r * (D * 2) + ((ch ^ (r & 7)) << 4));
-            }
     }
     tc_fence_before();
     __syncthreads();
     if (warp == 9) {
         tc_fence_after();
-        tmem_dealloc(tmem, 512);
+        tmem_dealloc(tmem, L::TM);
     }
     if (*abort_flag && tid == 0) {
         // let copies that were issued but never consumed land before the CTA's shared memory is reused
@@ -492,21 +580,21 @@ diff_attn_tc(const __grid_constant__ CUtensorMap tk, const __grid_constant__ CUt
 }
 
 // ================================================================ few rows
-// diff_attn_rows: at most 16 rows of a kv head (one token with its group's heads, or a few), bound by reading K and V.
+// diff_attn_rows: a few rows of a kv head (one token with its group's heads, or a few), bound by reading K and V.
 // A 128-row tile would spend its time on rows that do not exist; here mma.sync takes 16 rows (m16n8k16), which
 // is far from being the limit: 48 products for 16 keys of 8 KB.
 // Each warp streams its own 16-key slabs (slab w, w + W, ...) by TMA through a ring of its own, so warps never wait
 // for one another: scores, online softmax and O of both maps stay in the warp's registers. The warps' sums
 // are added up in shared memory at the end, the parts of split keys through the workspace.
 constexpr int SLAB = 16, RING = 3;
+constexpr int FEW = 64;   // rows up to which groups of 16 beat a tile of 128
 
 template <int D, int W>
 struct RowLay {
     static constexpr int BOX = SLAB * 128, HALF = SLAB * D * 2, STAGE = 2 * HALF;   // a slab's keys, then its values
     static constexpr int OFF_LAM = W * RING * STAGE, OFF_W = OFF_LAM + 16 * 4, OFF_BAR = OFF_W + D * 4;
     static constexpr int TOTAL = OFF_BAR + W * RING * 8 + 16;
-    // after the last slab: each warp's O [16][2][D] and its ref and l [2 maps][16] each
-    static constexpr int SUMS = 16 * 2 * D + 64;
+    static constexpr int SUMS = 16 * row_words(D);   // after the last slab, in a warp's ring
     static_assert(W * SUMS * 4 <= W * RING * STAGE, "the warps' sums fit in their rings");
 };
 
@@ -527,44 +615,6 @@ __device__ __forceinline__ void ldmatrix4(uint32_t (&r)[4], uint32_t at) {
         asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(at) : "memory");
 }
 
-// Adds up `count` sets of sums for one row, one warp: set i has O [2][D] of the row at o + i * stride, and ref and l of
-// map m at st + i * stride + m * rows and + (2 + m) * rows. Returns O (this lane's D / 32 columns), ref and l.
-template <int D, bool GLOBAL>
-__device__ __forceinline__ void add_up(const float * o, const float * st, size_t stride, int rows, int count, int lane,
-                                       float (&sum)[2][D / 32], float (&top)[2], float (&l)[2]) {
-    constexpr int E = D / 32;
-    auto rd = [&](const float * p) { return GLOBAL ? __ldcg(p) : *p; };
-#pragma unroll
-    for (int m = 0; m < 2; ++m) {
-        top[m] = -INFINITY;
-        l[m] = 0.0f;
-        for (int i = lane; i < count; i += 32) top[m] = fmaxf(top[m], rd(st + i * stride + m * rows));
-#pragma unroll
-        for (int x = 16; x; x >>= 1) top[m] = fmaxf(top[m], __shfl_xor_sync(~0u, top[m], x));
-        const float ref = top[m] == -INFINITY ? 0.0f : top[m];
-        for (int i = lane; i < count; i += 32) l[m] += ex2(rd(st + i * stride + m * rows) - ref) * rd(st + i * stride + (2 + m) * rows);
-#pragma unroll
-        for (int x = 16; x; x >>= 1) l[m] += __shfl_xor_sync(~0u, l[m], x);
-#pragma unroll
-        for (int e = 0; e < E; ++e) sum[m][e] = 0.0f;
-#pragma unroll 8
-        for (int i = 0; i < count; ++i) {
-            const float f = ex2(rd(st + i * stride + m * rows) - ref);
-            const float * at = o + i * stride + m * D + E * lane;
-            float v[E];
-            if constexpr (E == 4) {
-                const float4 x = GLOBAL ? __ldcg((const float4 *) at) : *(const float4 *) at;
-                v[0] = x.x; v[1] = x.y; v[2] = x.z; v[3] = x.w;
-            } else {
-                const float2 x = GLOBAL ? __ldcg((const float2 *) at) : *(const float2 *) at;
-                v[0] = x.x; v[1] = x.y;
-            }
-#pragma unroll
-            for (int e = 0; e < E; ++e) sum[m][e] = fmaf(f, v[e], sum[m][e]);
-        }
-    }
-}
-
 template <int D, bool BF16, int W>
 __global__ void __launch_bounds__(32 * W, W == 8 ? 1 : 2)
 diff_attn_rows(const __grid_constant__ CUtensorMap tk, const __grid_constant__ CUtensorMap tv, const __grid_constant__ Args p) {
@@ -581,12 +631,15 @@ diff_attn_rows(const __grid_constant__ CUtensorMap tk, const __grid_constant__ C
     uint64_t * full = (uint64_t *) (smem + L::OFF_BAR) + warp * RING;
     volatile int * flags = (volatile int *) (smem + L::OFF_BAR + W * RING * 8);   // abort, last to arrive
 
-    const unsigned gid = blockIdx.x / p.splits, split = blockIdx.x % p.splits;
-    const int hk = (int) (gid % a.Hk), b = (int) (gid / a.Hk), R = (int) p.R;
+    // groups of 16 rows next to one another read the same keys at about the same time
+    const int sixteens = (int) (p.R + 15) / 16;
+    const unsigned gid = blockIdx.x / (sixteens * p.splits) * sixteens + blockIdx.x % sixteens, split = blockIdx.x / sixteens % p.splits;
+    const int hk = (int) (gid / sixteens % a.Hk), b = (int) (gid / sixteens / a.Hk);
+    const int first = (int) (gid % sixteens) * 16, R = min(16, (int) p.R - first);   // row r: token (first + r) / G, head (first + r) % G
     const int n = a.key_len ? max(0, min(a.key_len[b], (int) a.Sk)) : (int) a.Sk;
     auto limit = [&](int r) {   // keys before which row r sees; rows past the last one see all
         if (!a.causal || r >= R) return n;
-        return (int) max(0ll, min((long long) n, (long long) (r / p.G) + n - (long long) a.Sq + 1));
+        return (int) max(0ll, min((long long) n, (long long) ((first + r) / p.G) + n - (long long) a.Sq + 1));
     };
     const int least = limit(0);
     // this CTA's slabs, and this warp's
@@ -615,14 +668,14 @@ diff_attn_rows(const __grid_constant__ CUtensorMap tk, const __grid_constant__ C
     if (lane == 0)
         for (int i = 0; i < RING && i < mine; ++i) request(i);
 
-    // lambda of each head of the group, the norm's weights
-    for (int g = warp; g < p.G; g += W) {
-        const long long h = (long long) (hk * p.G + g) * a.lam_sh;
+    // lambda of each row's head, the norm's weights
+    for (int r = warp; r < R; r += W) {
+        const long long h = (long long) (hk * p.G + (first + r) % p.G) * a.lam_sh;
         float z1 = 0.0f, z2 = 0.0f;
         for (int e = lane; e < d; e += 32) { z1 += a.lq1[h + e] * a.lk1[h + e]; z2 += a.lq2[h + e] * a.lk2[h + e]; }
 #pragma unroll
         for (int x = 16; x; x >>= 1) { z1 += __shfl_xor_sync(~0u, z1, x); z2 += __shfl_xor_sync(~0u, z2, x); }
-        if (lane == 0) lam[g] = expf(z1) - expf(z2) + a.lambda_init;
+        if (lane == 0) lam[r] = expf(z1) - expf(z2) + a.lambda_init;
     }
     for (int e = tid; e < D; e += 32 * W) nw[e] = (a.norm_w ? a.norm_w[e] : 1.0f) * (1.0f - a.lambda_init);
 
@@ -632,7 +685,7 @@ diff_attn_rows(const __grid_constant__ CUtensorMap tk, const __grid_constant__ C
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
         const int r = r0 + 8 * h;
-        const uint16_t * q = (const uint16_t *) a.q.p + b * a.q.sb + (long long) (r / p.G) * a.q.ss + (long long) (hk * p.G + r % p.G) * a.q.sh;
+        const uint16_t * q = (const uint16_t *) a.q.p + b * a.q.sb + (long long) ((first + r) / p.G) * a.q.ss + (long long) (hk * p.G + (first + r) % p.G) * a.q.sh;
 #pragma unroll
         for (int m = 0; m < 2; ++m)
 #pragma unroll
@@ -788,57 +841,33 @@ diff_attn_rows(const __grid_constant__ CUtensorMap tk, const __grid_constant__ C
             float t = l[m][h];
             t += __shfl_xor_sync(~0u, t, 1);
             t += __shfl_xor_sync(~0u, t, 2);
+            float * to = sums + r * row_words(D);
             if ((lane & 3) == 0) {
-                sums[16 * 2 * D + m * 16 + r] = ref[m][h];
-                sums[16 * 2 * D + (2 + m) * 16 + r] = poison[h] ? NAN : t;
+                to[2 * D + m] = ref[m][h];
+                to[2 * D + 2 + m] = poison[h] ? NAN : t;
             }
             if (r < R)
 #pragma unroll
-                for (int x = 0; x < D / 8; ++x)
-                    *(float2 *) (sums + (r * 2 + m) * D + 8 * x + c0) = make_float2(o[m][x][2 * h], o[m][x][2 * h + 1]);
+                for (int x = 0; x < D / 8; ++x) *(float2 *) (to + m * D + 8 * x + c0) = make_float2(o[m][x][2 * h], o[m][x][2 * h + 1]);
         }
     }
     __syncthreads();
-    auto finish = [&](int r, float (&sum)[2][E], float (&rl)[2]) {
-        const int g = r % p.G;
-        const float w1 = rl[0] == 0.0f ? 0.0f : 1.0f / rl[0], w2 = rl[1] == 0.0f ? 0.0f : lam[g] / rl[1];
-        float ss = 0.0f, v[E];
-#pragma unroll
-        for (int e = 0; e < E; ++e) {
-            v[e] = sum[0][e] * w1 - sum[1][e] * w2;
-            ss += v[e] * v[e];
-        }
-#pragma unroll
-        for (int x = 16; x; x >>= 1) ss += __shfl_xor_sync(~0u, ss, x);
-        const float f = ss < INFINITY ? rsqrtf(ss * (1.0f / D) + a.eps) : NAN;
-        uint32_t x[E / 2];
-#pragma unroll
-        for (int e = 0; e < E; e += 2) x[e / 2] = pack16<BF16>(v[e] * f * nw[E * lane + e], v[e + 1] * f * nw[E * lane + e + 1]);
-        uint16_t * out = (uint16_t *) a.out.p + b * a.out.sb + (long long) (r / p.G) * a.out.ss + (long long) (hk * p.G + g) * a.out.sh + E * lane;
-        if (flags[0]) return;
-        if constexpr (E == 4) *(uint2 *) out = make_uint2(x[0], x[1]);
-        else *(uint32_t *) out = x[0];
-    };
-    const float * all = (const float *) smem;
-    constexpr size_t STRIDE = (size_t) RING * L::STAGE / 4;
-    const size_t size = (size_t) R * (2 * D + 4);
-    float * part = p.part + (size_t) gid * p.splits * size;
-    for (int r = warp; r < R; r += W) {
+    const size_t size = (size_t) R * row_words(D);   // of a part
+    float * part = p.part + (size_t) gid * p.splits * (16 * row_words(D));
+    for (int r = warp; r < R && !flags[0]; r += W) {
         float sum[2][E], top[2], rl[2];
-        add_up<D, false>(all + r * 2 * D, all + 16 * 2 * D + r, STRIDE, 16, W, lane, sum, top, rl);
+        auto at = [&](int i, int k) { return (const float *) (smem + i * RING * L::STAGE) + r * row_words(D) + k; };
+        add_up<D>(W, lane, sum, top, rl, [&](int i, int k) { return *at(i, k); },
+                  [&](int i, int k, float * v) { read_words<E, false>(at(i, k), v); });
         if (p.splits == 1) {
-            finish(r, sum, rl);
+            write_row<D, BF16>(p, b, hk, (first + r) / p.G, (first + r) % p.G, lam[r], nw, lane, sum, rl);
         } else {
-            float * at = part + split * size;
+            float * to = part + split * size + r * row_words(D);
 #pragma unroll
             for (int m = 0; m < 2; ++m) {
-                float * to = at + (size_t) (r * 2 + m) * D + E * lane;
-                if constexpr (E == 4) *(float4 *) to = make_float4(sum[m][0], sum[m][1], sum[m][2], sum[m][3]);
-                else *(float2 *) to = make_float2(sum[m][0], sum[m][1]);
-                if (lane == 0) {
-                    at[(size_t) R * 2 * D + m * R + r] = top[m];
-                    at[(size_t) R * 2 * D + (2 + m) * R + r] = rl[m];
-                }
+                if constexpr (E == 4) *(float4 *) (to + m * D + E * lane) = make_float4(sum[m][0], sum[m][1], sum[m][2], sum[m][3]);
+                else *(float2 *) (to + m * D + E * lane) = make_float2(sum[m][0], sum[m][1]);
+                if (lane == 0) { to[2 * D + m] = top[m]; to[2 * D + 2 + m] = rl[m]; }
             }
         }
     }
@@ -853,10 +882,12 @@ diff_attn_rows(const __grid_constant__ CUtensorMap tk, const __grid_constant__ C
         }
         __syncthreads();
         if (flags[1])
-            for (int r = warp; r < R; r += W) {
+            for (int r = warp; r < R && !flags[0]; r += W) {
                 float sum[2][E], top[2], rl[2];
-                add_up<D, true>(part + (size_t) r * 2 * D, part + (size_t) R * 2 * D + r, size, R, p.splits, lane, sum, top, rl);
-                finish(r, sum, rl);
+                auto at = [&](int i, int k) { return part + i * size + r * row_words(D) + k; };
+                add_up<D>(p.splits, lane, sum, top, rl, [&](int i, int k) { return __ldcg(at(i, k)); },
+                          [&](int i, int k, float * v) { read_words<E, true>(at(i, k), v); });
+                write_row<D, BF16>(p, b, hk, (first + r) / p.G, (first + r) % p.G, lam[r], nw, lane, sum, rl);
             }
     }
     if (flags[0] && tid == 0) {
@@ -918,8 +949,17 @@ int workspace(DeviceCtx & c, bool capturing) {
 
 template <int D, bool BF16>
 cudaError_t launch_tc(const CUtensorMap & tk, const CUtensorMap & tv, const Args & p, unsigned grid, cudaStream_t s) {
-    diff_attn_tc<D, BF16><<<grid, THREADS, Lay<D>::TOTAL, s>>>(tk, tv, p);
-    return cudaGetLastError();
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3(grid);
+    cfg.blockDim = dim3(THREADS);
+    cfg.dynamicSmemBytes = Lay<D>::TOTAL;
+    cfg.stream = s;
+    cudaLaunchAttribute at{};
+    at.id = cudaLaunchAttributeClusterDimension;
+    at.val.clusterDim = {(unsigned) p.splits, 1, 1};
+    cfg.attrs = &at;
+    cfg.numAttrs = p.splits > 1 ? 1 : 0;
+    return cudaLaunchKernelEx(&cfg, diff_attn_tc<D, BF16>, tk, tv, p);
 }
 template <int D, bool BF16>
 cudaError_t launch_rows(const CUtensorMap & tk, const CUtensorMap & tv, const Args & p, unsigned grid, int warps, cudaStream_t s) {
@@ -986,9 +1026,8 @@ int diff_attn(DeviceCtx & c, const tsn_diff_attn_args & in) {
     p.G = (int) (a.H / a.Hk);
     p.R = (long long) a.Sq * p.G;
     p.err = c.d_err;
-    const bool rows = p.R <= 16;
-    const long long groups = (p.R + ROWS - 1) / ROWS * a.B * a.Hk;
-    if (groups > 0x7fffffffLL) return fail(TSN_ERR_ARG, "tsn_diff_attn: too many query rows");
+    const bool rows = p.R <= FEW;
+    const long long groups = (rows ? (p.R + 15) / 16 : (p.R + ROWS - 1) / ROWS) * a.B * a.Hk;
     int warps = 8;
     if (rows) {
         // Parts of 512 keys (four slabs for each of eight warps) while that is at most one CTA per SM, and none up to
@@ -1001,19 +1040,19 @@ int diff_attn(DeviceCtx & c, const tsn_diff_attn_args & in) {
             warps = 4;
             parts = std::min(parts, std::max(1ll, 8 * SMS / groups));
         }
-        const long long size = p.R * (4 * a.d + 4) * 4;
-        parts = std::min({parts, 64ll, std::max(1ll, (long long) (WORKSPACE - COUNTERS * 4) / (groups * size))});
+        parts = std::min({parts, 64ll, std::max(1ll, (long long) (WORKSPACE - COUNTERS * 4) / (groups * 16 * (4 * a.d + 4) * 4))});
         if (groups > (long long) COUNTERS) parts = 1;
         p.chunk = (int) std::max(1ll, (slabs + parts - 1) / parts);
         p.splits = (int) std::max(1ll, (slabs + p.chunk - 1) / p.chunk);
     } else {
-        // Split the keys where whole tiles leave SMs without work: as many parts as fill one wave, of two key tiles at
-        // least (a part costs its CTA's start and a trip through the workspace, about what two tiles take).
+        // Split the keys over a cluster where whole tiles leave SMs without work: as many parts as fill one wave, of four
+        // key tiles at least, eight at most (the largest portable cluster).
         const long long tiles = ((long long) a.Sk + KEYS - 1) / KEYS;
-        p.splits = (int) std::max(1ll, std::min(SMS / groups, tiles / 2));
-        p.wr = (int) std::min<long long>(ROWS, p.R);
+        p.splits = (int) std::max(1ll, std::min({SMS / groups, tiles / 4, 8ll}));
     }
-    if (p.splits > 1) {
+    if (groups * p.splits > 0x7fffffffLL) return fail(TSN_ERR_ARG, "tsn_diff_attn: too many query rows");
+    const bool shared = rows && p.splits > 1;   // through the workspace
+    if (shared) {
         cudaStreamCaptureStatus st = cudaStreamCaptureStatusNone;
         cudaError_t e = cudaStreamIsCapturing(c.stream, &st);
         if (e != cudaSuccess) return fail(TSN_ERR_CUDA, std::string("tsn_diff_attn: ") + cudaGetErrorString(e));
@@ -1022,7 +1061,6 @@ int diff_attn(DeviceCtx & c, const tsn_diff_attn_args & in) {
         p.count = (unsigned int *) c.split_ws;
         p.part = (float *) ((char *) c.split_ws + COUNTERS * 4);
     }
-    static_assert(SMS <= COUNTERS && (size_t) SMS * 128 * (2 * 128 + 4) * 4 <= ((size_t) 32 << 20), "one wave of partial results fits");
     CUtensorMap tk{}, tv{};
     if (a.Sk && (!make_kv_map(&tk, a, a.k, KB, rows ? SLAB : KEYS) || !make_kv_map(&tv, a, a.v, KB, rows ? SLAB : KEYS)))
         return fail(TSN_ERR_ARG, "tsn_diff_attn: k or v cannot be described to the tensor memory accelerator");
@@ -1035,7 +1073,7 @@ int diff_attn(DeviceCtx & c, const tsn_diff_attn_args & in) {
     else
         e = a.d == 32 ? (bf ? launch_tc<64, true>(tk, tv, p, grid, c.stream) : launch_tc<64, false>(tk, tv, p, grid, c.stream))
                       : (bf ? launch_tc<128, true>(tk, tv, p, grid, c.stream) : launch_tc<128, false>(tk, tv, p, grid, c.stream));
-    if (e == cudaSuccess && p.splits > 1) {
+    if (e == cudaSuccess && shared) {
         cudaStreamCaptureStatus st = cudaStreamCaptureStatusNone;
         e = cudaStreamIsCapturing(c.stream, &st);
         if (e == cudaSuccess && st == cudaStreamCaptureStatusNone) {
