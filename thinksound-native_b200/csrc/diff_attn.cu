@@ -17,7 +17,6 @@
 #include <cudaTypedefs.h>
 
 #include <algorithm>
-#include <mutex>
 
 namespace tsn {
 
@@ -58,10 +57,40 @@ __device__ __forceinline__ uint64_t ffma2(uint64_t a, uint64_t b, uint64_t c) {
     asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
     return d;
 }
+__device__ __forceinline__ uint64_t f2_neg(uint64_t a) { return a ^ 0x8000000080000000ull; }
 __device__ __forceinline__ uint64_t fadd2(uint64_t a, uint64_t b) {
     uint64_t d;
     asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
     return d;
+}
+// (2^x, 2^y) on the FMA pipe, x and y clamped to -126 or more: 2^i p(f), i the nearest whole number, f = x - i in [-1/2, 1/2],
+// p the polynomial of least relative error there (Remez exchange): 7.5e-5 at degree 3, 2.6e-6 at degree 4, each below
+// an eighth of half a unit of the 16-bit type that the result is rounded to. Adding 1.5 * 2^23 rounds to i and leaves
+// it in the low bits. NaN stays non-finite.
+template <bool BF16>
+__device__ __forceinline__ uint64_t ex2_fma(uint64_t xy) {
+    float x, y;
+    f2_unpack(xy, x, y);
+    asm("max.NaN.f32 %0, %0, %1;" : "+f"(x) : "f"(-126.0f));
+    asm("max.NaN.f32 %0, %0, %1;" : "+f"(y) : "f"(-126.0f));
+    const uint64_t v = f2_pack(x, y), magic = f2_pack(12582912.0f, 12582912.0f), r = fadd2(v, magic);
+    const uint64_t f = fadd2(v, fadd2(magic, f2_neg(r)));
+    auto two = [](float c) { return f2_pack(c, c); };
+    uint64_t q;
+    if (BF16) {
+        q = ffma2(two(0.0551716685f), f, two(0.242611125f));
+        q = ffma2(q, f, two(0.693260968f));
+        q = ffma2(q, f, two(0.999928057f));
+    } else {
+        q = ffma2(two(0.00957010221f), f, two(0.0559178591f));
+        q = ffma2(q, f, two(0.240247443f));
+        q = ffma2(q, f, two(0.693121791f));
+        q = ffma2(q, f, two(0.999999285f));
+    }
+    float a, b, i, j;
+    f2_unpack(q, a, b);
+    f2_unpack(r, i, j);
+    return f2_pack(__uint_as_float(__float_as_uint(a) + (__float_as_uint(i) << 23)), __uint_as_float(__float_as_uint(b) + (__float_as_uint(j) << 23)));
 }
 template <bool BF16>
 __device__ __forceinline__ uint32_t pack16(float a, float b) {
@@ -166,9 +195,12 @@ __device__ __forceinline__ void write_row(const Args & p, int b, int hk, int i, 
 // (16 exponentials a cycle) and 896 of the tensor cores (the products with N 64 wait for shared memory).
 // Parts of the keys: each CTA leaves its rows' sums in its shared memory and, after a cluster barrier, adds up its
 // share of the rows over the cluster, in the order of the parts.
+#ifndef FE
+#define FE 4
+#endif
 template <int D>
 struct Lay {
-    static constexpr int BUF = D == 128 ? 2 : 2;
+    static constexpr int BUF = 2;
     static constexpr int Q = ROWS * D * 2, BOX = KEYS * 128, TILE = KEYS * D * 2;   // boxes of 64 keys x 64 elements
     static constexpr int STAGES = 6;
     static constexpr int OFF_K = Q, OFF_V = OFF_K + STAGES * TILE, OFF_LAM = OFF_V + STAGES * TILE;
@@ -241,7 +273,7 @@ diff_attn_tc(const __grid_constant__ CUtensorMap tk, const __grid_constant__ CUt
             if (lane == 0) {
                 for (int j = 0; j < nt; ++j) {
                     const int s = j % L::STAGES;
-                    if (j >= L::STAGES && !mbar_wait(&empty[s], (j / L::STAGES - 1) & 1, abort_flag, p.err, DEV_TIMEOUT_EMPTY)) break;
+                    if (j >= L::STAGES && !mbar_wait_soon(&empty[s], (j / L::STAGES - 1) & 1, abort_flag, p.err, DEV_TIMEOUT_EMPTY)) break;
                     mbar_expect_tx(&full[s], 2 * L::TILE);
                     for (int x = 0; x < ATOMS; ++x) {
                         tma_load_4d(smem + L::OFF_K + s * L::TILE + x * L::BOX, &tk, &full[s], 64 * x, (t0 + j) * KEYS, hk, b * p.kv_b);
@@ -250,46 +282,59 @@ diff_attn_tc(const __grid_constant__ CUtensorMap tk, const __grid_constant__ CUt
                 }
             }
         } else if (warp == 11) {
-            for (int j = 0; j < nt && mend; ++j) {
-                const int base = (t0 + j) * KEYS, s = j % L::STAGES;
-                uint32_t kw[2], bad[2] = {0, 0};
+            uint32_t mb[2] = {};   // whether the keys of the next tile are seen
+            auto fetch = [&](int j) {
 #pragma unroll
                 for (int w = 0; w < 2; ++w) {
-                    const int key = base + 32 * w + lane;
-                    kw[w] = __ballot_sync(~0u, key < n && (!mask || mask[key] != 0));
+                    const int key = (t0 + j) * KEYS + 32 * w + lane;
+                    mb[w] = key < n && (!mask || mask[key] != 0);
                 }
-                if (!mbar_wait(&full[s], (j / L::STAGES) & 1, abort_flag, p.err, DEV_TIMEOUT_FULL)) break;
+            };
+            if (mend) fetch(0);
+            for (int j = 0; j < nt && mend; ++j) {
+                const int base = (t0 + j) * KEYS, s = j % L::STAGES;
+                uint32_t gone[2], bad[2] = {0, 0};
+#pragma unroll
+                for (int w = 0; w < 2; ++w) gone[w] = ~__ballot_sync(~0u, mb[w] != 0);
+                if (j + 1 < nt) fetch(j + 1);
+                if (!mbar_wait_soon(&full[s], (j / L::STAGES) & 1, abort_flag, p.err, DEV_TIMEOUT_FULL)) break;
                 __syncwarp();
-                const bool differ = mixed(base);
-                if ((kw[0] & kw[1]) != ~0u || differ) {
-                    constexpr int AT_ONCE = 32 / CH, AHEAD = 4;   // rows of one step, steps whose loads run together
-                    for (int key0 = 0; key0 < KEYS; key0 += AT_ONCE * AHEAD) {
-                        uint4 o[AHEAD];
-                        auto at = [&](int y) {
-                            const int key = key0 + y * AT_ONCE + lane / CH, ch = lane % CH;
-                            return (uint4 *) (smem + L::OFF_V + s * L::TILE + (ch >> 3) * L::BOX + key * 128 + (((ch & 7) ^ (key & 7)) << 4));
-                        };
-                        const uint32_t here = kw[key0 >> 5] >> (key0 & 31);
-                        if (differ)
+                constexpr int AT_ONCE = 32 / CH;   // rows of one step
+                const int sub = lane / CH, ch = lane % CH;
+                auto at = [&](int key) {
+                    return (uint4 *) (smem + L::OFF_V + s * L::TILE + (ch >> 3) * L::BOX + key * 128 + (((ch & 7) ^ (key & 7)) << 4));
+                };
+                // rows of masked keys
 #pragma unroll
-                            for (int y = 0; y < AHEAD; ++y) o[y] = *at(y);
+                for (int w = 0; w < 2; ++w)
+                    for (uint32_t g = gone[w]; g;) {
+                        int key = -1;
 #pragma unroll
-                        for (int y = 0; y < AHEAD; ++y) {
-                            if (!((here >> (y * AT_ONCE + lane / CH)) & 1u)) {
-                                *at(y) = make_uint4(0, 0, 0, 0);
-                            } else if (differ) {
-                                const uint4 f = make_uint4(finite_only<BF16>(o[y].x), finite_only<BF16>(o[y].y), finite_only<BF16>(o[y].z), finite_only<BF16>(o[y].w));
-                                if (o[y].x != f.x || o[y].y != f.y || o[y].z != f.z || o[y].w != f.w) {
-                                    *at(y) = f;
-                                    bad[key0 >> 5] |= 1u << ((key0 + y * AT_ONCE + lane / CH) & 31);
-                                }
+                        for (int y = 0; y < AT_ONCE; ++y) {
+                            if (g && sub == y) key = 32 * w + __ffs((int) g) - 1;
+                            g &= g - 1;
+                        }
+                        if (key >= 0) *at(key) = make_uint4(0, 0, 0, 0);
+                    }
+                __syncwarp();
+                // non-finite values, where some rows see the key and others do not
+                if (mixed(base))
+#pragma unroll
+                    for (int w = 0; w < 2; ++w) {
+#pragma unroll 4
+                        for (int y = 0; y < 32; y += AT_ONCE) {
+                            const int key = 32 * w + y + sub;
+                            const uint4 o = *at(key);
+                            const uint4 f = make_uint4(finite_only<BF16>(o.x), finite_only<BF16>(o.y), finite_only<BF16>(o.z), finite_only<BF16>(o.w));
+                            if (o.x != f.x || o.y != f.y || o.z != f.z || o.w != f.w) {
+                                *at(key) = f;
+                                bad[w] |= 1u << (key & 31);
                             }
                         }
+                        bad[w] = __reduce_or_sync(~0u, bad[w]);
                     }
-                    fence_proxy_async_smem();
-                }
-                bad[0] = __reduce_or_sync(~0u, bad[0]);
-                bad[1] = __reduce_or_sync(~0u, bad[1]);
+                fence_proxy_async_smem();
+                __syncwarp();
                 if (lane == 0) {
                     words[2 + 2 * s] = bad[0];
                     words[3 + 2 * s] = bad[1];
@@ -305,19 +350,19 @@ diff_attn_tc(const __grid_constant__ CUtensorMap tk, const __grid_constant__ CUt
             const uint32_t to = TM_O + D * mm, ts = tmem + KEYS * BUF * mm;
             auto qk = [&](int j) {
                 const int s = j % L::STAGES, x = j % BUF;
-                if (!mbar_wait(&full[s], (j / L::STAGES) & 1, abort_flag, p.err, DEV_TIMEOUT_FULL)) return false;
+                if (!mbar_wait_soon(&full[s], (j / L::STAGES) & 1, abort_flag, p.err, DEV_TIMEOUT_FULL)) return false;
                 const uint64_t k = kd + (uint64_t) (s * (L::TILE >> 4));
 #pragma unroll
                 for (int kk = 0; kk < d / 16; ++kk) umma_f16_if(lead, ts + KEYS * x, qd + 2 * kk, k + 2 * kk, id_s, kk != 0);
                 umma_commit_if(lead, &s_full[mm * BUF + x]);
                 return true;
             };
-            bool go = nt > 0 && mbar_wait(q_full, 0, abort_flag, p.err, DEV_TIMEOUT_FULL);
+            bool go = nt > 0 && mbar_wait_soon(q_full, 0, abort_flag, p.err, DEV_TIMEOUT_FULL);
             for (int j = 0; j < BUF && j < nt && go; ++j) go = qk(j);
             for (int j = 0; j < nt && go; ++j) {
                 const int s = j % L::STAGES, x = j % BUF;
-                if (!mbar_wait(&p_full[mm * BUF + x], (j / BUF) & 1, abort_flag, p.err, DEV_TIMEOUT_TMEM)) break;
-                if (mend && !mbar_wait(&v_ready[s], (j / L::STAGES) & 1, abort_flag, p.err, DEV_TIMEOUT_FULL)) break;
+                if (!mbar_wait_soon(&p_full[mm * BUF + x], (j / BUF) & 1, abort_flag, p.err, DEV_TIMEOUT_TMEM)) break;
+                if (mend && !mbar_wait_soon(&v_ready[s], (j / L::STAGES) & 1, abort_flag, p.err, DEV_TIMEOUT_FULL)) break;
                 tc_fence_after();
                 const uint64_t v = vd + (uint64_t) (s * (L::TILE >> 4));
 #pragma unroll
@@ -362,7 +407,7 @@ diff_attn_tc(const __grid_constant__ CUtensorMap tk, const __grid_constant__ CUt
             if (tid < D) nw[tid] = (a.norm_w ? a.norm_w[tid] : 1.0f) * (1.0f - a.lambda_init);
 
             const uint32_t to = TM_O + D * m + lane0;
-            const int lim = t < rows ? limit(t) : n;
+            const int lim = t < rows ? limit(t) : n;   // keys before which this row sees
             bool poison = false;
             uint32_t mb[2] = {};   // mask bytes of the next tile
             auto fetch_mask = [&](int j) {
@@ -372,99 +417,105 @@ diff_attn_tc(const __grid_constant__ CUtensorMap tk, const __grid_constant__ CUt
                     mb[w] = key < n ? mask[key] : 0u;
                 }
             };
-            // the keys of tile j that this row sees; clear: every row sees all of them
-            auto clear = [&](int j) { return !mask && (t0 + j + 1) * KEYS <= least; };
-            auto visible = [&](int j, uint32_t (&vis)[2]) {
-#pragma unroll
-                for (int w = 0; w < 2; ++w) {
-                    const int at = (t0 + j) * KEYS + 32 * w;
-                    vis[w] = (mask ? __ballot_sync(~0u, mb[w] != 0) : low_bits(n - at)) & low_bits(lim - at);
-                }
-            };
-            auto hide = [&](const uint32_t vis, uint32_t * s) {   // masks 32 keys
-                if (__any_sync(~0u, vis != ~0u))
-#pragma unroll
-                    for (int e = 0; e < 32; ++e)
-                        if (!((vis >> e) & 1u)) s[e] = 0xff800000u;   // -inf
-            };
-            if (mask && nt > 0) fetch_mask(0);
-            for (int j = 0; j < nt; ++j) {
-                const int x = m * BUF + j % BUF;
-                const uint32_t ts = tmem + KEYS * x + lane0;
-                uint32_t vis[2] = {~0u, ~0u};
-                if (!clear(j)) visible(j, vis);
-                if (mask && j + 1 < nt) fetch_mask(j + 1);
-                if (!mbar_wait(&s_full[x], (j / BUF) & 1, abort_flag, p.err, DEV_TIMEOUT_TMEM)) { ok = false; break; }
+            auto arrived = [&](int j) {   // tile j's scores
+                const bool go = mbar_wait_soon(&s_full[m * BUF + j % BUF], (j / BUF) & 1, abort_flag, p.err, DEV_TIMEOUT_TMEM);
                 __syncwarp();
                 tc_fence_after();
-                uint32_t s[KEYS], pk[KEYS / 2];
-                tmem_request32(ts, s);
-                tmem_request32(ts + 32, s + 32);
-                tmem_landed32(s);
-                tmem_landed32(s + 32);
-                if (!clear(j)) {
-                    hide(vis[0], s);
-                    hide(vis[1], s + 32);
-                }
-                // The exponentials are taken against the reference of the tiles before, and the maximum beside them, so that
-                // the SFU need not wait for it; the few tiles whose maximum is too far above the reference are done again.
-                uint64_t sum[2];
-                while (true) {
-                    const float neg = ref == -INFINITY ? 0.0f : -ref;
-                    const uint64_t c2 = f2_pack(p.c, p.c), neg2 = f2_pack(neg, neg);
-                    float mx[2] = {-INFINITY, -INFINITY};
-                    sum[0] = sum[1] = 0ull;
+                return go;
+            };
+            auto tiles = [&](auto masked, int from, int until) {
+                constexpr bool MASKED = decltype(masked)::value;
+                for (int j = from; j < until && ok; ++j) {
+                    const int base = (t0 + j) * KEYS, x = m * BUF + j % BUF;
+                    uint32_t s[KEYS], pk[KEYS / 2];
+                    tmem_request32(tmem + KEYS * x + lane0, s);
+                    tmem_request32(tmem + KEYS * x + lane0 + 32, s + 32);
+                    tmem_landed32(s);
+                    tmem_landed32(s + 32);
+                    uint32_t vis[2];   // the keys that this row sees
+                    if (MASKED) {
 #pragma unroll
-                    for (int e = 0; e < KEYS / 2; ++e) {
-                        const float a0 = __uint_as_float(s[2 * e]), a1 = __uint_as_float(s[2 * e + 1]);
-                        float y, z;
-                        f2_unpack(ffma2(f2_pack(a0, a1), c2, neg2), y, z);
-                        y = ex2(y);
-                        z = ex2(z);
-                        sum[e & 1] = fadd2(sum[e & 1], f2_pack(y, z));
-                        pk[e] = pack16<BF16>(y, z);
-                        mx[e & 1] = fmaxf(mx[e & 1], fmaxf(a0, a1));
+                        for (int w = 0; w < 2; ++w) {
+                            vis[w] = (mask ? __ballot_sync(~0u, mb[w] != 0) : low_bits(n - base - 32 * w)) & low_bits(lim - base - 32 * w);
+                            if (__any_sync(~0u, vis[w] != ~0u))
+#pragma unroll
+                                for (int e = 0; e < 32; ++e)
+                                    if (!((vis[w] >> e) & 1u)) s[32 * w + e] = 0xff800000u;   // -inf
+                        }
+                        if (mask && j + 1 < nt) fetch_mask(j + 1);
                     }
-                    const float top = fmaxf(mx[0], mx[1]) * p.c;
-                    const bool move = top > ref + LAZY;
-                    if (!__any_sync(~0u, move)) break;
-                    // a row moves its reference by itself, so its result does not depend on its neighbours
-                    const float f = move ? ex2(ref - top) : 1.0f;
-                    if (move) { ref = top; l *= f; }
-                    if (j > 0) {
-                        // O is complete up to tile j - 1: the scores issued after that product are there, or its own commit
-                        const int i = j - 1 + BUF;
-                        uint64_t * done = i < nt ? &s_full[m * BUF + i % BUF] : &o_full[m * BUF + nt - j];
-                        if (!mbar_wait(done, i < nt ? (i / BUF) & 1 : 0, abort_flag, p.err, DEV_TIMEOUT_TMEM)) { ok = false; break; }
-                        __syncwarp();
-                        tc_fence_after();
-#pragma unroll 1
-                        for (int y = 0; y < D; y += 16) {
-                            float o[16];
-                            tmem_ld16(to + y, o);
+                    // The exponentials are taken against the reference of the tiles before, and the maximum beside them, so that
+                    // the SFU need not wait for it; the few tiles whose maximum is too far above the reference are done again.
+                    uint64_t sum[2];
+                    while (true) {
+                        const float neg = ref == -INFINITY ? 0.0f : -ref;
+                        const uint64_t c2 = f2_pack(p.c, p.c), neg2 = f2_pack(neg, neg);
+                        float mx[2] = {-INFINITY, -INFINITY};
+                        sum[0] = sum[1] = 0ull;
 #pragma unroll
-                            for (int e = 0; e < 16; ++e) o[e] *= f;
-                            tmem_st16(to + y, (const uint32_t *) o);
+                        for (int e = 0; e < KEYS / 2; ++e) {
+                            const float a0 = __uint_as_float(s[2 * e]), a1 = __uint_as_float(s[2 * e + 1]);
+                            const uint64_t v = ffma2(f2_pack(a0, a1), c2, neg2);
+                            float y, z;
+                            if (!MASKED && e % FE == FE - 1) {
+                                f2_unpack(ex2_fma<BF16>(v), y, z);
+                            } else {
+                                f2_unpack(v, y, z);
+                                y = ex2(y);
+                                z = ex2(z);
+                            }
+                            sum[e & 1] = fadd2(sum[e & 1], f2_pack(y, z));
+                            pk[e] = pack16<BF16>(y, z);
+                            mx[e & 1] = fmaxf(mx[e & 1], fmaxf(a0, a1));
+                        }
+                        const float top = fmaxf(mx[0], mx[1]) * p.c;
+                        const bool move = top > ref + LAZY;
+                        if (!__any_sync(~0u, move)) break;
+                        // a row moves its reference by itself, so its result does not depend on its neighbours
+                        const float f = move ? ex2(ref - top) : 1.0f;
+                        if (move) { ref = top; l *= f; }
+                        if (j > 0) {
+                            // O is complete up to tile j - 1: the scores issued after that product are there, or its own commit
+                            const int i = j - 1 + BUF;
+                            uint64_t * done = i < nt ? &s_full[m * BUF + i % BUF] : &o_full[m * BUF + nt - j];
+                            if (!mbar_wait_soon(done, i < nt ? (i / BUF) & 1 : 0, abort_flag, p.err, DEV_TIMEOUT_TMEM)) { ok = false; break; }
+                            __syncwarp();
+                            tc_fence_after();
+#pragma unroll 1
+                            for (int y = 0; y < D; y += 16) {
+                                float o[16];
+                                tmem_ld16(to + y, o);
+#pragma unroll
+                                for (int e = 0; e < 16; ++e) o[e] *= f;
+                                tmem_st16(to + y, (const uint32_t *) o);
+                            }
                         }
                     }
+                    float y, z;
+                    f2_unpack(fadd2(sum[0], sum[1]), y, z);
+                    l += y + z;
+                    tmem_st32(tmem + KEYS * x + lane0, pk);
+                    if (j + 1 < nt && !arrived(j + 1)) ok = false;   // meanwhile; they need no more than the product of tile j - 1
+                    tmem_st_wait();
+                    if (MASKED && m == 0 && mixed(base)) {
+                        if (!mbar_wait_soon(&v_ready[j % L::STAGES], (j / L::STAGES) & 1, abort_flag, p.err, DEV_TIMEOUT_FULL)) ok = false;
+                        const volatile uint32_t * bad = words + 2 + 2 * (j % L::STAGES);
+                        poison |= (bad[0] & vis[0]) != 0 || (bad[1] & vis[1]) != 0;
+                    }
+                    tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(&p_full[x]);
                 }
-                if (!ok) break;
-                float y, z;
-                f2_unpack(fadd2(sum[0], sum[1]), y, z);
-                l += y + z;
-                tmem_st32(ts, pk);
-                tmem_st_wait();
-                if (m == 0 && mixed((t0 + j) * KEYS)) {
-                    if (!mbar_wait(&v_ready[j % L::STAGES], (j / L::STAGES) & 1, abort_flag, p.err, DEV_TIMEOUT_FULL)) { ok = false; break; }
-                    const volatile uint32_t * bad = words + 2 + 2 * (j % L::STAGES);
-                    poison |= (bad[0] & vis[0]) != 0 || (bad[1] & vis[1]) != 0;
-                }
-                tc_fence_before();
-                __syncwarp();
-                if (lane == 0) mbar_arrive(&p_full[x]);
+            };
+            if (nt > 0) {
+                if (mask) fetch_mask(0);
+                ok = arrived(0);
+                const int clear = mask ? 0 : min(nt, max(0, least / KEYS - t0));   // tiles that every row sees whole
+                tiles(std::false_type(), 0, clear);
+                tiles(std::true_type(), clear, nt);
             }
             if (poison) l = NAN;
-            if (ok && nt > 0) ok = mbar_wait(&o_full[m * BUF], 0, abort_flag, p.err, DEV_TIMEOUT_TMEM);
+            if (ok && nt > 0) ok = mbar_wait_soon(&o_full[m * BUF], 0, abort_flag, p.err, DEV_TIMEOUT_TMEM);
             __syncwarp();
             tc_fence_after();
         }
@@ -716,7 +767,7 @@ diff_attn_rows(const __grid_constant__ CUtensorMap tk, const __grid_constant__ C
         const int base = (s0 + warp + i * W) * SLAB;
         uint32_t there = low_bits(n - base) & 0xffffu;   // the keys that exist
         if (mask) there = __ballot_sync(~0u, lane < SLAB && base + lane < n && mask[base + lane] != 0);
-        if (!mbar_wait(&full[i % RING], (i / RING) & 1, flags, p.err, DEV_TIMEOUT_FULL)) break;
+        if (!mbar_wait_soon(&full[i % RING], (i / RING) & 1, flags, p.err, DEV_TIMEOUT_FULL)) break;
         __syncwarp();
         const uint32_t kt = smem_u32(ring + (i % RING) * L::STAGE), vt = kt + L::HALF;
         float s[2][2][4];

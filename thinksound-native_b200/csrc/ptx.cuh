@@ -65,6 +65,14 @@ __device__ __forceinline__ bool mbar_wait(uint64_t * bar, uint32_t parity, volat
         }
     }
 }
+// The same for waits that are usually short but not over: tries (each may sleep a little in hardware) before the clock
+// is read for the bound. Reading the global timer takes about as long as such a wait.
+__device__ __forceinline__ bool mbar_wait_soon(uint64_t * bar, uint32_t parity, volatile int * abort_flag, int * err, int code) {
+#pragma unroll 1
+    for (int i = 0; i < 256; ++i)
+        if (mbar_try_wait(bar, parity)) return true;
+    return mbar_wait(bar, parity, abort_flag, err, code);
+}
 
 // ---------------------------------------------------------------- TMA (no multicast)
 __device__ __forceinline__ void tma_prefetch(const CUtensorMap * m) {
