@@ -40,19 +40,24 @@ def _want(name, t, shape, dtype):
 
 
 def _put(view, name, t):
-    """Address and strides of a [., ., C] or [., ., ., C] tensor whose last dimension is contiguous."""
+    """Strides of a [., ., C] or [., ., ., C] tensor whose last dimension is contiguous."""
     st = t.stride()
     if st[-1] != 1 and t.shape[-1] > 1:
         raise ValueError(f"{name}: the last dimension must be contiguous")
     if not t.is_cuda:
         raise ValueError(f"{name} must be a CUDA tensor")
-    view.p = t.data_ptr()
     view.sb = st[0]
     if len(st) == 3:
         view.st = st[1]
     else:
         view.ss = st[1]
         view.sh = st[2]
+
+
+def _form(*tensors):
+    """What a call's checks go by: shape, strides, type and place of each tensor. A call of the same form as the
+    one before needs only its addresses set; the checks, several microseconds of Python, are those of a new form."""
+    return [None if t is None else (t.shape, t.stride(), t.dtype, t.is_cuda) for t in tensors]
 
 
 class BlockNorm:
@@ -76,12 +81,26 @@ class BlockNorm:
         a.C, a.post, a.pre, a.gate_tanh = C_, NORMS[post], NORMS[pre], int(gate_tanh)
         a.post_eps, a.pre_eps, a.res_scale = post_eps, pre_eps, 1.0 if vec is not None else residual_scale
         a.post_w, a.post_b, a.pre_w, a.pre_b, a.res_vec = (_address(t) for t in self._keep)
-        self._a, self._ref = a, C.byref(a)
+        self._a, self._ref, self._form, self._call = a, C.byref(a), None, lib().tsn_block_norm
+        self._views = a.x, a.y, a.gate, a.shift, a.scale, a.x_out, a.h
 
     def __call__(self, x, y=None, gate=None, shift=None, scale=None, x_out=None, h=None):
         """x, x_out [B, T, C] of the residual's type; y, h [B, T, C] of the branch's type, which is the residual's or
         narrower than its float32; gate, shift, scale [B or 1, T or 1, C] of the branch's type, each or None.
         x_out may be x and h may be y."""
+        tensors = (x, y, gate, shift, scale, x_out, h)
+        form = _form(*tensors)
+        if form != self._form:
+            self._form = None
+            self._check(*tensors)
+            self._form = form
+        for view, t in zip(self._views, tensors):
+            view.p = None if t is None else t.data_ptr()
+        rc = self._call(self.dev.h, self._ref)
+        if rc:
+            check(rc)
+
+    def _check(self, x, y, gate, shift, scale, x_out, h):
         a = self._a
         shape = x.shape
         if len(shape) != 3 or shape[2] != self.C:
@@ -93,28 +112,23 @@ class BlockNorm:
         a.B, a.T, a.xtype, a.type = shape[0], shape[1], TYPES[x.dtype], TYPES[dtype]
         _put(a.x, "x", x)
         for name, t, of in (("y", y, dtype), ("x_out", x_out, x.dtype), ("h", h, dtype)):
-            view = getattr(a, name)
-            if t is None:
-                view.p = None
-            else:
+            if t is not None:
                 _want(name, t, shape, of)
-                _put(view, name, t)
+                _put(getattr(a, name), name, t)
         for name, t in (("gate", gate), ("shift", shift), ("scale", scale)):
-            view = getattr(a, name)
             if t is None:
-                view.p = None
                 continue
             if t.dtype is not dtype:
                 raise TypeError(f"{name} is {t.dtype}, expected {dtype}")
             ts = t.shape
             if len(ts) != 3 or ts[2] != self.C or ts[0] not in (1, shape[0]) or ts[1] not in (1, shape[1]):
                 raise ValueError(f"{name} must be [B or 1, T or 1, {self.C}], got {tuple(ts)}")
+            view = getattr(a, name)
             _put(view, name, t)
             if ts[0] == 1:
                 view.sb = 0
             if ts[1] == 1:
                 view.st = 0
-        check(lib().tsn_block_norm(self.dev.h, self._ref))
 
 
 class RopeAxes:
@@ -141,44 +155,62 @@ class RopeAxes:
         a = RopeArgs()
         a.eps = eps
         a.q_norm, a.k_norm = (_address(t) for t in self._keep)
-        self._a, self._ref, self._plan_ref = a, C.byref(a), C.byref(self._plan)
+        self._a, self._ref, self._plan_ref, self._form = a, C.byref(a), C.byref(self._plan), None
+        self._call = lib().tsn_rope_axes
+        self._views = a.q, a.k, a.q_out, a.k_out
 
     def __call__(self, q, k, pos, q_out=None, k_out=None):
         """q [B, S, Hq, head_dim] and k [B, S, Hk, head_dim], either may be None; pos int32 [S, axes] or [B, S, axes].
         Results into q_out and k_out, or in place where those are None."""
+        if q_out is None:
+            q_out = q
+        if k_out is None:
+            k_out = k
+        tensors = (q, k, q_out, k_out)
+        form = _form(q, k, q_out, k_out, pos)
+        if form != self._form:
+            self._form = None
+            self._check(q, k, pos, q_out, k_out)
+            self._form = form
+        for view, t in zip(self._views, tensors):
+            view.p = None if t is None else t.data_ptr()
+        self._a.pos = pos.data_ptr()
+        rc = self._call(self.dev.h, self._plan_ref, self._ref)
+        if rc:
+            check(rc)
+
+    def _check(self, q, k, pos, q_out, k_out):
         a = self._a
         first = q if q is not None else k
+        if first is None or first.dim() != 4:
+            raise ValueError("q or k is wanted, [B, S, heads, head_dim]")
         B, S = first.shape[0], first.shape[1]
         dtype = first.dtype
         if dtype not in TYPES:
             raise TypeError("float32, float16 or bfloat16 tensors are wanted")
         a.B, a.S, a.type = B, S, TYPES[dtype]
         for name, t, out in (("q", q, q_out), ("k", k, k_out)):
-            view, res = getattr(a, name), getattr(a, name + "_out")
             if t is None:
-                view.p = res.p = None
                 continue
+            if t.dim() != 4:
+                raise ValueError(f"{name} must be [B, S, heads, head_dim]")
             H = t.shape[2]
             _want(name, t, (B, S, H, self.D), dtype)
-            _put(view, name, t)
+            _want(name + "_out", out, t.shape, dtype)
+            _put(getattr(a, name), name, t)
+            _put(getattr(a, name + "_out"), name + "_out", out)
             if name == "q":
                 a.Hq = H
             else:
                 a.Hk = H
-            if out is None:
-                out = t
-            else:
-                _want(name + "_out", out, t.shape, dtype)
-            _put(res, name + "_out", out)
         ps = pos.shape
         if pos.dtype is not torch.int32 or ps[-2:] != (S, self.axes) or (len(ps) == 3 and ps[0] not in (1, B)) or len(ps) > 3:
             raise ValueError(f"pos must be int32 [S, {self.axes}] or [B, S, {self.axes}]")
         st = pos.stride()
         if not pos.is_cuda or (st[-1] != 1 and self.axes > 1):
             raise ValueError("pos must be a CUDA tensor whose last dimension is contiguous")
-        a.pos, a.pos_ss = pos.data_ptr(), st[-2]
+        a.pos_ss = st[-2]
         a.pos_sb = st[0] if len(ps) == 3 and ps[0] > 1 else 0
-        check(lib().tsn_rope_axes(self.dev.h, self._plan_ref, self._ref))
 
 
 class DiffAttention:
@@ -200,13 +232,33 @@ class DiffAttention:
         a.d, a.lambda_init, a.eps, a.scale = d, lambda_init, eps, 0.0 if scale is None else scale
         a.lq1, a.lk1, a.lq2, a.lk2, a.norm_w = (_address(t) for t in self._keep)
         a.lam_sh = d if self.heads else 0
-        self._a, self._ref = a, C.byref(a)
+        self._a, self._ref, self._form, self._call = a, C.byref(a), None, lib().tsn_diff_attn
+        self._views = a.q, a.k, a.v, a.out
 
     def __call__(self, q, k, v, out, key_len=None, key_mask=None, causal: bool = False):
         """q, out [B, Sq, H, 2 d], k, v [B, Sk, Hk, 2 d], all float16 or bfloat16. key_len: int32 [B], the keys each
         sequence has; key_mask: uint8 or bool [B or 1, Sk], nonzero where a key is seen; causal: counted from the
         end, the last query sees the last key."""
         a = self._a
+        tensors = (q, k, v, out)
+        form = _form(q, k, v, out, key_len, key_mask)
+        if form != self._form:
+            self._form = None
+            self._check(q, k, v, out, key_len, key_mask)
+            self._form = form
+        for view, t in zip(self._views, tensors):
+            view.p = t.data_ptr()
+        a.key_len = None if key_len is None else key_len.data_ptr()
+        a.key_mask = None if key_mask is None else key_mask.data_ptr()
+        a.causal = 1 if causal else 0
+        rc = self._call(self.dev.h, self._ref)
+        if rc:
+            check(rc)
+
+    def _check(self, q, k, v, out, key_len, key_mask):
+        a = self._a
+        if q.dim() != 4 or k.dim() != 4:
+            raise ValueError("q and k must be [B, S, heads, 2 d]")
         B, Sq, H, D = q.shape
         Sk, Hk = k.shape[1], k.shape[2]
         dtype = q.dtype
@@ -219,24 +271,16 @@ class DiffAttention:
         _want("k", k, (B, Sk, Hk, D), dtype)
         _want("v", v, (B, Sk, Hk, D), dtype)
         _want("out", out, q.shape, dtype)
-        a.B, a.Sq, a.Sk, a.H, a.Hk, a.type, a.causal = B, Sq, Sk, H, Hk, TYPES[dtype], int(causal)
-        _put(a.q, "q", q)
-        _put(a.k, "k", k)
-        _put(a.v, "v", v)
-        _put(a.out, "out", out)
-        if key_len is None:
-            a.key_len = None
-        else:
-            if key_len.dtype is not torch.int32 or tuple(key_len.shape) != (B,) or not key_len.is_cuda or not key_len.is_contiguous():
-                raise ValueError("key_len must be a contiguous int32 CUDA tensor of shape [B]")
-            a.key_len = key_len.data_ptr()
-        if key_mask is None:
-            a.key_mask = None
-        else:
-            if key_mask.dtype not in (torch.uint8, torch.bool) or key_mask.shape[1:] != (Sk,) or key_mask.shape[0] not in (1, B):
+        a.B, a.Sq, a.Sk, a.H, a.Hk, a.type = B, Sq, Sk, H, Hk, TYPES[dtype]
+        for name, t in (("q", q), ("k", k), ("v", v), ("out", out)):
+            _put(getattr(a, name), name, t)
+        if key_len is not None and (key_len.dtype is not torch.int32 or tuple(key_len.shape) != (B,) or not key_len.is_cuda
+                                    or not key_len.is_contiguous()):
+            raise ValueError("key_len must be a contiguous int32 CUDA tensor of shape [B]")
+        if key_mask is not None:
+            ms = key_mask.shape
+            if key_mask.dtype not in (torch.uint8, torch.bool) or len(ms) != 2 or ms[1] != Sk or ms[0] not in (1, B):
                 raise ValueError("key_mask must be uint8 or bool [B or 1, Sk]")
             if not key_mask.is_cuda or (key_mask.stride(1) != 1 and Sk > 1):
                 raise ValueError("key_mask must be a CUDA tensor whose last dimension is contiguous")
-            a.key_mask = key_mask.data_ptr()
-            a.mask_sb = key_mask.stride(0) if key_mask.shape[0] > 1 else 0
-        check(lib().tsn_diff_attn(self.dev.h, self._ref))
+            a.mask_sb = key_mask.stride(0) if ms[0] > 1 else 0
