@@ -632,20 +632,22 @@ diff_attn_tc(const __grid_constant__ CUtensorMap tk, const __grid_constant__ CUt
 
 // ================================================================ few rows
 // diff_attn_rows: a few rows of a kv head (one token with its group's heads, or a few), bound by reading K and V.
-// A 128-row tile would spend its time on rows that do not exist; here mma.sync takes 16 rows (m16n8k16), which
-// is far from being the limit: 48 products for 16 keys of 8 KB.
+// A 128-row tile would spend its time on rows that do not exist; here mma.sync takes 8 rows, with the keys (and for
+// the product with V the columns) on its 16-row side: S^T = K Q^T, O^T = V^T P^T, 24 products for 16 keys of 8 KB.
+// P^T is S^T's layout transposed in registers (movmatrix). With the rows on the 16-row side, half of it empty, twice
+// the products and exponentials made one token over four caches of 32 768 keys take 97 us.
 // Each warp streams its own 16-key slabs (slab w, w + W, ...) by TMA through a ring of its own, so warps never wait
 // for one another: scores, online softmax and O of both maps stay in the warp's registers. The warps' sums
 // are added up in shared memory at the end, the parts of split keys through the workspace.
-constexpr int SLAB = 16, RING = 3;
-constexpr int FEW = 64;   // rows up to which groups of 16 beat a tile of 128
+constexpr int SLAB = 16, RING = 3, SOME = 8;   // keys of a slab, slabs of a ring, rows of a group
+constexpr int FEW = 32;                        // rows up to which groups of 8 beat a tile of 128
 
 template <int D, int W>
 struct RowLay {
     static constexpr int BOX = SLAB * 128, HALF = SLAB * D * 2, STAGE = 2 * HALF;   // a slab's keys, then its values
     static constexpr int OFF_LAM = W * RING * STAGE, OFF_W = OFF_LAM + 16 * 4, OFF_BAR = OFF_W + D * 4;
     static constexpr int TOTAL = OFF_BAR + W * RING * 8 + 16;
-    static constexpr int SUMS = 16 * row_words(D);   // after the last slab, in a warp's ring
+    static constexpr int SUMS = SOME * row_words(D);   // after the last slab, in a warp's ring
     static_assert(W * SUMS * 4 <= W * RING * STAGE, "the warps' sums fit in their rings");
 };
 
@@ -657,6 +659,12 @@ __device__ __forceinline__ void mma16816(float (&c)[4], const uint32_t (&a)[4], 
     else
         asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+// the 8 x 8 matrix of 16-bit elements that the warp holds, transposed
+__device__ __forceinline__ uint32_t movmatrix(uint32_t a) {
+    uint32_t d;
+    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(d) : "r"(a));
+    return d;
 }
 template <bool TRANS>
 __device__ __forceinline__ void ldmatrix4(uint32_t (&r)[4], uint32_t at) {
@@ -682,11 +690,12 @@ diff_attn_rows(const __grid_constant__ CUtensorMap tk, const __grid_constant__ C
     uint64_t * full = (uint64_t *) (smem + L::OFF_BAR) + warp * RING;
     volatile int * flags = (volatile int *) (smem + L::OFF_BAR + W * RING * 8);   // abort, last to arrive
 
-    // groups of 16 rows next to one another read the same keys at about the same time
-    const int sixteens = (int) (p.R + 15) / 16;
-    const unsigned gid = blockIdx.x / (sixteens * p.splits) * sixteens + blockIdx.x % sixteens, split = blockIdx.x / sixteens % p.splits;
-    const int hk = (int) (gid / sixteens % a.Hk), b = (int) (gid / sixteens / a.Hk);
-    const int first = (int) (gid % sixteens) * 16, R = min(16, (int) p.R - first);   // row r: token (first + r) / G, head (first + r) % G
+    // All groups of a part lie next to one another: the groups of 8 rows of a kv head read the same keys at about the same
+    // time, and the kv heads neighbouring ones (a head's row is 256 bytes, too little for DRAM by itself).
+    const int eights = (int) (p.R + SOME - 1) / SOME;
+    const unsigned groups = gridDim.x / p.splits, gid = blockIdx.x % groups, split = blockIdx.x / groups;
+    const int hk = (int) (gid / eights % a.Hk), b = (int) (gid / eights / a.Hk);
+    const int first = (int) (gid % eights) * SOME, R = min(SOME, (int) p.R - first);   // row r: token (first + r) / G, head (first + r) % G
     const int n = a.key_len ? max(0, min(a.key_len[b], (int) a.Sk)) : (int) a.Sk;
     auto limit = [&](int r) {   // keys before which row r sees; rows past the last one see all
         if (!a.causal || r >= R) return n;
@@ -730,60 +739,60 @@ diff_attn_rows(const __grid_constant__ CUtensorMap tk, const __grid_constant__ C
     }
     for (int e = tid; e < D; e += 32 * W) nw[e] = (a.norm_w ? a.norm_w[e] : 1.0f) * (1.0f - a.lambda_init);
 
-    // Q as A operands: rows lane / 4 and lane / 4 + 8, rows past the last one as zeros
-    const int r0 = lane >> 2, c0 = (lane & 3) * 2;
-    uint32_t qa[2][d / 16][4];
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-        const int r = r0 + 8 * h;
-        const uint16_t * q = (const uint16_t *) a.q.p + b * a.q.sb + (long long) ((first + r) / p.G) * a.q.ss + (long long) (hk * p.G + (first + r) % p.G) * a.q.sh;
+    // Q^T as B operands: row lane / 4, rows past the last one as zeros. Scores: keys lane / 4 (+ 8) by rows c0, c0 + 1.
+    const int g0 = lane >> 2, c0 = (lane & 3) * 2;
+    uint32_t qb[2][d / 16][2];
+    {
+        const int u = first + g0;
+        const uint16_t * q = (const uint16_t *) a.q.p + b * a.q.sb + (long long) (u / p.G) * a.q.ss + (long long) (hk * p.G + u % p.G) * a.q.sh;
 #pragma unroll
         for (int m = 0; m < 2; ++m)
 #pragma unroll
-            for (int k = 0; k < d / 16; ++k) {
-                qa[m][k][h] = r < R ? *(const uint32_t *) (q + m * d + 16 * k + c0) : 0u;
-                qa[m][k][2 + h] = r < R ? *(const uint32_t *) (q + m * d + 16 * k + c0 + 8) : 0u;
-            }
+            for (int k = 0; k < d / 16; ++k)
+#pragma unroll
+                for (int h = 0; h < 2; ++h) qb[m][k][h] = g0 < R ? *(const uint32_t *) (q + m * d + 16 * k + 8 * h + c0) : 0u;
     }
-    const int lim[2] = {limit(r0), limit(r0 + 8)};
+    const int lim[2] = {limit(c0), limit(c0 + 1)};
     const uint8_t * mask = a.key_mask ? a.key_mask + b * a.mask_sb : nullptr;
     __syncthreads();   // the abort flag, lambda and the weights are set
 
-    float o[2][D / 8][4], l[2][2] = {}, ref[2][2];
+    float o[2][D / 16][4], l[2][2] = {}, ref[2][2];   // O^T: columns 16 x + lane / 4 (+ 8) by rows c0, c0 + 1
 #pragma unroll
     for (int m = 0; m < 2; ++m) {
         ref[m][0] = ref[m][1] = -INFINITY;
 #pragma unroll
-        for (int x = 0; x < D / 8; ++x)
+        for (int x = 0; x < D / 16; ++x)
 #pragma unroll
             for (int k = 0; k < 4; ++k) o[m][x][k] = 0.0f;
     }
     bool poison[2] = {false, false};
-    // addresses of ldmatrix: K rows (key) with the two 8-element halves of a k step side by side, V rows (key)
-    // with two groups of 8 columns
-    const int krow = (lane & 7) + ((lane >> 4) << 3), kch = (lane >> 3) & 1;
-    const int vrow = (lane & 7) + (((lane >> 3) & 1) << 3), vch = lane >> 4;
+    // addresses of ldmatrix: K rows (key), two groups of 8 keys by two of 8 elements; V rows (key), two groups of 8 columns
+    // by two of 8 keys
+    const int krow = (lane & 7) + (((lane >> 3) & 1) << 3), kch = lane >> 4;
+    const int vrow = (lane & 7) + ((lane >> 4) << 3), vch = (lane >> 3) & 1;
+    uint32_t mb = mask && mine > 0 && lane < SLAB && (s0 + warp) * SLAB + lane < n ? mask[(s0 + warp) * SLAB + lane] : 0u;
     for (int i = 0; i < mine; ++i) {
         const int base = (s0 + warp + i * W) * SLAB;
         uint32_t there = low_bits(n - base) & 0xffffu;   // the keys that exist
-        if (mask) there = __ballot_sync(~0u, lane < SLAB && base + lane < n && mask[base + lane] != 0);
+        if (mask) {
+            there = __ballot_sync(~0u, mb != 0);
+            const int key = base + W * SLAB + lane;
+            mb = lane < SLAB && key < n ? mask[key] : 0u;
+        }
         if (!mbar_wait_soon(&full[i % RING], (i / RING) & 1, flags, p.err, DEV_TIMEOUT_FULL)) break;
         __syncwarp();
         const uint32_t kt = smem_u32(ring + (i % RING) * L::STAGE), vt = kt + L::HALF;
-        float s[2][2][4];
+        float s[2][4];
 #pragma unroll
         for (int m = 0; m < 2; ++m) {
 #pragma unroll
-            for (int x = 0; x < 2; ++x)
-#pragma unroll
-                for (int k = 0; k < 4; ++k) s[m][x][k] = 0.0f;
+            for (int k = 0; k < 4; ++k) s[m][k] = 0.0f;
 #pragma unroll
             for (int k = 0; k < d / 16; ++k) {
                 const int col = m * d + 16 * k;
                 uint32_t f[4];
                 ldmatrix4<false>(f, kt + (col / 64) * L::BOX + krow * 128 + ((((col % 64) / 8 + kch) ^ (krow & 7)) << 4));
-                mma16816<BF16>(s[m][0], qa[m][k], f[0], f[1]);
-                mma16816<BF16>(s[m][1], qa[m][k], f[2], f[3]);
+                mma16816<BF16>(s[m], f, qb[m][k][0], qb[m][k][1]);
             }
         }
         const bool gone = there != 0xffffu, mixed = a.causal && least < min(n, base + SLAB);
@@ -794,10 +803,8 @@ diff_attn_rows(const __grid_constant__ CUtensorMap tk, const __grid_constant__ C
 #pragma unroll
             for (int m = 0; m < 2; ++m)
 #pragma unroll
-                for (int x = 0; x < 2; ++x)
-#pragma unroll
-                    for (int k = 0; k < 4; ++k)
-                        if (!((vis[k >> 1] >> (8 * x + c0 + (k & 1))) & 1u)) s[m][x][k] = -INFINITY;
+                for (int k = 0; k < 4; ++k)
+                    if (!((vis[k & 1] >> (g0 + 8 * (k >> 1))) & 1u)) s[m][k] = -INFINITY;
         }
         bool move = false;
         float top[2][2];
@@ -805,7 +812,7 @@ diff_attn_rows(const __grid_constant__ CUtensorMap tk, const __grid_constant__ C
         for (int m = 0; m < 2; ++m)
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
-                top[m][h] = fmaxf(fmaxf(s[m][0][2 * h], s[m][0][2 * h + 1]), fmaxf(s[m][1][2 * h], s[m][1][2 * h + 1])) * p.c;
+                top[m][h] = fmaxf(s[m][h], s[m][2 + h]) * p.c;
                 move |= top[m][h] > ref[m][h] + LAZY;
             }
         if (__any_sync(~0u, move)) {
@@ -813,30 +820,28 @@ diff_attn_rows(const __grid_constant__ CUtensorMap tk, const __grid_constant__ C
             for (int m = 0; m < 2; ++m)
 #pragma unroll
                 for (int h = 0; h < 2; ++h) {
-                    float t = fmaxf(top[m][h], __shfl_xor_sync(~0u, top[m][h], 1));
-                    t = fmaxf(t, __shfl_xor_sync(~0u, t, 2));
+                    float t = top[m][h];
+#pragma unroll
+                    for (int x = 4; x < 32; x <<= 1) t = fmaxf(t, __shfl_xor_sync(~0u, t, x));
                     if (t > ref[m][h] + LAZY) {   // a row moves its reference by itself
                         const float f = ex2(ref[m][h] - t);
                         ref[m][h] = t;
                         l[m][h] *= f;
 #pragma unroll
-                        for (int x = 0; x < D / 8; ++x) { o[m][x][2 * h] *= f; o[m][x][2 * h + 1] *= f; }
+                        for (int x = 0; x < D / 16; ++x) { o[m][x][h] *= f; o[m][x][2 + h] *= f; }
                     }
                 }
         }
-        uint32_t pa[2][4];
+        uint32_t pb[2][2];
 #pragma unroll
         for (int m = 0; m < 2; ++m) {
             const float n0 = ref[m][0] == -INFINITY ? 0.0f : -ref[m][0], n1 = ref[m][1] == -INFINITY ? 0.0f : -ref[m][1];
-#pragma unroll
-            for (int x = 0; x < 2; ++x) {
-                const float e0 = ex2(fmaf(s[m][x][0], p.c, n0)), e1 = ex2(fmaf(s[m][x][1], p.c, n0));
-                const float e2 = ex2(fmaf(s[m][x][2], p.c, n1)), e3 = ex2(fmaf(s[m][x][3], p.c, n1));
-                l[m][0] += e0 + e1;
-                l[m][1] += e2 + e3;
-                pa[m][2 * x] = pack16<BF16>(e0, e1);
-                pa[m][2 * x + 1] = pack16<BF16>(e2, e3);
-            }
+            const float e0 = ex2(fmaf(s[m][0], p.c, n0)), e1 = ex2(fmaf(s[m][1], p.c, n1));
+            const float e2 = ex2(fmaf(s[m][2], p.c, n0)), e3 = ex2(fmaf(s[m][3], p.c, n1));
+            l[m][0] += e0 + e2;
+            l[m][1] += e1 + e3;
+            pb[m][0] = movmatrix(pack16<BF16>(e0, e1));
+            pb[m][1] = movmatrix(pack16<BF16>(e2, e3));
         }
         if (!gone && !mixed) {
 #pragma unroll
@@ -844,35 +849,29 @@ diff_attn_rows(const __grid_constant__ CUtensorMap tk, const __grid_constant__ C
                 uint32_t f[4];
                 ldmatrix4<true>(f, vt + (x / 4) * L::BOX + vrow * 128 + (((2 * (x % 4) + vch) ^ (vrow & 7)) << 4));
 #pragma unroll
-                for (int m = 0; m < 2; ++m) {
-                    mma16816<BF16>(o[m][2 * x], pa[m], f[0], f[1]);
-                    mma16816<BF16>(o[m][2 * x + 1], pa[m], f[2], f[3]);
-                }
+                for (int m = 0; m < 2; ++m) mma16816<BF16>(o[m][x], f, pb[m][0], pb[m][1]);
             }
         } else {
             // values behind masked keys count as zero; where rows differ, so do non-finite ones, and rows that see one are marked
             const auto word = [](uint32_t two) { return (two & 1u ? 0xffffu : 0u) | (two & 2u ? 0xffff0000u : 0u); };
-            const uint32_t keep0 = word(there >> c0), keep1 = word(there >> (c0 + 8));
+            const uint32_t keep[2] = {word(there >> c0), word(there >> (c0 + 8))};
             uint32_t bad = 0;
 #pragma unroll
             for (int x = 0; x < D / 16; ++x) {
                 uint32_t f[4];
                 ldmatrix4<true>(f, vt + (x / 4) * L::BOX + vrow * 128 + (((2 * (x % 4) + vch) ^ (vrow & 7)) << 4));
-                f[0] &= keep0; f[1] &= keep1; f[2] &= keep0; f[3] &= keep1;
-                if (mixed) {
 #pragma unroll
-                    for (int y = 0; y < 4; ++y) {
+                for (int y = 0; y < 4; ++y) {
+                    f[y] &= keep[y >> 1];
+                    if (mixed) {
                         const uint32_t g = finite_only<BF16>(f[y]), diff = f[y] ^ g;
-                        if (diff & 0xffffu) bad |= 1u << (c0 + 8 * (y & 1));
-                        if (diff >> 16) bad |= 2u << (c0 + 8 * (y & 1));
+                        if (diff & 0xffffu) bad |= 1u << (c0 + 8 * (y >> 1));
+                        if (diff >> 16) bad |= 2u << (c0 + 8 * (y >> 1));
                         f[y] = g;
                     }
                 }
 #pragma unroll
-                for (int m = 0; m < 2; ++m) {
-                    mma16816<BF16>(o[m][2 * x], pa[m], f[0], f[1]);
-                    mma16816<BF16>(o[m][2 * x + 1], pa[m], f[2], f[3]);
-                }
+                for (int m = 0; m < 2; ++m) mma16816<BF16>(o[m][x], f, pb[m][0], pb[m][1]);
             }
             bad = __reduce_or_sync(~0u, bad);
             poison[0] |= (bad & vis[0]) != 0;
@@ -885,26 +884,26 @@ diff_attn_rows(const __grid_constant__ CUtensorMap tk, const __grid_constant__ C
     // the warp's sums in its ring, then warp w adds up rows w, w + W, ... of all warps
     float * sums = (float *) ring;
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-        const int r = r0 + 8 * h;
+    for (int h = 0; h < 2; ++h)
 #pragma unroll
         for (int m = 0; m < 2; ++m) {
             float t = l[m][h];
-            t += __shfl_xor_sync(~0u, t, 1);
-            t += __shfl_xor_sync(~0u, t, 2);
-            float * to = sums + r * row_words(D);
-            if ((lane & 3) == 0) {
+#pragma unroll
+            for (int x = 4; x < 32; x <<= 1) t += __shfl_xor_sync(~0u, t, x);
+            float * to = sums + (c0 + h) * row_words(D);
+            if (g0 == 0) {
                 to[2 * D + m] = ref[m][h];
                 to[2 * D + 2 + m] = poison[h] ? NAN : t;
             }
-            if (r < R)
 #pragma unroll
-                for (int x = 0; x < D / 8; ++x) *(float2 *) (to + m * D + 8 * x + c0) = make_float2(o[m][x][2 * h], o[m][x][2 * h + 1]);
+            for (int x = 0; x < D / 16; ++x) {
+                to[m * D + 16 * x + g0] = o[m][x][h];
+                to[m * D + 16 * x + g0 + 8] = o[m][x][2 + h];
+            }
         }
-    }
     __syncthreads();
     const size_t size = (size_t) R * row_words(D);   // of a part
-    float * part = p.part + (size_t) gid * p.splits * (16 * row_words(D));
+    float * part = p.part + (size_t) gid * p.splits * (SOME * row_words(D));
     for (int r = warp; r < R && !flags[0]; r += W) {
         float sum[2][E], top[2], rl[2];
         auto at = [&](int i, int k) { return (const float *) (smem + i * RING * L::STAGE) + r * row_words(D) + k; };
@@ -1078,7 +1077,7 @@ int diff_attn(DeviceCtx & c, const tsn_diff_attn_args & in) {
     p.R = (long long) a.Sq * p.G;
     p.err = c.d_err;
     const bool rows = p.R <= FEW;
-    const long long groups = (rows ? (p.R + 15) / 16 : (p.R + ROWS - 1) / ROWS) * a.B * a.Hk;
+    const long long groups = (rows ? (p.R + SOME - 1) / SOME : (p.R + ROWS - 1) / ROWS) * a.B * a.Hk;
     int warps = 8;
     if (rows) {
         // Parts of 512 keys (four slabs for each of eight warps) while that is at most one CTA per SM, and none up to
@@ -1091,7 +1090,7 @@ int diff_attn(DeviceCtx & c, const tsn_diff_attn_args & in) {
             warps = 4;
             parts = std::min(parts, std::max(1ll, 8 * SMS / groups));
         }
-        parts = std::min({parts, 64ll, std::max(1ll, (long long) (WORKSPACE - COUNTERS * 4) / (groups * 16 * (4 * a.d + 4) * 4))});
+        parts = std::min({parts, 64ll, std::max(1ll, (long long) (WORKSPACE - COUNTERS * 4) / (groups * SOME * (4 * a.d + 4) * 4))});
         if (groups > (long long) COUNTERS) parts = 1;
         p.chunk = (int) std::max(1ll, (slabs + parts - 1) / parts);
         p.splits = (int) std::max(1ll, (slabs + p.chunk - 1) / p.chunk);
