@@ -125,32 +125,46 @@ __device__ __forceinline__ void read_words(const float * at, float * v) {
     }
 }
 
-// Adds up `count` sets of a row's sums, one warp: rd(i, k) is word k of set i, rdv(i, k, v) D / 32 words from k on.
-// Returns O (this lane's D / 32 columns), ref and l. The order is that of the sets.
+// Adds up `count` (1 to 64) sets of a row's sums, one warp: rd(i, k) is word k of set i, rdv(i, k, v) D / 32 words from k
+// on. Returns O (this lane's D / 32 columns), ref and l. The order is that of the sets. Eight sets are read at once.
 template <int D, class Rd, class RdV>
 __device__ __forceinline__ void add_up(int count, int lane, float (&sum)[2][D / 32], float (&top)[2], float (&l)[2], Rd rd, RdV rdv) {
     constexpr int E = D / 32;
+    const bool one = lane < count, two = lane + 32 < count;
+    float w[2][2];   // the factors of sets lane and lane + 32
 #pragma unroll
     for (int m = 0; m < 2; ++m) {
-        top[m] = -INFINITY;
-        l[m] = 0.0f;
-        for (int i = lane; i < count; i += 32) top[m] = fmaxf(top[m], rd(i, 2 * D + m));
+        const float r1 = one ? rd(lane, 2 * D + m) : -INFINITY, r2 = two ? rd(lane + 32, 2 * D + m) : -INFINITY;
+        const float l1 = one ? rd(lane, 2 * D + 2 + m) : 0.0f, l2 = two ? rd(lane + 32, 2 * D + 2 + m) : 0.0f;
+        top[m] = fmaxf(r1, r2);
 #pragma unroll
         for (int x = 16; x; x >>= 1) top[m] = fmaxf(top[m], __shfl_xor_sync(~0u, top[m], x));
         const float ref = top[m] == -INFINITY ? 0.0f : top[m];
-        for (int i = lane; i < count; i += 32) l[m] += ex2(rd(i, 2 * D + m) - ref) * rd(i, 2 * D + 2 + m);
+        w[m][0] = ex2(r1 - ref);
+        w[m][1] = ex2(r2 - ref);
+        l[m] = w[m][0] * l1 + w[m][1] * l2;
 #pragma unroll
         for (int x = 16; x; x >>= 1) l[m] += __shfl_xor_sync(~0u, l[m], x);
 #pragma unroll
         for (int e = 0; e < E; ++e) sum[m][e] = 0.0f;
-#pragma unroll 8
-        for (int i = 0; i < count; ++i) {
-            const float f = ex2(rd(i, 2 * D + m) - ref);
-            float v[4];
-            rdv(i, m * D + E * lane, v);
+    }
+#pragma unroll 1
+    for (int i = 0; i < count; i += 8) {
+        float v[2][8][4];
 #pragma unroll
-            for (int e = 0; e < E; ++e) sum[m][e] = fmaf(f, v[e], sum[m][e]);
-        }
+        for (int m = 0; m < 2; ++m)
+#pragma unroll
+            for (int k = 0; k < 8; ++k)
+                if (i + k < count) rdv(i + k, m * D + E * lane, v[m][k]);
+#pragma unroll
+        for (int m = 0; m < 2; ++m)
+#pragma unroll
+            for (int k = 0; k < 8; ++k) {
+                const float f = __shfl_sync(~0u, i < 32 ? w[m][0] : w[m][1], (i + k) & 31);
+                if (i + k < count)
+#pragma unroll
+                    for (int e = 0; e < E; ++e) sum[m][e] = fmaf(f, v[m][k][e], sum[m][e]);
+            }
     }
 }
 
@@ -639,10 +653,10 @@ diff_attn_tc(const __grid_constant__ CUtensorMap tk, const __grid_constant__ CUt
 // Each warp streams its own 16-key slabs (slab w, w + W, ...) by TMA through a ring of its own, so warps never wait
 // for one another: scores, online softmax and O of both maps stay in the warp's registers. The warps' sums
 // are added up in shared memory at the end, the parts of split keys through the workspace.
-constexpr int SLAB = 16, RING = 3, SOME = 8;   // keys of a slab, slabs of a ring, rows of a group
+constexpr int SLAB = 16, RING = 3, SOME = 8, W = 8;   // keys of a slab, slabs of a ring, rows of a group, warps
 constexpr int FEW = 32;                        // rows up to which groups of 8 beat a tile of 128
 
-template <int D, int W>
+template <int D>
 struct RowLay {
     static constexpr int BOX = SLAB * 128, HALF = SLAB * D * 2, STAGE = 2 * HALF;   // a slab's keys, then its values
     static constexpr int OFF_LAM = W * RING * STAGE, OFF_W = OFF_LAM + 16 * 4, OFF_BAR = OFF_W + D * 4;
@@ -674,10 +688,10 @@ __device__ __forceinline__ void ldmatrix4(uint32_t (&r)[4], uint32_t at) {
         asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(at) : "memory");
 }
 
-template <int D, bool BF16, int W>
-__global__ void __launch_bounds__(32 * W, W == 8 ? 1 : 2)
+template <int D, bool BF16>
+__global__ void __launch_bounds__(32 * W, 1)
 diff_attn_rows(const __grid_constant__ CUtensorMap tk, const __grid_constant__ CUtensorMap tv, const __grid_constant__ Args p) {
-    using L = RowLay<D, W>;
+    using L = RowLay<D>;
     constexpr int d = D / 2, E = D / 32;
     extern __shared__ __align__(1024) uint8_t smem[];
     const tsn_diff_attn_args & a = p.a;
@@ -1012,9 +1026,8 @@ cudaError_t launch_tc(const CUtensorMap & tk, const CUtensorMap & tv, const Args
     return cudaLaunchKernelEx(&cfg, diff_attn_tc<D, BF16>, tk, tv, p);
 }
 template <int D, bool BF16>
-cudaError_t launch_rows(const CUtensorMap & tk, const CUtensorMap & tv, const Args & p, unsigned grid, int warps, cudaStream_t s) {
-    if (warps == 8) diff_attn_rows<D, BF16, 8><<<grid, 256, RowLay<D, 8>::TOTAL, s>>>(tk, tv, p);
-    else diff_attn_rows<D, BF16, 4><<<grid, 128, RowLay<D, 4>::TOTAL, s>>>(tk, tv, p);
+cudaError_t launch_rows(const CUtensorMap & tk, const CUtensorMap & tv, const Args & p, unsigned grid, cudaStream_t s) {
+    diff_attn_rows<D, BF16><<<grid, 32 * W, RowLay<D>::TOTAL, s>>>(tk, tv, p);
     return cudaGetLastError();
 }
 
@@ -1025,14 +1038,10 @@ cudaError_t configure_diff_attn() {
     auto set = [&](auto * k, int bytes) {
         if (e == cudaSuccess) e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
     };
-    set(diff_attn_rows<64, false, 4>, RowLay<64, 4>::TOTAL);
-    set(diff_attn_rows<64, true, 4>, RowLay<64, 4>::TOTAL);
-    set(diff_attn_rows<128, false, 4>, RowLay<128, 4>::TOTAL);
-    set(diff_attn_rows<128, true, 4>, RowLay<128, 4>::TOTAL);
-    set(diff_attn_rows<64, false, 8>, RowLay<64, 8>::TOTAL);
-    set(diff_attn_rows<64, true, 8>, RowLay<64, 8>::TOTAL);
-    set(diff_attn_rows<128, false, 8>, RowLay<128, 8>::TOTAL);
-    set(diff_attn_rows<128, true, 8>, RowLay<128, 8>::TOTAL);
+    set(diff_attn_rows<64, false>, RowLay<64>::TOTAL);
+    set(diff_attn_rows<64, true>, RowLay<64>::TOTAL);
+    set(diff_attn_rows<128, false>, RowLay<128>::TOTAL);
+    set(diff_attn_rows<128, true>, RowLay<128>::TOTAL);
     set(diff_attn_tc<64, false>, Lay<64>::TOTAL);
     set(diff_attn_tc<64, true>, Lay<64>::TOTAL);
     set(diff_attn_tc<128, false>, Lay<128>::TOTAL);
@@ -1078,22 +1087,23 @@ int diff_attn(DeviceCtx & c, const tsn_diff_attn_args & in) {
     p.err = c.d_err;
     const bool rows = p.R <= FEW;
     const long long groups = (rows ? (p.R + SOME - 1) / SOME : (p.R + ROWS - 1) / ROWS) * a.B * a.Hk;
-    int warps = 8;
     if (rows) {
-        // Parts of 512 keys (four slabs for each of eight warps) while that is at most one CTA per SM, and none up to
-        // 1024 keys, where the trip through the workspace costs more than the keys. Beyond, CTAs of four warps, two
-        // per SM, in about four rounds, so that sequences of unequal length even out; at most 64 parts, as one CTA
-        // adds them up, and no more than the workspace holds.
-        const long long slabs = ((long long) a.Sk + SLAB - 1) / SLAB;
-        long long parts = slabs <= 64 ? 1 : (slabs + 31) / 32;
-        if (groups * parts > SMS) {
-            warps = 4;
-            parts = std::min(parts, std::max(1ll, 8 * SMS / groups));
+        // As many parts as take the least time, in units of what one CTA takes for a slab (93 ns): the start of a CTA is 30,
+        // a trip of the sums through the workspace 30 and a half for each part; past 74 CTAs at once (of 8 KB slabs) they
+        // wait for HBM. One token of 32 heads over 8, four caches of 32 768 keys: 87 us with one wave of 128 CTAs (6.2
+        // TB/s), 93 to 163 with two to sixteen; 16 heads over 704 keys: 9.6 us in one part or eight, 11.3 in two.
+        const long long slabs = ((long long) a.Sk + SLAB - 1) / SLAB, room = (long long) (WORKSPACE - COUNTERS * 4) / (SOME * (4 * a.d + 4) * 4);
+        double least = 0.0;
+        for (long long parts = 1; parts <= 64 && (parts == 1 || (groups <= (long long) COUNTERS && groups * parts <= room)); ++parts) {
+            const long long chunk = std::max(1ll, (slabs + parts - 1) / parts), ctas = groups * parts;
+            const double crowd = std::max(1.0, std::min<long long>(ctas, SMS) * (a.d / 64.0) / 74.0);
+            const double cost = (double) ((ctas + SMS - 1) / SMS) * (30.0 + chunk * crowd) + (parts > 1 ? 30.0 + 0.5 * parts : 0.0);
+            if (parts == 1 || cost < least) {
+                least = cost;
+                p.chunk = (int) chunk;
+                p.splits = (int) std::max(1ll, (slabs + chunk - 1) / chunk);
+            }
         }
-        parts = std::min({parts, 64ll, std::max(1ll, (long long) (WORKSPACE - COUNTERS * 4) / (groups * SOME * (4 * a.d + 4) * 4))});
-        if (groups > (long long) COUNTERS) parts = 1;
-        p.chunk = (int) std::max(1ll, (slabs + parts - 1) / parts);
-        p.splits = (int) std::max(1ll, (slabs + p.chunk - 1) / p.chunk);
     } else {
         // Split the keys over a cluster where whole tiles leave SMs without work: as many parts as fill one wave, of four
         // key tiles at least, eight at most (the largest portable cluster).
@@ -1118,8 +1128,8 @@ int diff_attn(DeviceCtx & c, const tsn_diff_attn_args & in) {
     const bool bf = a.type == TSN_BF16;
     cudaError_t e;
     if (rows)
-        e = a.d == 32 ? (bf ? launch_rows<64, true>(tk, tv, p, grid, warps, c.stream) : launch_rows<64, false>(tk, tv, p, grid, warps, c.stream))
-                      : (bf ? launch_rows<128, true>(tk, tv, p, grid, warps, c.stream) : launch_rows<128, false>(tk, tv, p, grid, warps, c.stream));
+        e = a.d == 32 ? (bf ? launch_rows<64, true>(tk, tv, p, grid, c.stream) : launch_rows<64, false>(tk, tv, p, grid, c.stream))
+                      : (bf ? launch_rows<128, true>(tk, tv, p, grid, c.stream) : launch_rows<128, false>(tk, tv, p, grid, c.stream));
     else
         e = a.d == 32 ? (bf ? launch_tc<64, true>(tk, tv, p, grid, c.stream) : launch_tc<64, false>(tk, tv, p, grid, c.stream))
                       : (bf ? launch_tc<128, true>(tk, tv, p, grid, c.stream) : launch_tc<128, false>(tk, tv, p, grid, c.stream));
