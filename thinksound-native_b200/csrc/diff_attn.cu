@@ -17,6 +17,7 @@
 #include <cudaTypedefs.h>
 
 #include <algorithm>
+#include <atomic>
 
 namespace tsn {
 
@@ -31,7 +32,7 @@ struct Args {
     tsn_diff_attn_args a;
     float c;                    // scale * log2(e)
     int G;                      // query heads per kv head
-    long long R;                // Sq * G rows of one kv head
+    int R;                      // Sq * G rows of one kv head
     int splits, kv_b;           // parts of the keys; 0: every batch reads the same keys
     int chunk;                  // few rows: slabs of a part
     float * part;
@@ -223,6 +224,7 @@ struct Lay {
     static_assert(TOTAL <= 227 * 1024, "one CTA's shared memory");
     static_assert(ROWS * row_words(D) * 4 <= 2 * STAGES * TILE, "the rows' sums fit in the ring");
     static_assert(TM_O + 2 * D <= TM, "tensor memory");
+    static_assert(ROWS * 8 * 8 <= Q, "the parts' factors fit in Q's place");
 };
 
 template <int D, bool BF16>
@@ -247,13 +249,12 @@ diff_attn_tc(const __grid_constant__ CUtensorMap tk, const __grid_constant__ CUt
     // this CTA's rows, keys and part of them; long rows of a causal call come first
     const unsigned gid = blockIdx.x / p.splits, split = blockIdx.x % p.splits;
     const int hk = (int) (gid % a.Hk), b = (int) (gid / a.Hk % a.B);
-    const long long qt = (p.R + ROWS - 1) / ROWS - 1 - gid / a.Hk / a.B, r0 = qt * ROWS;
-    const int rows = (int) min((long long) ROWS, p.R - r0);
-    const int i0 = (int) (r0 / p.G), rem0 = (int) (r0 % p.G);   // row t: token i0 + (rem0 + t) / G, head (rem0 + t) % G
+    const int r0 = (int) ((p.R + ROWS - 1) / ROWS - 1 - gid / a.Hk / a.B) * ROWS, rows = min(ROWS, p.R - r0);
+    const int i0 = r0 / p.G, rem0 = r0 % p.G;   // row t: token i0 + (rem0 + t) / G, head (rem0 + t) % G
     const int n = a.key_len ? max(0, min(a.key_len[b], (int) a.Sk)) : (int) a.Sk;
     auto limit = [&](int t) {   // keys before which row t sees
         if (!a.causal) return n;
-        return (int) max(0ll, min((long long) n, (long long) (i0 + (rem0 + t) / p.G) + n - (long long) a.Sq + 1));
+        return max(0, min(n, i0 + (rem0 + t) / p.G + n - (int) a.Sq + 1));   // at most 2^30 each
     };
     const int most = limit(rows - 1), least = limit(0);
     const int all_tiles = (most + KEYS - 1) / KEYS, per = (all_tiles + p.splits - 1) / p.splits;
@@ -392,6 +393,7 @@ diff_attn_tc(const __grid_constant__ CUtensorMap tk, const __grid_constant__ CUt
         if (p.splits > 1) {
             __syncthreads();
             cluster_sync_all();
+            __syncthreads();
             cluster_sync_all();
         } else {
             for (int i = 0; i < 4; ++i) __syncthreads();
@@ -399,13 +401,19 @@ diff_attn_tc(const __grid_constant__ CUtensorMap tk, const __grid_constant__ CUt
     } else {
         if (fits) {
             // Q into its swizzled boxes, rows past the last one as zeros; lambda of each head of the group; weights
-            for (int i = tid; i < ROWS * CH; i += 256) {
-                const int r = i / CH, ch = i % CH, u = rem0 + r;
-                uint4 x = make_uint4(0, 0, 0, 0);
+            uint4 x[ROWS * CH / 256];   // all on their way before the first is stored
+#pragma unroll
+            for (int y = 0; y < ROWS * CH / 256; ++y) {
+                const int r = (tid + 256 * y) / CH, ch = tid % CH, u = rem0 + r;
+                x[y] = make_uint4(0, 0, 0, 0);
                 if (r < rows)
-                    x = *(const uint4 *) ((const uint16_t *) a.q.p + b * a.q.sb + (long long) (i0 + u / p.G) * a.q.ss +
-                                          (long long) (hk * p.G + u % p.G) * a.q.sh + ch * 8);
-                *(uint4 *) (smem + (ch >> 3) * QBOX + r * 128 + (((ch & 7) ^ (r & 7)) << 4)) = x;
+                    x[y] = *(const uint4 *) ((const uint16_t *) a.q.p + b * a.q.sb + (long long) (i0 + u / p.G) * a.q.ss +
+                                             (long long) (hk * p.G + u % p.G) * a.q.sh + ch * 8);
+            }
+#pragma unroll
+            for (int y = 0; y < ROWS * CH / 256; ++y) {
+                const int r = (tid + 256 * y) / CH, ch = tid % CH;
+                *(uint4 *) (smem + (ch >> 3) * QBOX + r * 128 + (((ch & 7) ^ (r & 7)) << 4)) = x[y];
             }
             fence_proxy_async_smem();
             __syncwarp();
@@ -556,24 +564,65 @@ diff_attn_tc(const __grid_constant__ CUtensorMap tk, const __grid_constant__ CUt
                 to[2 * D + 2 + m] = l;
             }
             cluster_sync_all();
-            const int share = (rows + p.splits - 1) / p.splits, last = min(rows, ((int) split + 1) * share);
-            const uint32_t here = smem_u32(sums);
-            for (int r = (int) split * share + warp; r < last && !*abort_flag; r += 8) {
-                constexpr int E = D / 32;
-                float sum[2][E], top[2], rl[2];
-                auto at = [&](int i, int k) { return dsmem_map(here, (uint32_t) i) + (uint32_t) (r * row_words(D) + k) * 4; };
-                add_up<D>(p.splits, lane, sum, top, rl, [&](int i, int k) { return dsmem_ld1(at(i, k)); },
-                          [&](int i, int k, float * v) {
-                              if (E == 4) {
-                                  const float4 x = dsmem_ld4(at(i, k));
-                                  v[0] = x.x; v[1] = x.y; v[2] = x.z; v[3] = x.w;
-                              } else {
-                                  v[0] = dsmem_ld1(at(i, k));
-                                  v[1] = dsmem_ld1(at(i, k + 1));
-                              }
-                          });
-                const int u = rem0 + r, g = u % p.G;
-                write_row<D, BF16>(p, b, hk, i0 + u / p.G, g, lam[g], nw, lane, sum, rl);
+            // this CTA's share of the rows: first each part's factors, 2^(ref - greatest) / l and that times -lambda, in Q's
+            // place, then the parts' sums, a row by D / 4 lanes, four steps of rows at once
+            const int share = (rows + p.splits - 1) / p.splits, from = (int) split * share, here = max(0, min(rows - from, share));
+            const uint32_t at0 = smem_u32(sums) + from * row_words(D) * 4;
+            float2 * fac = (float2 *) smem;   // [row][8 parts]
+            if (tid < here) {
+                float4 st[8];   // ref and l of both maps
+                float2 top = make_float2(-INFINITY, -INFINITY), sum = make_float2(0.0f, 0.0f);
+#pragma unroll
+                for (int i = 0; i < 8; ++i)
+                    if (i < p.splits) {
+                        st[i] = dsmem_ld4(dsmem_map(at0 + (tid * row_words(D) + 2 * D) * 4, (uint32_t) i));
+                        top = make_float2(fmaxf(top.x, st[i].x), fmaxf(top.y, st[i].y));
+                    }
+                if (top.x == -INFINITY) top.x = 0.0f;
+                if (top.y == -INFINITY) top.y = 0.0f;
+#pragma unroll
+                for (int i = 0; i < 8; ++i)
+                    if (i < p.splits) {
+                        st[i].x = ex2(st[i].x - top.x);
+                        st[i].y = ex2(st[i].y - top.y);
+                        sum.x += st[i].x * st[i].z;
+                        sum.y += st[i].y * st[i].w;
+                    }
+                const float w1 = sum.x == 0.0f ? 0.0f : 1.0f / sum.x, w2 = sum.y == 0.0f ? 0.0f : -lam[(rem0 + from + tid) % p.G] / sum.y;
+#pragma unroll
+                for (int i = 0; i < 8; ++i)
+                    if (i < p.splits) fac[tid * 8 + i] = make_float2(st[i].x * w1, st[i].y * w2);
+            }
+            __syncthreads();
+            constexpr int LANES = D / 4, STEP = 8 * (32 / LANES), AT_ONCE = 4;   // of a row; rows of a step of all warps
+            const int col = (lane % LANES) * 4;
+            for (int y0 = warp * (32 / LANES) + lane / LANES; y0 < (here + STEP - 1) / STEP * STEP; y0 += STEP * AT_ONCE) {
+                float o[AT_ONCE][4] = {};
+                for (int i = 0; i < p.splits; ++i)
+#pragma unroll
+                    for (int y = 0; y < AT_ONCE; ++y) {
+                        const int r = y0 + y * STEP;
+                        if (r < here) {
+                            const uint32_t at = dsmem_map(at0 + (r * row_words(D) + col) * 4, (uint32_t) i);
+                            const float4 v = dsmem_ld4(at), w = dsmem_ld4(at + D * 4);
+                            const float2 f = fac[r * 8 + i];
+                            o[y][0] = fmaf(f.x, v.x, fmaf(f.y, w.x, o[y][0])); o[y][1] = fmaf(f.x, v.y, fmaf(f.y, w.y, o[y][1]));
+                            o[y][2] = fmaf(f.x, v.z, fmaf(f.y, w.z, o[y][2])); o[y][3] = fmaf(f.x, v.w, fmaf(f.y, w.w, o[y][3]));
+                        }
+                    }
+#pragma unroll
+                for (int y = 0; y < AT_ONCE; ++y) {
+                    const int r = y0 + y * STEP;
+                    float ss = o[y][0] * o[y][0] + o[y][1] * o[y][1] + o[y][2] * o[y][2] + o[y][3] * o[y][3];
+#pragma unroll
+                    for (int x = LANES / 2; x; x >>= 1) ss += __shfl_xor_sync(~0u, ss, x);
+                    if (r >= here || *abort_flag) continue;
+                    const float g = ss < INFINITY ? rsqrtf(ss * (1.0f / D) + a.eps) : NAN;
+                    const float4 w = *(const float4 *) (nw + col);
+                    const int u = rem0 + from + r;
+                    *(uint2 *) ((uint16_t *) a.out.p + b * a.out.sb + (long long) (i0 + u / p.G) * a.out.ss + (long long) (hk * p.G + u % p.G) * a.out.sh + col) =
+                        make_uint2(pack16<BF16>(o[y][0] * g * w.x, o[y][1] * g * w.y), pack16<BF16>(o[y][2] * g * w.z, o[y][3] * g * w.w));
+                }
             }
             cluster_sync_all();   // nobody leaves while its sums are read
         } else {
@@ -706,14 +755,14 @@ diff_attn_rows(const __grid_constant__ CUtensorMap tk, const __grid_constant__ C
 
     // All groups of a part lie next to one another: the groups of 8 rows of a kv head read the same keys at about the same
     // time, and the kv heads neighbouring ones (a head's row is 256 bytes, too little for DRAM by itself).
-    const int eights = (int) (p.R + SOME - 1) / SOME;
+    const int eights = (p.R + SOME - 1) / SOME;
     const unsigned groups = gridDim.x / p.splits, gid = blockIdx.x % groups, split = blockIdx.x / groups;
     const int hk = (int) (gid / eights % a.Hk), b = (int) (gid / eights / a.Hk);
-    const int first = (int) (gid % eights) * SOME, R = min(SOME, (int) p.R - first);   // row r: token (first + r) / G, head (first + r) % G
+    const int first = (int) (gid % eights) * SOME, R = min(SOME, p.R - first);   // row r: token (first + r) / G, head (first + r) % G
     const int n = a.key_len ? max(0, min(a.key_len[b], (int) a.Sk)) : (int) a.Sk;
     auto limit = [&](int r) {   // keys before which row r sees; rows past the last one see all
         if (!a.causal || r >= R) return n;
-        return (int) max(0ll, min((long long) n, (long long) ((first + r) / p.G) + n - (long long) a.Sq + 1));
+        return max(0, min(n, (first + r) / p.G + n - (int) a.Sq + 1));   // at most 2^30 each
     };
     const int least = limit(0);
     // this CTA's slabs, and this warp's
@@ -1031,6 +1080,9 @@ cudaError_t launch_rows(const CUtensorMap & tk, const CUtensorMap & tv, const Ar
     return cudaGetLastError();
 }
 
+// clusters of 1 to 8 CTAs of diff_attn_tc that run at once (one CTA per SM; a cluster lies within a GPC)
+std::atomic<int> g_clusters[9];
+
 } // namespace
 
 cudaError_t configure_diff_attn() {
@@ -1046,6 +1098,21 @@ cudaError_t configure_diff_attn() {
     set(diff_attn_tc<64, true>, Lay<64>::TOTAL);
     set(diff_attn_tc<128, false>, Lay<128>::TOTAL);
     set(diff_attn_tc<128, true>, Lay<128>::TOTAL);
+    g_clusters[1] = SMS;
+    for (unsigned n = 2; n <= 8 && e == cudaSuccess; ++n) {
+        cudaLaunchAttribute at{};
+        at.id = cudaLaunchAttributeClusterDimension;
+        at.val.clusterDim = {n, 1, 1};
+        cudaLaunchConfig_t cfg{};
+        cfg.gridDim = dim3(n * SMS);
+        cfg.blockDim = dim3(THREADS);
+        cfg.dynamicSmemBytes = Lay<128>::TOTAL;
+        cfg.attrs = &at;
+        cfg.numAttrs = 1;
+        int count = 0;
+        e = cudaOccupancyMaxActiveClusters(&count, diff_attn_tc<128, true>, &cfg);
+        g_clusters[n] = count;
+    }
     return e;
 }
 
@@ -1083,7 +1150,8 @@ int diff_attn(DeviceCtx & c, const tsn_diff_attn_args & in) {
     p.a = a;
     p.c = a.scale * LOG2E;
     p.G = (int) (a.H / a.Hk);
-    p.R = (long long) a.Sq * p.G;
+    if ((long long) a.Sq * p.G > (1ll << 30)) return fail(TSN_ERR_ARG, "tsn_diff_attn: more than 2^30 query rows of a kv head");
+    p.R = (int) a.Sq * p.G;
     p.err = c.d_err;
     const bool rows = p.R <= FEW;
     const long long groups = (rows ? (p.R + SOME - 1) / SOME : (p.R + ROWS - 1) / ROWS) * a.B * a.Hk;
@@ -1105,10 +1173,16 @@ int diff_attn(DeviceCtx & c, const tsn_diff_attn_args & in) {
             }
         }
     } else {
-        // Split the keys over a cluster where whole tiles leave SMs without work: as many parts as fill one wave, of four
-        // key tiles at least, eight at most (the largest portable cluster).
+        // As many parts of a cluster as take the least time, in microseconds: start and end of a CTA 7, a tile of a 64-wide map
+        // 1 (of a 32-wide one 0.7), adding up the parts 3; clusters of one size run g_clusters[size] at a time. Four key tiles
+        // a part at least, eight parts at most (the largest portable cluster).
         const long long tiles = ((long long) a.Sk + KEYS - 1) / KEYS;
-        p.splits = (int) std::max(1ll, std::min({SMS / groups, tiles / 4, 8ll}));
+        double least = 0.0;
+        for (int parts = 1; parts <= 8 && (parts == 1 || parts * 4 <= tiles); ++parts) {
+            const long long room = std::max(1, g_clusters[parts].load(std::memory_order_relaxed));
+            const double cost = (double) ((groups + room - 1) / room) * (7.0 + (double) ((tiles + parts - 1) / parts) * (a.d == 64 ? 1.0 : 0.7)) + (parts > 1 ? 3.0 : 0.0);
+            if (parts == 1 || cost < least) { least = cost; p.splits = parts; }
+        }
     }
     if (groups * p.splits > 0x7fffffffLL) return fail(TSN_ERR_ARG, "tsn_diff_attn: too many query rows");
     const bool shared = rows && p.splits > 1;   // through the workspace
