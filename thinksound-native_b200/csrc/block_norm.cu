@@ -19,6 +19,7 @@ namespace {
 struct NormArgs {
     tsn_block_norm_args a;
     unsigned rows;
+    int swapped;   // one row a block: the batch runs along x instead of y
 };
 
 // V elements of type T: 16-byte words where a piece has some, else the elements themselves.
@@ -138,12 +139,13 @@ __global__ void __launch_bounds__(most_threads(V, NV, BLOCK)) block_norm_kernel(
     const tsn_block_norm_args & a = n.a;
     const int C = (int) a.C;
     const float inv_C = 1.0f / (float) C;
-    const unsigned row = BLOCK ? blockIdx.x : blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5);
+    const unsigned row = blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5);
     if (!BLOCK && row >= n.rows) return;
     const int first = (BLOCK ? (int) threadIdx.x : (int) (threadIdx.x & 31)) * V, step = (BLOCK ? (int) blockDim.x : 32) * V;
     auto col = [&](int i) { return first + i * step; };
     auto at = [&](int i) { return col(i) < C; };
-    const unsigned b = row / a.T, t = row % a.T;
+    // a block's row is a block index in each direction: its addresses are the same in all threads and cost them nothing
+    const unsigned b = BLOCK ? (n.swapped ? blockIdx.x : blockIdx.y) : row / a.T, t = BLOCK ? (n.swapped ? blockIdx.y : blockIdx.x) : row % a.T;
     auto in = [&](const tsn_rows & r) { return b * r.sb + t * r.st; };
 
     constexpr bool EARLY = NV <= 2;
@@ -228,22 +230,23 @@ __global__ void __launch_bounds__(most_threads(V, NV, BLOCK)) block_norm_kernel(
 template <class TX, class T, int V>
 cudaError_t launch(const NormArgs & n, cudaStream_t s) {
     const int pieces = ((int) n.a.C + V - 1) / V;
+    const dim3 grid = n.swapped ? dim3(n.a.B, n.a.T) : dim3(n.a.T, n.a.B);
     if (pieces <= 32) {
         block_norm_kernel<TX, T, V, 1, false><<<(n.rows + 3) / 4, 128, 0, s>>>(n);
     } else if constexpr (V == 1) {   // unaligned rows
         const int threads = std::min(1024, (pieces + 127) / 128 * 32);
-        if (pieces <= 4 * threads) block_norm_kernel<TX, T, V, 4, true><<<n.rows, threads, 0, s>>>(n);
-        else block_norm_kernel<TX, T, V, 16, true><<<n.rows, threads, 0, s>>>(n);
+        if (pieces <= 4 * threads) block_norm_kernel<TX, T, V, 4, true><<<grid, threads, 0, s>>>(n);
+        else block_norm_kernel<TX, T, V, 16, true><<<grid, threads, 0, s>>>(n);
     } else {
         // One piece a thread while a block of 512 holds the row: the least latency where there are few rows (658
         // rows of 1024: 4.2 us, 4.8 with two pieces, 8.6 with four), and no slower where rows fill the GPU (32 500 of
         // 2048: 174, 175 and 233 us).
         const int per = pieces > 2048 ? 8 : pieces > 1024 ? 4 : pieces > 512 ? 2 : 1;
         const int threads = (pieces + 32 * per - 1) / (32 * per) * 32;
-        if (per == 1) block_norm_kernel<TX, T, V, 1, true><<<n.rows, threads, 0, s>>>(n);
-        else if (per == 2) block_norm_kernel<TX, T, V, 2, true><<<n.rows, threads, 0, s>>>(n);
-        else if (per == 4) block_norm_kernel<TX, T, V, 4, true><<<n.rows, threads, 0, s>>>(n);
-        else if constexpr (V < 8) block_norm_kernel<TX, T, V, 8, true><<<n.rows, threads, 0, s>>>(n);   // 2048 pieces of 8 are 16384
+        if (per == 1) block_norm_kernel<TX, T, V, 1, true><<<grid, threads, 0, s>>>(n);
+        else if (per == 2) block_norm_kernel<TX, T, V, 2, true><<<grid, threads, 0, s>>>(n);
+        else if (per == 4) block_norm_kernel<TX, T, V, 4, true><<<grid, threads, 0, s>>>(n);
+        else if constexpr (V < 8) block_norm_kernel<TX, T, V, 8, true><<<grid, threads, 0, s>>>(n);   // 2048 pieces of 8 are 16384
     }
     return cudaGetLastError();
 }
@@ -287,7 +290,7 @@ int block_norm(DeviceCtx & c, const tsn_block_norm_args & a) {
         !aligned(a.shift, e) || !aligned(a.scale, e) ||
         (((uintptr_t) a.post_w | (uintptr_t) a.post_b | (uintptr_t) a.pre_w | (uintptr_t) a.pre_b | (uintptr_t) a.res_vec) & 3))
         return fail(TSN_ERR_ARG, "tsn_block_norm: an address that is no multiple of its element's size");
-    const NormArgs n{a, (unsigned) rows};
+    const NormArgs n{a, (unsigned) rows, a.B > 65535};   // then T is less: there are no more than 2^31 - 1 rows
     cudaError_t rc;
     if (a.type == TSN_F32) rc = launch<float, float>(n, c.stream);
     else if (a.type == TSN_F16) rc = a.xtype == TSN_F32 ? launch<float, __half>(n, c.stream) : launch<__half, __half>(n, c.stream);
