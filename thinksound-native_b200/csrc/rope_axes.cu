@@ -216,10 +216,12 @@ cudaError_t launch(const tsn_rope_plan_t & p, const tsn_rope_args & a, cudaStrea
     if (p.D % 8 == 0 && a.B <= 65535 && rows16(a.q, a.Hq) && rows16(a.k, a.Hk) && (!a.q.p || rows16(a.q_out, a.Hq)) && (!a.k.p || rows16(a.k_out, a.Hk))) {
         int lph = 1;
         while (lph * 8 < (int) p.D) lph *= 2;
-        // Tokens of a block: 8 share its start; fewer while blocks would not fill the SMs.
-        const int tok = (int) std::min<long long>(MAX_TOK, std::max(1ll, tokens / (4 * 148)));
+        // Tokens of a block: 8 share its start; fewer while four blocks per SM take them all (not a few more, which would
+        // be a second wave).
         const int side = 32 / lph, chunks = (int) ((a.q.p ? a.Hq : 0) + side - 1) / side + (int) ((a.k.p ? a.Hk : 0) + side - 1) / side;
-        const dim3 blocks((a.S + tok - 1) / tok, a.B, (chunks + WARPS - 1) / WARPS);
+        const long long turns = (chunks + WARPS - 1) / WARPS;
+        const int tok = (int) std::min<long long>(MAX_TOK, (tokens * turns + 4 * 148 - 1) / (4 * 148));
+        const dim3 blocks((a.S + tok - 1) / tok, a.B, (unsigned) turns);
         const int pair = p.layout == TSN_ROPE_INTERLEAVED ? NEXT : p.P % 8 == 0 ? LANES : SHARED;
         auto go = [&](auto L) {
             constexpr int LPH = decltype(L)::value;
