@@ -1,5 +1,5 @@
 // diff_attn.cu — differential attention (tsn_diff_attn): diff_attn_tc on the tcgen05 tensor cores, and
-// diff_attn_rows for at most 16 query rows.
+// diff_attn_rows for at most 32 query rows of a kv head.
 //
 //   o = O_1 / l_1 - lambda O_2 / l_2,   O_m = sum_j p_mj v_j,  l_m = sum_j p_mj,  p_mj = 2^(c q_m.k_mj - ref_m)
 // in one pass over the keys: ref_m follows the running maximum of the row, O_m and l_m are rescaled when it
@@ -67,8 +67,8 @@ __device__ __forceinline__ uint64_t fadd2(uint64_t a, uint64_t b) {
 // (2^x, 2^y) on the FMA pipe, x and y clamped to -126 or more: 2^i p(f), i the nearest whole number, f = x - i in [-1/2, 1/2],
 // p the polynomial of least relative error there (Remez exchange): 7.5e-5 at degree 3, 2.6e-6 at degree 4, each below
 // an eighth of half a unit of the 16-bit type that the result is rounded to. Adding 1.5 * 2^23 rounds to i and leaves
-// it in the low bits. NaN stays non-finite.
-template <bool BF16>
+// it in the low bits. NaN stays non-finite. ZERO: what was clamped becomes 0 (p(0) < 1, so 2^-126 p(0) is subnormal).
+template <bool BF16, bool ZERO>
 __device__ __forceinline__ uint64_t ex2_fma(uint64_t xy) {
     float x, y;
     f2_unpack(xy, x, y);
@@ -91,7 +91,9 @@ __device__ __forceinline__ uint64_t ex2_fma(uint64_t xy) {
     float a, b, i, j;
     f2_unpack(q, a, b);
     f2_unpack(r, i, j);
-    return f2_pack(__uint_as_float(__float_as_uint(a) + (__float_as_uint(i) << 23)), __uint_as_float(__float_as_uint(b) + (__float_as_uint(j) << 23)));
+    uint64_t e = f2_pack(__uint_as_float(__float_as_uint(a) + (__float_as_uint(i) << 23)), __uint_as_float(__float_as_uint(b) + (__float_as_uint(j) << 23)));
+    if (ZERO) asm("mul.rn.ftz.f32x2 %0, %0, %1;" : "+l"(e) : "l"(two(1.0f)));
+    return e;
 }
 template <bool BF16>
 __device__ __forceinline__ uint32_t pack16(float a, float b) {
@@ -109,6 +111,39 @@ __device__ __forceinline__ uint32_t finite_only(uint32_t v) {
     if ((v & e) == e) v &= 0xffff0000u;
     if ((v & (e << 16)) == (e << 16)) v &= 0x0000ffffu;
     return v;
+}
+
+// 32 scores s of a row become 2^(c s + neg): P as 16-bit pairs, and their sum. Every fourth pair takes the FMA pipe.
+template <bool BF16, bool MASKED>
+__device__ __forceinline__ void exponentials(const uint32_t * s, uint32_t * pk, float c, float ref, uint64_t (&sum)[2]) {
+    const float neg = ref == -INFINITY ? 0.0f : -ref;
+    const uint64_t c2 = f2_pack(c, c), neg2 = f2_pack(neg, neg);
+#pragma unroll
+    for (int e = 0; e < 16; ++e) {
+        const uint64_t v = ffma2(f2_pack(__uint_as_float(s[2 * e]), __uint_as_float(s[2 * e + 1])), c2, neg2);
+        float y, z;
+        if (e % 4 == 3) {
+            f2_unpack(ex2_fma<BF16, MASKED>(v), y, z);
+        } else {
+            f2_unpack(v, y, z);
+            y = ex2(y);
+            z = ex2(z);
+        }
+        sum[e & 1] = fadd2(sum[e & 1], f2_pack(y, z));
+        pk[e] = pack16<BF16>(y, z);
+    }
+}
+__device__ __forceinline__ float greatest(const uint32_t * s) {   // of 32
+    float mx[2] = {-INFINITY, -INFINITY};
+#pragma unroll
+    for (int e = 0; e < 32; e += 2) mx[(e >> 1) & 1] = fmaxf(mx[(e >> 1) & 1], fmaxf(__uint_as_float(s[e]), __uint_as_float(s[e + 1])));
+    return fmaxf(mx[0], mx[1]);
+}
+__device__ __forceinline__ void hide(uint32_t * s, uint32_t vis) {   // scores of the keys that the row does not see
+    if (__any_sync(~0u, vis != ~0u))
+#pragma unroll
+        for (int e = 0; e < 32; ++e)
+            if (!((vis >> e) & 1u)) s[e] = 0xff800000u;   // -inf
 }
 
 // A row's sums as they are added up over warps, CTAs or parts of the keys: O [2 maps][D], then ref and l of both maps.
@@ -207,12 +242,13 @@ __device__ __forceinline__ void write_row(const Args & p, int b, int hk, int i, 
 // TMEM at d = 64: S in two buffers per map (4 x 64 columns), so that a map's next scores are there when its
 // softmax is done, and O_1, O_2 (128 each): all 512 columns.
 // What bounds it: 2 exponentials for 12 d operations. At d = 64 a 128 x 64 tile pair takes 1024 cycles of the SFU
-// (16 exponentials a cycle) and 896 of the tensor cores (the products with N 64 wait for shared memory).
+// (16 exponentials a cycle), 768 with every fourth pair on the FMA pipe, and 896 of the tensor cores (the products with
+// N 64 wait for shared memory). 8125 tokens of 16 heads take 850 to 870 us, 0.94 PFLOP/s, about 1650 cycles a tile pair at
+// the 1.7 GHz that the power limit leaves: both maps' warps tend to compute, and to wait for TMEM, at the same time.
+// Measured and left: 32-key tiles on 16 softmax warps (1050 us), turns of the maps for the SFU (975 to 1080), 128-key
+// tiles with one buffer (1287), the next tile's scores requested a half tile ahead (960).
 // Parts of the keys: each CTA leaves its rows' sums in its shared memory and, after a cluster barrier, adds up its
 // share of the rows over the cluster, in the order of the parts.
-#ifndef FE
-#define FE 4
-#endif
 template <int D>
 struct Lay {
     static constexpr int BUF = 2;
@@ -272,6 +308,17 @@ diff_attn_tc(const __grid_constant__ CUtensorMap tk, const __grid_constant__ CUt
     }
     if (warp == 8 && lane == 0 && nt > 0) { tma_prefetch(&tk); tma_prefetch(&tv); }
     if (warp == 9) tmem_alloc(words, L::TM);
+    uint4 q[ROWS * CH / 256];   // Q, on its way while the barriers and tensor memory are set up
+    if (warp < 8) {
+#pragma unroll
+        for (int y = 0; y < ROWS * CH / 256; ++y) {
+            const int r = (tid + 256 * y) / CH, ch = tid % CH, u = rem0 + r;
+            q[y] = make_uint4(0, 0, 0, 0);
+            if (r < rows)
+                q[y] = *(const uint4 *) ((const uint16_t *) a.q.p + b * a.q.sb + (long long) (i0 + u / p.G) * a.q.ss +
+                                         (long long) (hk * p.G + u % p.G) * a.q.sh + ch * 8);
+        }
+    }
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
@@ -382,7 +429,7 @@ diff_attn_tc(const __grid_constant__ CUtensorMap tk, const __grid_constant__ CUt
                 const uint64_t v = vd + (uint64_t) (s * (L::TILE >> 4));
 #pragma unroll
                 for (int kk = 0; kk < KEYS / 16; ++kk)
-                    umma_f16_ts_if(lead, to, ts + KEYS * x + 8 * kk, v + 128 * kk, id_pv, j > 0 || kk > 0);
+                    umma_f16_ts_if(lead, to, ts + KEYS * x + 32 + 8 * kk, v + 128 * kk, id_pv, j > 0 || kk > 0);
                 umma_commit_if(lead, &empty[s]);
                 if (j + BUF < nt) go = qk(j + BUF);
                 else umma_commit_if(lead, &o_full[mm * BUF + nt - 1 - j]);   // the last BUF tiles, [0] the last
@@ -401,19 +448,10 @@ diff_attn_tc(const __grid_constant__ CUtensorMap tk, const __grid_constant__ CUt
     } else {
         if (fits) {
             // Q into its swizzled boxes, rows past the last one as zeros; lambda of each head of the group; weights
-            uint4 x[ROWS * CH / 256];   // all on their way before the first is stored
-#pragma unroll
-            for (int y = 0; y < ROWS * CH / 256; ++y) {
-                const int r = (tid + 256 * y) / CH, ch = tid % CH, u = rem0 + r;
-                x[y] = make_uint4(0, 0, 0, 0);
-                if (r < rows)
-                    x[y] = *(const uint4 *) ((const uint16_t *) a.q.p + b * a.q.sb + (long long) (i0 + u / p.G) * a.q.ss +
-                                             (long long) (hk * p.G + u % p.G) * a.q.sh + ch * 8);
-            }
 #pragma unroll
             for (int y = 0; y < ROWS * CH / 256; ++y) {
                 const int r = (tid + 256 * y) / CH, ch = tid % CH;
-                *(uint4 *) (smem + (ch >> 3) * QBOX + r * 128 + (((ch & 7) ^ (r & 7)) << 4)) = x[y];
+                *(uint4 *) (smem + (ch >> 3) * QBOX + r * 128 + (((ch & 7) ^ (r & 7)) << 4)) = q[y];
             }
             fence_proxy_async_smem();
             __syncwarp();
@@ -445,81 +483,76 @@ diff_attn_tc(const __grid_constant__ CUtensorMap tk, const __grid_constant__ CUt
                 tc_fence_after();
                 return go;
             };
+            // A tile is taken in two halves of 32 keys, so that a half's scores come from TMEM while the other half's
+            // exponentials run. P replaces the second half's scores; the first half's stay until the tile is done.
+            uint32_t s1[32], vis[2] = {~0u, ~0u};
+            uint64_t sum[2];
+            // the first half of tile j, whose scores are there, and the maximum over both
+            auto first_half = [&](auto masked, int j) {
+                constexpr bool MASKED = decltype(masked)::value;
+                const uint32_t at = tmem + KEYS * (m * BUF + j % BUF) + lane0;
+                uint32_t s0[32], pk[16];
+                tmem_request32(at, s0);
+                if (MASKED) {
+                    const int base = (t0 + j) * KEYS;
+#pragma unroll
+                    for (int w = 0; w < 2; ++w)
+                        vis[w] = (mask ? __ballot_sync(~0u, mb[w] != 0) : low_bits(n - base - 32 * w)) & low_bits(lim - base - 32 * w);
+                    if (mask && j + 1 < nt) fetch_mask(j + 1);
+                }
+                tmem_landed32(s0);
+                tmem_request32(at + 32, s1);
+                if (MASKED) hide(s0, vis[0]);
+                // against the reference of the tiles before; the few tiles whose maximum is too far above it are done again
+                sum[0] = sum[1] = 0ull;
+                exponentials<BF16, MASKED>(s0, pk, p.c, ref, sum);
+                const float top0 = greatest(s0);
+                tmem_landed32(s1);
+                if (MASKED) hide(s1, vis[1]);
+                const float top = fmaxf(top0, greatest(s1)) * p.c;
+                const bool move = top > ref + LAZY;
+                if (__any_sync(~0u, move)) {
+                    // a row moves its reference by itself, so its result does not depend on its neighbours
+                    const float f = move ? ex2(ref - top) : 1.0f;
+                    if (move) { ref = top; l *= f; }
+                    if (j > 0) {
+                        // O is complete up to tile j - 1: the scores issued after that product are there, or its own commit
+                        const int i = j - 1 + BUF;
+                        uint64_t * done = i < nt ? &s_full[m * BUF + i % BUF] : &o_full[m * BUF + nt - j];
+                        if (!mbar_wait_soon(done, i < nt ? (i / BUF) & 1 : 0, abort_flag, p.err, DEV_TIMEOUT_TMEM)) ok = false;
+                        __syncwarp();
+                        tc_fence_after();
+#pragma unroll 1
+                        for (int y = 0; y < D && ok; y += 16) {
+                            float o[16];
+                            tmem_ld16(to + y, o);
+#pragma unroll
+                            for (int e = 0; e < 16; ++e) o[e] *= f;
+                            tmem_st16(to + y, (const uint32_t *) o);
+                        }
+                    }
+                    tmem_request32(at, s0);
+                    tmem_landed32(s0);
+                    if (MASKED) hide(s0, vis[0]);
+                    sum[0] = sum[1] = 0ull;
+                    exponentials<BF16, MASKED>(s0, pk, p.c, ref, sum);
+                }
+                tmem_st16(at + 32, pk);
+            };
             auto tiles = [&](auto masked, int from, int until) {
                 constexpr bool MASKED = decltype(masked)::value;
                 for (int j = from; j < until && ok; ++j) {
-                    const int base = (t0 + j) * KEYS, x = m * BUF + j % BUF;
-                    uint32_t s[KEYS], pk[KEYS / 2];
-                    tmem_request32(tmem + KEYS * x + lane0, s);
-                    tmem_request32(tmem + KEYS * x + lane0 + 32, s + 32);
-                    tmem_landed32(s);
-                    tmem_landed32(s + 32);
-                    uint32_t vis[2];   // the keys that this row sees
-                    if (MASKED) {
-#pragma unroll
-                        for (int w = 0; w < 2; ++w) {
-                            vis[w] = (mask ? __ballot_sync(~0u, mb[w] != 0) : low_bits(n - base - 32 * w)) & low_bits(lim - base - 32 * w);
-                            if (__any_sync(~0u, vis[w] != ~0u))
-#pragma unroll
-                                for (int e = 0; e < 32; ++e)
-                                    if (!((vis[w] >> e) & 1u)) s[32 * w + e] = 0xff800000u;   // -inf
-                        }
-                        if (mask && j + 1 < nt) fetch_mask(j + 1);
-                    }
-                    // The exponentials are taken against the reference of the tiles before, and the maximum beside them, so that
-                    // the SFU need not wait for it; the few tiles whose maximum is too far above the reference are done again.
-                    uint64_t sum[2];
-                    while (true) {
-                        const float neg = ref == -INFINITY ? 0.0f : -ref;
-                        const uint64_t c2 = f2_pack(p.c, p.c), neg2 = f2_pack(neg, neg);
-                        float mx[2] = {-INFINITY, -INFINITY};
-                        sum[0] = sum[1] = 0ull;
-#pragma unroll
-                        for (int e = 0; e < KEYS / 2; ++e) {
-                            const float a0 = __uint_as_float(s[2 * e]), a1 = __uint_as_float(s[2 * e + 1]);
-                            const uint64_t v = ffma2(f2_pack(a0, a1), c2, neg2);
-                            float y, z;
-                            if (!MASKED && e % FE == FE - 1) {
-                                f2_unpack(ex2_fma<BF16>(v), y, z);
-                            } else {
-                                f2_unpack(v, y, z);
-                                y = ex2(y);
-                                z = ex2(z);
-                            }
-                            sum[e & 1] = fadd2(sum[e & 1], f2_pack(y, z));
-                            pk[e] = pack16<BF16>(y, z);
-                            mx[e & 1] = fmaxf(mx[e & 1], fmaxf(a0, a1));
-                        }
-                        const float top = fmaxf(mx[0], mx[1]) * p.c;
-                        const bool move = top > ref + LAZY;
-                        if (!__any_sync(~0u, move)) break;
-                        // a row moves its reference by itself, so its result does not depend on its neighbours
-                        const float f = move ? ex2(ref - top) : 1.0f;
-                        if (move) { ref = top; l *= f; }
-                        if (j > 0) {
-                            // O is complete up to tile j - 1: the scores issued after that product are there, or its own commit
-                            const int i = j - 1 + BUF;
-                            uint64_t * done = i < nt ? &s_full[m * BUF + i % BUF] : &o_full[m * BUF + nt - j];
-                            if (!mbar_wait_soon(done, i < nt ? (i / BUF) & 1 : 0, abort_flag, p.err, DEV_TIMEOUT_TMEM)) { ok = false; break; }
-                            __syncwarp();
-                            tc_fence_after();
-#pragma unroll 1
-                            for (int y = 0; y < D; y += 16) {
-                                float o[16];
-                                tmem_ld16(to + y, o);
-#pragma unroll
-                                for (int e = 0; e < 16; ++e) o[e] *= f;
-                                tmem_st16(to + y, (const uint32_t *) o);
-                            }
-                        }
-                    }
+                    if (!arrived(j)) { ok = false; break; }
+                    first_half(masked, j);
+                    const int x = m * BUF + j % BUF;
+                    uint32_t pk[16];
+                    exponentials<BF16, MASKED>(s1, pk, p.c, ref, sum);
+                    tmem_st16(tmem + KEYS * x + lane0 + 48, pk);
                     float y, z;
                     f2_unpack(fadd2(sum[0], sum[1]), y, z);
                     l += y + z;
-                    tmem_st32(tmem + KEYS * x + lane0, pk);
-                    if (j + 1 < nt && !arrived(j + 1)) ok = false;   // meanwhile; they need no more than the product of tile j - 1
                     tmem_st_wait();
-                    if (MASKED && m == 0 && mixed(base)) {
+                    if (MASKED && m == 0 && mixed((t0 + j) * KEYS)) {
                         if (!mbar_wait_soon(&v_ready[j % L::STAGES], (j / L::STAGES) & 1, abort_flag, p.err, DEV_TIMEOUT_FULL)) ok = false;
                         const volatile uint32_t * bad = words + 2 + 2 * (j % L::STAGES);
                         poison |= (bad[0] & vis[0]) != 0 || (bad[1] & vis[1]) != 0;
@@ -531,7 +564,6 @@ diff_attn_tc(const __grid_constant__ CUtensorMap tk, const __grid_constant__ CUt
             };
             if (nt > 0) {
                 if (mask) fetch_mask(0);
-                ok = arrived(0);
                 const int clear = mask ? 0 : min(nt, max(0, least / KEYS - t0));   // tiles that every row sees whole
                 tiles(std::false_type(), 0, clear);
                 tiles(std::true_type(), clear, nt);
