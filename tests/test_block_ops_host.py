@@ -81,3 +81,23 @@ def test_binding_without_torch():
     code = "import sys; sys.path.insert(0, %r); import tsn; tsn.lib(); assert 'torch' not in sys.modules" % os.path.join(
         ROOT, "thinksound-native_b200")
     subprocess.run(["python3", "-c", code], check=True)
+
+
+def test_tensors_of_another_gpu_are_refused():
+    """An operator's tensors lie on its handle's GPU: not on another one, not in host memory."""
+    from tsn import block_ops
+
+    class Dev:
+        ordinal = 1
+
+    class On:
+        def __init__(self, gpu):
+            self.gpu = gpu
+
+        def get_device(self):
+            return self.gpu
+
+    block_ops._here(Dev, ("x", On(1)), ("y", None))
+    for gpu in (0, 2, -1):
+        with pytest.raises(ValueError, match="y must be a CUDA tensor on GPU 1"):
+            block_ops._here(Dev, ("x", On(1)), ("y", On(gpu)))

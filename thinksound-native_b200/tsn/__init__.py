@@ -229,6 +229,7 @@ class Device:
         h = C.c_void_p()
         check(lib().tsn_device_create(ordinal, C.byref(h)))
         self.h = h
+        self.ordinal = ordinal
         self._models = weakref.WeakSet()   # models must be freed before their device
         if stream is not None:
             check(lib().tsn_device_set_stream(self.h, C.c_void_p(stream)))

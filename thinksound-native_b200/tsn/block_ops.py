@@ -4,7 +4,9 @@
 Each object holds a layer's weights and options (kept alive by it) and is called with the tensors of one
 pass; results go into tensors that the caller owns. Calls are issued on the device handle's stream and do
 not synchronise. Tensors may have any strides whose last dimension is contiguous; what the library refuses
-raises :class:`tsn.TsnError`, what does not fit together raises :class:`ValueError` or :class:`TypeError`.
+raises :class:`tsn.TsnError`, what does not fit together, or lies on another GPU than the handle's, raises
+:class:`ValueError` or :class:`TypeError`. An object holds the arguments of its last call, so one thread at a time
+calls it.
 """
 from __future__ import annotations
 
@@ -19,12 +21,13 @@ NORMS = {"none": 0, "rms": 1, "layer": 2}
 LAYOUTS = {"interleaved": 0, "half": 1}
 
 
-def _weights(name, t, shape):
-    """A float32 weight on the GPU, contiguous; None stays None."""
+def _weights(dev, name, t, shape):
+    """A float32 weight on the handle's GPU, contiguous; None stays None."""
     if t is None:
         return None
-    if tuple(t.shape) != tuple(shape) or t.dtype is not torch.float32 or not t.is_cuda:
-        raise ValueError(f"{name} must be a float32 CUDA tensor of shape {tuple(shape)}")
+    if tuple(t.shape) != tuple(shape) or t.dtype is not torch.float32:
+        raise ValueError(f"{name} must be a float32 tensor of shape {tuple(shape)}")
+    _here(dev, (name, t))
     return t.contiguous()
 
 
@@ -44,8 +47,6 @@ def _put(view, name, t):
     st = t.stride()
     if st[-1] != 1 and t.shape[-1] > 1:
         raise ValueError(f"{name}: the last dimension must be contiguous")
-    if not t.is_cuda:
-        raise ValueError(f"{name} must be a CUDA tensor")
     view.sb = st[0]
     if len(st) == 3:
         view.st = st[1]
@@ -54,10 +55,17 @@ def _put(view, name, t):
         view.sh = st[2]
 
 
+def _here(dev, *named):
+    """Every tensor lies on the handle's GPU."""
+    for name, t in named:
+        if t is not None and t.get_device() != dev.ordinal:
+            raise ValueError(f"{name} must be a CUDA tensor on GPU {dev.ordinal}")
+
+
 def _form(*tensors):
     """What a call's checks go by: shape, strides, type and place of each tensor. A call of the same form as the
     one before needs only its addresses set; the checks, several microseconds of Python, are those of a new form."""
-    return [None if t is None else (t.shape, t.stride(), t.dtype, t.is_cuda) for t in tensors]
+    return [None if t is None else (t.shape, t.stride(), t.dtype, t.get_device()) for t in tensors]
 
 
 class BlockNorm:
@@ -74,7 +82,7 @@ class BlockNorm:
             raise ValueError("post and pre must be 'rms', 'layer' or 'none'")
         self.dev, self.C = dev, C_
         vec = residual_scale if isinstance(residual_scale, torch.Tensor) else None
-        self._keep = [_weights(n, t, (C_,)) for n, t in (("post_weight", post_weight), ("post_bias", post_bias),
+        self._keep = [_weights(dev, n, t, (C_,)) for n, t in (("post_weight", post_weight), ("post_bias", post_bias),
                                                          ("pre_weight", pre_weight), ("pre_bias", pre_bias),
                                                          ("residual_scale", vec))]
         a = BlockNormArgs()
@@ -102,6 +110,7 @@ class BlockNorm:
 
     def _check(self, x, y, gate, shift, scale, x_out, h):
         a = self._a
+        _here(self.dev, ("x", x), ("y", y), ("gate", gate), ("shift", shift), ("scale", scale), ("x_out", x_out), ("h", h))
         shape = x.shape
         if len(shape) != 3 or shape[2] != self.C:
             raise ValueError(f"x must be [B, T, {self.C}], got {tuple(shape)}")
@@ -151,7 +160,7 @@ class RopeAxes:
         self._plan = RopePlan()
         check(lib().tsn_rope_plan(head_dim, n, (C.c_uint32 * n)(*pairs), (C.c_double * n)(*theta),
                                   (C.c_double * n)(*scale), LAYOUTS[layout], C.byref(self._plan)))
-        self._keep = [_weights("q_norm", q_norm, (head_dim,)), _weights("k_norm", k_norm, (head_dim,))]
+        self._keep = [_weights(dev, "q_norm", q_norm, (head_dim,)), _weights(dev, "k_norm", k_norm, (head_dim,))]
         a = RopeArgs()
         a.eps = eps
         a.q_norm, a.k_norm = (_address(t) for t in self._keep)
@@ -181,6 +190,7 @@ class RopeAxes:
 
     def _check(self, q, k, pos, q_out, k_out):
         a = self._a
+        _here(self.dev, ("q", q), ("k", k), ("pos", pos), ("q_out", q_out), ("k_out", k_out))
         first = q if q is not None else k
         if first is None or first.dim() != 4:
             raise ValueError("q or k is wanted, [B, S, heads, head_dim]")
@@ -207,8 +217,8 @@ class RopeAxes:
         if pos.dtype is not torch.int32 or ps[-2:] != (S, self.axes) or (len(ps) == 3 and ps[0] not in (1, B)) or len(ps) > 3:
             raise ValueError(f"pos must be int32 [S, {self.axes}] or [B, S, {self.axes}]")
         st = pos.stride()
-        if not pos.is_cuda or (st[-1] != 1 and self.axes > 1):
-            raise ValueError("pos must be a CUDA tensor whose last dimension is contiguous")
+        if st[-1] != 1 and self.axes > 1:
+            raise ValueError("pos: the last dimension must be contiguous")
         a.pos_ss = st[-2]
         a.pos_sb = st[0] if len(ps) == 3 and ps[0] > 1 else 0
 
@@ -227,7 +237,7 @@ class DiffAttention:
         if shape[-1:] != (d,) or len(shape) > 2:
             raise ValueError(f"the lambda vectors must be [{d}] or [H, {d}]")
         self.heads = shape[0] if len(shape) == 2 else None
-        self._keep = [_weights(n, t, shape) for n, t in vectors] + [_weights("norm_weight", norm_weight, (2 * d,))]
+        self._keep = [_weights(dev, n, t, shape) for n, t in vectors] + [_weights(dev, "norm_weight", norm_weight, (2 * d,))]
         a = DiffAttnArgs()
         a.d, a.lambda_init, a.eps, a.scale = d, lambda_init, eps, 0.0 if scale is None else scale
         a.lq1, a.lk1, a.lq2, a.lk2, a.norm_w = (_address(t) for t in self._keep)
@@ -257,6 +267,7 @@ class DiffAttention:
 
     def _check(self, q, k, v, out, key_len, key_mask):
         a = self._a
+        _here(self.dev, ("q", q), ("k", k), ("v", v), ("out", out), ("key_len", key_len), ("key_mask", key_mask))
         if q.dim() != 4 or k.dim() != 4:
             raise ValueError("q and k must be [B, S, heads, 2 d]")
         B, Sq, H, D = q.shape
@@ -274,13 +285,13 @@ class DiffAttention:
         a.B, a.Sq, a.Sk, a.H, a.Hk, a.type = B, Sq, Sk, H, Hk, TYPES[dtype]
         for name, t in (("q", q), ("k", k), ("v", v), ("out", out)):
             _put(getattr(a, name), name, t)
-        if key_len is not None and (key_len.dtype is not torch.int32 or tuple(key_len.shape) != (B,) or not key_len.is_cuda
+        if key_len is not None and (key_len.dtype is not torch.int32 or tuple(key_len.shape) != (B,)
                                     or not key_len.is_contiguous()):
-            raise ValueError("key_len must be a contiguous int32 CUDA tensor of shape [B]")
+            raise ValueError("key_len must be a contiguous int32 tensor of shape [B]")
         if key_mask is not None:
             ms = key_mask.shape
             if key_mask.dtype not in (torch.uint8, torch.bool) or len(ms) != 2 or ms[1] != Sk or ms[0] not in (1, B):
                 raise ValueError("key_mask must be uint8 or bool [B or 1, Sk]")
-            if not key_mask.is_cuda or (key_mask.stride(1) != 1 and Sk > 1):
-                raise ValueError("key_mask must be a CUDA tensor whose last dimension is contiguous")
+            if key_mask.stride(1) != 1 and Sk > 1:
+                raise ValueError("key_mask: the last dimension must be contiguous")
             a.mask_sb = key_mask.stride(0) if ms[0] > 1 else 0
