@@ -7,9 +7,10 @@
 // once; with more the modulation is read when it is needed, as it would not fit in registers. The mean and the sum of
 // squared distances from it are two reductions: one pass over squares would lose the variance of a row whose
 // mean is large.
-// 32 500 rows of 2048 bf16 elements with a modulation of each token take 171 us (932 MB, 5.45 TB/s, 0.83 of the measured
-// copy), 658 rows of 1024 4.1 us (latency: two reductions after the loads).
+// 32 500 rows of 2048 bf16 elements with a modulation of each token take 170 us (932 MB, 5.47 TB/s, 0.84 of the measured
+// copy), 658 rows of 1024 4.0 us (latency: two reductions after the loads).
 #include "block_ops.h"
+#include "kernels.h"
 
 #include <algorithm>
 #include <type_traits>
@@ -138,6 +139,7 @@ constexpr int most_threads(int V, int NV, bool block) { return !block ? 128 : V 
 template <class TX, class T, int V, int NV, bool BLOCK>
 __global__ void __launch_bounds__(most_threads(V, NV, BLOCK)) block_norm_kernel(const __grid_constant__ NormArgs n) {
     __shared__ float red[BLOCK ? 128 : 1];
+    pdl_wait();   // and no trigger: the next kernel's blocks beside this one's made 658 rows take 5.0 us instead of 4.0
     const tsn_block_norm_args & a = n.a;
     const int C = (int) a.C;
     const float inv_C = 1.0f / (float) C;
@@ -233,24 +235,27 @@ template <class TX, class T, int V>
 cudaError_t launch(const NormArgs & n, cudaStream_t s) {
     const int pieces = ((int) n.a.C + V - 1) / V;
     const dim3 grid = n.swapped ? dim3(n.a.B, n.a.T) : dim3(n.a.T, n.a.B);
+    cudaError_t e = cudaSuccess;
+    auto go = [&](void (*kernel)(NormArgs), int threads) { e = launch_cl(kernel, grid, dim3((unsigned) threads), 0, s, dim3(1), n); };
     if (pieces <= 32) {
-        block_norm_kernel<TX, T, V, 1, false><<<(n.rows + 3) / 4, 128, 0, s>>>(n);
+        e = launch_cl(block_norm_kernel<TX, T, V, 1, false>, dim3((n.rows + 3) / 4), dim3(128), 0, s, dim3(1), n);
     } else if constexpr (V == 1) {   // unaligned rows
         const int threads = std::min(1024, (pieces + 127) / 128 * 32);
-        if (pieces <= 4 * threads) block_norm_kernel<TX, T, V, 4, true><<<grid, threads, 0, s>>>(n);
-        else block_norm_kernel<TX, T, V, 16, true><<<grid, threads, 0, s>>>(n);
+        if (pieces <= 4 * threads) go(block_norm_kernel<TX, T, V, 4, true>, threads);
+        else go(block_norm_kernel<TX, T, V, 16, true>, threads);
     } else {
         // One piece a thread while a block of 512 holds the row: the least latency where there are few rows (658
         // rows of 1024: 4.2 us, 4.8 with two pieces, 8.6 with four), and no slower where rows fill the GPU (32 500 of
         // 2048: 174, 175 and 233 us).
         const int per = pieces > 2048 ? 8 : pieces > 1024 ? 4 : pieces > 512 ? 2 : 1;
         const int threads = (pieces + 32 * per - 1) / (32 * per) * 32;
-        if (per == 1) block_norm_kernel<TX, T, V, 1, true><<<grid, threads, 0, s>>>(n);
-        else if (per == 2) block_norm_kernel<TX, T, V, 2, true><<<grid, threads, 0, s>>>(n);
-        else if (per == 4) block_norm_kernel<TX, T, V, 4, true><<<grid, threads, 0, s>>>(n);
-        else if constexpr (V < 8) block_norm_kernel<TX, T, V, 8, true><<<grid, threads, 0, s>>>(n);   // 2048 pieces of 8 are 16384
+        if (per == 1) go(block_norm_kernel<TX, T, V, 1, true>, threads);
+        else if (per == 2) go(block_norm_kernel<TX, T, V, 2, true>, threads);
+        else if (per == 4) go(block_norm_kernel<TX, T, V, 4, true>, threads);
+        else if constexpr (V < 8) go(block_norm_kernel<TX, T, V, 8, true>, threads);   // 2048 pieces of 8 are 16384
     }
-    return cudaGetLastError();
+    if (e != cudaSuccess) cudaGetLastError();
+    return e;
 }
 
 template <class TX, class T>

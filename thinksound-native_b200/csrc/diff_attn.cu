@@ -12,6 +12,7 @@
 // key is marked: its result is NaN.
 // Every wait is bounded; barriers of a whole block or cluster are on paths that all threads take.
 #include "block_ops.h"
+#include "kernels.h"
 #include "ptx.cuh"
 
 #include <cudaTypedefs.h>
@@ -282,6 +283,18 @@ diff_attn_tc(const __grid_constant__ CUtensorMap tk, const __grid_constant__ CUt
     volatile int * abort_flag = (volatile int *) (words + 1);
     static_assert((1 + 3 * L::STAGES + 6 * BUF) * 8 + (2 + 2 * L::STAGES) * 4 <= 320, "barriers");
 
+    if (tid == 0) {
+        mbar_init(q_full, 8);
+        for (int s = 0; s < L::STAGES; ++s) { mbar_init(&full[s], 1); mbar_init(&empty[s], 2); mbar_init(&v_ready[s], 1); }
+        for (int x = 0; x < 2 * BUF; ++x) { mbar_init(&s_full[x], 1); mbar_init(&p_full[x], 4); mbar_init(&o_full[x], 1); }
+        *abort_flag = 0;
+        fence_mbar_init();
+    }
+    if (warp == 8 && lane == 0 && a.Sk > 0) { tma_prefetch(&tk); tma_prefetch(&tv); }
+    pdl_wait();   // from here on memory that earlier work may have written or may still read
+    // Tensor memory after the wait and before the trigger: of two kernels on one SM, neither can hold what the other waits for.
+    if (warp == 9) tmem_alloc(words, L::TM);
+
     // this CTA's rows, keys and part of them; long rows of a causal call come first
     const unsigned gid = blockIdx.x / p.splits, split = blockIdx.x % p.splits;
     const int hk = (int) (gid % a.Hk), b = (int) (gid / a.Hk % a.B);
@@ -299,15 +312,6 @@ diff_attn_tc(const __grid_constant__ CUtensorMap tk, const __grid_constant__ CUt
     auto mixed = [&](int base) { return a.causal && least < min(n, base + KEYS); };   // rows see different keys of the tile
     const bool mend = nt > 0 && (mask || (t0 + nt) * KEYS > n || mixed((t0 + nt - 1) * KEYS));
 
-    if (tid == 0) {
-        mbar_init(q_full, 8);
-        for (int s = 0; s < L::STAGES; ++s) { mbar_init(&full[s], 1); mbar_init(&empty[s], 2); mbar_init(&v_ready[s], 1); }
-        for (int x = 0; x < 2 * BUF; ++x) { mbar_init(&s_full[x], 1); mbar_init(&p_full[x], 4); mbar_init(&o_full[x], 1); }
-        *abort_flag = 0;
-        fence_mbar_init();
-    }
-    if (warp == 8 && lane == 0 && nt > 0) { tma_prefetch(&tk); tma_prefetch(&tv); }
-    if (warp == 9) tmem_alloc(words, L::TM);
     uint4 q[ROWS * CH / 256];   // Q, on its way while the barriers and tensor memory are set up
     if (warp < 8) {
 #pragma unroll
@@ -434,6 +438,7 @@ diff_attn_tc(const __grid_constant__ CUtensorMap tk, const __grid_constant__ CUt
         }
         // the barriers of the other warps' results
         __syncwarp();
+        pdl_trigger();
         if (p.splits > 1) {
             __syncthreads();
             cluster_sync_all();
@@ -570,6 +575,7 @@ diff_attn_tc(const __grid_constant__ CUtensorMap tk, const __grid_constant__ CUt
             __syncwarp();
             tc_fence_after();
         }
+        pdl_trigger();
         // ------------------------------------------------------------ results
         if (p.splits > 1) {
             // this part's sums in place of K and V: [row][row_words], a row 16 bytes past a multiple of all banks
@@ -731,8 +737,8 @@ diff_attn_tc(const __grid_constant__ CUtensorMap tk, const __grid_constant__ CUt
 // Each warp streams its own 16-key slabs (slab w, w + W, ...) by TMA through a ring of its own, so warps never wait
 // for one another: scores, online softmax and O of both maps stay in the warp's registers. The warps' sums
 // are added up in shared memory at the end, the parts of split keys through the workspace.
-// One token over four caches of 20 480 to 32 768 keys (32 heads over 8, bf16) takes 74.6 us: 436 MB, 5.85 TB/s, 0.89 of the
-// measured copy; one over two caches of up to 704 keys 9.1 us, most of it the way from the launch to the first keys.
+// One token over four caches of 20 480 to 32 768 keys (32 heads over 8, bf16) takes 73.2 us: 436 MB, 5.95 TB/s, 0.91 of the
+// measured copy; one over two caches of up to 704 keys 8.8 us, most of it the way from the launch to the first keys.
 constexpr int SLAB = 16, RING = 3, SOME = 8, W = 8;   // keys of a slab, slabs of a ring, rows of a group, warps
 constexpr int FEW = 32;                        // rows up to which groups of 8 beat a tile of 128
 
@@ -790,6 +796,12 @@ diff_attn_rows(const __grid_constant__ CUtensorMap tk, const __grid_constant__ C
     const unsigned groups = gridDim.x / p.splits, gid = blockIdx.x % groups, split = blockIdx.x / groups;
     const int hk = (int) (gid / eights % a.Hk), b = (int) (gid / eights / a.Hk);
     const int first = (int) (gid % eights) * SOME, R = min(SOME, p.R - first);   // row r: token (first + r) / G, head (first + r) % G
+    if (lane == 0) {
+        if (a.Sk > 0) { tma_prefetch(&tk); tma_prefetch(&tv); }
+        for (int s = 0; s < RING; ++s) mbar_init(&full[s], 1);
+        fence_mbar_init();
+    }
+    pdl_wait();
     const int n = a.key_len ? max(0, min(a.key_len[b], (int) a.Sk)) : (int) a.Sk;
     auto limit = [&](int r) {   // keys before which row r sees; rows past the last one see all
         if (!a.causal || r >= R) return n;
@@ -802,11 +814,6 @@ diff_attn_rows(const __grid_constant__ CUtensorMap tk, const __grid_constant__ C
     const int mine = s1 - s0 > warp ? (s1 - s0 - warp + W - 1) / W : 0;
 
     if (tid == 0) flags[0] = 0;
-    if (lane == 0) {
-        if (mine > 0) { tma_prefetch(&tk); tma_prefetch(&tv); }
-        for (int s = 0; s < RING; ++s) mbar_init(&full[s], 1);
-        fence_mbar_init();
-    }
     __syncwarp();
     uint8_t * ring = smem + warp * RING * L::STAGE;
     auto request = [&](int i) {   // slab i of this warp, one lane
@@ -975,6 +982,7 @@ diff_attn_rows(const __grid_constant__ CUtensorMap tk, const __grid_constant__ C
         if (lane == 0 && i + RING < mine) request(i + RING);
     }
 
+    pdl_trigger();   // from here on little memory is read: the next kernel's blocks would have taken bandwidth before
     // the warp's sums in its ring, then warp w adds up rows w, w + W, ... of all warps
     float * sums = (float *) ring;
 #pragma unroll
@@ -1093,22 +1101,11 @@ int workspace(DeviceCtx & c, bool capturing) {
 
 template <int D, bool BF16>
 cudaError_t launch_tc(const CUtensorMap & tk, const CUtensorMap & tv, const Args & p, unsigned grid, cudaStream_t s) {
-    cudaLaunchConfig_t cfg{};
-    cfg.gridDim = dim3(grid);
-    cfg.blockDim = dim3(THREADS);
-    cfg.dynamicSmemBytes = Lay<D>::TOTAL;
-    cfg.stream = s;
-    cudaLaunchAttribute at{};
-    at.id = cudaLaunchAttributeClusterDimension;
-    at.val.clusterDim = {(unsigned) p.splits, 1, 1};
-    cfg.attrs = &at;
-    cfg.numAttrs = p.splits > 1 ? 1 : 0;
-    return cudaLaunchKernelEx(&cfg, diff_attn_tc<D, BF16>, tk, tv, p);
+    return launch_cl(diff_attn_tc<D, BF16>, dim3(grid), dim3(THREADS), Lay<D>::TOTAL, s, dim3((unsigned) p.splits), tk, tv, p);
 }
 template <int D, bool BF16>
 cudaError_t launch_rows(const CUtensorMap & tk, const CUtensorMap & tv, const Args & p, unsigned grid, cudaStream_t s) {
-    diff_attn_rows<D, BF16><<<grid, 32 * W, RowLay<D>::TOTAL, s>>>(tk, tv, p);
-    return cudaGetLastError();
+    return launch_cl(diff_attn_rows<D, BF16>, dim3(grid), dim3(32 * W), RowLay<D>::TOTAL, s, dim3(1), tk, tv, p);
 }
 
 // clusters of 1 to 8 CTAs of diff_attn_tc that run at once (one CTA per SM; a cluster lies within a GPC)
@@ -1238,6 +1235,7 @@ int diff_attn(DeviceCtx & c, const tsn_diff_attn_args & in) {
     else
         e = a.d == 32 ? (bf ? launch_tc<64, true>(tk, tv, p, grid, c.stream) : launch_tc<64, false>(tk, tv, p, grid, c.stream))
                       : (bf ? launch_tc<128, true>(tk, tv, p, grid, c.stream) : launch_tc<128, false>(tk, tv, p, grid, c.stream));
+    if (e != cudaSuccess) cudaGetLastError();
     if (e == cudaSuccess && shared) {
         cudaStreamCaptureStatus st = cudaStreamCaptureStatusNone;
         e = cudaStreamIsCapturing(c.stream, &st);

@@ -12,6 +12,7 @@
 #include <type_traits>
 
 #include "block_ops.h"
+#include "kernels.h"
 
 namespace tsn {
 
@@ -52,7 +53,7 @@ enum { NEXT, LANES, SHARED };   // interleaved: its own; halves: another lane's 
 // D / 8 up. Block (x, b, z): tokens x * tok .. of sequence b, chunks 8 z .. of 32 / LPH heads. A warp takes one chunk,
 // queries' or keys', through the block's tokens, so that a token costs its lanes a load, a store and the
 // arithmetic; with fewer chunks than warps, several warps share a chunk's tokens.
-// Loads run one round ahead of the arithmetic: 32 500 tokens x 64 heads of 64, bf16, written head-major, take 102 us
+// Loads run one round ahead of the arithmetic: 32 500 tokens x 64 heads of 64, bf16, written head-major, take 101 us
 // (5.2 TB/s, 0.80 of the measured copy) with two tokens a round at four blocks per SM; 110 with one, 108 with four at
 // fewer blocks, 113 without the round ahead. With 16 tokens a block 104, with 32 113.
 template <class T, int LPH, int PAIR>
@@ -60,6 +61,7 @@ __global__ void __launch_bounds__(32 * WARPS, 4) rope_rows8(const __grid_constan
     constexpr int SIDE = 32 / LPH, AHEAD = sizeof(T) == 4 ? 1 : 2;   // tokens of a round: 16 or 32 bytes a lane each
     __shared__ __align__(16) float2 turn[MAX_TOK * TSN_ROPE_MAX_PAIRS + 8];
     __shared__ float mate[PAIR == SHARED ? WARPS : 1][32 * 9];   // a lane's 8 elements, one word of padding between lanes
+    pdl_wait();
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int D = (int) p.D, P = (int) p.P, Hq = a.q.p ? (int) a.Hq : 0, Hk = a.k.p ? (int) a.Hk : 0;
     const long long b = blockIdx.y, s0 = (long long) blockIdx.x * tok;
@@ -177,6 +179,7 @@ __global__ void __launch_bounds__(32 * WARPS, 4) rope_rows8(const __grid_constan
 template <class T>
 __global__ void __launch_bounds__(32 * WARPS) rope_rows1(const __grid_constant__ tsn_rope_plan_t p, const __grid_constant__ tsn_rope_args a) {
     __shared__ float buf[WARPS][2 * TSN_ROPE_MAX_PAIRS];
+    pdl_wait();
     const int lane = threadIdx.x & 31, D = (int) p.D, P = (int) p.P, Hq = a.q.p ? (int) a.Hq : 0, H = Hq + (a.k.p ? (int) a.Hk : 0);
     const long long item = (long long) blockIdx.x * WARPS + (threadIdx.x >> 5);
     if (item >= (long long) a.B * a.S * H) return;
@@ -213,6 +216,7 @@ cudaError_t launch(const tsn_rope_plan_t & p, const tsn_rope_args & a, cudaStrea
     };
     const long long tokens = (long long) a.B * a.S;
     const int H = (int) ((a.q.p ? a.Hq : 0) + (a.k.p ? a.Hk : 0));
+    cudaError_t e = cudaSuccess;
     if (p.D % 8 == 0 && a.B <= 65535 && rows16(a.q, a.Hq) && rows16(a.k, a.Hk) && (!a.q.p || rows16(a.q_out, a.Hq)) && (!a.k.p || rows16(a.k_out, a.Hk))) {
         int lph = 1;
         while (lph * 8 < (int) p.D) lph *= 2;
@@ -225,9 +229,9 @@ cudaError_t launch(const tsn_rope_plan_t & p, const tsn_rope_args & a, cudaStrea
         const int pair = p.layout == TSN_ROPE_INTERLEAVED ? NEXT : p.P % 8 == 0 ? LANES : SHARED;
         auto go = [&](auto L) {
             constexpr int LPH = decltype(L)::value;
-            if (pair == NEXT) rope_rows8<T, LPH, NEXT><<<blocks, 32 * WARPS, 0, s>>>(p, a, tok);
-            else if (pair == LANES) rope_rows8<T, LPH, LANES><<<blocks, 32 * WARPS, 0, s>>>(p, a, tok);
-            else rope_rows8<T, LPH, SHARED><<<blocks, 32 * WARPS, 0, s>>>(p, a, tok);
+            if (pair == NEXT) e = launch_cl(rope_rows8<T, LPH, NEXT>, blocks, dim3(32 * WARPS), 0, s, dim3(1), p, a, tok);
+            else if (pair == LANES) e = launch_cl(rope_rows8<T, LPH, LANES>, blocks, dim3(32 * WARPS), 0, s, dim3(1), p, a, tok);
+            else e = launch_cl(rope_rows8<T, LPH, SHARED>, blocks, dim3(32 * WARPS), 0, s, dim3(1), p, a, tok);
         };
         if (lph == 1) go(std::integral_constant<int, 1>());
         else if (lph == 2) go(std::integral_constant<int, 2>());
@@ -236,9 +240,10 @@ cudaError_t launch(const tsn_rope_plan_t & p, const tsn_rope_args & a, cudaStrea
         else if (lph == 16) go(std::integral_constant<int, 16>());
         else go(std::integral_constant<int, 32>());
     } else {
-        rope_rows1<T><<<(unsigned) ((tokens * H + WARPS - 1) / WARPS), 32 * WARPS, 0, s>>>(p, a);
+        e = launch_cl(rope_rows1<T>, dim3((unsigned) ((tokens * H + WARPS - 1) / WARPS)), dim3(32 * WARPS), 0, s, dim3(1), p, a);
     }
-    return cudaGetLastError();
+    if (e != cudaSuccess) cudaGetLastError();
+    return e;
 }
 
 } // namespace
