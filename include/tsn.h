@@ -421,6 +421,29 @@ typedef struct tsn_diff_attn_args {
 } tsn_diff_attn_args;
 int tsn_diff_attn(tsn_device * dev, const tsn_diff_attn_args * a);
 
+/* For a Python binding of the three operators: a call whose tensors have the form of the call before (shape,
+ * strides, type, place) needs no checks, only their addresses. `view` is the function of the tensor type's DLPack
+ * exchange table that describes an object as a DLTensor, `item` the interpreter's PyTuple_GetItem, `type` the objects'
+ * exact type, `none` the None object. tsn_form_take takes a tuple of n objects, writes their addresses (null for
+ * None) to *to[i] and returns 1 if every one has
+ * the recorded form, or, with `record`, records the forms. Otherwise it returns 0, what lies at *to[i] is undefined,
+ * and nothing is recorded any more. The caller holds the interpreter's lock. Host only. */
+enum { TSN_FORM_TENSORS = 7 };
+typedef struct tsn_form_tensor {
+    int32_t there, device_type, device, ndim;
+    uint32_t dtype;
+    int64_t shape[4], strides[4];
+} tsn_form_tensor;
+typedef struct tsn_form {
+    int (*view)(void * object, void * dl_tensor);
+    void * (*item)(void * tuple, intptr_t i);
+    void * type, * none;
+    uint32_t n, valid;
+    void ** to[TSN_FORM_TENSORS];
+    tsn_form_tensor t[TSN_FORM_TENSORS];
+} tsn_form;
+int tsn_form_take(tsn_form * f, int record, void * tuple);
+
 /* ------------------------------------------------------------------ fixtures */
 /* Write the seeded synthetic DiT GGUF (with_prep adds the conditioning-prep tensors). Host only. */
 int tsn_gguf_write_synthetic(const char * path, const tsn_dit_geom * g, uint64_t seed, int with_prep);

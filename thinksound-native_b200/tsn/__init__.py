@@ -82,7 +82,18 @@ class DiffAttnArgs(C.Structure):
                 + [("lam_sh", C.c_int64), ("norm_w", C.c_void_p)])
 
 
+class FormTensor(C.Structure):
+    _fields_ = ([(n, C.c_int32) for n in ("there", "device_type", "device", "ndim")] + [("dtype", C.c_uint32)]
+                + [(n, C.c_int64 * 4) for n in ("shape", "strides")])
+
+
+class Form(C.Structure):
+    _fields_ = [("view", C.c_void_p), ("item", C.c_void_p), ("type", C.c_void_p), ("none", C.c_void_p), ("n", C.c_uint32), ("valid", C.c_uint32),
+                ("to", C.c_void_p * 7), ("t", FormTensor * 7)]
+
+
 _lib = None
+_form_take = None
 
 # (name, restype, argtypes)
 _SIGS = [
@@ -201,6 +212,17 @@ def lib():
             fn.argtypes = args
         _lib = L
     return _lib
+
+
+def form_take():
+    """tsn_form_take, called with the interpreter's lock held: it looks into Python objects."""
+    global _form_take
+    if _form_take is None:
+        lib()
+        fn = C.PyDLL(LIB_PATH).tsn_form_take
+        fn.restype, fn.argtypes = C.c_int, [C.POINTER(Form), C.c_int, C.py_object]
+        _form_take = fn
+    return _form_take
 
 
 def check(rc: int):

@@ -11,10 +11,11 @@ calls it.
 from __future__ import annotations
 
 import ctypes as C
+import sys
 
 import torch
 
-from . import BlockNormArgs, DiffAttnArgs, RopeArgs, RopePlan, check, lib
+from . import BlockNormArgs, DiffAttnArgs, Form, RopeArgs, RopePlan, check, form_take, lib
 
 TYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
 NORMS = {"none": 0, "rms": 1, "layer": 2}
@@ -58,14 +59,54 @@ def _put(view, name, t):
 def _here(dev, *named):
     """Every tensor lies on the handle's GPU."""
     for name, t in named:
-        if t is not None and t.get_device() != dev.ordinal:
+        if t is not None and (t.get_device() != dev.ordinal or getattr(t, "is_meta", False)):
             raise ValueError(f"{name} must be a CUDA tensor on GPU {dev.ordinal}")
 
 
-def _form(*tensors):
-    """What a call's checks go by: shape, strides, type and place of each tensor. A call of the same form as the
-    one before needs only its addresses set; the checks, several microseconds of Python, are those of a new form."""
-    return [None if t is None else (t.shape, t.stride(), t.dtype, t.get_device()) for t in tensors]
+def _view():
+    """The address of the function that describes a torch tensor as a DLTensor, from torch's DLPack exchange table
+    (ABI version 1: version, previous table, then five functions, this one the fourth); 0 where there is none."""
+    table = getattr(torch.Tensor, "__dlpack_c_exchange_api__", None)
+    if table is None or object.__basicsize__ != 16 or not getattr(sys, "_is_gil_enabled", lambda: True)():
+        return 0
+    get = C.PyDLL(None).PyCapsule_GetPointer
+    get.restype, get.argtypes = C.c_void_p, [C.py_object, C.c_char_p]
+    at = get(table, b"dlpack_exchange_api")
+    if C.c_uint32.from_address(at).value != 1:
+        return 0
+    return C.c_void_p.from_address(at + 5 * C.sizeof(C.c_void_p)).value or 0
+
+
+_VIEW, _take, _python = _view(), form_take(), C.PyDLL(None)
+
+
+def _form_of(*places):
+    """A call's form and a reference to it: the tensors' addresses go to `places`."""
+    f = Form()
+    f.view, f.item = _VIEW, C.cast(_python.PyTuple_GetItem, C.c_void_p)
+    f.type, f.none, f.n = id(torch.Tensor), id(None), len(places)
+    for i, p in enumerate(places):
+        f.to[i] = p
+    return f, C.byref(f)
+
+
+def _known(ref, tensors):
+    """Whether the tensors have the form of the call before; then their addresses are set. What the view refuses (a
+    tensor without storage, say) goes through the checks instead."""
+    try:
+        return _take(ref, 0, tensors)
+    except (BufferError, RuntimeError):
+        return 0
+
+
+def _record(ref, tensors):
+    """Records the form of tensors that have passed the checks, several microseconds of Python, for the next call."""
+    if not _VIEW:
+        return
+    try:
+        _take(ref, 1, tensors)
+    except (BufferError, RuntimeError):
+        pass
 
 
 class BlockNorm:
@@ -89,21 +130,20 @@ class BlockNorm:
         a.C, a.post, a.pre, a.gate_tanh = C_, NORMS[post], NORMS[pre], int(gate_tanh)
         a.post_eps, a.pre_eps, a.res_scale = post_eps, pre_eps, 1.0 if vec is not None else residual_scale
         a.post_w, a.post_b, a.pre_w, a.pre_b, a.res_vec = (_address(t) for t in self._keep)
-        self._a, self._ref, self._form, self._call = a, C.byref(a), None, lib().tsn_block_norm
+        self._a, self._ref, self._call = a, C.byref(a), lib().tsn_block_norm
         self._views = a.x, a.y, a.gate, a.shift, a.scale, a.x_out, a.h
+        self._form, self._formed = _form_of(*(C.addressof(v) for v in self._views))
 
     def __call__(self, x, y=None, gate=None, shift=None, scale=None, x_out=None, h=None):
         """x, x_out [B, T, C] of the residual's type; y, h [B, T, C] of the branch's type, which is the residual's or
         narrower than its float32; gate, shift, scale [B or 1, T or 1, C] of the branch's type, each or None.
         x_out may be x and h may be y."""
-        tensors = (x, y, gate, shift, scale, x_out, h)
-        form = _form(*tensors)
-        if form != self._form:
-            self._form = None
+        tensors = x, y, gate, shift, scale, x_out, h
+        if not _known(self._formed, tensors):
             self._check(*tensors)
-            self._form = form
-        for view, t in zip(self._views, tensors):
-            view.p = None if t is None else t.data_ptr()
+            _record(self._formed, tensors)
+            for view, t in zip(self._views, tensors):
+                view.p = _address(t)
         rc = self._call(self.dev.h, self._ref)
         if rc:
             check(rc)
@@ -164,9 +204,10 @@ class RopeAxes:
         a = RopeArgs()
         a.eps = eps
         a.q_norm, a.k_norm = (_address(t) for t in self._keep)
-        self._a, self._ref, self._plan_ref, self._form = a, C.byref(a), C.byref(self._plan), None
+        self._a, self._ref, self._plan_ref = a, C.byref(a), C.byref(self._plan)
         self._call = lib().tsn_rope_axes
         self._views = a.q, a.k, a.q_out, a.k_out
+        self._form, self._formed = _form_of(*(C.addressof(v) for v in self._views), C.addressof(a) + RopeArgs.pos.offset)
 
     def __call__(self, q, k, pos, q_out=None, k_out=None):
         """q [B, S, Hq, head_dim] and k [B, S, Hk, head_dim], either may be None; pos int32 [S, axes] or [B, S, axes].
@@ -175,15 +216,13 @@ class RopeAxes:
             q_out = q
         if k_out is None:
             k_out = k
-        tensors = (q, k, q_out, k_out)
-        form = _form(q, k, q_out, k_out, pos)
-        if form != self._form:
-            self._form = None
+        tensors = q, k, q_out, k_out, pos
+        if not _known(self._formed, tensors):
             self._check(q, k, pos, q_out, k_out)
-            self._form = form
-        for view, t in zip(self._views, tensors):
-            view.p = None if t is None else t.data_ptr()
-        self._a.pos = pos.data_ptr()
+            _record(self._formed, tensors)
+            for view, t in zip(self._views, tensors):
+                view.p = _address(t)
+            self._a.pos = pos.data_ptr()
         rc = self._call(self.dev.h, self._plan_ref, self._ref)
         if rc:
             check(rc)
@@ -242,24 +281,23 @@ class DiffAttention:
         a.d, a.lambda_init, a.eps, a.scale = d, lambda_init, eps, 0.0 if scale is None else scale
         a.lq1, a.lk1, a.lq2, a.lk2, a.norm_w = (_address(t) for t in self._keep)
         a.lam_sh = d if self.heads else 0
-        self._a, self._ref, self._form, self._call = a, C.byref(a), None, lib().tsn_diff_attn
+        self._a, self._ref, self._call = a, C.byref(a), lib().tsn_diff_attn
         self._views = a.q, a.k, a.v, a.out
+        self._form, self._formed = _form_of(*(C.addressof(v) for v in self._views), C.addressof(a) + DiffAttnArgs.key_len.offset,
+                                            C.addressof(a) + DiffAttnArgs.key_mask.offset)
 
     def __call__(self, q, k, v, out, key_len=None, key_mask=None, causal: bool = False):
         """q, out [B, Sq, H, 2 d], k, v [B, Sk, Hk, 2 d], all float16 or bfloat16. key_len: int32 [B], the keys each
         sequence has; key_mask: uint8 or bool [B or 1, Sk], nonzero where a key is seen; causal: counted from the
         end, the last query sees the last key."""
         a = self._a
-        tensors = (q, k, v, out)
-        form = _form(q, k, v, out, key_len, key_mask)
-        if form != self._form:
-            self._form = None
-            self._check(q, k, v, out, key_len, key_mask)
-            self._form = form
-        for view, t in zip(self._views, tensors):
-            view.p = t.data_ptr()
-        a.key_len = None if key_len is None else key_len.data_ptr()
-        a.key_mask = None if key_mask is None else key_mask.data_ptr()
+        tensors = q, k, v, out, key_len, key_mask
+        if not _known(self._formed, tensors):
+            self._check(*tensors)
+            _record(self._formed, tensors)
+            for view, t in zip(self._views, tensors):
+                view.p = t.data_ptr()
+            a.key_len, a.key_mask = _address(key_len), _address(key_mask)
         a.causal = 1 if causal else 0
         rc = self._call(self.dev.h, self._ref)
         if rc:
