@@ -7,7 +7,7 @@
 // once; with more the modulation is read when it is needed, as it would not fit in registers. The mean and the sum of
 // squared distances from it are two reductions: one pass over squares would lose the variance of a row whose
 // mean is large.
-// 32 500 rows of 2048 bf16 elements with a modulation of each token take 170 us (932 MB, 5.47 TB/s, 0.84 of the measured
+// 32 500 rows of 2048 bf16 elements with a modulation of each token take 153 us (932 MB, 6.08 TB/s, 0.93 of the measured
 // copy), 658 rows of 1024 4.0 us (latency: two reductions after the loads).
 #include "block_ops.h"
 #include "kernels.h"
@@ -62,12 +62,17 @@ template <int V>
 __device__ __forceinline__ float2 at2(const float * v, int k) { return make_float2(v[k], V == 1 ? 0.0f : v[k + (V > 1)]); }
 __device__ __forceinline__ float2 both(float v) { return make_float2(v, v); }
 
-// tanh(x) = 1 - 2 / (e^(2x) + 1). For 16-bit gates: off by 2^-22 at most, where the gate itself is known to 2^-12
-// of its value; the library's tanhf, exact to its last bits near 0 as well, would cost more than the row's traffic.
+// tanh of a gate. bf16 gates, known to 2^-9 of their value, take the hardware's (off by 2^-11 of it). f16 gates take
+// 1 - 2 / (e^(2x) + 1), off by 2^-22 at most, where the gate itself is known to 2^-12 of its value; the library's tanhf,
+// exact to its last bits near 0 as well, would cost more than the row's traffic.
 template <class T>
 __device__ __forceinline__ float gate_tanh(float x) {
     if (sizeof(T) == 4) return tanhf(x);
     float e, r;
+    if (std::is_same<T, __nv_bfloat16>::value) {
+        asm("tanh.approx.f32 %0, %1;" : "=f"(r) : "f"(x));
+        return r;
+    }
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(x * 2.88539008177792681f));
     asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(e + 1.0f));
     return fmaf(-2.0f, r, 1.0f);
@@ -245,9 +250,11 @@ cudaError_t launch(const NormArgs & n, cudaStream_t s) {
         else go(block_norm_kernel<TX, T, V, 16, true>, threads);
     } else {
         // One piece a thread while a block of 512 holds the row: the least latency where there are few rows (658
-        // rows of 1024: 4.2 us, 4.8 with two pieces, 8.6 with four), and no slower where rows fill the GPU (32 500 of
-        // 2048: 174, 175 and 233 us).
-        const int per = pieces > 2048 ? 8 : pieces > 1024 ? 4 : pieces > 512 ? 2 : 1;
+        // rows of 1024: 4.0 us, 4.8 with two pieces, 8.6 with four). Two, half the reductions, where the rows fill the GPU
+        // eight times (32 500 of 2048 bf16: 153 us, 166 with one; 2400: 18.1 and 17.1), and for wide rows of 16 bits
+        // from eight rows an SM on (2400 of 4096: 32.6 and 35.5; 600: no difference).
+        const bool two = pieces > 64 && ((long long) n.rows * pieces >= 8ll * 148 * 2048 || (V == 8 && pieces > 256 && n.rows >= 8 * 148));
+        const int per = pieces > 2048 ? 8 : pieces > 1024 ? 4 : pieces > 512 || two ? 2 : 1;
         const int threads = (pieces + 32 * per - 1) / (32 * per) * 32;
         if (per == 1) go(block_norm_kernel<TX, T, V, 1, true>, threads);
         else if (per == 2) go(block_norm_kernel<TX, T, V, 2, true>, threads);
