@@ -196,7 +196,7 @@ _SIGS = [
     ("tsn_gguf_write_synthetic_vae", C.c_int, [C.c_char_p, C.c_uint32, C.c_uint32, C.c_uint32, C.c_uint64]),
 ]
 
-EXPORTED = [s[0] for s in _SIGS]
+EXPORTED = [s[0] for s in _SIGS] + ["tsn_form_take"]   # bound by form_take
 
 
 def lib():
