@@ -343,7 +343,7 @@ typedef struct tsn_heads { void * p; int64_t sb, ss, sh; } tsn_heads;
  * (0), weights (1), biases (0); x_out or h may be absent, not both. x and x_out are of xtype, which
  * is `type` or TSN_F32; y, h, gate, shift and scale are of `type`; weights, biases and res_vec are f32.
  * x_out may be x, and h may be y, at the same strides. C 1..16384; any strides and alignment (rows that
- * all start at 16-byte boundaries are read 16 bytes at a time). */
+ * all start at 16-byte boundaries are read 16 bytes at a time, at pairs of elements a pair at a time). */
 typedef struct tsn_block_norm_args {
     uint32_t B, T, C;
     int32_t xtype, type, post, pre, gate_tanh;

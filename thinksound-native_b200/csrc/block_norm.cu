@@ -25,23 +25,36 @@ struct NormArgs {
     int swapped;   // one row a block: the batch runs along x instead of y
 };
 
-// V elements of type T: 16-byte words where a piece has some, else the elements themselves.
+// V elements of type T: 16-byte words where a piece has some, else a pair in one word or the element itself.
 template <class T, int V>
 struct Piece {
     static constexpr bool WIDE = sizeof(T) * V >= 16;
-    typename std::conditional<WIDE, Words<T, WIDE ? V : 16>, T>::type r;
+    using Pair = typename std::conditional<sizeof(T) == 4, float2, uint32_t>::type;
+    typename std::conditional<WIDE, Words<T, WIDE ? V : 16>, typename std::conditional<V == 2, Pair, T>::type>::type r;
     __device__ __forceinline__ void load(const T * p) {
         if constexpr (WIDE) r = load_words<T, V>(p);
+        else if constexpr (V == 2) r = *(const Pair *) p;
         else r = *p;
     }
     __device__ __forceinline__ void get(float * v) const {
-        if constexpr (WIDE) to_floats<T, V>(r, v);
-        else *v = to_f32(r);
+        if constexpr (WIDE) {
+            to_floats<T, V>(r, v);
+        } else if constexpr (V == 2) {
+            float2 f;
+            if constexpr (sizeof(T) == 4) f = r;
+            else f = unpack2<T>(r);
+            v[0] = f.x;
+            v[1] = f.y;
+        } else {
+            *v = to_f32(r);
+        }
     }
 };
 template <class T, int V>
 __device__ __forceinline__ void store(T * p, const float * v) {
     if constexpr (Piece<T, V>::WIDE) store_words<T, V>(p, v);
+    else if constexpr (V == 2 && sizeof(T) == 4) *(float2 *) p = make_float2(v[0], v[1]);
+    else if constexpr (V == 2) *(uint32_t *) p = pack2<T>(v[0], v[1]);
     else *p = from_f32<T>(*v);
 }
 // v[k] = f(v[k], ...) over a piece, two at a time where it has two
@@ -138,7 +151,7 @@ __device__ __forceinline__ void norm(float (&u)[NV][V], float inv_C, int kind, f
 }
 
 // The most threads of a block: with several 16-byte pieces a thread, half as many at twice the registers.
-constexpr int most_threads(int V, int NV, bool block) { return !block ? 128 : V > 1 && NV > 1 ? 512 : 1024; }
+constexpr int most_threads(int V, int NV, bool block) { return !block ? 128 : V > 2 && NV > 1 ? 512 : 1024; }
 
 // One row per block (BLOCK) or per warp.
 template <class TX, class T, int V, int NV, bool BLOCK>
@@ -244,10 +257,10 @@ cudaError_t launch(const NormArgs & n, cudaStream_t s) {
     auto go = [&](void (*kernel)(NormArgs), int threads) { e = launch_cl(kernel, grid, dim3((unsigned) threads), 0, s, dim3(1), n); };
     if (pieces <= 32) {
         e = launch_cl(block_norm_kernel<TX, T, V, 1, false>, dim3((n.rows + 3) / 4), dim3(128), 0, s, dim3(1), n);
-    } else if constexpr (V == 1) {   // unaligned rows
+    } else if constexpr (V <= 2) {   // unaligned rows
         const int threads = std::min(1024, (pieces + 127) / 128 * 32);
         if (pieces <= 4 * threads) go(block_norm_kernel<TX, T, V, 4, true>, threads);
-        else go(block_norm_kernel<TX, T, V, 16, true>, threads);
+        else go(block_norm_kernel<TX, T, V, 16 / V, true>, threads);   // 16384 elements in 1024 threads
     } else {
         // One piece a thread while a block of 512 holds the row: the least latency where there are few rows (658
         // rows of 1024: 4.0 us, 4.8 with two pieces, 8.6 with four). Two, half the reductions, where the rows fill the GPU
@@ -269,15 +282,19 @@ template <class TX, class T>
 cudaError_t launch(const NormArgs & n, cudaStream_t s) {
     constexpr int V = 16 / sizeof(T);
     const tsn_block_norm_args & a = n.a;
-    auto rows16 = [&](const tsn_rows & r, size_t size) {   // every row starts at a 16-byte boundary
-        return !r.p || (((uintptr_t) r.p | (uintptr_t) (a.B > 1 ? r.sb : 0) * size | (uintptr_t) (a.T > 1 ? r.st : 0) * size) & 15) == 0;
+    // every row, and every vector, starts at a multiple of some elements' bytes, 16 at most
+    auto aligned = [&](uintptr_t elements) {
+        auto rows = [&](const tsn_rows & r, size_t size) {
+            const uintptr_t bytes = std::min<uintptr_t>(16, elements * size);
+            return !r.p || (((uintptr_t) r.p | (uintptr_t) (a.B > 1 ? r.sb : 0) * size | (uintptr_t) (a.T > 1 ? r.st : 0) * size) & (bytes - 1)) == 0;
+        };
+        auto vec = [&](const float * p) { return ((uintptr_t) p & (std::min<uintptr_t>(16, elements * 4) - 1)) == 0; };
+        return a.C % elements == 0 && rows(a.x, sizeof(TX)) && rows(a.x_out, sizeof(TX)) && rows(a.y, sizeof(T)) && rows(a.h, sizeof(T)) &&
+               rows(a.gate, sizeof(T)) && rows(a.scale, sizeof(T)) && rows(a.shift, sizeof(T)) && vec(a.post_w) && vec(a.post_b) &&
+               vec(a.pre_w) && vec(a.pre_b) && vec(a.res_vec);
     };
-    auto vec16 = [&](const float * p) { return ((uintptr_t) p & 15) == 0; };
-    const bool wide = a.C % V == 0 && rows16(a.x, sizeof(TX)) && rows16(a.x_out, sizeof(TX)) && rows16(a.y, sizeof(T)) &&
-                      rows16(a.h, sizeof(T)) && rows16(a.gate, sizeof(T)) && rows16(a.scale, sizeof(T)) &&
-                      rows16(a.shift, sizeof(T)) && vec16(a.post_w) && vec16(a.post_b) && vec16(a.pre_w) && vec16(a.pre_b) &&
-                      vec16(a.res_vec);
-    return wide ? launch<TX, T, V>(n, s) : launch<TX, T, 1>(n, s);
+    // pairs where 16 bytes do not fit: 5400 rows of 1462, f16 with an f32 residual, 50 us (2.9 TB/s), 89 by single elements
+    return aligned(V) ? launch<TX, T, V>(n, s) : aligned(2) ? launch<TX, T, 2>(n, s) : launch<TX, T, 1>(n, s);
 }
 
 } // namespace
