@@ -205,6 +205,14 @@ __device__ __forceinline__ void add_up(int count, int lane, float (&sum)[2][D / 
     }
 }
 
+// The norm's factor of a row from its sum of squares and both maps' sums: NaN where o is not finite. A row that sees no
+// key has no sums; its o is zero and stays so, also with an eps of 0 (0 * 1 / sqrt(0) would be NaN).
+template <int D>
+__device__ __forceinline__ float norm_factor(float ss, float eps, float l1, float l2) {
+    if (l1 == 0.0f && l2 == 0.0f) return 0.0f;
+    return ss < INFINITY ? rsqrtf(ss * (1.0f / D) + eps) : NAN;
+}
+
 // The result of one row from its sums, one warp: lam lambda of its head, nw the norm's weights.
 template <int D, bool BF16>
 __device__ __forceinline__ void write_row(const Args & p, int b, int hk, int i, int g, float lam, const float * nw, int lane,
@@ -220,7 +228,7 @@ __device__ __forceinline__ void write_row(const Args & p, int b, int hk, int i, 
     }
 #pragma unroll
     for (int x = 16; x; x >>= 1) ss += __shfl_xor_sync(~0u, ss, x);
-    const float f = ss < INFINITY ? rsqrtf(ss * (1.0f / D) + a.eps) : NAN;
+    const float f = norm_factor<D>(ss, a.eps, l[0], l[1]);
     uint32_t x[E / 2];
 #pragma unroll
     for (int e = 0; e < E; e += 2) x[e / 2] = pack16<BF16>(v[e] * f * nw[E * lane + e], v[e + 1] * f * nw[E * lane + e + 1]);
@@ -261,7 +269,7 @@ struct Lay {
     static_assert(TOTAL <= 227 * 1024, "one CTA's shared memory");
     static_assert(ROWS * row_words(D) * 4 <= 2 * STAGES * TILE, "the rows' sums fit in the ring");
     static_assert(TM_O + 2 * D <= TM, "tensor memory");
-    static_assert(ROWS * 8 * 8 <= Q, "the parts' factors fit in Q's place");
+    static_assert(ROWS * (8 * 8 + 8) <= Q, "the parts' factors and the rows' sums fit in Q's place");
 };
 
 template <int D, bool BF16>
@@ -603,7 +611,7 @@ diff_attn_tc(const __grid_constant__ CUtensorMap tk, const __grid_constant__ CUt
             // place, then the parts' sums, a row by D / 4 lanes, four steps of rows at once
             const int share = (rows + p.splits - 1) / p.splits, from = (int) split * share, here = max(0, min(rows - from, share));
             const uint32_t at0 = smem_u32(sums) + from * row_words(D) * 4;
-            float2 * fac = (float2 *) smem;   // [row][8 parts]
+            float2 * fac = (float2 *) smem, * rl = fac + ROWS * 8;   // [row][8 parts]; [row] sums of both maps
             if (tid < here) {
                 float4 st[8];   // ref and l of both maps
                 float2 top = make_float2(-INFINITY, -INFINITY), sum = make_float2(0.0f, 0.0f);
@@ -627,6 +635,7 @@ diff_attn_tc(const __grid_constant__ CUtensorMap tk, const __grid_constant__ CUt
 #pragma unroll
                 for (int i = 0; i < 8; ++i)
                     if (i < p.splits) fac[tid * 8 + i] = make_float2(st[i].x * w1, st[i].y * w2);
+                rl[tid] = sum;
             }
             __syncthreads();
             constexpr int LANES = D / 4, STEP = 8 * (32 / LANES), AT_ONCE = 4;   // of a row; rows of a step of all warps
@@ -652,7 +661,7 @@ diff_attn_tc(const __grid_constant__ CUtensorMap tk, const __grid_constant__ CUt
 #pragma unroll
                     for (int x = LANES / 2; x; x >>= 1) ss += __shfl_xor_sync(~0u, ss, x);
                     if (r >= here || *abort_flag) continue;
-                    const float g = ss < INFINITY ? rsqrtf(ss * (1.0f / D) + a.eps) : NAN;
+                    const float g = norm_factor<D>(ss, a.eps, rl[r].x, rl[r].y);
                     const float4 w = *(const float4 *) (nw + col);
                     const int u = rem0 + from + r;
                     *(uint2 *) ((uint16_t *) a.out.p + b * a.out.sb + (long long) (i0 + u / p.G) * a.out.ss + (long long) (hk * p.G + u % p.G) * a.out.sh + col) =
@@ -664,14 +673,15 @@ diff_attn_tc(const __grid_constant__ CUtensorMap tk, const __grid_constant__ CUt
             // o = O_1 / l_1 - lambda O_2 / l_2, thread (row t, half m of the columns); RMSNorm over both halves; the result
             // through Q's place, so that whole rows are written. In place of K: row sums [2][128], sums of squares [2][128]
             float * rl = (float *) (smem + L::OFF_K), * rss = rl + 256;
-            float o[d];
+            float o[d], l1, l2;
             tc_fence_before();
             __syncthreads();   // both maps are done with the ring, and their O is there
             tc_fence_after();
             rl[tid] = l;
             __syncthreads();
             {
-                const float l1 = rl[t], l2 = rl[128 + t];
+                l1 = rl[t];
+                l2 = rl[128 + t];
                 const float w1 = l1 == 0.0f ? 0.0f : 1.0f / l1;
                 const float w2 = l2 == 0.0f ? 0.0f : t < rows ? lam[(rem0 + t) % p.G] / l2 : 0.0f;
 #pragma unroll
@@ -694,7 +704,7 @@ diff_attn_tc(const __grid_constant__ CUtensorMap tk, const __grid_constant__ CUt
             __syncthreads();
             {
                 const float ss = rss[t] + rss[128 + t];
-                const float g = ss < INFINITY ? rsqrtf(ss * (1.0f / D) + a.eps) : NAN;
+                const float g = norm_factor<D>(ss, a.eps, l1, l2);
 #pragma unroll
                 for (int e = 0; e < d; e += 8) {
                     uint32_t x[4];
