@@ -338,7 +338,7 @@ typedef struct tsn_heads { void * p; int64_t sb, ss, sh; } tsn_heads;
 /* Norms before and after a block, fused with the block's gate and residual scale. Per row of C:
  *   x_out = r * x + act(gate) * Npost(y)          h = Npre(x_out) * (1 + scale) + shift
  * RMS: N(u) = u / sqrt(mean(u^2) + eps) * w (+ b); LAYER: N(u) = (u - mean) / sqrt(var + eps) * w (+ b);
- * NONE: N(u) = u. r is res_vec [C] where given, else res_scale; act is tanh if gate_tanh. Npre sees
+ * NONE: N(u) = u. r is res_vec [C] where given, else res_scale; act is tanh if gate_tanh, to 2^-20 of its value. Npre sees
  * x_out before it is rounded to xtype. Absent terms: y (then x_out = r * x), gate (1), scale (0), shift
  * (0), weights (1), biases (0); x_out or h may be absent, not both. x and x_out are of xtype, which
  * is `type` or TSN_F32; y, h, gate, shift and scale are of `type`; weights, biases and res_vec are f32.
