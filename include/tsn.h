@@ -401,7 +401,8 @@ int tsn_rope_axes(tsn_device * dev, const tsn_rope_plan_t * plan, const tsn_rope
  * and infinities included; a row that sees a non-finite value is NaN.
  * lq1 .. lk2: f32 vectors of d, one per query head lam_sh elements apart (0: shared). norm_w: f32 [2 d] or
  * null for ones.
- * The probabilities are rounded to `type` before the product with v, as the tensor cores take them.
+ * The probabilities are rounded to `type` before the product with v, as the tensor cores take them, and their sum is
+ * that of the rounded ones.
  * Few query rows over many keys split the keys over several CTAs through a workspace that the device handle
  * allocates at its first such call and keeps: make one such call before capturing it in a CUDA graph. Calls on
  * different streams take turns at it; a graph's replays do not know of them, so let a replay that holds such a

@@ -68,7 +68,7 @@ __device__ __forceinline__ uint64_t fadd2(uint64_t a, uint64_t b) {
 // (2^x, 2^y) on the FMA pipe, x and y clamped to -126 or more: 2^i p(f), i the nearest whole number, f = x - i in [-1/2, 1/2],
 // p the polynomial of least relative error there (Remez exchange): 7.5e-5 at degree 3, 2.6e-6 at degree 4, each below
 // an eighth of half a unit of the 16-bit type that the result is rounded to. Adding 1.5 * 2^23 rounds to i and leaves
-// it in the low bits. NaN stays non-finite. ZERO: what was clamped becomes 0 (p(0) < 1, so 2^-126 p(0) is subnormal).
+// it in the low bits. NaN becomes 0x7f7fffff, which rounds to infinity in either 16-bit type. ZERO: what was clamped becomes 0 (p(0) < 1, so 2^-126 p(0) is subnormal).
 template <bool BF16, bool ZERO>
 __device__ __forceinline__ uint64_t ex2_fma(uint64_t xy) {
     float x, y;
@@ -103,6 +103,12 @@ __device__ __forceinline__ uint32_t pack16(float a, float b) {
     else asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(b), "f"(a));
     return r;
 }
+// a and b += the two 16-bit values of a word, in f32
+template <bool BF16>
+__device__ __forceinline__ void add_rounded(float & a, float & b, uint32_t two) {
+    if (BF16) asm("{\n .reg .b16 l, h;\n mov.b32 {l, h}, %2;\n add.rn.f32.bf16 %0, l, %0;\n add.rn.f32.bf16 %1, h, %1;\n}" : "+f"(a), "+f"(b) : "r"(two));
+    else asm("{\n .reg .b16 l, h;\n mov.b32 {l, h}, %2;\n add.rn.f32.f16 %0, l, %0;\n add.rn.f32.f16 %1, h, %1;\n}" : "+f"(a), "+f"(b) : "r"(two));
+}
 // the low n bits of a word, n of any sign and size
 __device__ __forceinline__ uint32_t low_bits(int n) { return n >= 32 ? 0xffffffffu : n <= 0 ? 0u : (1u << n) - 1u; }
 // of two 16-bit values, the non-finite ones set to zero
@@ -114,9 +120,10 @@ __device__ __forceinline__ uint32_t finite_only(uint32_t v) {
     return v;
 }
 
-// 32 scores s of a row become 2^(c s + neg): P as 16-bit pairs, and their sum. Every fourth pair takes the FMA pipe.
+// 32 scores s of a row become 2^(c s + neg): P as 16-bit pairs, and the sum of these rounded values, so that what rounding
+// takes from a key's share in the product it takes from the divisor too. Every fourth pair takes the FMA pipe.
 template <bool BF16, bool MASKED>
-__device__ __forceinline__ void exponentials(const uint32_t * s, uint32_t * pk, float c, float ref, uint64_t (&sum)[2]) {
+__device__ __forceinline__ void exponentials(const uint32_t * s, uint32_t * pk, float c, float ref, float (&sum)[4]) {
     const float neg = ref == -INFINITY ? 0.0f : -ref;
     const uint64_t c2 = f2_pack(c, c), neg2 = f2_pack(neg, neg);
 #pragma unroll
@@ -130,8 +137,8 @@ __device__ __forceinline__ void exponentials(const uint32_t * s, uint32_t * pk, 
             y = ex2(y);
             z = ex2(z);
         }
-        sum[e & 1] = fadd2(sum[e & 1], f2_pack(y, z));
         pk[e] = pack16<BF16>(y, z);
+        add_rounded<BF16>(sum[2 * (e & 1)], sum[2 * (e & 1) + 1], pk[e]);
     }
 }
 __device__ __forceinline__ float greatest(const uint32_t * s) {   // of 32
@@ -496,7 +503,7 @@ diff_attn_tc(const __grid_constant__ CUtensorMap tk, const __grid_constant__ CUt
             // A tile is taken in two halves of 32 keys, so that a half's scores come from TMEM while the other half's
             // exponentials run. P replaces the second half's scores; the first half's stay until the tile is done.
             uint32_t s1[32], vis[2] = {~0u, ~0u};
-            uint64_t sum[2];
+            float sum[4];
             // the first half of tile j, whose scores are there, and the maximum over both
             auto first_half = [&](auto masked, int j) {
                 constexpr bool MASKED = decltype(masked)::value;
@@ -514,7 +521,7 @@ diff_attn_tc(const __grid_constant__ CUtensorMap tk, const __grid_constant__ CUt
                 tmem_request32(at + 32, s1);
                 if (MASKED) hide(s0, vis[0]);
                 // against the reference of the tiles before; the few tiles whose maximum is too far above it are done again
-                sum[0] = sum[1] = 0ull;
+                sum[0] = sum[1] = sum[2] = sum[3] = 0.0f;
                 exponentials<BF16, MASKED>(s0, pk, p.c, ref, sum);
                 const float top0 = greatest(s0);
                 tmem_landed32(s1);
@@ -544,7 +551,7 @@ diff_attn_tc(const __grid_constant__ CUtensorMap tk, const __grid_constant__ CUt
                     tmem_request32(at, s0);
                     tmem_landed32(s0);
                     if (MASKED) hide(s0, vis[0]);
-                    sum[0] = sum[1] = 0ull;
+                    sum[0] = sum[1] = sum[2] = sum[3] = 0.0f;
                     exponentials<BF16, MASKED>(s0, pk, p.c, ref, sum);
                 }
                 tmem_st16(at + 32, pk);
@@ -558,9 +565,7 @@ diff_attn_tc(const __grid_constant__ CUtensorMap tk, const __grid_constant__ CUt
                     uint32_t pk[16];
                     exponentials<BF16, MASKED>(s1, pk, p.c, ref, sum);
                     tmem_st16(tmem + KEYS * x + lane0 + 48, pk);
-                    float y, z;
-                    f2_unpack(fadd2(sum[0], sum[1]), y, z);
-                    l += y + z;
+                    l += (sum[0] + sum[2]) + (sum[1] + sum[3]);
                     tmem_st_wait();
                     if (MASKED && m == 0 && mixed((t0 + j) * KEYS)) {
                         if (!mbar_wait_soon(&v_ready[j % L::STAGES], (j / L::STAGES) & 1, abort_flag, p.err, DEV_TIMEOUT_FULL)) ok = false;
@@ -949,10 +954,11 @@ diff_attn_rows(const __grid_constant__ CUtensorMap tk, const __grid_constant__ C
             const float n0 = ref[m][0] == -INFINITY ? 0.0f : -ref[m][0], n1 = ref[m][1] == -INFINITY ? 0.0f : -ref[m][1];
             const float e0 = ex2(fmaf(s[m][0], p.c, n0)), e1 = ex2(fmaf(s[m][1], p.c, n1));
             const float e2 = ex2(fmaf(s[m][2], p.c, n0)), e3 = ex2(fmaf(s[m][3], p.c, n1));
-            l[m][0] += e0 + e2;
-            l[m][1] += e1 + e3;
-            pb[m][0] = movmatrix(pack16<BF16>(e0, e1));
-            pb[m][1] = movmatrix(pack16<BF16>(e2, e3));
+            const uint32_t p0 = pack16<BF16>(e0, e1), p1 = pack16<BF16>(e2, e3);
+            add_rounded<BF16>(l[m][0], l[m][1], p0);   // the sums are of what the product takes
+            add_rounded<BF16>(l[m][0], l[m][1], p1);
+            pb[m][0] = movmatrix(p0);
+            pb[m][1] = movmatrix(p1);
         }
         if (!gone && !mixed) {
 #pragma unroll
