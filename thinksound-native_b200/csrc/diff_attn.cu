@@ -1096,8 +1096,9 @@ bool make_kv_map(CUtensorMap * m, const tsn_diff_attn_args & a, const tsn_heads 
 constexpr size_t COUNTERS = 4096, WORKSPACE = COUNTERS * 4 + ((size_t) 32 << 20);
 constexpr int SMS = 148;
 
-// The device's workspace, ordered after the last call that used it on another stream.
-int workspace(DeviceCtx & c, bool capturing) {
+// The device's workspace, ordered after the last call that used it on another stream. Streams are told apart by their id,
+// which no other stream of the process ever has: a handle may stand for one stream per thread, or be given out again.
+int workspace(DeviceCtx & c, bool capturing, unsigned long long stream) {
     if (!c.split_ws) {
         if (capturing) return fail(TSN_ERR_STATE, "tsn_diff_attn: a first call that splits its keys cannot be captured");
         void * p = nullptr;
@@ -1108,7 +1109,7 @@ int workspace(DeviceCtx & c, bool capturing) {
         if (e != cudaSuccess) { cudaFree(p); return fail(TSN_ERR_CUDA, std::string("tsn_diff_attn: ") + cudaGetErrorString(e)); }
         c.split_ws = p;
     }
-    if (!capturing && c.split_used && c.split_stream != c.stream) {
+    if (!capturing && c.split_used && c.split_stream != stream) {
         cudaError_t e = cudaStreamWaitEvent(c.stream, c.split_ev, 0);
         if (e != cudaSuccess) return fail(TSN_ERR_CUDA, std::string("tsn_diff_attn: ") + cudaGetErrorString(e));
     }
@@ -1230,11 +1231,13 @@ int diff_attn(DeviceCtx & c, const tsn_diff_attn_args & in) {
     }
     if (groups * p.splits > 0x7fffffffLL) return fail(TSN_ERR_ARG, "tsn_diff_attn: too many query rows");
     const bool shared = rows && p.splits > 1;   // through the workspace
+    cudaStreamCaptureStatus st = cudaStreamCaptureStatusNone;
+    unsigned long long stream = 0;
     if (shared) {
-        cudaStreamCaptureStatus st = cudaStreamCaptureStatusNone;
         cudaError_t e = cudaStreamIsCapturing(c.stream, &st);
+        if (e == cudaSuccess && st == cudaStreamCaptureStatusNone) e = cudaStreamGetId(c.stream, &stream);
         if (e != cudaSuccess) return fail(TSN_ERR_CUDA, std::string("tsn_diff_attn: ") + cudaGetErrorString(e));
-        int rc = workspace(c, st != cudaStreamCaptureStatusNone);
+        int rc = workspace(c, st != cudaStreamCaptureStatusNone, stream);
         if (rc) return rc;
         p.count = (unsigned int *) c.split_ws;
         p.part = (float *) ((char *) c.split_ws + COUNTERS * 4);
@@ -1252,14 +1255,10 @@ int diff_attn(DeviceCtx & c, const tsn_diff_attn_args & in) {
         e = a.d == 32 ? (bf ? launch_tc<64, true>(tk, tv, p, grid, c.stream) : launch_tc<64, false>(tk, tv, p, grid, c.stream))
                       : (bf ? launch_tc<128, true>(tk, tv, p, grid, c.stream) : launch_tc<128, false>(tk, tv, p, grid, c.stream));
     if (e != cudaSuccess) cudaGetLastError();
-    if (e == cudaSuccess && shared) {
-        cudaStreamCaptureStatus st = cudaStreamCaptureStatusNone;
-        e = cudaStreamIsCapturing(c.stream, &st);
-        if (e == cudaSuccess && st == cudaStreamCaptureStatusNone) {
-            e = cudaEventRecord(c.split_ev, c.stream);
-            c.split_used = true;
-            c.split_stream = c.stream;
-        }
+    if (e == cudaSuccess && shared && st == cudaStreamCaptureStatusNone) {
+        e = cudaEventRecord(c.split_ev, c.stream);
+        c.split_used = true;
+        c.split_stream = stream;
     }
     if (e != cudaSuccess) return fail(TSN_ERR_CUDA, std::string("tsn_diff_attn: ") + cudaGetErrorString(e));
     return TSN_OK;

@@ -39,10 +39,11 @@ struct DeviceCtx {
     void * col = nullptr;
     size_t col_bytes = 0;
     // transformer-block operators: partial results of calls that split their keys, allocated once at
-    // its full size; split_ev follows the last call that used it, so calls on other streams wait for it
+    // its full size; split_ev follows the last call that used it, on the stream of id split_stream, so calls on
+    // other streams wait for it
     void * split_ws = nullptr;
     cudaEvent_t split_ev = nullptr;
-    cudaStream_t split_stream = nullptr;
+    unsigned long long split_stream = 0;
     bool split_used = false;
     int activate();                  // cudaSetDevice(ordinal)
     int check_device_error();        // after a sync: TSN_ERR_TIMEOUT if a kernel gave up
