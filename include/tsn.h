@@ -403,10 +403,11 @@ int tsn_rope_axes(tsn_device * dev, const tsn_rope_plan_t * plan, const tsn_rope
  * null for ones.
  * The probabilities are rounded to `type` before the product with v, as the tensor cores take them, and their sum is
  * that of the rounded ones.
- * Few query rows over many keys split the keys over several CTAs through a workspace that the device handle
- * allocates at its first such call and keeps: make one such call before capturing it in a CUDA graph. Calls on
- * different streams take turns at it; a graph's replays do not know of them, so let a replay that holds such a
- * call not run beside another one of the same device handle. At most 2^30 queries, keys and query rows of a kv
+ * Few query rows over many keys split the keys over several CTAs, whose sums meet in a workspace. Calls take turns at
+ * the device handle's (32 MiB, allocated at its first such call and kept), whatever streams they are on. A call captured
+ * in a CUDA graph has one of its own size that belongs to the graph, so replays may run beside one another and beside
+ * other calls; executables made from one graph share it, as they share the results. A graph is replayed while the handle
+ * is there (its error word is the handle's). At most 2^30 queries, keys and query rows of a kv
  * head (Sq * H / Hk), 65535 sequences and heads. */
 typedef struct tsn_diff_attn_args {
     uint32_t B, Sq, Sk, H, Hk, d;

@@ -77,6 +77,7 @@ int tsn_device_destroy(tsn_device * dev) {
     if (c.split_used) cudaEventSynchronize(c.split_ev);
     if (c.split_ws) cudaFree(c.split_ws);
     if (c.split_ev) cudaEventDestroy(c.split_ev);
+    release_diff_attn(c.ordinal);
     if (c.d_err) cudaFree(c.d_err);
     if (c.ev0) cudaEventDestroy(c.ev0);
     if (c.ev1) cudaEventDestroy(c.ev1);

@@ -14,6 +14,7 @@ int rope_plan(uint32_t D, uint32_t axes, const uint32_t * pairs, const double * 
 int rope_axes(DeviceCtx & c, const tsn_rope_plan_t & p, const tsn_rope_args & a);
 cudaError_t configure_diff_attn();   // once per device, before the first launch
 int diff_attn(DeviceCtx & c, const tsn_diff_attn_args & a);
+void release_diff_attn(int ordinal);   // with the device: workspaces of graphs that are gone
 
 inline bool known_type(int t) { return t == TSN_F32 || t == TSN_F16 || t == TSN_BF16; }
 inline size_t type_size(int t) { return t == TSN_F32 ? 4 : 2; }

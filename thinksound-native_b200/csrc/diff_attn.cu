@@ -19,6 +19,7 @@
 
 #include <algorithm>
 #include <atomic>
+#include <mutex>
 
 namespace tsn {
 
@@ -1096,23 +1097,95 @@ bool make_kv_map(CUtensorMap * m, const tsn_diff_attn_args & a, const tsn_heads 
 constexpr size_t COUNTERS = 4096, WORKSPACE = COUNTERS * 4 + ((size_t) 32 << 20);
 constexpr int SMS = 148;
 
-// The device's workspace, ordered after the last call that used it on another stream. Streams are told apart by their id,
-// which no other stream of the process ever has: a handle may stand for one stream per thread, or be given out again.
-int workspace(DeviceCtx & c, bool capturing, unsigned long long stream) {
+// Host calls that touch no stream of the program, so that they also work while one of them is being captured.
+struct Uncaptured {
+    cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
+    Uncaptured() { cudaThreadExchangeStreamCaptureMode(&mode); }
+    ~Uncaptured() { cudaThreadExchangeStreamCaptureMode(&mode); }
+};
+cudaError_t zero(void * p, size_t bytes) {   // and waits for it
+    Uncaptured u;
+    cudaStream_t s = nullptr;
+    cudaError_t e = cudaStreamCreateWithFlags(&s, cudaStreamNonBlocking);
+    if (e == cudaSuccess) e = cudaMemsetAsync(p, 0, bytes, s);
+    if (e == cudaSuccess) e = cudaStreamSynchronize(s);
+    if (s) cudaStreamDestroy(s);
+    return e;
+}
+cudaError_t allocate(void ** p, size_t bytes) {
+    Uncaptured u;
+    return cudaMalloc(p, bytes);
+}
+int failed(cudaError_t e) {
+    cudaGetLastError();
+    return fail(e == cudaErrorMemoryAllocation ? TSN_ERR_OOM : TSN_ERR_CUDA, std::string("tsn_diff_attn: ") + cudaGetErrorString(e));
+}
+
+// The device's workspace, ordered after the last call that used it. Streams are told apart by their id, which no other
+// stream of the process ever has: a handle may stand for one stream per thread, or be given out again.
+int workspace(DeviceCtx & c, unsigned long long stream) {
+    cudaError_t e = cudaSuccess;
     if (!c.split_ws) {
-        if (capturing) return fail(TSN_ERR_STATE, "tsn_diff_attn: a first call that splits its keys cannot be captured");
         void * p = nullptr;
-        if (cudaMalloc(&p, WORKSPACE) != cudaSuccess) { cudaGetLastError(); return fail(TSN_ERR_OOM, "tsn_diff_attn: workspace"); }
-        cudaError_t e = cudaMemset(p, 0, COUNTERS * 4);
-        if (e == cudaSuccess) e = cudaDeviceSynchronize();
+        e = allocate(&p, WORKSPACE);
+        if (e == cudaSuccess) e = zero(p, COUNTERS * 4);
         if (e == cudaSuccess && !c.split_ev) e = cudaEventCreateWithFlags(&c.split_ev, cudaEventDisableTiming);
-        if (e != cudaSuccess) { cudaFree(p); return fail(TSN_ERR_CUDA, std::string("tsn_diff_attn: ") + cudaGetErrorString(e)); }
+        if (e != cudaSuccess) { cudaFree(p); return failed(e); }
         c.split_ws = p;
     }
-    if (!capturing && c.split_used && c.split_stream != stream) {
-        cudaError_t e = cudaStreamWaitEvent(c.stream, c.split_ev, 0);
-        if (e != cudaSuccess) return fail(TSN_ERR_CUDA, std::string("tsn_diff_attn: ") + cudaGetErrorString(e));
+    if (c.split_used && c.split_stream != stream) e = cudaStreamWaitEvent(c.stream, c.split_ev, 0);
+    return e == cudaSuccess ? TSN_OK : failed(e);
+}
+
+// Workspaces of captured calls. One belongs to its call's graph, so that replays need no order among themselves or with other
+// calls; when the graph and its executables are gone it lies here until another capture, or the device's end, takes it.
+struct Block {
+    void * p;
+    size_t bytes;
+    int ordinal;
+    Block * next;
+};
+std::mutex g_idle_mu;
+Block * g_idle = nullptr;
+
+void CUDART_CB make_idle(void * block) {   // no CUDA calls in here
+    std::lock_guard<std::mutex> lk(g_idle_mu);
+    Block * b = (Block *) block;
+    b->next = g_idle;
+    g_idle = b;
+}
+
+int graph_workspace(const DeviceCtx & c, cudaGraph_t graph, size_t bytes, void ** out) {
+    size_t size = (size_t) 1 << 18;   // powers of two, so that they fit the calls of later captures
+    while (size < bytes) size *= 2;
+    Block * b = nullptr;
+    {
+        std::lock_guard<std::mutex> lk(g_idle_mu);
+        for (Block ** at = &g_idle; *at; at = &(*at)->next)
+            if ((*at)->ordinal == c.ordinal && (*at)->bytes == size) {
+                b = *at;
+                *at = b->next;
+                break;
+            }
     }
+    if (!b) {
+        b = new Block{nullptr, size, c.ordinal, nullptr};
+        const cudaError_t e = allocate(&b->p, size);
+        if (e != cudaSuccess) { delete b; return failed(e); }
+    }
+    cudaUserObject_t object = nullptr;
+    cudaError_t e = zero(b->p, size);
+    if (e == cudaSuccess) e = cudaUserObjectCreate(&object, b, make_idle, 1, cudaUserObjectNoDestructorSync);
+    if (e != cudaSuccess) {
+        make_idle(b);
+        return failed(e);
+    }
+    e = cudaGraphRetainUserObject(graph, object, 1, cudaGraphUserObjectMove);
+    if (e != cudaSuccess) {
+        cudaUserObjectRelease(object, 1);
+        return failed(e);
+    }
+    *out = b->p;
     return TSN_OK;
 }
 
@@ -1159,6 +1232,26 @@ cudaError_t configure_diff_attn() {
         g_clusters[n] = count;
     }
     return e;
+}
+
+void release_diff_attn(int ordinal) {
+    Block * gone = nullptr;
+    {
+        std::lock_guard<std::mutex> lk(g_idle_mu);
+        for (Block ** at = &g_idle; *at;) {
+            Block * b = *at;
+            if (b->ordinal != ordinal) { at = &b->next; continue; }
+            *at = b->next;
+            b->next = gone;
+            gone = b;
+        }
+    }
+    while (gone) {   // without the lock: freeing may wait for a thread of the driver's that is in make_idle
+        Block * b = gone;
+        gone = b->next;
+        cudaFree(b->p);
+        delete b;
+    }
 }
 
 int diff_attn(DeviceCtx & c, const tsn_diff_attn_args & in) {
@@ -1231,16 +1324,27 @@ int diff_attn(DeviceCtx & c, const tsn_diff_attn_args & in) {
     }
     if (groups * p.splits > 0x7fffffffLL) return fail(TSN_ERR_ARG, "tsn_diff_attn: too many query rows");
     const bool shared = rows && p.splits > 1;   // through the workspace
-    cudaStreamCaptureStatus st = cudaStreamCaptureStatusNone;
+    cudaStreamCaptureStatus capture = cudaStreamCaptureStatusNone;
     unsigned long long stream = 0;
     if (shared) {
-        cudaError_t e = cudaStreamIsCapturing(c.stream, &st);
-        if (e == cudaSuccess && st == cudaStreamCaptureStatusNone) e = cudaStreamGetId(c.stream, &stream);
-        if (e != cudaSuccess) return fail(TSN_ERR_CUDA, std::string("tsn_diff_attn: ") + cudaGetErrorString(e));
-        int rc = workspace(c, st != cudaStreamCaptureStatusNone, stream);
+        cudaGraph_t graph = nullptr;
+        cudaError_t e = cudaStreamGetCaptureInfo(c.stream, &capture, nullptr, &graph, nullptr, nullptr);
+        if (e == cudaSuccess && capture == cudaStreamCaptureStatusInvalidated) e = cudaErrorStreamCaptureInvalidated;
+        if (e == cudaSuccess && capture == cudaStreamCaptureStatusNone) e = cudaStreamGetId(c.stream, &stream);
+        if (e != cudaSuccess) return failed(e);
+        size_t counters = COUNTERS * 4;
+        void * ws = nullptr;
+        int rc;
+        if (capture == cudaStreamCaptureStatusNone) {
+            rc = workspace(c, stream);
+            ws = c.split_ws;
+        } else {
+            counters = ((size_t) groups * 4 + 255) & ~(size_t) 255;
+            rc = graph_workspace(c, graph, counters + (size_t) groups * p.splits * (SOME * (4 * a.d + 4) * 4), &ws);
+        }
         if (rc) return rc;
-        p.count = (unsigned int *) c.split_ws;
-        p.part = (float *) ((char *) c.split_ws + COUNTERS * 4);
+        p.count = (unsigned int *) ws;
+        p.part = (float *) ((char *) ws + counters);
     }
     CUtensorMap tk{}, tv{};
     if (a.Sk && (!make_kv_map(&tk, a, a.k, KB, rows ? SLAB : KEYS) || !make_kv_map(&tv, a, a.v, KB, rows ? SLAB : KEYS)))
@@ -1255,7 +1359,7 @@ int diff_attn(DeviceCtx & c, const tsn_diff_attn_args & in) {
         e = a.d == 32 ? (bf ? launch_tc<64, true>(tk, tv, p, grid, c.stream) : launch_tc<64, false>(tk, tv, p, grid, c.stream))
                       : (bf ? launch_tc<128, true>(tk, tv, p, grid, c.stream) : launch_tc<128, false>(tk, tv, p, grid, c.stream));
     if (e != cudaSuccess) cudaGetLastError();
-    if (e == cudaSuccess && shared && st == cudaStreamCaptureStatusNone) {
+    if (e == cudaSuccess && shared && capture == cudaStreamCaptureStatusNone) {
         e = cudaEventRecord(c.split_ev, c.stream);
         c.split_used = true;
         c.split_stream = stream;

@@ -40,7 +40,7 @@ struct DeviceCtx {
     size_t col_bytes = 0;
     // transformer-block operators: partial results of calls that split their keys, allocated once at
     // its full size; split_ev follows the last call that used it, on the stream of id split_stream, so calls on
-    // other streams wait for it
+    // other streams wait for it (captured calls have workspaces of their own)
     void * split_ws = nullptr;
     cudaEvent_t split_ev = nullptr;
     unsigned long long split_stream = 0;
