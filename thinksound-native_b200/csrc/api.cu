@@ -177,7 +177,7 @@ int tsn_dispatch(tsn_device * dev, const char * kernel, const uint32_t grid[3], 
     std::lock_guard<std::mutex> lk(dev->ctx.mu);
     DeviceCtx & c = dev->ctx;
     TRY(c.activate());
-    if (!c.pending) { CKR(cudaEventRecord(c.ev0, c.stream)); c.pending = true; }
+    TRY(c.begin());
     return compat_dispatch(c, kernel, grid, block, bufs, nbufs, params, nparams);
 }
 
@@ -256,7 +256,7 @@ int tsn_selftest_gemv_jobs(tsn_device * dev, const void * W, const void * bias, 
     std::lock_guard<std::mutex> lk(dev->ctx.mu);                        \
     DeviceCtx & c = dev->ctx;                                            \
     TRY(c.activate());                                                   \
-    if (!c.pending) { CKR(cudaEventRecord(c.ev0, c.stream)); c.pending = true; }
+    TRY(c.begin());
 
 int tsn_gemm(tsn_device * dev, int wf16, const void * W, const void * X, void * Y, const void * bias,
              uint32_t M, uint32_t N, uint32_t K, uint32_t ldx, uint32_t ldw, uint32_t ldy) {

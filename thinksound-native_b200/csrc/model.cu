@@ -36,6 +36,17 @@ int DeviceCtx::activate() {
     return TSN_OK;
 }
 
+int DeviceCtx::begin() {
+    if (pending) return TSN_OK;
+    // a captured call is no work yet, and an event recorded in a capture has no time
+    cudaStreamCaptureStatus st = cudaStreamCaptureStatusNone;
+    CKR(cudaStreamIsCapturing(stream, &st));
+    if (st != cudaStreamCaptureStatusNone) return TSN_OK;
+    CKR(cudaEventRecord(ev0, stream));
+    pending = true;
+    return TSN_OK;
+}
+
 int DeviceCtx::check_device_error() {
     int h = 0;
     CKR(cudaMemcpy(&h, d_err, sizeof(int), cudaMemcpyDeviceToHost));

@@ -46,6 +46,7 @@ struct DeviceCtx {
     unsigned long long split_stream = 0;
     bool split_used = false;
     int activate();                  // cudaSetDevice(ordinal)
+    int begin();                     // before a call's work: the batch's first event
     int check_device_error();        // after a sync: TSN_ERR_TIMEOUT if a kernel gave up
     int sync();                      // stream sync + device error word
 };
