@@ -29,7 +29,10 @@ def _weights(dev, name, t, shape):
     if tuple(t.shape) != tuple(shape) or t.dtype is not torch.float32:
         raise ValueError(f"{name} must be a float32 tensor of shape {tuple(shape)}")
     _here(dev, (name, t))
-    return t.contiguous()
+    if not t.is_contiguous():
+        t = t.contiguous()
+        torch.cuda.current_stream(t.device).synchronize()   # the copy's stream; calls are issued on the handle's
+    return t
 
 
 def _address(t):
