@@ -1292,7 +1292,7 @@ int diff_attn(DeviceCtx & c, const tsn_diff_attn_args & in) {
     p.R = (int) a.Sq * p.G;
     p.err = c.d_err;
     const bool rows = p.R <= FEW;
-    const long long groups = (rows ? (p.R + SOME - 1) / SOME : (p.R + ROWS - 1) / ROWS) * a.B * a.Hk;
+    const long long groups = (long long) (rows ? (p.R + SOME - 1) / SOME : (p.R + ROWS - 1) / ROWS) * a.B * a.Hk;   // below 2^60
     if (rows) {
         // As many parts as take the least time, in units of what one CTA takes for a slab (93 ns): the start of a CTA is 30,
         // a trip of the sums through the workspace 30 and a half for each part; past 74 CTAs at once (of 8 KB slabs) they
