@@ -368,7 +368,7 @@ typedef struct tsn_rope_plan_t {
     uint64_t turn[TSN_ROPE_MAX_PAIRS];
     uint8_t axis[TSN_ROPE_MAX_PAIRS];
 } tsn_rope_plan_t;
-/* D even, 2..256, 2 P <= D; theta > 0, scale finite. */
+/* D even, 2..256, 2 P <= D; theta > 0, scale and the turns that they give finite. */
 int tsn_rope_plan(uint32_t D, uint32_t axes, const uint32_t * pairs, const double * theta, const double * scale,
                   int layout, tsn_rope_plan_t * out);
 /* q [B, S, Hq, D] and k [B, S, Hk, D] of `type` into q_out and k_out (the inputs themselves, at the same

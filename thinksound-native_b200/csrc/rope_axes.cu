@@ -262,6 +262,7 @@ int rope_plan(uint32_t D, uint32_t axes, const uint32_t * pairs, const double * 
         if (pairs[x] > D / 2 || p.P + pairs[x] > D / 2) return fail(TSN_ERR_ARG, "tsn_rope_plan: more pairs than D / 2");
         for (uint32_t i = 0; i < pairs[x]; ++i, ++p.P) {
             const double turns = scale[x] * std::pow(theta[x], -(double) i / pairs[x]) / (2.0 * 3.14159265358979323846);
+            if (!std::isfinite(turns)) return fail(TSN_ERR_ARG, "tsn_rope_plan: theta and scale give turns that are not finite");
             const double part = turns - std::floor(turns);   // whole turns per position turn nothing
             p.turn[p.P] = part >= 1.0 ? 0 : (uint64_t) std::ldexp(part, 64);
             p.axis[p.P] = (uint8_t) x;
