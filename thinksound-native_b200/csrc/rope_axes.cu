@@ -274,7 +274,7 @@ int rope_plan(uint32_t D, uint32_t axes, const uint32_t * pairs, const double * 
 
 int rope_axes(DeviceCtx & c, const tsn_rope_plan_t & p, const tsn_rope_args & a) {
     if (!known_type(a.type)) return fail(TSN_ERR_ARG, "tsn_rope_axes: unknown type");
-    if (p.D < 2 || p.D > 2 * TSN_ROPE_MAX_PAIRS || p.D % 2 || 2 * p.P > p.D || p.axes < 1 || p.axes > TSN_ROPE_MAX_AXES)
+    if (p.D < 2 || p.D > 2 * TSN_ROPE_MAX_PAIRS || p.D % 2 || p.P > p.D / 2 || p.axes < 1 || p.axes > TSN_ROPE_MAX_AXES)
         return fail(TSN_ERR_ARG, "tsn_rope_axes: not a plan of tsn_rope_plan");
     for (uint32_t j = 0; j < p.P; ++j)
         if (p.axis[j] >= p.axes) return fail(TSN_ERR_ARG, "tsn_rope_axes: not a plan of tsn_rope_plan");
