@@ -39,7 +39,9 @@ class StreamingBlock:
         self.middle = tsn.BlockNorm(dev, C, post="rms", pre="rms", post_weight=ones(C), pre_weight=ones(C), residual_scale=0.9,
                                     gate_tanh=True)
         self.last = tsn.BlockNorm(dev, C, post="rms", pre="none", post_weight=ones(C), residual_scale=0.9, gate_tanh=True)
-        self.rope = tsn.RopeAxes(dev, d, axis_pairs, q_norm=ones(d), k_norm=ones(d))
+        q_norm, k_norm = ones(d), ones(d)
+        self.rope = tsn.RopeAxes(dev, d, axis_pairs, q_norm=q_norm, k_norm=k_norm)
+        self.rope_k = tsn.RopeAxes(dev, d, axis_pairs, k_norm=k_norm)   # an object for each place: calls of one form skip the checks
         self.attention = tsn.DiffAttention(dev, d, *(0.1 * r(d) for _ in range(4)), lambda_init=0.4, norm_weight=ones(2 * d))
         self.k_cache = torch.empty(batch, kv_heads, cache, 2 * d, dtype=torch.float16, device="cuda")   # head-major
         self.v_cache = torch.empty_like(self.k_cache)
@@ -65,7 +67,7 @@ class StreamingBlock:
         self.v_cache[:, :, at:end].copy_(self._linear(h, self.wv).view(B, T, Hk, 2 * d).transpose(1, 2))
         cached = self.k_cache[:, :, at:end].transpose(1, 2)                                    # [B, T, Hk, 2 d]
         for half in (0, 1):   # the maps' halves of the cache's heads
-            self.rope(None, k[:, :, half::2], pos, k_out=cached[..., half * d:(half + 1) * d])
+            self.rope_k(None, k[:, :, half::2], pos, k_out=cached[..., half * d:(half + 1) * d])
         self.rope(q, None, pos)
         o = torch.empty(B, T, H, 2 * d, dtype=torch.float16, device="cuda")
         self.attention(q.view(B, T, H, 2 * d), self.k_cache[:, :, :end].transpose(1, 2), self.v_cache[:, :, :end].transpose(1, 2), o,
