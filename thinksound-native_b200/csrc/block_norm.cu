@@ -1,14 +1,16 @@
 // block_norm.cu — norms before and after a block, fused with gate and residual scale (tsn_block_norm).
 //
 // Per row of C elements: x' = r x + act(g) Npost(y), h = Npre(x') (1 + scale) + shift. Bound by HBM: x, y and
-// the modulation rows are read once, x' and h written once. A row stays in registers from the first load to
-// the last store, each thread holding NV pieces of V elements (16 bytes of the branch's type). Up to two pieces a
+// the modulation rows are read once, x' and h written once. A row stays with its threads from the first load to
+// the last store, each holding NV pieces of V elements (16 bytes of the branch's type) in registers; only rows of more
+// than 4096 single elements (V 1, NV 16) spill, 290 to 700 bytes a thread. Up to two pieces a
 // thread, everything the row needs is requested before the first reduction, so its threads wait for memory
 // once; with more the modulation is read when it is needed, as it would not fit in registers. The mean and the sum of
 // squared distances from it are two reductions: one pass over squares would lose the variance of a row whose
 // mean is large.
-// 32 500 rows of 2048 bf16 elements with a modulation of each token take 164 us (932 MB, 5.7 TB/s, 0.87 of the measured
-// copy), 658 rows of 1024 4.0 us (latency: two reductions after the loads).
+// 32 500 rows of 2048 bf16 elements with a modulation of each token take 164 us in one long run of them, 180 us
+// with other inputs from call to call (932 MB, 5.7 and 5.2 TB/s, 0.87 and 0.79 of the measured copy), 658 rows of 1024
+// 4.0 us (latency: two reductions after the loads).
 #include "block_ops.h"
 #include "kernels.h"
 
@@ -266,8 +268,8 @@ cudaError_t launch(const NormArgs & n, cudaStream_t s) {
     } else {
         // One piece a thread while a block of 512 holds the row: the least latency where there are few rows (658
         // rows of 1024: 4.0 us, 4.8 with two pieces, 8.6 with four). Two, half the reductions, where the rows fill the GPU
-        // eight times (32 500 of 2048 bf16: 153 us, 166 with one; 2400: 18.1 and 17.1), and for wide rows of 16 bits
-        // from eight rows an SM on (2400 of 4096: 32.6 and 35.5; 600: no difference).
+        // eight times (with tanh gates 32 500 of 2048 bf16 take 161 us, 195 with one; 2400 of 2048 17.9 and 18.1), and for
+        // wide rows of 16 bits from eight rows an SM on (2400 of 4096: 33.1 and 36.7; 600: 12.5 and 12.0).
         const bool two = pieces > 64 && ((long long) n.rows * pieces >= 8ll * 148 * 2048 || (V == 8 && pieces > 256 && n.rows >= 8 * 148));
         const int per = pieces > 2048 ? 8 : pieces > 1024 ? 4 : pieces > 512 || two ? 2 : 1;
         const int threads = (pieces + 32 * per - 1) / (32 * per) * 32;
@@ -295,7 +297,8 @@ cudaError_t launch(const NormArgs & n, cudaStream_t s) {
                rows(a.gate, sizeof(T)) && rows(a.scale, sizeof(T)) && rows(a.shift, sizeof(T)) && vec(a.post_w) && vec(a.post_b) &&
                vec(a.pre_w) && vec(a.pre_b) && vec(a.res_vec);
     };
-    // pairs where 16 bytes do not fit: 5400 rows of 1462, f16 with an f32 residual, 50 us (2.9 TB/s), 89 by single elements
+    // pairs where 16 bytes do not fit: 5400 rows of 1462, f16 with an f32 residual, 50 us (2.9 TB/s); by single elements 89, and
+    // 91 for rows of 1461 (1.6 TB/s). Both are bound by narrow loads, which keep few bytes on their way.
     return aligned(V) ? launch<TX, T, V>(n, s) : aligned(2) ? launch<TX, T, 2>(n, s) : launch<TX, T, 1>(n, s);
 }
 

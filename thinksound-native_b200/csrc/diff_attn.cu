@@ -260,9 +260,10 @@ __device__ __forceinline__ void write_row(const Args & p, int b, int hk, int i, 
 // softmax is done, and O_1, O_2 (128 each): all 512 columns.
 // What bounds it: 2 exponentials for 12 d operations. At d = 64 a 128 x 64 tile pair takes 1024 cycles of the SFU
 // (16 exponentials a cycle), 768 with every fourth pair on the FMA pipe, and 896 of the tensor cores (the products with
-// N 64 wait for shared memory). 8125 tokens of 16 heads take 850 to 870 us, 0.94 PFLOP/s, about 1650 cycles a tile pair at
-// the 1.7 GHz that the power limit leaves: both maps' warps tend to compute, and to wait for TMEM, at the same time.
-// Measured and left: 32-key tiles on 16 softmax warps (1050 us), turns of the maps for the SFU (975 to 1080), 128-key
+// N 64 wait for shared memory). 8125 tokens of 16 heads take 890 to 930 us, 0.87 to 0.91 PFLOP/s, about 1650 cycles a
+// tile pair at the 1.65 GHz that the power limit leaves: both maps' warps tend to compute, and to wait for TMEM, at the same time.
+// The sums of the rounded probabilities are one mixed add a value; with the unrounded ones, two to a packed add, it
+// was 870. Measured before that, and left: 32-key tiles on 16 softmax warps (1050 us), turns of the maps for the SFU (975 to 1080), 128-key
 // tiles with one buffer (1287), the next tile's scores requested a half tile ahead (960).
 // Parts of the keys: each CTA leaves its rows' sums in its shared memory and, after a cluster barrier, adds up its
 // share of the rows over the cluster, in the order of the parts.
@@ -753,10 +754,15 @@ diff_attn_tc(const __grid_constant__ CUtensorMap tk, const __grid_constant__ CUt
 // Each warp streams its own 16-key slabs (slab w, w + W, ...) by TMA through a ring of its own, so warps never wait
 // for one another: scores, online softmax and O of both maps stay in the warp's registers. The warps' sums
 // are added up in shared memory at the end, the parts of split keys through the workspace.
-// One token over four caches of 20 480 to 32 768 keys (32 heads over 8, bf16) takes 73.2 us: 436 MB, 5.95 TB/s, 0.91 of the
-// measured copy; one over two caches of up to 704 keys 8.8 us, most of it the way from the launch to the first keys.
+// One token over four caches of 20 480 to 32 768 keys (32 heads over 8, bf16) takes 73.5 us: 436 MB, 5.93 TB/s, 0.91 of the
+// measured copy; one over two caches of up to 704 keys 9.0 us, most of it the way from the launch to the first keys.
 constexpr int SLAB = 16, RING = 3, SOME = 8, W = 8;   // keys of a slab, slabs of a ring, rows of a group, warps
-constexpr int FEW = 32;                        // rows up to which groups of 8 beat a tile of 128
+// Rows up to which groups of 8 are taken instead of a tile of 128. bf16, d 64, causal, us by groups / by tiles at 8, 32 and 64
+// rows a kv head: one head over 32 768 keys 18.6/59.5, 20.5/60.3, 29.2/61.6 (parts go to more SMs than a cluster has); 8 over
+// 4096 13.6/15.5, 15.6/16.6, 21.4/18.1; 2 x 8 over 704 10.3/12.3, 11.1/12.9, 11.3/14.2. Each group reads the keys anew, so
+// where there are more groups than SMs tiles are ahead from 24 rows on: 8 x 8 over 512 10.2/13.2, 19.1/13.8, 36.4/15.2;
+// 4 x 8 over 8192 31.9/37.1, 54.3/37.9, 133/39.8. The bound takes only the rows into account.
+constexpr int FEW = 32;
 
 template <int D>
 struct RowLay {

@@ -55,7 +55,8 @@ enum { NEXT, LANES, SHARED };   // interleaved: its own; halves: another lane's 
 // arithmetic; with fewer chunks than warps, several warps share a chunk's tokens.
 // Loads run one round ahead of the arithmetic: 32 500 tokens x 64 heads of 64, bf16, written head-major, take 101 us
 // (5.2 TB/s, 0.80 of the measured copy) with two tokens a round at four blocks per SM; 110 with one, 108 with four at
-// fewer blocks, 113 without the round ahead. With 16 tokens a block 104, with 32 113.
+// fewer blocks, 113 without the round ahead. With 16 tokens a block 104, with 32 113. (With other inputs from call to call
+// 108.) Four blocks leave a thread 64 registers: the 16-bit forms spill 8 to 44 bytes, with SHARED up to 124.
 template <class T, int LPH, int PAIR>
 __global__ void __launch_bounds__(32 * WARPS, 4) rope_rows8(const __grid_constant__ tsn_rope_plan_t p, const __grid_constant__ tsn_rope_args a, int tok) {
     constexpr int SIDE = 32 / LPH, AHEAD = sizeof(T) == 4 ? 1 : 2;   // tokens of a round: 16 or 32 bytes a lane each
