@@ -398,7 +398,8 @@ int tsn_rope_axes(tsn_device * dev, const tsn_rope_plan_t * plan, const tsn_rope
  * Visible keys of query i in batch b, with n = key_len[b] (int32, clamped to 0..Sk; null: Sk): j < n; and
  * key_mask[b * mask_sb + j] != 0 (bytes; null: all); and with causal j <= i + n - Sq, so the last query
  * sees the last key. A row that sees no key is zero, whatever eps is. What masked keys and values hold has no effect, NaN
- * and infinities included; a row that sees a non-finite value is NaN.
+ * and infinities included; a row that sees a non-finite value, or has a score that is NaN or +infinity, is NaN; a key
+ * whose score is -infinity has no share in that map.
  * lq1 .. lk2: f32 vectors of d, one per query head lam_sh elements apart (0: shared). norm_w: f32 [2 d] or
  * null for ones.
  * The probabilities are rounded to `type` before the product with v, as the tensor cores take them, and their sum is

@@ -585,6 +585,8 @@ diff_attn_tc(const __grid_constant__ CUtensorMap tk, const __grid_constant__ CUt
                 tiles(std::false_type(), 0, clear);
                 tiles(std::true_type(), clear, nt);
             }
+            // no score above -inf: the FMA pipe's exponentials gave its keys 2^-126 each
+            if (ref == -INFINITY && l < INFINITY) l = 0.0f;
             if (poison) l = NAN;
             if (ok && nt > 0) ok = mbar_wait_soon(&o_full[m * BUF], 0, abort_flag, p.err, DEV_TIMEOUT_TMEM);
             __syncwarp();
