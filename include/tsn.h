@@ -424,14 +424,90 @@ typedef struct tsn_diff_attn_args {
 } tsn_diff_attn_args;
 int tsn_diff_attn(tsn_device * dev, const tsn_diff_attn_args * a);
 
-/* For a Python binding of the three operators: a call whose tensors have the form of the call before (shape,
+/* ---- a key/value cache in pages that many sequences share: appending to it, attention over it.
+ * B sequences. The cache is P pages of `page` tokens each (a power of two, 16..1024) of Hk heads of D elements, keys in k and
+ * values in v: slot t of page p, head h starts at element p * sb + t * ss + h * sh, any order of the three. Place j of
+ * sequence b (its j-th token) lies in page table[b * table_sb + j / page], slot j % page; M entries a sequence. An entry
+ * outside 0..P - 1 is no page: what would be written there is dropped, and its keys are not seen.
+ * A call brings N rows of new tokens. Those of sequence b are rows q_start[b] .. q_start[b + 1] - 1 (q_start: B + 1 ascending
+ * numbers, 0..N; null: N = B, row b). len[b] counts the sequence's tokens in the cache, the new ones included: the i-th
+ * of n new tokens has place len[b] - n + i. Places below 0 or from M * page on are in no page. Rows that belong
+ * to no sequence are left as they were. table, len and q_start are int32 and read on the device; whatever they hold, nothing
+ * outside the pages is touched. Sequences may share pages that a call only reads.
+ * k and v are of `type`, TSN_F16 or TSN_BF16; base addresses and strides are multiples of 16 bytes, strides positive. At most
+ * 65535 sequences and heads, 2^30 new tokens and places of a sequence, 2^31 - 1 pages. */
+typedef struct tsn_paged {
+    uint32_t B, N, P, M, page, Hk, D;
+    int32_t type;
+    tsn_heads k, v;
+    const int32_t * table;
+    int64_t table_sb;
+    const int32_t * len, * q_start;
+} tsn_paged;
+
+/* Appends new tokens: an optional RMSNorm and the rotary positions of `plan` for queries and keys, as tsn_rope_axes does it, keys
+ * and values into their pages. q [N, Hq, D] into q_out (Hq 0 or q.p null: keys and values only), k and v [N, Hk, D]: row i,
+ * head h starts at element i * sb + h * st. q, k and v are of xtype, which is c.type or TSN_F32; q_out is of c.type, and may be
+ * q at the same strides where the types agree. D is a multiple of 8, 8..256; addresses and strides are multiples of 16 bytes.
+ * pos: int32, axis a of row i at pos[i * pos_ss + a]; null: the token's place (plans of one axis).
+ * means (or p null): of c.type, page p, head h at element p * sb + h * st: the mean over the keys that the page holds of its
+ * sequence, as they are stored, for every page that a new token went into. Sequences that share a page
+ * they write to, or a row of means, leave it undefined. */
+typedef struct tsn_cache_append_args {
+    tsn_paged c;
+    uint32_t Hq;
+    int32_t xtype;
+    float eps;
+    tsn_rows q, k, v, q_out, means;
+    const int32_t * pos;
+    int64_t pos_ss;
+    const float * q_norm, * k_norm;
+} tsn_cache_append_args;
+int tsn_cache_append(tsn_device * dev, const tsn_rope_plan_t * plan, const tsn_cache_append_args * a);
+
+/* Attention of the new tokens over their sequences' caches (appended before): out = softmax(scale q k^T) v over the visible keys.
+ * q and out [N, H, D] of c.type, row i, head h at element i * sb + h * st; query head h reads kv head h / (H / Hk), H / Hk at
+ * most 128; D is 64 or 128. scale 0 means 1 / sqrt(D). A token at place p sees place j of its sequence where j < len[b];
+ * with causal j <= p; and with window > 0 (causal only) j > p - window. A row that sees no key is zero.
+ * What unseen keys and values hold has no effect, NaN and infinities included; what seen ones hold enters as the arithmetic has
+ * it (a row with a score of NaN or +infinity is NaN, a key whose score is -infinity has no share).
+ * The probabilities are rounded to `type` before the product with v, as the tensor cores take them, and their sum is that of the
+ * rounded ones. most: new tokens of a sequence at most, as far as the caller knows (0: not known); it decides which kernel
+ * runs, never the result's extent. Split keys meet in a workspace, as those of tsn_diff_attn do. */
+typedef struct tsn_paged_attn_args {
+    tsn_paged c;
+    uint32_t H, most;
+    int32_t causal;
+    uint32_t window;
+    float scale;
+    tsn_rows q, out;
+} tsn_paged_attn_args;
+int tsn_paged_attn(tsn_device * dev, const tsn_paged_attn_args * a);
+
+/* Causal attention over `picks` pages of the cache, chosen for each new token and kv head by a cheap score: page x scores
+ * (sum of the group's query heads) . means[x], in 64 bits. For a token at place p, with its own page o = p / page, the
+ * candidates are pages 0..o; pages below `first` and above o - last (the token's own among them; last at least 1) come before
+ * all others, then higher scores, and of equal scores the lower page. chosen [N, Hk, picks], int32: the chosen pages in
+ * ascending order, then -1 where there are fewer. out as tsn_paged_attn with causal over the keys of the chosen pages. means is
+ * what tsn_cache_append keeps, all finite; entries of the table that are no page score as zero means do. A token at a place
+ * below 0 or from M * page on chooses nothing and gets zeros. first + last <= picks <= 1024; M at most 16384. */
+typedef struct tsn_sparse_attn_args {
+    tsn_paged c;
+    uint32_t H, picks, first, last;
+    float scale;
+    tsn_rows q, out, means;
+    int32_t * chosen;
+} tsn_sparse_attn_args;
+int tsn_sparse_attn(tsn_device * dev, const tsn_sparse_attn_args * a);
+
+/* For a Python binding of the operators on tensors: a call whose tensors have the form of the call before (shape,
  * strides, type, place) needs no checks, only their addresses. `view` is the function of the tensor type's DLPack
  * exchange table that describes an object as a DLTensor, `item` the interpreter's PyTuple_GetItem, `type` the objects'
  * exact type, `none` the None object. tsn_form_take takes a tuple of n objects, writes their addresses (null for
  * None) to *to[i] and returns 1 if every one has
  * the recorded form, or, with `record`, records the forms. Otherwise it returns 0, what lies at *to[i] is undefined,
  * and nothing is recorded any more. The caller holds the interpreter's lock. Host only. */
-enum { TSN_FORM_TENSORS = 7 };
+enum { TSN_FORM_TENSORS = 11 };
 typedef struct tsn_form_tensor {
     int32_t there, device_type, device, ndim;
     uint32_t dtype;

@@ -7,8 +7,10 @@
 #include <unistd.h>
 
 #include "block_ops.h"
+#include "split_ws.h"
 #include "compat.h"
 #include "gguf_io.h"
+#include "paged.h"
 #include "runtime.h"
 
 using namespace tsn;
@@ -61,6 +63,7 @@ int tsn_device_create(int ordinal, tsn_device ** out) {
     CKR(configure_gemv());
     CKR(configure_gemv_tc());
     CKR(configure_diff_attn());
+    CKR(configure_paged());
     *out = d.release();
     return TSN_OK;
 }
@@ -77,7 +80,7 @@ int tsn_device_destroy(tsn_device * dev) {
     if (c.split_used) cudaEventSynchronize(c.split_ev);
     if (c.split_ws) cudaFree(c.split_ws);
     if (c.split_ev) cudaEventDestroy(c.split_ev);
-    release_diff_attn(c.ordinal);
+    release_split(c.ordinal);
     if (c.d_err) cudaFree(c.d_err);
     if (c.ev0) cudaEventDestroy(c.ev0);
     if (c.ev1) cudaEventDestroy(c.ev1);
@@ -310,6 +313,15 @@ static int guarded(tsn_device * dev, const void * args, F && f) {
     }
 }
 
+template <class F>
+static int refused(F && check) {
+    try {
+        return check();
+    } catch (...) {
+        return TSN_ERR_OOM;
+    }
+}
+
 extern "C" {
 
 int tsn_block_norm(tsn_device * dev, const tsn_block_norm_args * a) {
@@ -328,6 +340,19 @@ int tsn_rope_axes(tsn_device * dev, const tsn_rope_plan_t * plan, const tsn_rope
 }
 int tsn_diff_attn(tsn_device * dev, const tsn_diff_attn_args * a) {
     return guarded(dev, a, [&](DeviceCtx & c) { return diff_attn(c, *a); });
+}
+// the paged cache's: what is refused is refused before the device is looked at
+int tsn_cache_append(tsn_device * dev, const tsn_rope_plan_t * plan, const tsn_cache_append_args * a) {
+    if (int rc = refused([&] { return check_cache_append(plan, a); })) return rc;
+    return guarded(dev, a, [&](DeviceCtx & c) { return cache_append(c, *plan, *a); });
+}
+int tsn_paged_attn(tsn_device * dev, const tsn_paged_attn_args * a) {
+    if (int rc = refused([&] { return check_paged_attn(a); })) return rc;
+    return guarded(dev, a, [&](DeviceCtx & c) { return paged_attn(c, *a); });
+}
+int tsn_sparse_attn(tsn_device * dev, const tsn_sparse_attn_args * a) {
+    if (int rc = refused([&] { return check_sparse_attn(a); })) return rc;
+    return guarded(dev, a, [&](DeviceCtx & c) { return sparse_attn(c, *a); });
 }
 
 // ------------------------------------------------------------------------------- model face

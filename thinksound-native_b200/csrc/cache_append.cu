@@ -1,0 +1,259 @@
+// cache_append.cu — new tokens into a paged key/value cache, with the heads' norm and the rotary positions (tsn_cache_append).
+//
+// Bound by HBM: q, k and v are read once, q_out and the pages written once. As in tsn_rope_axes a block takes a few whole
+// tokens, computes their cosines and sines once into shared memory (64-bit phases), and its warps run over the heads, 8 elements a
+// lane, loads one round ahead. What the cache adds is a chain of small reads for each token (its sequence, length and page), one
+// warp a token, while the heads' loads are on their way.
+// The means of the pages are a second kernel, which reads the touched pages' keys after the first has written them.
+#include <algorithm>
+#include <type_traits>
+
+#include "kernels.h"
+#include "paged.h"
+
+namespace tsn {
+
+namespace {
+
+__device__ __forceinline__ float phase(int pos, uint64_t turn) {   // pos * turn modulo one turn, in [-1/2, 1/2) turns
+    const uint64_t p = (uint64_t) (long long) pos * turn;
+    return (float) (int) (p >> 32) * 0x1p-32f;
+}
+
+constexpr int WARPS = 8, MAX_TOK = 8;
+enum { NEXT, LANES, SHARED };   // where the other element of a lane's pairs is: with the lane, another lane, shared memory
+
+struct Append {
+    tsn_cache_append_args a;
+    int page_log2, tok;   // tokens of a block
+};
+
+// Block (x, z): tokens x * tok .., chunks 8 z .. of 32 / LPH heads: the queries', then the keys', then the values'.
+template <class TX, class T, int LPH, int PAIR>
+__global__ void __launch_bounds__(32 * WARPS, 4) cache_append_kernel(const __grid_constant__ tsn_rope_plan_t p, const __grid_constant__ Append n) {
+    constexpr int SIDE = 32 / LPH;
+    __shared__ __align__(16) float2 turn[MAX_TOK * TSN_ROPE_MAX_PAIRS + 8];
+    __shared__ float mate[PAIR == SHARED ? WARPS : 1][32 * 9];   // a lane's 8 elements, one word of padding between lanes
+    __shared__ int place[MAX_TOK], spot[MAX_TOK], slot[MAX_TOK];   // spot: the page, -1: none
+    pdl_wait();
+    const tsn_cache_append_args & a = n.a;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int D = (int) p.D, P = (int) p.P, Hq = (int) a.Hq, Hk = (int) a.c.Hk, tok = n.tok;
+    const long long s0 = (long long) blockIdx.x * tok;
+    const int here = (int) min((long long) tok, a.c.N - s0);
+    const int sub = lane / LPH, at = (lane & (LPH - 1)) * 8;
+    const int q_chunks = (Hq + SIDE - 1) / SIDE, k_chunks = (Hk + SIDE - 1) / SIDE, chunks = q_chunks + 2 * k_chunks;
+    const int sharing = chunks < WARPS ? WARPS / chunks : 1;   // warps of a chunk
+    const float inv_D = 1.0f / (float) D;
+    const int row = (P + 1) & ~1;   // a token's pairs in the table, from a 16-byte boundary on
+
+    const int chunk = sharing > 1 ? (warp < sharing * chunks ? warp % chunks : chunks) : (int) blockIdx.y * WARPS + warp;
+    const int what = chunk < q_chunks ? 0 : chunk < q_chunks + k_chunks ? 1 : 2;   // q, k, v
+    const tsn_rows & in = what == 0 ? a.q : what == 1 ? a.k : a.v;
+    const float * wp = what == 0 ? a.q_norm : what == 1 ? a.k_norm : nullptr;
+    const int head = (chunk - (what == 0 ? 0 : what == 1 ? q_chunks : q_chunks + k_chunks)) * SIDE + sub, from = sharing > 1 ? warp / chunks : 0;
+    const bool mine = chunk < chunks && at < D && head < (what == 0 ? Hq : Hk);
+    const TX * x = (const TX *) in.p + (s0 + from) * in.sb + head * in.st + at;
+    const long long dx = sharing * in.sb;
+    Words<TX, 8> raw, next;
+    auto fetch = [&](int k) {
+        if (mine && k < here) next = load_words<TX, 8>(x);
+        x += dx;
+    };
+    fetch(from);   // before the table: the loads are on their way
+    float2 w[4];
+    if (wp)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) w[i] = mine ? make_float2(wp[at + 2 * i], wp[at + 2 * i + 1]) : make_float2(0.0f, 0.0f);
+    if (warp < here) {
+        const int i = (int) s0 + warp, b = seq_of_row(a.c, i);
+        const int at_place = b < 0 ? 0 : place_of_row(a.c, b, i);
+        if (lane == 0) {
+            place[warp] = at_place;
+            spot[warp] = b < 0 ? -2 : page_of(a.c, b, at_place >> n.page_log2);   // -2: a row of no sequence
+            slot[warp] = at_place & ((1 << n.page_log2) - 1);
+        }
+    }
+    __syncthreads();
+    for (int i = threadIdx.x; i < here * P; i += 32 * WARPS) {
+        const int k = i / P, j = i % P;
+        const int pos = a.pos ? a.pos[(s0 + k) * a.pos_ss + p.axis[j]] : place[k];
+        float sn, cs;
+        sincospif(2.0f * phase(pos, p.turn[j]), &sn, &cs);
+        turn[k * row + j] = make_float2(cs, sn);
+    }
+    __syncthreads();
+    if (chunk >= chunks) return;
+
+    for (int k = from; k < here; k += sharing) {
+        raw = next;
+        fetch(k + sharing);
+        float u[8];
+        to_floats<TX, 8>(raw, u);
+        if (wp) {
+            float2 q = make_float2(0.0f, 0.0f);
+#pragma unroll
+            for (int i = 0; i < 8; i += 2) q = fma2(make_float2(u[i], u[i + 1]), make_float2(u[i], u[i + 1]), q);
+            float ss = mine ? q.x + q.y : 0.0f;
+#pragma unroll
+            for (int o = LPH >> 1; o; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+            const float inv = rsqrtf(fmaf(ss, inv_D, a.eps));
+#pragma unroll
+            for (int i = 0; i < 8; i += 2) {
+                const float2 r = mul2(make_float2(u[i], u[i + 1]), mul2(w[i / 2], make_float2(inv, inv)));
+                u[i] = r.x;
+                u[i + 1] = r.y;
+            }
+        }
+        const float2 * tr = turn + k * row;
+        if (what == 2) {
+        } else if (PAIR == NEXT) {
+#pragma unroll
+            for (int i = 0; i < 8; i += 4) {
+                const int j = (at + i) >> 1;
+                const float4 cs = *(const float4 *) (tr + (j < row ? j : 0));
+                const float2 v = make_float2(u[i], u[i + 2]);
+                if (j < P) {
+                    u[i] = v.x * cs.x - u[i + 1] * cs.y;
+                    u[i + 1] = v.x * cs.y + u[i + 1] * cs.x;
+                }
+                if (j + 1 < P) {
+                    u[i + 2] = v.y * cs.z - u[i + 3] * cs.w;
+                    u[i + 3] = v.y * cs.w + u[i + 3] * cs.z;
+                }
+            }
+        } else if (PAIR == LANES) {
+            const bool low = at < P, turned = at < 2 * P;
+            const int other = turned ? (low ? lane + P / 8 : lane - P / 8) : lane;
+            const float4 * cs = (const float4 *) (tr + (turned ? (low ? at : at - P) : 0));
+#pragma unroll
+            for (int i = 0; i < 8; i += 2) {
+                const float4 c2 = cs[i / 2];
+                const float m0 = __shfl_sync(0xffffffffu, u[i], other), m1 = __shfl_sync(0xffffffffu, u[i + 1], other);
+                if (turned) {
+                    u[i] = fmaf(u[i], c2.x, low ? -m0 * c2.y : m0 * c2.y);
+                    u[i + 1] = fmaf(u[i + 1], c2.z, low ? -m1 * c2.w : m1 * c2.w);
+                }
+            }
+        } else {
+            float * m = mate[warp];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) m[lane * 9 + i] = u[i];
+            __syncwarp();
+            const int base = lane & ~(LPH - 1);   // the head's first lane
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const int e = at + i;
+                if (e < 2 * P) {
+                    const int o = e < P ? e + P : e - P;
+                    const float v = m[(base + (o >> 3)) * 9 + (o & 7)];
+                    const float2 cs = tr[e < P ? e : e - P];
+                    u[i] = fmaf(u[i], cs.x, e < P ? -v * cs.y : v * cs.y);
+                }
+            }
+            __syncwarp();
+        }
+        if (!mine) continue;
+        if (what == 0) {
+            if (spot[k] != -2) store_words<T, 8>((T *) a.q_out.p + (s0 + k) * a.q_out.sb + head * a.q_out.st + at, u);
+        } else if (spot[k] >= 0) {
+            const tsn_heads & to = what == 1 ? a.c.k : a.c.v;
+            store_words<T, 8>((T *) to.p + spot[k] * to.sb + slot[k] * to.ss + head * to.sh + at, u);
+        }
+    }
+}
+
+// The mean key of every page that a new token went into: the work of the token that is the page's last, a warp a head. Sums are
+// f32, over the keys in the order of lanes, then of the lanes.
+template <class T, int LPH>
+__global__ void __launch_bounds__(32 * WARPS) cache_means_kernel(const __grid_constant__ Append n) {
+    constexpr int SIDE = 32 / LPH, AHEAD = 8;   // keys of a step, steps whose loads run at once
+    pdl_wait();
+    const tsn_cache_append_args & a = n.a;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, D = (int) a.c.D, Hk = (int) a.c.Hk;
+    const int sub = lane / LPH, at = (lane & (LPH - 1)) * 8;
+    const bool mine = at < D;
+    const long long s0 = (long long) blockIdx.x * n.tok;
+    const int here = (int) min((long long) n.tok, a.c.N - s0);
+    for (int k = 0; k < here; ++k) {
+        const int i = (int) s0 + k, b = seq_of_row(a.c, i);
+        if (b < 0) continue;
+        const int pl = place_of_row(a.c, b, i), slot = pl & ((1 << n.page_log2) - 1);
+        if (slot + 1 != (1 << n.page_log2) && i + 1 != seq_start(a.c, b + 1)) continue;
+        const int id = page_of(a.c, b, pl >> n.page_log2);
+        if (id < 0) continue;
+        for (int h = warp; h < Hk; h += WARPS) {
+            const T * key = (const T *) a.c.k.p + id * a.c.k.sb + h * a.c.k.sh + at;
+            float sum[8] = {};
+            for (int t = sub; t <= slot; t += SIDE * AHEAD) {
+                Words<T, 8> r[AHEAD];
+#pragma unroll
+                for (int y = 0; y < AHEAD; ++y)
+                    if (mine && t + y * SIDE <= slot) r[y] = load_words<T, 8>(key + (t + y * SIDE) * a.c.k.ss);
+#pragma unroll
+                for (int y = 0; y < AHEAD; ++y)
+                    if (mine && t + y * SIDE <= slot) {
+                        float u[8];
+                        to_floats<T, 8>(r[y], u);
+#pragma unroll
+                        for (int e = 0; e < 8; ++e) sum[e] += u[e];
+                    }
+            }
+            __syncwarp();
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+#pragma unroll
+                for (int o = LPH; o < 32; o <<= 1) sum[e] += __shfl_xor_sync(~0u, sum[e], o);
+                sum[e] /= (float) (slot + 1);
+            }
+            if (mine && sub == 0) store_words<T, 8>((T *) a.means.p + id * a.means.sb + h * a.means.st + at, sum);
+        }
+    }
+}
+
+template <class TX, class T>
+cudaError_t launch(const tsn_rope_plan_t & p, Append & n, cudaStream_t s) {
+    const tsn_cache_append_args & a = n.a;
+    int lph = 1;
+    while (lph * 8 < (int) p.D) lph *= 2;
+    const int side = 32 / lph, chunks = (int) ((a.Hq + side - 1) / side + 2 * ((a.c.Hk + side - 1) / side));
+    const long long turns = (chunks + WARPS - 1) / WARPS;
+    // Tokens of a block: 8 share its start; fewer while four blocks per SM take them all.
+    n.tok = (int) std::min<long long>(MAX_TOK, ((long long) a.c.N * turns + 4 * 148 - 1) / (4 * 148));
+    const dim3 blocks((a.c.N + n.tok - 1) / n.tok, (unsigned) turns);
+    const int pair = p.layout == TSN_ROPE_INTERLEAVED ? NEXT : p.P % 8 == 0 ? LANES : SHARED;
+    const int mean_tok = (int) std::max(1u, std::min(32u, a.c.N / 1024));
+    cudaError_t e = cudaSuccess;
+    auto go = [&](auto L) {
+        constexpr int LPH = decltype(L)::value;
+        if (pair == NEXT) e = launch_cl(cache_append_kernel<TX, T, LPH, NEXT>, blocks, dim3(32 * WARPS), 0, s, dim3(1), p, n);
+        else if (pair == LANES) e = launch_cl(cache_append_kernel<TX, T, LPH, LANES>, blocks, dim3(32 * WARPS), 0, s, dim3(1), p, n);
+        else e = launch_cl(cache_append_kernel<TX, T, LPH, SHARED>, blocks, dim3(32 * WARPS), 0, s, dim3(1), p, n);
+        if (e != cudaSuccess || !a.means.p) return;
+        n.tok = mean_tok;
+        e = launch_cl(cache_means_kernel<T, LPH>, dim3((a.c.N + mean_tok - 1) / mean_tok), dim3(32 * WARPS), 0, s, dim3(1), n);
+    };
+    if (lph == 1) go(std::integral_constant<int, 1>());
+    else if (lph == 2) go(std::integral_constant<int, 2>());
+    else if (lph == 4) go(std::integral_constant<int, 4>());
+    else if (lph == 8) go(std::integral_constant<int, 8>());
+    else if (lph == 16) go(std::integral_constant<int, 16>());
+    else go(std::integral_constant<int, 32>());
+    if (e != cudaSuccess) cudaGetLastError();
+    return e;
+}
+
+} // namespace
+
+int cache_append(DeviceCtx & c, const tsn_rope_plan_t & p, const tsn_cache_append_args & a) {
+    if (a.c.N == 0 || a.c.B == 0) return TSN_OK;
+    Append n{a, log2_of(a.c.page), 1};
+    if (!n.a.q.p) n.a.Hq = 0;
+    const bool wide = a.xtype == TSN_F32;
+    const cudaError_t e = a.c.type == TSN_F16 ? (wide ? launch<float, __half>(p, n, c.stream) : launch<__half, __half>(p, n, c.stream))
+                                              : (wide ? launch<float, __nv_bfloat16>(p, n, c.stream) : launch<__nv_bfloat16, __nv_bfloat16>(p, n, c.stream));
+    if (e != cudaSuccess) return fail(TSN_ERR_CUDA, std::string("tsn_cache_append: ") + cudaGetErrorString(e));
+    return TSN_OK;
+}
+
+} // namespace tsn

@@ -11,15 +11,12 @@
 // causal rows differ in what they see, non-finite values of a V row become zero and each row that sees such a
 // key is marked: its result is NaN.
 // Every wait is bounded; barriers of a whole block or cluster are on paths that all threads take.
-#include "block_ops.h"
+#include "attn_ops.cuh"
 #include "kernels.h"
-#include "ptx.cuh"
-
-#include <cudaTypedefs.h>
+#include "split_ws.h"
 
 #include <algorithm>
 #include <atomic>
-#include <mutex>
 
 namespace tsn {
 
@@ -42,133 +39,8 @@ struct Args {
     int * err;
 };
 
-__device__ __forceinline__ float ex2(float x) {
-    float y;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-    return y;
-}
-__device__ __forceinline__ uint64_t f2_pack(float a, float b) {
-    uint64_t r;
-    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
-    return r;
-}
-__device__ __forceinline__ void f2_unpack(uint64_t r, float & a, float & b) {
-    asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(r));
-}
-__device__ __forceinline__ uint64_t ffma2(uint64_t a, uint64_t b, uint64_t c) {
-    uint64_t d;
-    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
-    return d;
-}
-__device__ __forceinline__ uint64_t f2_neg(uint64_t a) { return a ^ 0x8000000080000000ull; }
-__device__ __forceinline__ uint64_t fadd2(uint64_t a, uint64_t b) {
-    uint64_t d;
-    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
-    return d;
-}
-// (2^x, 2^y) on the FMA pipe, x and y clamped to -126 or more: 2^i p(f), i the nearest whole number, f = x - i in [-1/2, 1/2],
-// p the polynomial of least relative error there (Remez exchange): 7.5e-5 at degree 3, 2.6e-6 at degree 4, each below
-// an eighth of half a unit of the 16-bit type that the result is rounded to. Adding 1.5 * 2^23 rounds to i and leaves
-// it in the low bits. NaN becomes 0x7f7fffff, which rounds to infinity in either 16-bit type. ZERO: what was clamped becomes 0 (p(0) < 1, so 2^-126 p(0) is subnormal).
-template <bool BF16, bool ZERO>
-__device__ __forceinline__ uint64_t ex2_fma(uint64_t xy) {
-    float x, y;
-    f2_unpack(xy, x, y);
-    asm("max.NaN.f32 %0, %0, %1;" : "+f"(x) : "f"(-126.0f));
-    asm("max.NaN.f32 %0, %0, %1;" : "+f"(y) : "f"(-126.0f));
-    const uint64_t v = f2_pack(x, y), magic = f2_pack(12582912.0f, 12582912.0f), r = fadd2(v, magic);
-    const uint64_t f = fadd2(v, fadd2(magic, f2_neg(r)));
-    auto two = [](float c) { return f2_pack(c, c); };
-    uint64_t q;
-    if (BF16) {
-        q = ffma2(two(0.0551716685f), f, two(0.242611125f));
-        q = ffma2(q, f, two(0.693260968f));
-        q = ffma2(q, f, two(0.999928057f));
-    } else {
-        q = ffma2(two(0.00957010221f), f, two(0.0559178591f));
-        q = ffma2(q, f, two(0.240247443f));
-        q = ffma2(q, f, two(0.693121791f));
-        q = ffma2(q, f, two(0.999999285f));
-    }
-    float a, b, i, j;
-    f2_unpack(q, a, b);
-    f2_unpack(r, i, j);
-    uint64_t e = f2_pack(__uint_as_float(__float_as_uint(a) + (__float_as_uint(i) << 23)), __uint_as_float(__float_as_uint(b) + (__float_as_uint(j) << 23)));
-    if (ZERO) asm("mul.rn.ftz.f32x2 %0, %0, %1;" : "+l"(e) : "l"(two(1.0f)));
-    return e;
-}
-template <bool BF16>
-__device__ __forceinline__ uint32_t pack16(float a, float b) {
-    uint32_t r;
-    if (BF16) asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(b), "f"(a));
-    else asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(b), "f"(a));
-    return r;
-}
-// a and b += the two 16-bit values of a word, in f32
-template <bool BF16>
-__device__ __forceinline__ void add_rounded(float & a, float & b, uint32_t two) {
-    if (BF16) asm("{\n .reg .b16 l, h;\n mov.b32 {l, h}, %2;\n add.rn.f32.bf16 %0, l, %0;\n add.rn.f32.bf16 %1, h, %1;\n}" : "+f"(a), "+f"(b) : "r"(two));
-    else asm("{\n .reg .b16 l, h;\n mov.b32 {l, h}, %2;\n add.rn.f32.f16 %0, l, %0;\n add.rn.f32.f16 %1, h, %1;\n}" : "+f"(a), "+f"(b) : "r"(two));
-}
-// the low n bits of a word, n of any sign and size
-__device__ __forceinline__ uint32_t low_bits(int n) { return n >= 32 ? 0xffffffffu : n <= 0 ? 0u : (1u << n) - 1u; }
-// of two 16-bit values, the non-finite ones set to zero
-template <bool BF16>
-__device__ __forceinline__ uint32_t finite_only(uint32_t v) {
-    const uint32_t e = BF16 ? 0x7f80u : 0x7c00u;
-    if ((v & e) == e) v &= 0xffff0000u;
-    if ((v & (e << 16)) == (e << 16)) v &= 0x0000ffffu;
-    return v;
-}
-
-// 32 scores s of a row become 2^(c s + neg): P as 16-bit pairs, and the sum of these rounded values, so that what rounding
-// takes from a key's share in the product it takes from the divisor too. Every fourth pair takes the FMA pipe.
-template <bool BF16, bool MASKED>
-__device__ __forceinline__ void exponentials(const uint32_t * s, uint32_t * pk, float c, float ref, float (&sum)[4]) {
-    const float neg = ref == -INFINITY ? 0.0f : -ref;
-    const uint64_t c2 = f2_pack(c, c), neg2 = f2_pack(neg, neg);
-#pragma unroll
-    for (int e = 0; e < 16; ++e) {
-        const uint64_t v = ffma2(f2_pack(__uint_as_float(s[2 * e]), __uint_as_float(s[2 * e + 1])), c2, neg2);
-        float y, z;
-        if (e % 4 == 3) {
-            f2_unpack(ex2_fma<BF16, MASKED>(v), y, z);
-        } else {
-            f2_unpack(v, y, z);
-            y = ex2(y);
-            z = ex2(z);
-        }
-        pk[e] = pack16<BF16>(y, z);
-        add_rounded<BF16>(sum[2 * (e & 1)], sum[2 * (e & 1) + 1], pk[e]);
-    }
-}
-__device__ __forceinline__ float greatest(const uint32_t * s) {   // of 32
-    float mx[2] = {-INFINITY, -INFINITY};
-#pragma unroll
-    for (int e = 0; e < 32; e += 2) mx[(e >> 1) & 1] = fmaxf(mx[(e >> 1) & 1], fmaxf(__uint_as_float(s[e]), __uint_as_float(s[e + 1])));
-    return fmaxf(mx[0], mx[1]);
-}
-__device__ __forceinline__ void hide(uint32_t * s, uint32_t vis) {   // scores of the keys that the row does not see
-    if (__any_sync(~0u, vis != ~0u))
-#pragma unroll
-        for (int e = 0; e < 32; ++e)
-            if (!((vis >> e) & 1u)) s[e] = 0xff800000u;   // -inf
-}
-
 // A row's sums as they are added up over warps, CTAs or parts of the keys: O [2 maps][D], then ref and l of both maps.
 constexpr int row_words(int D) { return 2 * D + 4; }
-
-// E (2 or 4) words of shared or, past the L1 cache, global memory
-template <int E, bool GLOBAL>
-__device__ __forceinline__ void read_words(const float * at, float * v) {
-    if (E == 4) {
-        const float4 x = GLOBAL ? __ldcg((const float4 *) at) : *(const float4 *) at;
-        v[0] = x.x; v[1] = x.y; v[2] = x.z; v[3] = x.w;
-    } else {
-        const float2 x = GLOBAL ? __ldcg((const float2 *) at) : *(const float2 *) at;
-        v[0] = x.x; v[1] = x.y;
-    }
-}
 
 // Adds up `count` (1 to 64) sets of a row's sums, one warp: rd(i, k) is word k of set i, rdv(i, k, v) D / 32 words from k
 // on. Returns O (this lane's D / 32 columns), ref and l. The order is that of the sets. Eight sets are read at once.
@@ -775,29 +647,6 @@ struct RowLay {
     static_assert(W * SUMS * 4 <= W * RING * STAGE, "the warps' sums fit in their rings");
 };
 
-template <bool BF16>
-__device__ __forceinline__ void mma16816(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-    if (BF16)
-        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-                     : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
-    else
-        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-                     : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
-}
-// the 8 x 8 matrix of 16-bit elements that the warp holds, transposed
-__device__ __forceinline__ uint32_t movmatrix(uint32_t a) {
-    uint32_t d;
-    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(d) : "r"(a));
-    return d;
-}
-template <bool TRANS>
-__device__ __forceinline__ void ldmatrix4(uint32_t (&r)[4], uint32_t at) {
-    if (TRANS)
-        asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(at) : "memory");
-    else
-        asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(at) : "memory");
-}
-
 template <int D, bool BF16>
 __global__ void __launch_bounds__(32 * W, 1)
 diff_attn_rows(const __grid_constant__ CUtensorMap tk, const __grid_constant__ CUtensorMap tv, const __grid_constant__ Args p) {
@@ -1075,22 +924,10 @@ diff_attn_rows(const __grid_constant__ CUtensorMap tk, const __grid_constant__ C
 }
 
 // ---------------------------------------------------------------- host
-PFN_cuTensorMapEncodeTiled_v12000 encoder() {
-    static const PFN_cuTensorMapEncodeTiled_v12000 enc = [] {
-        cudaDriverEntryPointQueryResult q{};
-        void * fn = nullptr;
-        if (cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &fn, 12000, cudaEnableDefault, &q) != cudaSuccess ||
-            q != cudaDriverEntryPointSuccess)
-            fn = nullptr;
-        return (PFN_cuTensorMapEncodeTiled_v12000) fn;
-    }();
-    return enc;
-}
-
 // {2 d, Sk, Hk, B} view of keys or values with {64, box_keys, 1, 1} boxes. A dimension of one element has a
 // stride that is never taken: any valid one stands in.
 bool make_kv_map(CUtensorMap * m, const tsn_diff_attn_args & a, const tsn_heads & t, uint32_t B, uint32_t box_keys) {
-    const PFN_cuTensorMapEncodeTiled_v12000 enc = encoder();
+    const PFN_cuTensorMapEncodeTiled_v12000 enc = tensor_map_encoder();
     if (!enc) return false;
     const cuuint64_t row = 2 * a.d * 2;
     const cuuint64_t dims[4] = {2 * a.d, a.Sk, a.Hk, B};
@@ -1102,100 +939,7 @@ bool make_kv_map(CUtensorMap * m, const tsn_diff_attn_args & a, const tsn_heads 
                CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-constexpr size_t COUNTERS = 4096, WORKSPACE = COUNTERS * 4 + ((size_t) 32 << 20);
 constexpr int SMS = 148;
-
-// Host calls that touch no stream of the program, so that they also work while one of them is being captured.
-struct Uncaptured {
-    cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
-    Uncaptured() { cudaThreadExchangeStreamCaptureMode(&mode); }
-    ~Uncaptured() { cudaThreadExchangeStreamCaptureMode(&mode); }
-};
-cudaError_t zero(void * p, size_t bytes) {   // and waits for it
-    Uncaptured u;
-    cudaStream_t s = nullptr;
-    cudaError_t e = cudaStreamCreateWithFlags(&s, cudaStreamNonBlocking);
-    if (e == cudaSuccess) e = cudaMemsetAsync(p, 0, bytes, s);
-    if (e == cudaSuccess) e = cudaStreamSynchronize(s);
-    if (s) cudaStreamDestroy(s);
-    return e;
-}
-cudaError_t allocate(void ** p, size_t bytes) {
-    Uncaptured u;
-    return cudaMalloc(p, bytes);
-}
-int failed(cudaError_t e) {
-    cudaGetLastError();
-    return fail(e == cudaErrorMemoryAllocation ? TSN_ERR_OOM : TSN_ERR_CUDA, std::string("tsn_diff_attn: ") + cudaGetErrorString(e));
-}
-
-// The device's workspace, ordered after the last call that used it. Streams are told apart by their id, which no other
-// stream of the process ever has: a handle may stand for one stream per thread, or be given out again.
-int workspace(DeviceCtx & c, unsigned long long stream) {
-    cudaError_t e = cudaSuccess;
-    if (!c.split_ws) {
-        void * p = nullptr;
-        e = allocate(&p, WORKSPACE);
-        if (e == cudaSuccess) e = zero(p, COUNTERS * 4);
-        if (e == cudaSuccess && !c.split_ev) e = cudaEventCreateWithFlags(&c.split_ev, cudaEventDisableTiming);
-        if (e != cudaSuccess) { cudaFree(p); return failed(e); }
-        c.split_ws = p;
-    }
-    if (c.split_used && c.split_stream != stream) e = cudaStreamWaitEvent(c.stream, c.split_ev, 0);
-    return e == cudaSuccess ? TSN_OK : failed(e);
-}
-
-// Workspaces of captured calls. One belongs to its call's graph, so that replays need no order among themselves or with other
-// calls; when the graph and its executables are gone it lies here until another capture, or the device's end, takes it.
-struct Block {
-    void * p;
-    size_t bytes;
-    int ordinal;
-    Block * next;
-};
-std::mutex g_idle_mu;
-Block * g_idle = nullptr;
-
-void CUDART_CB make_idle(void * block) {   // no CUDA calls in here
-    std::lock_guard<std::mutex> lk(g_idle_mu);
-    Block * b = (Block *) block;
-    b->next = g_idle;
-    g_idle = b;
-}
-
-int graph_workspace(const DeviceCtx & c, cudaGraph_t graph, size_t bytes, void ** out) {
-    size_t size = (size_t) 1 << 18;   // powers of two, so that they fit the calls of later captures
-    while (size < bytes) size *= 2;
-    Block * b = nullptr;
-    {
-        std::lock_guard<std::mutex> lk(g_idle_mu);
-        for (Block ** at = &g_idle; *at; at = &(*at)->next)
-            if ((*at)->ordinal == c.ordinal && (*at)->bytes == size) {
-                b = *at;
-                *at = b->next;
-                break;
-            }
-    }
-    if (!b) {
-        b = new Block{nullptr, size, c.ordinal, nullptr};
-        const cudaError_t e = allocate(&b->p, size);
-        if (e != cudaSuccess) { delete b; return failed(e); }
-    }
-    cudaUserObject_t object = nullptr;
-    cudaError_t e = zero(b->p, size);
-    if (e == cudaSuccess) e = cudaUserObjectCreate(&object, b, make_idle, 1, cudaUserObjectNoDestructorSync);
-    if (e != cudaSuccess) {
-        make_idle(b);
-        return failed(e);
-    }
-    e = cudaGraphRetainUserObject(graph, object, 1, cudaGraphUserObjectMove);
-    if (e != cudaSuccess) {
-        cudaUserObjectRelease(object, 1);
-        return failed(e);
-    }
-    *out = b->p;
-    return TSN_OK;
-}
 
 template <int D, bool BF16>
 cudaError_t launch_tc(const CUtensorMap & tk, const CUtensorMap & tv, const Args & p, unsigned grid, cudaStream_t s) {
@@ -1242,26 +986,6 @@ cudaError_t configure_diff_attn() {
     return e;
 }
 
-void release_diff_attn(int ordinal) {
-    Block * gone = nullptr;
-    {
-        std::lock_guard<std::mutex> lk(g_idle_mu);
-        for (Block ** at = &g_idle; *at;) {
-            Block * b = *at;
-            if (b->ordinal != ordinal) { at = &b->next; continue; }
-            *at = b->next;
-            b->next = gone;
-            gone = b;
-        }
-    }
-    while (gone) {   // without the lock: freeing may wait for a thread of the driver's that is in make_idle
-        Block * b = gone;
-        gone = b->next;
-        cudaFree(b->p);
-        delete b;
-    }
-}
-
 int diff_attn(DeviceCtx & c, const tsn_diff_attn_args & in) {
     tsn_diff_attn_args a = in;
     if (a.type != TSN_F16 && a.type != TSN_BF16) return fail(TSN_ERR_ARG, "tsn_diff_attn: type must be TSN_F16 or TSN_BF16");
@@ -1306,9 +1030,9 @@ int diff_attn(DeviceCtx & c, const tsn_diff_attn_args & in) {
         // a trip of the sums through the workspace 30 and a half for each part; past 74 CTAs at once (of 8 KB slabs) they
         // wait for HBM. One token of 32 heads over 8, four caches of 32 768 keys: 87 us with one wave of 128 CTAs (6.2
         // TB/s), 93 to 163 with two to sixteen; 16 heads over 704 keys: 9.6 us in one part or eight, 11.3 in two.
-        const long long slabs = ((long long) a.Sk + SLAB - 1) / SLAB, room = (long long) (WORKSPACE - COUNTERS * 4) / (SOME * (4 * a.d + 4) * 4);
+        const long long slabs = ((long long) a.Sk + SLAB - 1) / SLAB, room = (long long) SPLIT_BYTES / (SOME * (4 * a.d + 4) * 4);
         double least = 0.0;
-        for (long long parts = 1; parts <= 64 && (parts == 1 || (groups <= (long long) COUNTERS && groups * parts <= room)); ++parts) {
+        for (long long parts = 1; parts <= 64 && (parts == 1 || (groups <= (long long) SPLIT_GROUPS && groups * parts <= room)); ++parts) {
             const long long chunk = std::max(1ll, (slabs + parts - 1) / parts), ctas = groups * parts;
             const double crowd = std::max(1.0, std::min<long long>(ctas, SMS) * (a.d / 64.0) / 74.0);
             const double cost = (double) ((ctas + SMS - 1) / SMS) * (30.0 + chunk * crowd) + (parts > 1 ? 30.0 + 0.5 * parts : 0.0);
@@ -1332,27 +1056,12 @@ int diff_attn(DeviceCtx & c, const tsn_diff_attn_args & in) {
     }
     if (groups * p.splits > 0x7fffffffLL) return fail(TSN_ERR_ARG, "tsn_diff_attn: too many query rows");
     const bool shared = rows && p.splits > 1;   // through the workspace
-    cudaStreamCaptureStatus capture = cudaStreamCaptureStatusNone;
-    unsigned long long stream = 0;
+    SplitUse use;
     if (shared) {
-        cudaGraph_t graph = nullptr;
-        cudaError_t e = cudaStreamGetCaptureInfo(c.stream, &capture, nullptr, &graph, nullptr, nullptr);
-        if (e == cudaSuccess && capture == cudaStreamCaptureStatusInvalidated) e = cudaErrorStreamCaptureInvalidated;
-        if (e == cudaSuccess && capture == cudaStreamCaptureStatusNone) e = cudaStreamGetId(c.stream, &stream);
-        if (e != cudaSuccess) return failed(e);
-        size_t counters = COUNTERS * 4;
-        void * ws = nullptr;
-        int rc;
-        if (capture == cudaStreamCaptureStatusNone) {
-            rc = workspace(c, stream);
-            ws = c.split_ws;
-        } else {
-            counters = ((size_t) groups * 4 + 255) & ~(size_t) 255;
-            rc = graph_workspace(c, graph, counters + (size_t) groups * p.splits * (SOME * (4 * a.d + 4) * 4), &ws);
-        }
+        const int rc = split_begin(c, "tsn_diff_attn", (size_t) groups, (size_t) groups * p.splits * (SOME * (4 * a.d + 4) * 4), use);
         if (rc) return rc;
-        p.count = (unsigned int *) ws;
-        p.part = (float *) ((char *) ws + counters);
+        p.count = use.count;
+        p.part = use.part;
     }
     CUtensorMap tk{}, tv{};
     if (a.Sk && (!make_kv_map(&tk, a, a.k, KB, rows ? SLAB : KEYS) || !make_kv_map(&tv, a, a.v, KB, rows ? SLAB : KEYS)))
@@ -1367,11 +1076,7 @@ int diff_attn(DeviceCtx & c, const tsn_diff_attn_args & in) {
         e = a.d == 32 ? (bf ? launch_tc<64, true>(tk, tv, p, grid, c.stream) : launch_tc<64, false>(tk, tv, p, grid, c.stream))
                       : (bf ? launch_tc<128, true>(tk, tv, p, grid, c.stream) : launch_tc<128, false>(tk, tv, p, grid, c.stream));
     if (e != cudaSuccess) cudaGetLastError();
-    if (e == cudaSuccess && shared && capture == cudaStreamCaptureStatusNone) {
-        e = cudaEventRecord(c.split_ev, c.stream);
-        c.split_used = true;
-        c.split_stream = stream;
-    }
+    if (e == cudaSuccess && shared) e = split_end(c, use);
     if (e != cudaSuccess) return fail(TSN_ERR_CUDA, std::string("tsn_diff_attn: ") + cudaGetErrorString(e));
     return TSN_OK;
 }

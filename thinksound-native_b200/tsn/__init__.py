@@ -82,6 +82,29 @@ class DiffAttnArgs(C.Structure):
                 + [("lam_sh", C.c_int64), ("norm_w", C.c_void_p)])
 
 
+class Paged(C.Structure):
+    """tsn_paged: a key/value cache in pages, and the batch of new tokens that a call brings."""
+    _fields_ = ([(n, C.c_uint32) for n in ("B", "N", "P", "M", "page", "Hk", "D")] + [("type", C.c_int32)]
+                + [(n, Heads) for n in ("k", "v")]
+                + [("table", C.c_void_p), ("table_sb", C.c_int64), ("len", C.c_void_p), ("q_start", C.c_void_p)])
+
+
+class CacheAppendArgs(C.Structure):
+    _fields_ = ([("c", Paged), ("Hq", C.c_uint32), ("xtype", C.c_int32), ("eps", C.c_float)]
+                + [(n, Rows) for n in ("q", "k", "v", "q_out", "means")]
+                + [("pos", C.c_void_p), ("pos_ss", C.c_int64), ("q_norm", C.c_void_p), ("k_norm", C.c_void_p)])
+
+
+class PagedAttnArgs(C.Structure):
+    _fields_ = ([("c", Paged), ("H", C.c_uint32), ("most", C.c_uint32), ("causal", C.c_int32), ("window", C.c_uint32),
+                 ("scale", C.c_float)] + [(n, Rows) for n in ("q", "out")])
+
+
+class SparseAttnArgs(C.Structure):
+    _fields_ = ([("c", Paged)] + [(n, C.c_uint32) for n in ("H", "picks", "first", "last")] + [("scale", C.c_float)]
+                + [(n, Rows) for n in ("q", "out", "means")] + [("chosen", C.c_void_p)])
+
+
 class FormTensor(C.Structure):
     _fields_ = ([(n, C.c_int32) for n in ("there", "device_type", "device", "ndim")] + [("dtype", C.c_uint32)]
                 + [(n, C.c_int64 * 4) for n in ("shape", "strides")])
@@ -89,7 +112,7 @@ class FormTensor(C.Structure):
 
 class Form(C.Structure):
     _fields_ = [("view", C.c_void_p), ("item", C.c_void_p), ("type", C.c_void_p), ("none", C.c_void_p), ("n", C.c_uint32), ("valid", C.c_uint32),
-                ("to", C.c_void_p * 7), ("t", FormTensor * 7)]
+                ("to", C.c_void_p * 11), ("t", FormTensor * 11)]
 
 
 _lib = None
@@ -192,6 +215,9 @@ _SIGS = [
                                 C.POINTER(C.c_double), C.c_int, C.POINTER(RopePlan)]),
     ("tsn_rope_axes", C.c_int, [C.c_void_p, C.POINTER(RopePlan), C.POINTER(RopeArgs)]),
     ("tsn_diff_attn", C.c_int, [C.c_void_p, C.POINTER(DiffAttnArgs)]),
+    ("tsn_cache_append", C.c_int, [C.c_void_p, C.POINTER(RopePlan), C.POINTER(CacheAppendArgs)]),
+    ("tsn_paged_attn", C.c_int, [C.c_void_p, C.POINTER(PagedAttnArgs)]),
+    ("tsn_sparse_attn", C.c_int, [C.c_void_p, C.POINTER(SparseAttnArgs)]),
     ("tsn_gguf_write_synthetic", C.c_int, [C.c_char_p, C.POINTER(Geom), C.c_uint64, C.c_int]),
     ("tsn_gguf_write_synthetic_vae", C.c_int, [C.c_char_p, C.c_uint32, C.c_uint32, C.c_uint32, C.c_uint64]),
 ]
@@ -626,4 +652,7 @@ def __getattr__(name):
     if name in ("BlockNorm", "RopeAxes", "DiffAttention"):
         from . import block_ops
         return getattr(block_ops, name)
+    if name in ("CacheAppend", "PagedAttention", "SparseAttention"):
+        from . import paged_ops
+        return getattr(paged_ops, name)
     raise AttributeError(f"module {__name__!r} has no attribute {name!r}")
