@@ -3,11 +3,12 @@
 //
 //   o = sum_j p_j v_j / sum_j p_j,  p_j = 2^(c q.k_j - ref),  ref the running maximum, in one pass over the keys.
 // A warp takes one query head: each lane holds D / 32 elements of q and o.
+#include <algorithm>
 #include <cmath>
 
-#include "attn_ops.cuh"
 #include "kernels.h"
-#include "paged.h"
+#include "paged_attn.h"
+#include "split_ws.h"
 
 namespace tsn {
 
@@ -15,19 +16,8 @@ cudaError_t configure_page_select();
 
 namespace {
 
-constexpr float LOG2E = 1.44269504088896341f;
-
-struct Args {
-    tsn_paged c;
-    uint32_t H, window, picks;
-    int causal, page_log2;
-    float scale;   // times log2(e)
-    tsn_rows q, out;
-    const int * chosen;   // null: every page
-};
-
 template <class T, int D>
-__global__ void __launch_bounds__(128) paged_attn_warp(const __grid_constant__ Args p) {
+__global__ void __launch_bounds__(128) paged_attn_warp(const __grid_constant__ PagedArgs p) {
     constexpr int E = D / 32;
     pdl_wait();
     const int lane = threadIdx.x & 31;
@@ -71,34 +61,103 @@ __global__ void __launch_bounds__(128) paged_attn_warp(const __grid_constant__ A
     for (int e = 0; e < E; ++e) out[e] = from_f32<T>(l == 0.0f ? 0.0f : o[e] / l);
 }
 
-cudaError_t launch(const Args & p, cudaStream_t s) {
+cudaError_t launch(const PagedArgs & p, cudaStream_t s) {
     const dim3 grid((unsigned) (((long long) p.c.N * p.H + 3) / 4));
     const bool bf = p.c.type == TSN_BF16;
-    cudaError_t e;
-    if (p.c.D == 64) e = bf ? launch_cl(paged_attn_warp<__nv_bfloat16, 64>, grid, dim3(128), 0, s, dim3(1), p) : launch_cl(paged_attn_warp<__half, 64>, grid, dim3(128), 0, s, dim3(1), p);
-    else e = bf ? launch_cl(paged_attn_warp<__nv_bfloat16, 128>, grid, dim3(128), 0, s, dim3(1), p) : launch_cl(paged_attn_warp<__half, 128>, grid, dim3(128), 0, s, dim3(1), p);
-    if (e != cudaSuccess) cudaGetLastError();
-    return e;
+    if (p.c.D == 64) return bf ? launch_cl(paged_attn_warp<__nv_bfloat16, 64>, grid, dim3(128), 0, s, dim3(1), p) : launch_cl(paged_attn_warp<__half, 64>, grid, dim3(128), 0, s, dim3(1), p);
+    return bf ? launch_cl(paged_attn_warp<__nv_bfloat16, 128>, grid, dim3(128), 0, s, dim3(1), p) : launch_cl(paged_attn_warp<__half, 128>, grid, dim3(128), 0, s, dim3(1), p);
+}
+
+PagedArgs args_of(const DeviceCtx & c, const tsn_paged & cache, uint32_t H, float scale) {
+    PagedArgs p{};
+    p.c = cache;
+    if (p.c.P == 0) p.c.M = 0;   // no page: no key
+    p.H = (int) H;
+    p.G = (int) (H / cache.Hk);
+    p.page_log2 = log2_of(cache.page);
+    p.scale = (scale == 0.0f ? 1.0f / std::sqrt((float) cache.D) : scale) * PAGED_LOG2E;
+    p.err = c.d_err;
+    return p;
+}
+
+// Rows of a kv head up to which groups of 8 or 16 are taken
+constexpr uint64_t FEW = 32;
+
+// The few-rows kernel with what it needs of the workspace.
+int few_rows(DeviceCtx & c, const char * name, PagedArgs & p, uint32_t most) {
+    size_t groups = 0, bytes = 0;
+    SplitUse use;
+    plan_paged_rows(p, most, &groups, &bytes);
+    if (groups) {
+        if (const int rc = split_begin(c, name, groups, bytes, use)) return rc;
+        p.count = use.count;
+        p.part = use.part;
+    }
+    cudaError_t e = launch_paged_rows(p, most, c.stream);
+    if (e == cudaSuccess && groups) e = split_end(c, use);
+    if (e == cudaSuccess) return TSN_OK;
+    cudaGetLastError();
+    return fail(TSN_ERR_CUDA, std::string(name) + ": " + cudaGetErrorString(e));
 }
 
 } // namespace
 
-cudaError_t configure_paged() { return configure_page_select(); }
+// {D, page, Hk, P} views with {64, tokens, 1, 1} boxes. A dimension of one element has a stride that is never taken: any valid one
+// stands in. Without pages nothing is loaded, but the map of some page has to be valid.
+bool make_page_maps(const tsn_paged & c, uint32_t tokens, CUtensorMap * tk, CUtensorMap * tv) {
+    const PFN_cuTensorMapEncodeTiled_v12000 enc = tensor_map_encoder();
+    if (!enc) return false;
+    if (c.P == 0) return true;
+    bool ok = true;
+    for (int i = 0; i < 2; ++i) {
+        const tsn_heads & t = i ? c.v : c.k;
+        const cuuint64_t row = c.D * 2;
+        const cuuint64_t dims[4] = {c.D, c.page, c.Hk, c.P};
+        const cuuint64_t strides[3] = {(cuuint64_t) t.ss * 2, c.Hk > 1 ? (cuuint64_t) t.sh * 2 : row, c.P > 1 ? (cuuint64_t) t.sb * 2 : row};
+        const cuuint32_t box[4] = {64, tokens, 1, 1}, es[4] = {1, 1, 1, 1};
+        ok = ok && enc(i ? tv : tk, c.type == TSN_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4, t.p, dims, strides, box, es,
+                       CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                       CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+    }
+    return ok;
+}
+
+cudaError_t configure_paged() {
+    cudaError_t e = configure_page_select();
+    if (e == cudaSuccess) e = configure_paged_rows();
+    return e;
+}
 
 int paged_attn(DeviceCtx & c, const tsn_paged_attn_args & a) {
     if (a.c.N == 0 || a.c.B == 0) return TSN_OK;
-    Args p{a.c, a.H, a.window, 0, a.causal, log2_of(a.c.page), (a.scale == 0.0f ? 1.0f / std::sqrt((float) a.c.D) : a.scale) * LOG2E, a.q, a.out, nullptr};
+    PagedArgs p = args_of(c, a.c, a.H, a.scale);
+    p.q = a.q;
+    p.out = a.out;
+    p.causal = a.causal != 0;
+    p.window = (int) a.window;
+    const uint32_t most = !a.c.q_start ? 1 : a.most ? std::min(a.most, a.c.N) : a.c.N;
+    if ((uint64_t) most * p.G <= FEW) return few_rows(c, "tsn_paged_attn", p, most);
     const cudaError_t e = launch(p, c.stream);
-    return e == cudaSuccess ? TSN_OK : fail(TSN_ERR_CUDA, std::string("tsn_paged_attn: ") + cudaGetErrorString(e));
+    if (e == cudaSuccess) return TSN_OK;
+    cudaGetLastError();
+    return fail(TSN_ERR_CUDA, std::string("tsn_paged_attn: ") + cudaGetErrorString(e));
 }
 
 int sparse_attn(DeviceCtx & c, const tsn_sparse_attn_args & a) {
     if (a.c.N == 0 || a.c.B == 0) return TSN_OK;
-    cudaError_t e = launch_page_select(a, c.stream);
-    Args p{a.c, a.H, 0, a.picks, 1, log2_of(a.c.page), (a.scale == 0.0f ? 1.0f / std::sqrt((float) a.c.D) : a.scale) * LOG2E, a.q, a.out, a.chosen};
-    if (e == cudaSuccess) e = launch(p, c.stream);
-    else cudaGetLastError();
-    return e == cudaSuccess ? TSN_OK : fail(TSN_ERR_CUDA, std::string("tsn_sparse_attn: ") + cudaGetErrorString(e));
+    PagedArgs p = args_of(c, a.c, a.H, a.scale);
+    p.q = a.q;
+    p.out = a.out;
+    p.causal = 1;
+    p.picks = (int) a.picks;
+    p.chosen = a.chosen;
+    if ((uint64_t) a.c.N * a.c.Hk * ((p.G + 7) / 8) > 0x7fffffffu) return fail(TSN_ERR_ARG, "tsn_sparse_attn: too many query rows");
+    const cudaError_t e = launch_page_select(a, c.stream);
+    if (e != cudaSuccess) {
+        cudaGetLastError();
+        return fail(TSN_ERR_CUDA, std::string("tsn_sparse_attn: ") + cudaGetErrorString(e));
+    }
+    return few_rows(c, "tsn_sparse_attn", p, 1);
 }
 
 } // namespace tsn
