@@ -63,4 +63,8 @@ cudaError_t configure_paged_rows();
 void plan_paged_rows(PagedArgs & p, uint32_t most, size_t * groups, size_t * bytes);
 cudaError_t launch_paged_rows(const PagedArgs & p, uint32_t most, cudaStream_t s);
 
+cudaError_t configure_paged_tiles();
+// 256 query rows of a kv head at a time
+cudaError_t launch_paged_tiles(PagedArgs p, cudaStream_t s);
+
 } // namespace tsn

@@ -1,0 +1,520 @@
+// paged_tiles.cu — attention over the paged cache for many query rows of a kv head, on the tcgen05 tensor cores.
+//
+//   o = sum_j p_j v_j / l,  l = sum_j p_j,  p_j = 2^(c q.k_j - ref)
+// in one pass over the keys; ref follows the row's running maximum and moves, with o and l rescaled, when that has grown by more than
+// 2^8. P is rounded to 16 bits, as the tensor cores take it, and l is the sum of the rounded ones, so that rounding cancels for a key
+// that dominates; scores, maxima, sums and o are f32.
+// A unit is 256 query rows of a sequence and kv head, (token, head of the group), as two tiles of 128, so that heads of a group share
+// the keys; a CTA takes a unit or, where there are few, a part of its keys, the parts of a cluster adding up their sums. 384 threads:
+//   warps 0-3, 4-7  softmax of a tile, one row a thread: S from TMEM, mask, maximum, exponentials, P over S's columns
+//   warp 8          TMA: 128 keys, then their values, through one ring of stages; a tile may lie in several pages, a lane a box
+//   warps 9, 10     issue a tile's products: P_j V, then Q K_j+1 (so that S_j+1 being there means that O holds tile j)
+//   warp 11         where some keys are not seen by all rows: makes the tiles' V rows fit for the product
+// While one tile's products run, the other's exponentials do. TMEM: S of both tiles (2 x 128 columns) and O (2 x D).
+// Values behind keys that are not there may be NaN, and 0 * NaN is NaN: those rows of V are cleared. Where rows differ in what they
+// see, values that are not finite are cleared too and added again to the rows that do see them.
+// Every wait is bounded; barriers of a whole block or cluster are on paths that all threads take.
+#include "kernels.h"
+#include "paged_attn.h"
+
+#include <algorithm>
+#include <atomic>
+
+namespace tsn {
+
+namespace {
+
+constexpr int ROWS = 256, KEYS = 128, THREADS = 384;
+constexpr float LAZY = 8.0f;   // log2 units that a maximum may grow before o is rescaled
+
+template <int D>
+struct Lay {
+    static constexpr int ATOMS = D / 64, BOX = KEYS * 128, TILE = KEYS * D * 2;   // boxes of 128 rows x 64 elements
+    static constexpr int STAGES = D == 128 ? 5 : 10, DEEP = 16;                   // DEEP: above the tiles on their way
+    static constexpr int OFF_RING = 2 * TILE, OFF_BAR = OFF_RING + STAGES * TILE, TOTAL = OFF_BAR + 640;   // Q's two tiles first
+    static constexpr int SUM_ROW = D + 4;
+    static constexpr uint32_t TM_O = 2 * KEYS, TM = 512;
+    static_assert(TOTAL + 64 <= 227 * 1024, "one CTA's shared memory");
+    static_assert(ROWS * SUM_ROW * 4 <= STAGES * TILE, "the rows' sums fit in the ring");
+    static_assert(TM_O + 2 * D <= TM, "tensor memory");
+    static_assert((8 + 3 * STAGES) * 8 + (2 + DEEP + 4 * STAGES) * 4 <= 640, "barriers");
+};
+
+__device__ __forceinline__ void bar_n(int id, int n) { asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(n) : "memory"); }
+
+template <int D, bool BF16>
+__global__ void __launch_bounds__(THREADS, 1)
+paged_tiles_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant__ CUtensorMap tv, const __grid_constant__ PagedArgs p) {
+    using L = Lay<D>;
+    constexpr int CH = D / 8, STAGES = L::STAGES;   // CH: 16-byte pieces of a head
+    extern __shared__ __align__(1024) uint8_t smem[];
+    __shared__ int unit_of[4];   // sequence, its first row, its new tokens, unit in it
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const bool fits = (smem_u32(smem) & 1023) == 0;   // the swizzled tiles need 1024-byte alignment
+    if (!fits && tid == 0 && p.err) atomicCAS(p.err, 0, DEV_BAD_ARGS);
+    uint64_t * bar = (uint64_t *) (smem + L::OFF_BAR);
+    // v_ready is a tile's, of the last STAGES: a stage holds keys one time and values another
+    uint64_t * q_full = bar, * s_full = bar + 2, * p_full = bar + 4, * o_full = bar + 6, * full = bar + 8, * empty = full + STAGES, * v_ready = empty + STAGES;
+    uint32_t * words = (uint32_t *) (v_ready + STAGES);   // TMEM address, abort flag, slabs with pages [DEEP tiles], keys of a tile that are not finite [STAGES tiles][4]
+    volatile int * abort_flag = (volatile int *) (words + 1);
+    volatile uint32_t * paged = words + 2, * not_finite = paged + L::DEEP;
+
+    if (tid == 0) {
+        for (int t = 0; t < 2; ++t) { mbar_init(&q_full[t], 4); mbar_init(&s_full[t], 1); mbar_init(&p_full[t], 4); mbar_init(&o_full[t], 1); }
+        for (int s = 0; s < STAGES; ++s) { mbar_init(&full[s], 1); mbar_init(&empty[s], 2); mbar_init(&v_ready[s], 1); }
+        *abort_flag = 0;
+        fence_mbar_init();
+    }
+    if (warp == 8 && lane == 0 && p.c.P) { tma_prefetch(&tk); tma_prefetch(&tv); }
+    pdl_wait();   // from here on memory that earlier work may have written or may still read
+    // Tensor memory after the wait and before the trigger: of two kernels on one SM, neither can hold what the other waits for.
+    if (warp == 9) tmem_alloc(words, L::TM);
+
+    // this CTA's unit: units of a sequence are (group of rows, kv head), the last rows, which see most, first
+    const unsigned split = blockIdx.x % p.parts;
+    if (warp == 0) {
+        const long long gid = blockIdx.x / p.parts;
+        long long before = 0;
+        if (lane == 0) unit_of[0] = -1;
+        __syncwarp();
+        for (int b0 = 0; b0 < (int) p.c.B && before <= gid; b0 += 32) {
+            const int b = b0 + lane;
+            int start = 0, n = 0;
+            if (b < (int) p.c.B) {
+                start = seq_start(p.c, b);
+                n = max(0, seq_start(p.c, b + 1) - start);
+            }
+            const long long mine = ((long long) n * p.G + ROWS - 1) / ROWS * p.c.Hk;
+            long long upto = mine;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const long long v = __shfl_up_sync(~0u, upto, o);
+                if (lane >= o) upto += v;
+            }
+            const long long at = before + upto - mine;
+            if (at <= gid && gid < at + mine) {
+                unit_of[0] = b;
+                unit_of[1] = start;
+                unit_of[2] = n;
+                unit_of[3] = (int) (gid - at);
+            }
+            before += __shfl_sync(~0u, upto, 31);
+        }
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = __shfl_sync(~0u, words[0], 0), TM_O = tmem + L::TM_O;
+    const int b = unit_of[0];
+    if (b < 0) {   // more CTAs than units, the whole cluster of them
+        __syncthreads();
+        if (warp == 9) tmem_dealloc(tmem, L::TM);
+        return;
+    }
+    const int row0 = unit_of[1], fresh = unit_of[2], hk = unit_of[3] % (int) p.c.Hk;
+    const int all_rows = fresh * p.G;   // at most 2^30
+    const int r0 = ((all_rows + ROWS - 1) / ROWS - 1 - unit_of[3] / (int) p.c.Hk) * ROWS, R = min(ROWS, all_rows - r0);
+    const int len = p.c.len[b], n = cached(p, len), place0 = first_place(len, fresh);
+    // row t: token (r0 + t) / G, head (r0 + t) % G; keys lo .. hi - 1
+    auto place_of = [&](int t) { return place0 + (r0 + t) / p.G; };
+    auto hi_of = [&](int t) { return seen_to(p, place_of(t), n); };
+    auto lo_of = [&](int t) { return min(seen_from(p, place_of(t)), n); };
+    // tiles of keys that some row sees, this part of them
+    const int tile0 = lo_of(0) / KEYS, all_tiles = max(0, (hi_of(R - 1) + KEYS - 1) / KEYS - tile0);
+    const int per = (all_tiles + p.parts - 1) / p.parts;
+    const int t0 = tile0 + min(all_tiles, (int) split * per), nt = fits ? tile0 + min(all_tiles, ((int) split + 1) * per) - t0 : 0;
+    const int least = hi_of(0), latest = lo_of(R - 1);   // before least and from latest on every row sees
+    auto mixed = [&](int base) { return least < min(n, base + KEYS) || base < latest; };   // rows see different keys of the tile
+    const bool mend = nt > 0 && ((t0 + nt) * KEYS > n || mixed(t0 * KEYS) || mixed((t0 + nt - 1) * KEYS));
+    // the part's tiles that tile t of the rows sees: ja .. jb - 1
+    auto from_of = [&](int t) { return 128 * t < R ? min(nt, max(0, lo_of(128 * t) / KEYS - t0)) : 0; };
+    auto until_of = [&](int t) { return 128 * t < R ? max(from_of(t), min(nt, (hi_of(min(R, 128 * t + 128) - 1) + KEYS - 1) / KEYS - t0)) : 0; };
+
+    if (warp >= 8) {
+        if (warp == 8) {
+            // Pages of a tile: a lane each of its boxes' rows, read one tile ahead
+            const int box = min(KEYS, 1 << p.page_log2), pieces = KEYS / box;
+            const int piece = lane % pieces, atom = lane / pieces;
+            auto page_at = [&](int j) {
+                const int key = (t0 + j) * KEYS + piece * box;
+                return key < n ? page_of(p.c, b, key >> p.page_log2) : (int) p.c.P;   // what is behind the end counts as there, but is not loaded
+            };
+            int next = nt > 0 ? page_at(0) : 0;
+            bool go = true;
+            for (int j = 0; j < nt && go; ++j) {
+                const int id = next;
+                if (j + 1 < nt) next = page_at(j + 1);
+                const uint32_t gone = __ballot_sync(~0u, lane < pieces && id < 0);
+                uint32_t slabs = 0xffu;
+                if (gone)
+                    for (int x = 0; x < pieces; ++x)
+                        if ((gone >> x) & 1u) slabs &= ~(((1u << (box / 16)) - 1u) << (x * (box / 16)));
+                const int slot = ((t0 + j) * KEYS + piece * box) & ((1 << p.page_log2) - 1), page = id < 0 ? (int) p.c.P : id;   // past the last page: zeros
+#pragma unroll
+                for (int kv = 0; kv < 2; ++kv) {
+                    const int i = 2 * j + kv, s = i % STAGES;
+                    if (i >= STAGES && !mbar_wait_soon(&empty[s], (i / STAGES - 1) & 1, abort_flag, p.err, DEV_TIMEOUT_EMPTY)) go = false;
+                    go = __all_sync(~0u, go);
+                    if (!go) break;
+                    if (lane == 0) {
+                        if (kv == 0) paged[j % L::DEEP] = slabs;
+                        mbar_expect_tx(&full[s], L::TILE);
+                    }
+                    __syncwarp();
+                    if (atom < L::ATOMS)
+                        tma_load_4d(smem + L::OFF_RING + s * L::TILE + atom * L::BOX + piece * box * 128, kv ? &tv : &tk, &full[s], 64 * atom, slot, hk, page);
+                }
+            }
+        } else if (warp == 11) {
+            for (int j = 0; j < nt && mend; ++j) {
+                const int base = (t0 + j) * KEYS, i = 2 * j + 1, s = i % STAGES;
+                if (!mbar_wait_soon(&full[s], (i / STAGES) & 1, abort_flag, p.err, DEV_TIMEOUT_FULL)) break;
+                __syncwarp();
+                uint8_t * v = smem + L::OFF_RING + s * L::TILE;
+                const bool mix = mixed(base);
+                // rows of keys that are not there, a lane a key
+                for (int key = max(0, n - base) + lane; key < KEYS; key += 32)
+#pragma unroll
+                    for (int y = 0; y < CH; ++y) *(uint4 *) (v + key * 128 + (y >> 3) * L::BOX + (y & 7) * 16) = make_uint4(0, 0, 0, 0);
+                __syncwarp();
+                uint32_t bad[4] = {0, 0, 0, 0};
+                if (mix) {
+                    constexpr int AT_ONCE = 32 / CH;   // rows of one step
+                    const int sub = lane / CH, ch = lane % CH;
+#pragma unroll
+                    for (int w = 0; w < 4; ++w) {
+#pragma unroll 4
+                        for (int y = 0; y < 32; y += AT_ONCE) {
+                            const int key = 32 * w + y + sub;
+                            uint4 * at = (uint4 *) (v + (ch >> 3) * L::BOX + key * 128 + (ch & 7) * 16);   // whichever piece lies there
+                            const uint4 o = *at;
+                            const uint4 f = make_uint4(finite_only<BF16>(o.x), finite_only<BF16>(o.y), finite_only<BF16>(o.z), finite_only<BF16>(o.w));
+                            if (o.x != f.x || o.y != f.y || o.z != f.z || o.w != f.w) {
+                                *at = f;
+                                bad[w] |= 1u << (key & 31);
+                            }
+                        }
+                        bad[w] = __reduce_or_sync(~0u, bad[w]);
+                    }
+                }
+                fence_proxy_async_smem();
+                __syncwarp();
+                if (lane == 0) {
+                    for (int w = 0; w < 4; ++w) not_finite[4 * (j % STAGES) + w] = bad[w];
+                    mbar_arrive(&v_ready[j % STAGES]);
+                }
+            }
+        } else {
+            const int t = warp - 9, ja = from_of(t), jb = until_of(t);
+            const uint32_t lead = elect_lane(), id_s = umma_idesc_f16(KEYS, BF16), id_pv = umma_idesc_f16(D, BF16, 1);
+            const uint64_t qd = umma_desc_sw128(smem + t * L::TILE), kd = umma_desc_sw128(smem + L::OFF_RING), vd = umma_desc_sw128_mn(smem + L::OFF_RING, L::BOX);
+            const uint32_t ts = tmem + KEYS * t, to = TM_O + D * t;
+            auto landed = [&](int i) { return mbar_wait_soon(&full[i % STAGES], (i / STAGES) & 1, abort_flag, p.err, DEV_TIMEOUT_FULL); };
+            auto fit = [&](int j) { return mbar_wait_soon(&v_ready[j % STAGES], (j / STAGES) & 1, abort_flag, p.err, DEV_TIMEOUT_FULL); };
+            auto pass = [&](int i) {   // a stage that this tile does not use
+                if (!landed(i)) return false;
+                if (mend && (i & 1) && !fit(i / 2)) return false;
+                if (lead) mbar_arrive(&empty[i % STAGES]);
+                return true;
+            };
+            auto qk = [&](int j) {
+                const int i = 2 * j, s = i % STAGES;
+                if (!landed(i)) return false;
+                const uint64_t k = kd + (uint64_t) (s * (L::TILE >> 4));
+#pragma unroll
+                for (int kk = 0; kk < D / 16; ++kk)
+                    umma_f16_if(lead, ts, qd + (kk / 4) * (L::BOX >> 4) + 2 * (kk % 4), k + (kk / 4) * (L::BOX >> 4) + 2 * (kk % 4), id_s, kk != 0);
+                umma_commit_if(lead, &s_full[t]);
+                umma_commit_if(lead, &empty[s]);
+                return true;
+            };
+            bool go = true;
+            for (int i = 0; i < 2 * ja && go; ++i) go = pass(i);
+            if (go && ja < jb) go = mbar_wait_soon(&q_full[t], 0, abort_flag, p.err, DEV_TIMEOUT_FULL) && qk(ja);
+            for (int j = ja; j < jb && go; ++j) {
+                const int i = 2 * j + 1, s = i % STAGES;
+                if (!mbar_wait_soon(&p_full[t], (j - ja) & 1, abort_flag, p.err, DEV_TIMEOUT_TMEM)) break;
+                if (!landed(i)) break;
+                if (mend && !fit(j)) break;
+                tc_fence_after();
+                const uint64_t v = vd + (uint64_t) (s * (L::TILE >> 4));
+#pragma unroll
+                for (int kk = 0; kk < KEYS / 16; ++kk) umma_f16_ts_if(lead, to, ts + 8 * kk, v + 128 * kk, id_pv, j > ja || kk > 0);
+                umma_commit_if(lead, &empty[s]);
+                if (j + 1 < jb) go = qk(j + 1);
+                else umma_commit_if(lead, &o_full[t]);
+            }
+            for (int i = 2 * jb; i < 2 * nt && go; ++i) go = pass(i);
+        }
+        __syncwarp();
+        pdl_trigger();
+        if (p.parts > 1) {
+            cluster_sync_all();
+            cluster_sync_all();
+        }
+    } else {
+        const int t = warp >> 2, row = tid & 127, ja = from_of(t), jb = until_of(t), mine = 128 * t + row;   // row of the unit
+        const uint32_t lane0 = (uint32_t) ((warp & 3) * 32) << 16, ts = tmem + KEYS * t + lane0, to = TM_O + D * t + lane0;
+        const bool there = mine < R;
+        auto address = [&](const tsn_rows & x, int r) {   // of row r of the unit
+            const int u = r0 + r;
+            return (uint16_t *) x.p + (long long) (row0 + u / p.G) * x.sb + (long long) (hk * p.G + u % p.G) * x.st;
+        };
+        uint8_t * qs = smem + t * L::TILE;
+        if (ja < jb) {   // Q into its swizzled boxes, rows past the last one as zeros
+            constexpr int AT_ONCE = 8;
+#pragma unroll
+            for (int y0 = 0; y0 < CH; y0 += AT_ONCE) {
+                uint4 q[AT_ONCE];
+#pragma unroll
+                for (int y = 0; y < AT_ONCE; ++y) {
+                    const int r = (row + 128 * (y0 + y)) / CH, ch = row % CH;
+                    q[y] = make_uint4(0, 0, 0, 0);
+                    if (128 * t + r < R) q[y] = *(const uint4 *) (address(p.q, 128 * t + r) + ch * 8);
+                }
+#pragma unroll
+                for (int y = 0; y < AT_ONCE; ++y) {
+                    const int r = (row + 128 * (y0 + y)) / CH, ch = row % CH;
+                    *(uint4 *) (qs + (ch >> 3) * L::BOX + r * 128 + (((ch & 7) ^ (r & 7)) << 4)) = q[y];
+                }
+            }
+            fence_proxy_async_smem();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&q_full[t]);
+        }
+        const int hi = there ? hi_of(mine) : n, lo = there ? lo_of(mine) : 0;
+        const int rows_end = min(R, 128 * t + 128);
+        const int sure_hi = ja < jb ? hi_of(128 * t) : 0, sure_lo = ja < jb ? lo_of(rows_end - 1) : 0;   // every row of the tile sees keys sure_lo .. sure_hi - 1
+        float l = 0.0f, ref = -INFINITY;
+        bool ok = true, poison = false;
+        // Tile j. Exponentials run against the reference of the tiles before while the maximum is found; the few tiles whose maximum is
+        // too far above it are done again. P waits in registers for that, and S stays where it is.
+        auto tile = [&](auto masked, int j) {
+            constexpr bool MASKED = decltype(masked)::value;
+            const int base = (t0 + j) * KEYS;
+            uint32_t vis[4] = {~0u, ~0u, ~0u, ~0u};
+            if (MASKED) {
+                const uint32_t slabs = paged[j % L::DEEP];
+#pragma unroll
+                for (int w = 0; w < 4; ++w)
+                    vis[w] = low_bits(hi - base - 32 * w) & ~low_bits(lo - base - 32 * w) & ((slabs >> (2 * w) & 1u ? 0xffffu : 0u) | (slabs >> (2 * w) & 2u ? 0xffff0000u : 0u));
+            }
+            uint32_t pk[64], s[2][32];
+            float sum[4], top = -INFINITY;
+            auto pass = [&](bool find) {
+                sum[0] = sum[1] = sum[2] = sum[3] = 0.0f;
+                tmem_request32(ts, s[0]);
+#pragma unroll
+                for (int w = 0; w < 4; ++w) {
+                    tmem_landed32(s[w & 1]);
+                    if (w < 3) tmem_request32(ts + 32 * (w + 1), s[(w + 1) & 1]);
+                    if (MASKED) hide(s[w & 1], vis[w]);
+                    exponentials<BF16, MASKED>(s[w & 1], pk + 16 * w, p.scale, ref, sum);
+                    if (find) top = fmaxf(top, greatest(s[w & 1]));
+                }
+            };
+            pass(true);
+            top *= p.scale;
+            const bool move = top > ref + LAZY;
+            if (__any_sync(~0u, move)) {
+                // a row moves its reference by itself, so its result does not depend on its neighbours
+                const float f = move ? ex2(ref - top) : 1.0f;
+                if (move) { ref = top; l *= f; }
+                if (j > ja) {   // O holds the tiles before: their products were issued before these scores'
+#pragma unroll 1
+                    for (int y = 0; y < D; y += 16) {
+                        float o[16];
+                        tmem_ld16(to + y, o);
+#pragma unroll
+                        for (int e = 0; e < 16; ++e) o[e] *= f;
+                        tmem_st16(to + y, (const uint32_t *) o);
+                    }
+                }
+                pass(false);
+            }
+#pragma unroll
+            for (int w = 0; w < 4; ++w) tmem_st16(ts + 16 * w, pk + 16 * w);
+            l += (sum[0] + sum[2]) + (sum[1] + sum[3]);
+            if (mend && mixed(base)) {
+                if (!mbar_wait_soon(&v_ready[j % STAGES], (j / STAGES) & 1, abort_flag, p.err, DEV_TIMEOUT_FULL)) ok = false;
+#pragma unroll
+                for (int w = 0; w < 4; ++w) poison |= (not_finite[4 * (j % STAGES) + w] & vis[w]) != 0;
+            }
+            tmem_st_wait();
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&p_full[t]);
+        };
+        for (int j = ja; j < jb && ok; ++j) {
+            if (!mbar_wait_soon(&s_full[t], (j - ja) & 1, abort_flag, p.err, DEV_TIMEOUT_TMEM)) { ok = false; break; }
+            __syncwarp();
+            tc_fence_after();
+            const int base = (t0 + j) * KEYS;
+            if (base >= sure_lo && base + KEYS <= sure_hi && paged[j % L::DEEP] == 0xffu) tile(std::false_type(), j);
+            else tile(std::true_type(), j);
+        }
+        // no score above -inf: the FMA pipe's exponentials gave its keys 2^-126 each
+        if (ref == -INFINITY && l < INFINITY) l = 0.0f;
+        if (ok && ja < jb) ok = mbar_wait_soon(&o_full[t], 0, abort_flag, p.err, DEV_TIMEOUT_TMEM);
+        __syncwarp();
+        tc_fence_after();
+        pdl_trigger();
+        // ------------------------------------------------------------ results
+        auto piece = [&](int x, float * o) {   // 32 columns of O
+            if (ja < jb) {
+                tmem_ld32(to + x, o);
+            } else {
+#pragma unroll
+                for (int e = 0; e < 32; ++e) o[e] = 0.0f;
+            }
+            if (poison && there)
+                for (int j = ja; j < jb; ++j)
+                    if (mixed((t0 + j) * KEYS))
+                        add_not_finite<BF16, 32>(p, b, hk, max(lo, (t0 + j) * KEYS), min(hi, (t0 + j + 1) * KEYS), x, o);
+        };
+        if (p.parts > 1) {
+            bar_n(3, 256);   // both tiles are done with the ring
+            float * sums = (float *) (smem + L::OFF_RING);
+            {
+                float * dst = sums + mine * L::SUM_ROW;
+#pragma unroll 1
+                for (int x = 0; x < D; x += 32) {
+                    float o[32];
+                    piece(x, o);
+#pragma unroll
+                    for (int e = 0; e < 32; e += 4) *(float4 *) (dst + x + e) = make_float4(o[e], o[e + 1], o[e + 2], o[e + 3]);
+                }
+                dst[D] = ref;
+                dst[D + 1] = l;
+            }
+            cluster_sync_all();
+            // this CTA's share of the rows, a warp a row, D / 32 columns a lane
+            constexpr int E = D / 32;
+            const int share = (R + p.parts - 1) / p.parts, from = (int) split * share, until = min(R, from + share);
+            for (int r = from + warp; r < until && !*abort_flag; r += 8) {
+                const uint32_t at = smem_u32(sums + r * L::SUM_ROW);
+                float f[8], top = -INFINITY, sum = 0.0f, o[E] = {}, v[8][4];
+                float4 st[8];
+#pragma unroll
+                for (int i = 0; i < 8; ++i)
+                    if (i < p.parts) {
+                        st[i] = dsmem_ld4(dsmem_map(at + D * 4, (uint32_t) i));
+                        const float4 x = dsmem_ld4(dsmem_map(at + (E * lane / 4) * 16, (uint32_t) i));
+                        if (E == 4) { v[i][0] = x.x; v[i][1] = x.y; v[i][2] = x.z; v[i][3] = x.w; }
+                        else { v[i][0] = lane & 1 ? x.z : x.x; v[i][1] = lane & 1 ? x.w : x.y; }
+                        top = fmaxf(top, st[i].x);
+                    }
+                const float low = top == -INFINITY ? 0.0f : top;
+#pragma unroll
+                for (int i = 0; i < 8; ++i)
+                    if (i < p.parts) {
+                        f[i] = ex2(st[i].x - low);
+                        sum += f[i] * st[i].y;
+#pragma unroll
+                        for (int e = 0; e < E; ++e) o[e] = fmaf(f[i], v[i][e], o[e]);
+                    }
+                const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+                uint16_t * out = address(p.out, r) + E * lane;
+                if constexpr (E == 4) *(uint2 *) out = sum == 0.0f ? make_uint2(0, 0) : make_uint2(pack16<BF16>(o[0] * inv, o[1] * inv), pack16<BF16>(o[2] * inv, o[3] * inv));
+                else *(uint32_t *) out = sum == 0.0f ? 0u : pack16<BF16>(o[0] * inv, o[1] * inv);
+            }
+            cluster_sync_all();   // nobody leaves while its sums are read
+        } else {
+            // through Q's place, so that whole rows are written
+            const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+#pragma unroll 1
+            for (int x = 0; x < D; x += 32) {
+                float o[32];
+                piece(x, o);
+#pragma unroll
+                for (int e = 0; e < 32; e += 8) {
+                    uint32_t w[4];
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) w[k] = l == 0.0f ? 0u : pack16<BF16>(o[e + 2 * k] * inv, o[e + 2 * k + 1] * inv);
+                    const int ch = (x + e) / 8;
+                    *(uint4 *) (qs + row * (D * 2) + ((ch ^ (row & 7)) << 4)) = make_uint4(w[0], w[1], w[2], w[3]);
+                }
+            }
+            bar_n(1 + t, 128);
+            if (!*abort_flag && fits)
+                for (int i = row; i < (rows_end - 128 * t) * CH; i += 128) {
+                    const int r = i / CH, ch = i % CH;
+                    *(uint4 *) (address(p.out, 128 * t + r) + ch * 8) = *(const uint4 *) (qs + r * (D * 2) + ((ch ^ (r & 7)) << 4));
+                }
+        }
+    }
+    tc_fence_before();
+    __syncthreads();
+    if (warp == 9) {
+        tc_fence_after();
+        tmem_dealloc(tmem, L::TM);
+    }
+    if (*abort_flag && tid == 0) {
+        // let copies that were issued but never consumed land before the CTA's shared memory is reused
+        const uint64_t t1 = global_ns();
+        while (global_ns() - t1 < 20000ull) {}
+    }
+}
+
+// clusters of 1 to 8 CTAs that run at once (one CTA per SM; a cluster lies within a GPC)
+std::atomic<int> g_clusters[9];
+
+template <int D, bool BF16>
+cudaError_t launch(const PagedArgs & p, unsigned grid, cudaStream_t s) {
+    CUtensorMap tk{}, tv{};
+    if (!make_page_maps(p.c, (uint32_t) std::min(KEYS, 1 << p.page_log2), &tk, &tv)) return cudaErrorInvalidValue;
+    return launch_cl(paged_tiles_kernel<D, BF16>, dim3(grid), dim3(THREADS), Lay<D>::TOTAL, s, dim3((unsigned) p.parts), tk, tv, p);
+}
+
+} // namespace
+
+cudaError_t configure_paged_tiles() {
+    cudaError_t e = cudaSuccess;
+    auto set = [&](auto * k, int bytes) {
+        if (e == cudaSuccess) e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+    };
+    set(paged_tiles_kernel<64, false>, Lay<64>::TOTAL);
+    set(paged_tiles_kernel<64, true>, Lay<64>::TOTAL);
+    set(paged_tiles_kernel<128, false>, Lay<128>::TOTAL);
+    set(paged_tiles_kernel<128, true>, Lay<128>::TOTAL);
+    g_clusters[1] = SMS;
+    for (unsigned n = 2; n <= 8 && e == cudaSuccess; ++n) {
+        cudaLaunchAttribute at{};
+        at.id = cudaLaunchAttributeClusterDimension;
+        at.val.clusterDim = {n, 1, 1};
+        cudaLaunchConfig_t cfg{};
+        cfg.gridDim = dim3(n * SMS);
+        cfg.blockDim = dim3(THREADS);
+        cfg.dynamicSmemBytes = Lay<128>::TOTAL;
+        cfg.attrs = &at;
+        cfg.numAttrs = 1;
+        int count = 0;
+        e = cudaOccupancyMaxActiveClusters(&count, paged_tiles_kernel<128, true>, &cfg);
+        g_clusters[n] = count;
+    }
+    return e;
+}
+
+cudaError_t launch_paged_tiles(PagedArgs p, cudaStream_t s) {
+    // units at most: a sequence has a last one that is not full
+    const long long rows = (long long) p.c.N * p.G, units = std::min<long long>(p.c.N, rows / ROWS + p.c.B) * p.c.Hk;
+    // As many parts of a cluster as take the least time, in microseconds: start and end of a CTA 7, a tile 1.2, adding up the parts
+    // 3; clusters of one size run g_clusters[size] at a time. Four key tiles a part at least, eight parts at most (the largest portable
+    // cluster). The keys are what the tables have room for: lengths are on the device.
+    long long keys = (long long) p.c.M << p.page_log2;
+    if (p.window) keys = std::min<long long>(keys, (long long) p.window + ROWS);
+    const long long tiles = (keys + KEYS - 1) / KEYS;
+    double least = 0.0;
+    for (int parts = 1; parts <= 8 && (parts == 1 || parts * 4 <= tiles); ++parts) {
+        const long long room = std::max(1, g_clusters[parts].load(std::memory_order_relaxed));
+        const double cost = (double) ((units + room - 1) / room) * (7.0 + (double) ((tiles + parts - 1) / parts) * 1.2) + (parts > 1 ? 3.0 : 0.0);
+        if (parts == 1 || cost < least) { least = cost; p.parts = parts; }
+    }
+    if (units * p.parts > 0x7fffffffLL) return cudaErrorInvalidValue;
+    const unsigned grid = (unsigned) (units * p.parts);
+    const bool bf = p.c.type == TSN_BF16;
+    if (p.c.D == 64) return bf ? launch<64, true>(p, grid, s) : launch<64, false>(p, grid, s);
+    return bf ? launch<128, true>(p, grid, s) : launch<128, false>(p, grid, s);
+}
+
+} // namespace tsn
