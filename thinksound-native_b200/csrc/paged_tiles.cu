@@ -8,7 +8,7 @@
 // the keys; a CTA takes a unit or, where there are few, a part of its keys, the parts of a cluster adding up their sums. 384 threads:
 //   warps 0-3, 4-7  softmax of a tile, one row a thread: S from TMEM, mask, maximum, exponentials, P over S's columns
 //   warp 8          TMA: 128 keys, then their values, through one ring of stages; a tile may lie in several pages, a lane a box
-//   warps 9, 10     issue a tile's products: P_j V, then Q K_j+1 (so that S_j+1 being there means that O holds tile j)
+//   warp 9          issues a tile's products: P_j V, then Q K_j+1 (so that S_j+1 being there means that O holds tile j)
 //   warp 11         where some keys are not seen by all rows: makes the tiles' V rows fit for the product
 // While one tile's products run, the other's exponentials do. TMEM: S of both tiles (2 x 128 columns) and O (2 x D).
 // Values behind keys that are not there may be NaN, and 0 * NaN is NaN: those rows of V are cleared. Where rows differ in what they
@@ -33,6 +33,7 @@ struct Lay {
     static constexpr int STAGES = D == 128 ? 5 : 10, DEEP = 16;                   // DEEP: above the tiles on their way
     static constexpr int OFF_RING = 2 * TILE, OFF_BAR = OFF_RING + STAGES * TILE, TOTAL = OFF_BAR + 640;   // Q's two tiles first
     static constexpr int SUM_ROW = D + 4;
+    static constexpr int EVERY = D == 128 ? 8 : 4;   // one pair of exponentials of so many takes the FMA pipe
     static constexpr uint32_t TM_O = 2 * KEYS, TM = 512;
     static_assert(TOTAL + 64 <= 227 * 1024, "one CTA's shared memory");
     static_assert(ROWS * SUM_ROW * 4 <= STAGES * TILE, "the rows' sums fit in the ring");
@@ -49,7 +50,9 @@ paged_tiles_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant
     constexpr int CH = D / 8, STAGES = L::STAGES;   // CH: 16-byte pieces of a head
     extern __shared__ __align__(1024) uint8_t smem[];
     __shared__ int unit_of[4];   // sequence, its first row, its new tokens, unit in it
-    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    // the warp's number as the compiler knows it to be one for all lanes: products issued under a branch that it takes for divergent
+    // cost 100 cycles and more each
+    const int tid = threadIdx.x, warp = __shfl_sync(~0u, tid >> 5, 0), lane = tid & 31;
     const bool fits = (smem_u32(smem) & 1023) == 0;   // the swizzled tiles need 1024-byte alignment
     if (!fits && tid == 0 && p.err) atomicCAS(p.err, 0, DEV_BAD_ARGS);
     uint64_t * bar = (uint64_t *) (smem + L::OFF_BAR);
@@ -61,7 +64,7 @@ paged_tiles_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant
 
     if (tid == 0) {
         for (int t = 0; t < 2; ++t) { mbar_init(&q_full[t], 4); mbar_init(&s_full[t], 1); mbar_init(&p_full[t], 4); mbar_init(&o_full[t], 1); }
-        for (int s = 0; s < STAGES; ++s) { mbar_init(&full[s], 1); mbar_init(&empty[s], 2); mbar_init(&v_ready[s], 1); }
+        for (int s = 0; s < STAGES; ++s) { mbar_init(&full[s], 1); mbar_init(&empty[s], 1); mbar_init(&v_ready[s], 1); }
         *abort_flag = 0;
         fence_mbar_init();
     }
@@ -204,47 +207,56 @@ paged_tiles_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant
                     mbar_arrive(&v_ready[j % STAGES]);
                 }
             }
-        } else {
-            const int t = warp - 9, ja = from_of(t), jb = until_of(t);
+        } else if (warp == 9) {
+            // In steps j = -1 .. nt - 1, for one tile of rows after the other: P_j V, then Q K_j+1. One warp for both, so that a tile's
+            // products come one after the other: two warps' ran side by side, and both tiles' exponentials did after them.
+            const auto one = [](int x) { return __shfl_sync(~0u, x, 0); };   // as warp
+            const int tiles = one(nt), ja[2] = {one(from_of(0)), one(from_of(1))}, jb[2] = {one(until_of(0)), one(until_of(1))};
+            const bool fitted = one(mend) != 0;
             const uint32_t lead = elect_lane(), id_s = umma_idesc_f16(KEYS, BF16), id_pv = umma_idesc_f16(D, BF16, 1);
-            const uint64_t qd = umma_desc_sw128(smem + t * L::TILE), kd = umma_desc_sw128(smem + L::OFF_RING), vd = umma_desc_sw128_mn(smem + L::OFF_RING, L::BOX);
-            const uint32_t ts = tmem + KEYS * t, to = TM_O + D * t;
-            auto landed = [&](int i) { return mbar_wait_soon(&full[i % STAGES], (i / STAGES) & 1, abort_flag, p.err, DEV_TIMEOUT_FULL); };
-            auto fit = [&](int j) { return mbar_wait_soon(&v_ready[j % STAGES], (j / STAGES) & 1, abort_flag, p.err, DEV_TIMEOUT_FULL); };
-            auto pass = [&](int i) {   // a stage that this tile does not use
-                if (!landed(i)) return false;
-                if (mend && (i & 1) && !fit(i / 2)) return false;
-                if (lead) mbar_arrive(&empty[i % STAGES]);
-                return true;
-            };
-            auto qk = [&](int j) {
-                const int i = 2 * j, s = i % STAGES;
-                if (!landed(i)) return false;
-                const uint64_t k = kd + (uint64_t) (s * (L::TILE >> 4));
-#pragma unroll
-                for (int kk = 0; kk < D / 16; ++kk)
-                    umma_f16_if(lead, ts, qd + (kk / 4) * (L::BOX >> 4) + 2 * (kk % 4), k + (kk / 4) * (L::BOX >> 4) + 2 * (kk % 4), id_s, kk != 0);
-                umma_commit_if(lead, &s_full[t]);
-                umma_commit_if(lead, &empty[s]);
-                return true;
-            };
+            const uint64_t qd = umma_desc_sw128(smem), kd = umma_desc_sw128(smem + L::OFF_RING), vd = umma_desc_sw128_mn(smem + L::OFF_RING, L::BOX);
+            auto wait = [&](uint64_t * at, int parity, int code) { return __all_sync(~0u, mbar_wait_soon(at, (uint32_t) parity, abort_flag, p.err, code)) != 0; };
             bool go = true;
-            for (int i = 0; i < 2 * ja && go; ++i) go = pass(i);
-            if (go && ja < jb) go = mbar_wait_soon(&q_full[t], 0, abort_flag, p.err, DEV_TIMEOUT_FULL) && qk(ja);
-            for (int j = ja; j < jb && go; ++j) {
-                const int i = 2 * j + 1, s = i % STAGES;
-                if (!mbar_wait_soon(&p_full[t], (j - ja) & 1, abort_flag, p.err, DEV_TIMEOUT_TMEM)) break;
-                if (!landed(i)) break;
-                if (mend && !fit(j)) break;
-                tc_fence_after();
-                const uint64_t v = vd + (uint64_t) (s * (L::TILE >> 4));
+            for (int j = -1; j < tiles && go; ++j) {
+                const int iv = 2 * j + 1, ik = 2 * j + 2, sv = iv % STAGES, sk = ik % STAGES;   // the stages of V_j and K_j+1
+                bool v_there = j < 0, k_there = j + 1 >= tiles;
+                auto values = [&] {
+                    if (v_there) return true;
+                    v_there = true;
+                    return wait(&full[sv], (iv / STAGES) & 1, DEV_TIMEOUT_FULL) && (!fitted || wait(&v_ready[j % STAGES], (j / STAGES) & 1, DEV_TIMEOUT_FULL));
+                };
+                auto keys = [&] {
+                    if (k_there) return true;
+                    k_there = true;
+                    return wait(&full[sk], (ik / STAGES) & 1, DEV_TIMEOUT_FULL);
+                };
 #pragma unroll
-                for (int kk = 0; kk < KEYS / 16; ++kk) umma_f16_ts_if(lead, to, ts + 8 * kk, v + 128 * kk, id_pv, j > ja || kk > 0);
-                umma_commit_if(lead, &empty[s]);
-                if (j + 1 < jb) go = qk(j + 1);
-                else umma_commit_if(lead, &o_full[t]);
+                for (int t = 0; t < 2; ++t) {
+                    if (go && j >= ja[t] && j < jb[t]) {
+                        go = values() && wait(&p_full[t], (j - ja[t]) & 1, DEV_TIMEOUT_TMEM);
+                        if (go) {
+                            tc_fence_after();
+                            const uint64_t v = vd + (uint64_t) (sv * (L::TILE >> 4));
+#pragma unroll
+                            for (int kk = 0; kk < KEYS / 16; ++kk)
+                                umma_f16_ts_if(lead, TM_O + D * t, tmem + KEYS * t + 8 * kk, v + 128 * kk, id_pv, j > ja[t] || kk > 0);
+                            if (j + 1 == jb[t]) umma_commit_if(lead, &o_full[t]);
+                        }
+                    }
+                    if (t == 1 && j >= 0 && go && (go = values())) umma_commit_if(lead, &empty[sv]);
+                    if (go && j + 1 >= ja[t] && j + 1 < jb[t]) {
+                        go = keys() && (j + 1 > ja[t] || wait(&q_full[t], 0, DEV_TIMEOUT_FULL));
+                        if (go) {
+                            const uint64_t q = qd + (uint64_t) (t * (L::TILE >> 4)), k = kd + (uint64_t) (sk * (L::TILE >> 4));
+#pragma unroll
+                            for (int kk = 0; kk < D / 16; ++kk)
+                                umma_f16_if(lead, tmem + KEYS * t, q + (kk / 4) * (L::BOX >> 4) + 2 * (kk % 4), k + (kk / 4) * (L::BOX >> 4) + 2 * (kk % 4), id_s, kk != 0);
+                            umma_commit_if(lead, &s_full[t]);
+                        }
+                    }
+                    if (t == 1 && j + 1 < tiles && go && (go = keys())) umma_commit_if(lead, &empty[sk]);
+                }
             }
-            for (int i = 2 * jb; i < 2 * nt && go; ++i) go = pass(i);
         }
         __syncwarp();
         pdl_trigger();
@@ -288,35 +300,52 @@ paged_tiles_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant
         float l = 0.0f, ref = -INFINITY;
         bool ok = true, poison = false;
         // Tile j. Exponentials run against the reference of the tiles before while the maximum is found; the few tiles whose maximum is
-        // too far above it are done again. P waits in registers for that, and S stays where it is.
-        auto tile = [&](auto masked, int j) {
-            constexpr bool MASKED = decltype(masked)::value;
+        // too far above it are done again. P waits in registers for that, and S stays where it is. There is one copy of this
+        // code: with copies for tiles that all rows see whole and for the second time round, the warps waited for instructions.
+        auto tile = [&](int j) {
             const int base = (t0 + j) * KEYS;
-            uint32_t vis[4] = {~0u, ~0u, ~0u, ~0u};
-            if (MASKED) {
-                const uint32_t slabs = paged[j % L::DEEP];
+            uint32_t vis[4] = {~0u, ~0u, ~0u, ~0u}, pk[64], s[2][32];
+            const uint32_t slabs = paged[j % L::DEEP];
+            if (base < sure_lo || base + KEYS > sure_hi || slabs != 0xffu)
 #pragma unroll
                 for (int w = 0; w < 4; ++w)
                     vis[w] = low_bits(hi - base - 32 * w) & ~low_bits(lo - base - 32 * w) & ((slabs >> (2 * w) & 1u ? 0xffffu : 0u) | (slabs >> (2 * w) & 2u ? 0xffff0000u : 0u));
-            }
-            uint32_t pk[64], s[2][32];
-            float sum[4], top = -INFINITY;
-            auto pass = [&](bool find) {
-                sum[0] = sum[1] = sum[2] = sum[3] = 0.0f;
+            uint64_t sum[2];
+            const uint64_t c2 = f2_pack(p.scale, p.scale);
+#pragma unroll 1
+            for (bool first = true;; first = false) {
+                const float neg = ref == -INFINITY ? 0.0f : -ref;
+                const uint64_t neg2 = f2_pack(neg, neg);
+                float top = -INFINITY;
+                sum[0] = sum[1] = 0;
                 tmem_request32(ts, s[0]);
 #pragma unroll
                 for (int w = 0; w < 4; ++w) {
-                    tmem_landed32(s[w & 1]);
+                    uint32_t * x = s[w & 1];
+                    tmem_landed32(x);
                     if (w < 3) tmem_request32(ts + 32 * (w + 1), s[(w + 1) & 1]);
-                    if (MASKED) hide(s[w & 1], vis[w]);
-                    exponentials<BF16, MASKED>(s[w & 1], pk + 16 * w, p.scale, ref, sum);
-                    if (find) top = fmaxf(top, greatest(s[w & 1]));
+                    hide(x, vis[w]);
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) {
+                        uint64_t v = ffma2(f2_pack(__uint_as_float(x[2 * e]), __uint_as_float(x[2 * e + 1])), c2, neg2);
+                        float y, z;
+                        if (e % L::EVERY == L::EVERY - 1) {
+                            v = ex2_fma<BF16, true>(v);
+                            f2_unpack(v, y, z);
+                        } else {
+                            f2_unpack(v, y, z);
+                            y = ex2(y);
+                            z = ex2(z);
+                            v = f2_pack(y, z);
+                        }
+                        sum[e & 1] = fadd2(sum[e & 1], v);
+                        pk[16 * w + e] = pack16<BF16>(y, z);
+                    }
+                    top = fmaxf(top, greatest(x));
                 }
-            };
-            pass(true);
-            top *= p.scale;
-            const bool move = top > ref + LAZY;
-            if (__any_sync(~0u, move)) {
+                top *= p.scale;
+                const bool move = top > ref + LAZY;
+                if (!first || !__any_sync(~0u, move)) break;
                 // a row moves its reference by itself, so its result does not depend on its neighbours
                 const float f = move ? ex2(ref - top) : 1.0f;
                 if (move) { ref = top; l *= f; }
@@ -330,11 +359,15 @@ paged_tiles_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant
                         tmem_st16(to + y, (const uint32_t *) o);
                     }
                 }
-                pass(false);
             }
-#pragma unroll
-            for (int w = 0; w < 4; ++w) tmem_st16(ts + 16 * w, pk + 16 * w);
-            l += (sum[0] + sum[2]) + (sum[1] + sum[3]);
+            tmem_st32(ts, pk);
+            tmem_st32(ts + 32, pk + 32);
+            {
+                float a, b, c, d;
+                f2_unpack(sum[0], a, b);
+                f2_unpack(sum[1], c, d);
+                l += (a + c) + (b + d);
+            }
             if (mend && mixed(base)) {
                 if (!mbar_wait_soon(&v_ready[j % STAGES], (j / STAGES) & 1, abort_flag, p.err, DEV_TIMEOUT_FULL)) ok = false;
 #pragma unroll
@@ -349,9 +382,7 @@ paged_tiles_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant
             if (!mbar_wait_soon(&s_full[t], (j - ja) & 1, abort_flag, p.err, DEV_TIMEOUT_TMEM)) { ok = false; break; }
             __syncwarp();
             tc_fence_after();
-            const int base = (t0 + j) * KEYS;
-            if (base >= sure_lo && base + KEYS <= sure_hi && paged[j % L::DEEP] == 0xffu) tile(std::false_type(), j);
-            else tile(std::true_type(), j);
+            tile(j);
         }
         // no score above -inf: the FMA pipe's exponentials gave its keys 2^-126 each
         if (ref == -INFINITY && l < INFINITY) l = 0.0f;
