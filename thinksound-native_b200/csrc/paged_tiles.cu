@@ -38,7 +38,7 @@ struct Lay {
     static_assert(TOTAL + 64 <= 227 * 1024, "one CTA's shared memory");
     static_assert(ROWS * SUM_ROW * 4 <= STAGES * TILE, "the rows' sums fit in the ring");
     static_assert(TM_O + 2 * D <= TM, "tensor memory");
-    static_assert((8 + 3 * STAGES) * 8 + (2 + DEEP + 4 * STAGES) * 4 <= 640, "barriers");
+    static_assert((10 + 3 * STAGES) * 8 + (2 + DEEP + 4 * STAGES) * 4 <= 640, "barriers");
 };
 
 __device__ __forceinline__ void bar_n(int id, int n) { asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(n) : "memory"); }
@@ -57,13 +57,13 @@ paged_tiles_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant
     if (!fits && tid == 0 && p.err) atomicCAS(p.err, 0, DEV_BAD_ARGS);
     uint64_t * bar = (uint64_t *) (smem + L::OFF_BAR);
     // v_ready is a tile's, of the last STAGES: a stage holds keys one time and values another
-    uint64_t * q_full = bar, * s_full = bar + 2, * p_full = bar + 4, * o_full = bar + 6, * full = bar + 8, * empty = full + STAGES, * v_ready = empty + STAGES;
+    uint64_t * q_full = bar, * s_full = bar + 2, * p_full = bar + 4, * o_full = bar + 6, * p_half = bar + 8, * full = bar + 10, * empty = full + STAGES, * v_ready = empty + STAGES;
     uint32_t * words = (uint32_t *) (v_ready + STAGES);   // TMEM address, abort flag, slabs with pages [DEEP tiles], keys of a tile that are not finite [STAGES tiles][4]
     volatile int * abort_flag = (volatile int *) (words + 1);
     volatile uint32_t * paged = words + 2, * not_finite = paged + L::DEEP;
 
     if (tid == 0) {
-        for (int t = 0; t < 2; ++t) { mbar_init(&q_full[t], 4); mbar_init(&s_full[t], 1); mbar_init(&p_full[t], 4); mbar_init(&o_full[t], 1); }
+        for (int t = 0; t < 2; ++t) { mbar_init(&q_full[t], 4); mbar_init(&s_full[t], 1); mbar_init(&p_full[t], 4); mbar_init(&o_full[t], 1); mbar_init(&p_half[t], 4); }
         for (int s = 0; s < STAGES; ++s) { mbar_init(&full[s], 1); mbar_init(&empty[s], 1); mbar_init(&v_ready[s], 1); }
         *abort_flag = 0;
         fence_mbar_init();
@@ -233,13 +233,20 @@ paged_tiles_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant
 #pragma unroll
                 for (int t = 0; t < 2; ++t) {
                     if (go && j >= ja[t] && j < jb[t]) {
-                        go = values() && wait(&p_full[t], (j - ja[t]) & 1, DEV_TIMEOUT_TMEM);
+                        const uint64_t v = vd + (uint64_t) (sv * (L::TILE >> 4));
+                        go = values() && wait(&p_half[t], (j - ja[t]) & 1, DEV_TIMEOUT_TMEM);
                         if (go) {
                             tc_fence_after();
-                            const uint64_t v = vd + (uint64_t) (sv * (L::TILE >> 4));
 #pragma unroll
-                            for (int kk = 0; kk < KEYS / 16; ++kk)
+                            for (int kk = 0; kk < KEYS / 32; ++kk)
                                 umma_f16_ts_if(lead, TM_O + D * t, tmem + KEYS * t + 8 * kk, v + 128 * kk, id_pv, j > ja[t] || kk > 0);
+                            go = wait(&p_full[t], (j - ja[t]) & 1, DEV_TIMEOUT_TMEM);
+                        }
+                        if (go) {
+                            tc_fence_after();
+#pragma unroll
+                            for (int kk = KEYS / 32; kk < KEYS / 16; ++kk)
+                                umma_f16_ts_if(lead, TM_O + D * t, tmem + KEYS * t + 8 * kk, v + 128 * kk, id_pv, 1);
                             if (j + 1 == jb[t]) umma_commit_if(lead, &o_full[t]);
                         }
                     }
@@ -299,53 +306,34 @@ paged_tiles_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant
         const int sure_hi = ja < jb ? hi_of(128 * t) : 0, sure_lo = ja < jb ? lo_of(rows_end - 1) : 0;   // every row of the tile sees keys sure_lo .. sure_hi - 1
         float l = 0.0f, ref = -INFINITY;
         bool ok = true, poison = false;
-        // Tile j. Exponentials run against the reference of the tiles before while the maximum is found; the few tiles whose maximum is
-        // too far above it are done again. P waits in registers for that, and S stays where it is. There is one copy of this
-        // code: with copies for tiles that all rows see whole and for the second time round, the warps waited for instructions.
+        // Tile j: all its scores into registers, the maximum, then the exponentials; P replaces S half by half, and the first half's
+        // product may start while the second half's exponentials run.
         auto tile = [&](int j) {
             const int base = (t0 + j) * KEYS;
-            uint32_t vis[4] = {~0u, ~0u, ~0u, ~0u}, pk[64], s[2][32];
+            uint32_t x[128];
+#pragma unroll
+            for (int w = 0; w < 4; ++w) tmem_request32(ts + 32 * w, x + 32 * w);
             const uint32_t slabs = paged[j % L::DEEP];
-            if (base < sure_lo || base + KEYS > sure_hi || slabs != 0xffu)
+            const bool masked = base < sure_lo || base + KEYS > sure_hi || slabs != 0xffu;
+            uint32_t vis[4] = {~0u, ~0u, ~0u, ~0u};
+            if (masked)
 #pragma unroll
                 for (int w = 0; w < 4; ++w)
                     vis[w] = low_bits(hi - base - 32 * w) & ~low_bits(lo - base - 32 * w) & ((slabs >> (2 * w) & 1u ? 0xffffu : 0u) | (slabs >> (2 * w) & 2u ? 0xffff0000u : 0u));
-            uint64_t sum[2];
-            const uint64_t c2 = f2_pack(p.scale, p.scale);
-#pragma unroll 1
-            for (bool first = true;; first = false) {
-                const float neg = ref == -INFINITY ? 0.0f : -ref;
-                const uint64_t neg2 = f2_pack(neg, neg);
-                float top = -INFINITY;
-                sum[0] = sum[1] = 0;
-                tmem_request32(ts, s[0]);
 #pragma unroll
-                for (int w = 0; w < 4; ++w) {
-                    uint32_t * x = s[w & 1];
-                    tmem_landed32(x);
-                    if (w < 3) tmem_request32(ts + 32 * (w + 1), s[(w + 1) & 1]);
-                    hide(x, vis[w]);
+            for (int w = 0; w < 4; ++w) tmem_landed32(x + 32 * w);
+            if (masked)
 #pragma unroll
-                    for (int e = 0; e < 16; ++e) {
-                        uint64_t v = ffma2(f2_pack(__uint_as_float(x[2 * e]), __uint_as_float(x[2 * e + 1])), c2, neg2);
-                        float y, z;
-                        if (e % L::EVERY == L::EVERY - 1) {
-                            v = ex2_fma<BF16, true>(v);
-                            f2_unpack(v, y, z);
-                        } else {
-                            f2_unpack(v, y, z);
-                            y = ex2(y);
-                            z = ex2(z);
-                            v = f2_pack(y, z);
-                        }
-                        sum[e & 1] = fadd2(sum[e & 1], v);
-                        pk[16 * w + e] = pack16<BF16>(y, z);
-                    }
-                    top = fmaxf(top, greatest(x));
-                }
-                top *= p.scale;
-                const bool move = top > ref + LAZY;
-                if (!first || !__any_sync(~0u, move)) break;
+                for (int w = 0; w < 4; ++w)
+#pragma unroll
+                    for (int e = 0; e < 32; ++e)
+                        if (!((vis[w] >> e) & 1u)) x[32 * w + e] = 0xff800000u;   // -inf
+            float mx[4];
+#pragma unroll
+            for (int w = 0; w < 4; ++w) mx[w] = greatest(x + 32 * w);
+            const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * p.scale;
+            const bool move = top > ref + LAZY;
+            if (__any_sync(~0u, move)) {
                 // a row moves its reference by itself, so its result does not depend on its neighbours
                 const float f = move ? ex2(ref - top) : 1.0f;
                 if (move) { ref = top; l *= f; }
@@ -360,8 +348,36 @@ paged_tiles_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant
                     }
                 }
             }
-            tmem_st32(ts, pk);
-            tmem_st32(ts + 32, pk + 32);
+            const float neg = ref == -INFINITY ? 0.0f : -ref;
+            const uint64_t neg2 = f2_pack(neg, neg), c2 = f2_pack(p.scale, p.scale);
+            uint64_t sum[2] = {0, 0};
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                uint32_t pk[32];
+#pragma unroll
+                for (int e = 0; e < 32; ++e) {
+                    uint64_t v = ffma2(f2_pack(__uint_as_float(x[64 * h + 2 * e]), __uint_as_float(x[64 * h + 2 * e + 1])), c2, neg2);
+                    float y, z;
+                    if (e % L::EVERY == L::EVERY - 1) {
+                        v = ex2_fma<BF16, true>(v);
+                        f2_unpack(v, y, z);
+                    } else {
+                        f2_unpack(v, y, z);
+                        y = ex2(y);
+                        z = ex2(z);
+                        v = f2_pack(y, z);
+                    }
+                    sum[e & 1] = fadd2(sum[e & 1], v);
+                    pk[e] = pack16<BF16>(y, z);
+                }
+                tmem_st32(ts + 32 * h, pk);
+                if (h == 0) {
+                    tmem_st_wait();
+                    tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(&p_half[t]);
+                }
+            }
             {
                 float a, b, c, d;
                 f2_unpack(sum[0], a, b);
