@@ -8,7 +8,7 @@
 // the keys; a CTA takes a unit or, where there are few, a part of its keys, the parts of a cluster adding up their sums. 384 threads:
 //   warps 0-3, 4-7  softmax of a tile, one row a thread: S from TMEM, mask, maximum, exponentials, P over S's columns
 //   warp 8          TMA: 128 keys, then their values, through one ring of stages; a tile may lie in several pages, a lane a box
-//   warp 9          issues a tile's products: P_j V, then Q K_j+1 (so that S_j+1 being there means that O holds tile j)
+//   warps 9, 10     issue a tile's products: P_j V, then Q K_j+1 (so that S_j+1 being there means that O holds tile j)
 //   warp 11         where some keys are not seen by all rows: makes the tiles' V rows fit for the product
 // While one tile's products run, the other's exponentials do. TMEM: S of both tiles (2 x 128 columns) and O (2 x D).
 // Values behind keys that are not there may be NaN, and 0 * NaN is NaN: those rows of V are cleared. Where rows differ in what they
@@ -38,7 +38,7 @@ struct Lay {
     static_assert(TOTAL + 64 <= 227 * 1024, "one CTA's shared memory");
     static_assert(ROWS * SUM_ROW * 4 <= STAGES * TILE, "the rows' sums fit in the ring");
     static_assert(TM_O + 2 * D <= TM, "tensor memory");
-    static_assert((10 + 3 * STAGES) * 8 + (2 + DEEP + 4 * STAGES) * 4 <= 640, "barriers");
+    static_assert((12 + 3 * STAGES) * 8 + (2 + DEEP + 4 * STAGES) * 4 <= 640, "barriers");
 };
 
 __device__ __forceinline__ void bar_n(int id, int n) { asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(n) : "memory"); }
@@ -56,15 +56,15 @@ paged_tiles_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant
     const bool fits = (smem_u32(smem) & 1023) == 0;   // the swizzled tiles need 1024-byte alignment
     if (!fits && tid == 0 && p.err) atomicCAS(p.err, 0, DEV_BAD_ARGS);
     uint64_t * bar = (uint64_t *) (smem + L::OFF_BAR);
-    // v_ready is a tile's, of the last STAGES: a stage holds keys one time and values another
-    uint64_t * q_full = bar, * s_full = bar + 2, * p_full = bar + 4, * o_full = bar + 6, * p_half = bar + 8, * full = bar + 10, * empty = full + STAGES, * v_ready = empty + STAGES;
+    // v_ready counts the tiles that pass through warp 11: a stage holds keys one time and values another
+    uint64_t * q_full = bar, * s_full = bar + 2, * p_full = bar + 4, * o_full = bar + 6, * p_half = bar + 8, * turn = bar + 10, * full = bar + 12, * empty = full + STAGES, * v_ready = empty + STAGES;
     uint32_t * words = (uint32_t *) (v_ready + STAGES);   // TMEM address, abort flag, slabs with pages [DEEP tiles], keys of a tile that are not finite [STAGES tiles][4]
     volatile int * abort_flag = (volatile int *) (words + 1);
     volatile uint32_t * paged = words + 2, * not_finite = paged + L::DEEP;
 
     if (tid == 0) {
-        for (int t = 0; t < 2; ++t) { mbar_init(&q_full[t], 4); mbar_init(&s_full[t], 1); mbar_init(&p_full[t], 4); mbar_init(&o_full[t], 1); mbar_init(&p_half[t], 4); }
-        for (int s = 0; s < STAGES; ++s) { mbar_init(&full[s], 1); mbar_init(&empty[s], 1); mbar_init(&v_ready[s], 1); }
+        for (int t = 0; t < 2; ++t) { mbar_init(&q_full[t], 4); mbar_init(&s_full[t], 1); mbar_init(&p_full[t], 4); mbar_init(&o_full[t], 1); mbar_init(&p_half[t], 4); mbar_init(&turn[t], 1); }
+        for (int s = 0; s < STAGES; ++s) { mbar_init(&full[s], 1); mbar_init(&empty[s], 2); mbar_init(&v_ready[s], 1); }
         *abort_flag = 0;
         fence_mbar_init();
     }
@@ -128,7 +128,7 @@ paged_tiles_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant
     const int t0 = tile0 + min(all_tiles, (int) split * per), nt = fits ? tile0 + min(all_tiles, ((int) split + 1) * per) - t0 : 0;
     const int least = hi_of(0), latest = lo_of(R - 1);   // before least and from latest on every row sees
     auto mixed = [&](int base) { return least < min(n, base + KEYS) || base < latest; };   // rows see different keys of the tile
-    const bool mend = nt > 0 && ((t0 + nt) * KEYS > n || mixed(t0 * KEYS) || mixed((t0 + nt - 1) * KEYS));
+    auto unfit = [&](int base) { return base + KEYS > n || mixed(base); };                           // its values pass through warp 11
     // the part's tiles that tile t of the rows sees: ja .. jb - 1
     auto from_of = [&](int t) { return 128 * t < R ? min(nt, max(0, lo_of(128 * t) / KEYS - t0)) : 0; };
     auto until_of = [&](int t) { return 128 * t < R ? max(from_of(t), min(nt, (hi_of(min(R, 128 * t + 128) - 1) + KEYS - 1) / KEYS - t0)) : 0; };
@@ -169,10 +169,14 @@ paged_tiles_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant
                 }
             }
         } else if (warp == 11) {
-            for (int j = 0; j < nt && mend; ++j) {
+            int seen = 0;
+            for (int j = 0; j < nt; ++j) {
                 const int base = (t0 + j) * KEYS, i = 2 * j + 1, s = i % STAGES;
-                if (!mbar_wait_soon(&full[s], (i / STAGES) & 1, abort_flag, p.err, DEV_TIMEOUT_FULL)) break;
+                // every use of a stage in turn: a parity tells a use only from the one before
+                if (!mbar_wait_soon(&full[(i - 1) % STAGES], ((i - 1) / STAGES) & 1, abort_flag, p.err, DEV_TIMEOUT_FULL) ||
+                    !mbar_wait_soon(&full[s], (i / STAGES) & 1, abort_flag, p.err, DEV_TIMEOUT_FULL)) break;
                 __syncwarp();
+                if (!unfit(base)) continue;
                 uint8_t * v = smem + L::OFF_RING + s * L::TILE;
                 const bool mix = mixed(base);
                 // rows of keys that are not there, a lane a key
@@ -203,66 +207,66 @@ paged_tiles_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant
                 fence_proxy_async_smem();
                 __syncwarp();
                 if (lane == 0) {
-                    for (int w = 0; w < 4; ++w) not_finite[4 * (j % STAGES) + w] = bad[w];
-                    mbar_arrive(&v_ready[j % STAGES]);
+                    for (int w = 0; w < 4; ++w) not_finite[4 * (seen % STAGES) + w] = bad[w];
+                    mbar_arrive(&v_ready[seen % STAGES]);
                 }
+                ++seen;
             }
-        } else if (warp == 9) {
-            // In steps j = -1 .. nt - 1, for one tile of rows after the other: P_j V, then Q K_j+1. One warp for both, so that a tile's
-            // products come one after the other: two warps' ran side by side, and both tiles' exponentials did after them.
+        } else {
+            // In steps j = -1 .. nt - 1: P_j V, then Q K_j+1 of this warp's tile of rows. What follows P's second half is issued by turns where
+            // both tiles have some: side by side, both would end late, and both tiles' exponentials would run at the same time.
             const auto one = [](int x) { return __shfl_sync(~0u, x, 0); };   // as warp
-            const int tiles = one(nt), ja[2] = {one(from_of(0)), one(from_of(1))}, jb[2] = {one(until_of(0)), one(until_of(1))};
-            const bool fitted = one(mend) != 0;
+            const int t = warp - 9, tiles = one(nt), ja = one(from_of(t)), jb = one(until_of(t)), other_a = one(from_of(1 - t)), other_b = one(until_of(1 - t));
             const uint32_t lead = elect_lane(), id_s = umma_idesc_f16(KEYS, BF16), id_pv = umma_idesc_f16(D, BF16, 1);
-            const uint64_t qd = umma_desc_sw128(smem), kd = umma_desc_sw128(smem + L::OFF_RING), vd = umma_desc_sw128_mn(smem + L::OFF_RING, L::BOX);
+            const uint64_t qd = umma_desc_sw128(smem + t * L::TILE), kd = umma_desc_sw128(smem + L::OFF_RING), vd = umma_desc_sw128_mn(smem + L::OFF_RING, L::BOX);
+            const uint32_t ts = tmem + KEYS * t, to = TM_O + D * t;
             auto wait = [&](uint64_t * at, int parity, int code) { return __all_sync(~0u, mbar_wait_soon(at, (uint32_t) parity, abort_flag, p.err, code)) != 0; };
             bool go = true;
+            int turns = 0, fits_seen = 0;
             for (int j = -1; j < tiles && go; ++j) {
                 const int iv = 2 * j + 1, ik = 2 * j + 2, sv = iv % STAGES, sk = ik % STAGES;   // the stages of V_j and K_j+1
-                bool v_there = j < 0, k_there = j + 1 >= tiles;
-                auto values = [&] {
-                    if (v_there) return true;
-                    v_there = true;
-                    return wait(&full[sv], (iv / STAGES) & 1, DEV_TIMEOUT_FULL) && (!fitted || wait(&v_ready[j % STAGES], (j / STAGES) & 1, DEV_TIMEOUT_FULL));
-                };
-                auto keys = [&] {
-                    if (k_there) return true;
-                    k_there = true;
-                    return wait(&full[sk], (ik / STAGES) & 1, DEV_TIMEOUT_FULL);
-                };
-#pragma unroll
-                for (int t = 0; t < 2; ++t) {
-                    if (go && j >= ja[t] && j < jb[t]) {
-                        const uint64_t v = vd + (uint64_t) (sv * (L::TILE >> 4));
-                        go = values() && wait(&p_half[t], (j - ja[t]) & 1, DEV_TIMEOUT_TMEM);
-                        if (go) {
-                            tc_fence_after();
-#pragma unroll
-                            for (int kk = 0; kk < KEYS / 32; ++kk)
-                                umma_f16_ts_if(lead, TM_O + D * t, tmem + KEYS * t + 8 * kk, v + 128 * kk, id_pv, j > ja[t] || kk > 0);
-                            go = wait(&p_full[t], (j - ja[t]) & 1, DEV_TIMEOUT_TMEM);
-                        }
-                        if (go) {
-                            tc_fence_after();
-#pragma unroll
-                            for (int kk = KEYS / 32; kk < KEYS / 16; ++kk)
-                                umma_f16_ts_if(lead, TM_O + D * t, tmem + KEYS * t + 8 * kk, v + 128 * kk, id_pv, 1);
-                            if (j + 1 == jb[t]) umma_commit_if(lead, &o_full[t]);
-                        }
+                const bool pv = j >= ja && j < jb, qk = j + 1 >= ja && j + 1 < jb;
+                const bool by_turns = (pv || qk) && j + 1 >= other_a && j < other_b && other_a < other_b;
+                if (j >= 0) {
+                    go = wait(&full[sv], (iv / STAGES) & 1, DEV_TIMEOUT_FULL);
+                    if (one(unfit((t0 + j) * KEYS))) {
+                        go = go && wait(&v_ready[fits_seen % STAGES], (fits_seen / STAGES) & 1, DEV_TIMEOUT_FULL);
+                        ++fits_seen;
                     }
-                    if (t == 1 && j >= 0 && go && (go = values())) umma_commit_if(lead, &empty[sv]);
-                    if (go && j + 1 >= ja[t] && j + 1 < jb[t]) {
-                        go = keys() && (j + 1 > ja[t] || wait(&q_full[t], 0, DEV_TIMEOUT_FULL));
-                        if (go) {
-                            const uint64_t q = qd + (uint64_t) (t * (L::TILE >> 4)), k = kd + (uint64_t) (sk * (L::TILE >> 4));
-#pragma unroll
-                            for (int kk = 0; kk < D / 16; ++kk)
-                                umma_f16_if(lead, tmem + KEYS * t, q + (kk / 4) * (L::BOX >> 4) + 2 * (kk % 4), k + (kk / 4) * (L::BOX >> 4) + 2 * (kk % 4), id_s, kk != 0);
-                            umma_commit_if(lead, &s_full[t]);
-                        }
-                    }
-                    if (t == 1 && j + 1 < tiles && go && (go = keys())) umma_commit_if(lead, &empty[sk]);
                 }
+                if (j + 1 < tiles) go = go && wait(&full[sk], (ik / STAGES) & 1, DEV_TIMEOUT_FULL);
+                if (qk && j + 1 == ja) go = go && wait(&q_full[t], 0, DEV_TIMEOUT_FULL);
+                const uint64_t v = vd + (uint64_t) (sv * (L::TILE >> 4)), k = kd + (uint64_t) (sk * (L::TILE >> 4));
+                if (pv && go && (go = wait(&p_half[t], (j - ja) & 1, DEV_TIMEOUT_TMEM))) {
+                    tc_fence_after();
+#pragma unroll
+                    for (int kk = 0; kk < KEYS / 32; ++kk) umma_f16_ts_if(lead, to, ts + 8 * kk, v + 128 * kk, id_pv, j > ja || kk > 0);
+                    go = wait(&p_full[t], (j - ja) & 1, DEV_TIMEOUT_TMEM);
+                }
+                if (by_turns && go) {
+                    if (t || turns) go = wait(&turn[t], (turns - 1 + t) & 1, DEV_TIMEOUT_TMEM);
+                    ++turns;
+                }
+                if (!go) break;
+                if (pv) {
+                    tc_fence_after();
+#pragma unroll
+                    for (int kk = KEYS / 32; kk < KEYS / 16; ++kk) umma_f16_ts_if(lead, to, ts + 8 * kk, v + 128 * kk, id_pv, 1);
+                    umma_commit_if(lead, &empty[sv]);
+                    if (j + 1 == jb) umma_commit_if(lead, &o_full[t]);
+                } else if (j >= 0 && lead) {
+                    mbar_arrive(&empty[sv]);   // a stage that this tile does not use
+                }
+                if (qk) {
+#pragma unroll
+                    for (int kk = 0; kk < D / 16; ++kk)
+                        umma_f16_if(lead, ts, qd + (kk / 4) * (L::BOX >> 4) + 2 * (kk % 4), k + (kk / 4) * (L::BOX >> 4) + 2 * (kk % 4), id_s, kk != 0);
+                    umma_commit_if(lead, &s_full[t]);
+                    umma_commit_if(lead, &empty[sk]);
+                } else if (j + 1 < tiles && lead) {
+                    mbar_arrive(&empty[sk]);
+                }
+                if (by_turns && lead) mbar_arrive(&turn[1 - t]);
             }
         }
         __syncwarp();
@@ -306,6 +310,8 @@ paged_tiles_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant
         const int sure_hi = ja < jb ? hi_of(128 * t) : 0, sure_lo = ja < jb ? lo_of(rows_end - 1) : 0;   // every row of the tile sees keys sure_lo .. sure_hi - 1
         float l = 0.0f, ref = -INFINITY;
         bool ok = true, poison = false;
+        int fits_seen = 0;   // tiles of the part whose values passed through warp 11
+        for (int j = 0; j < ja; ++j) fits_seen += unfit((t0 + j) * KEYS);
         // Tile j: all its scores into registers, the maximum, then the exponentials; P replaces S half by half, and the first half's
         // product may start while the second half's exponentials run.
         auto tile = [&](int j) {
@@ -384,10 +390,13 @@ paged_tiles_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant
                 f2_unpack(sum[1], c, d);
                 l += (a + c) + (b + d);
             }
-            if (mend && mixed(base)) {
-                if (!mbar_wait_soon(&v_ready[j % STAGES], (j / STAGES) & 1, abort_flag, p.err, DEV_TIMEOUT_FULL)) ok = false;
+            if (unfit(base)) {
+                if (mixed(base)) {
+                    if (!mbar_wait_soon(&v_ready[fits_seen % STAGES], (fits_seen / STAGES) & 1, abort_flag, p.err, DEV_TIMEOUT_FULL)) ok = false;
 #pragma unroll
-                for (int w = 0; w < 4; ++w) poison |= (not_finite[4 * (j % STAGES) + w] & vis[w]) != 0;
+                    for (int w = 0; w < 4; ++w) poison |= (not_finite[4 * (fits_seen % STAGES) + w] & vis[w]) != 0;
+                }
+                ++fits_seen;
             }
             tmem_st_wait();
             tc_fence_before();
