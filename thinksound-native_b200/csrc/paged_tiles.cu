@@ -33,7 +33,7 @@ struct Lay {
     static constexpr int STAGES = D == 128 ? 5 : 10, DEEP = 16;                   // DEEP: above the tiles on their way
     static constexpr int OFF_RING = 2 * TILE, OFF_BAR = OFF_RING + STAGES * TILE, TOTAL = OFF_BAR + 640;   // Q's two tiles first
     static constexpr int SUM_ROW = D + 4;
-    static constexpr int EVERY = D == 128 ? 8 : 4;   // one pair of exponentials of so many takes the FMA pipe
+    static constexpr int EVERY = 8;   // one pair of exponentials of so many takes the FMA pipe
     static constexpr uint32_t TM_O = 2 * KEYS, TM = 512;
     static_assert(TOTAL + 64 <= 227 * 1024, "one CTA's shared memory");
     static_assert(ROWS * SUM_ROW * 4 <= STAGES * TILE, "the rows' sums fit in the ring");
@@ -213,8 +213,8 @@ paged_tiles_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant
                 ++seen;
             }
         } else {
-            // In steps j = -1 .. nt - 1: P_j V, then Q K_j+1 of this warp's tile of rows. What follows P's second half is issued by turns where
-            // both tiles have some: side by side, both would end late, and both tiles' exponentials would run at the same time.
+            // In steps j = -1 .. nt - 1: P_j V, then Q K_j+1 of this warp's tile of rows, by turns where both tiles have some: side
+            // by side, both would end late, and both tiles' exponentials would run at the same time (980 us for 816).
             const auto one = [](int x) { return __shfl_sync(~0u, x, 0); };   // as warp
             const int t = warp - 9, tiles = one(nt), ja = one(from_of(t)), jb = one(until_of(t)), other_a = one(from_of(1 - t)), other_b = one(until_of(1 - t));
             const uint32_t lead = elect_lane(), id_s = umma_idesc_f16(KEYS, BF16), id_pv = umma_idesc_f16(D, BF16, 1);
@@ -237,15 +237,16 @@ paged_tiles_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant
                 if (j + 1 < tiles) go = go && wait(&full[sk], (ik / STAGES) & 1, DEV_TIMEOUT_FULL);
                 if (qk && j + 1 == ja) go = go && wait(&q_full[t], 0, DEV_TIMEOUT_FULL);
                 const uint64_t v = vd + (uint64_t) (sv * (L::TILE >> 4)), k = kd + (uint64_t) (sk * (L::TILE >> 4));
-                if (pv && go && (go = wait(&p_half[t], (j - ja) & 1, DEV_TIMEOUT_TMEM))) {
+                if (pv && go) go = wait(&p_half[t], (j - ja) & 1, DEV_TIMEOUT_TMEM);
+                if (by_turns && go) {
+                    if (t || turns) go = wait(&turn[t], (turns - 1 + t) & 1, DEV_TIMEOUT_TMEM);
+                    ++turns;
+                }
+                if (pv && go) {
                     tc_fence_after();
 #pragma unroll
                     for (int kk = 0; kk < KEYS / 32; ++kk) umma_f16_ts_if(lead, to, ts + 8 * kk, v + 128 * kk, id_pv, j > ja || kk > 0);
                     go = wait(&p_full[t], (j - ja) & 1, DEV_TIMEOUT_TMEM);
-                }
-                if (by_turns && go) {
-                    if (t || turns) go = wait(&turn[t], (turns - 1 + t) & 1, DEV_TIMEOUT_TMEM);
-                    ++turns;
                 }
                 if (!go) break;
                 if (pv) {
