@@ -49,7 +49,9 @@ paged_tiles_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant
     using L = Lay<D>;
     constexpr int CH = D / 8, STAGES = L::STAGES;   // CH: 16-byte pieces of a head
     extern __shared__ __align__(1024) uint8_t smem[];
-    __shared__ int unit_of[4];   // sequence, its first row, its new tokens, unit in it
+    // sequence, its first row, kv head, first query row, query rows, length, new tokens, tokens of rows 127 and the last; (token, head) of the rows
+    __shared__ int unit_of[9];
+    __shared__ uint16_t row_of[ROWS];
     // the warp's number as the compiler knows it to be one for all lanes: products issued under a branch that it takes for divergent
     // cost 100 cycles and more each
     const int tid = threadIdx.x, warp = __shfl_sync(~0u, tid >> 5, 0), lane = tid & 31;
@@ -82,12 +84,13 @@ paged_tiles_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant
         __syncwarp();
         for (int b0 = 0; b0 < (int) p.c.B && before <= gid; b0 += 32) {
             const int b = b0 + lane;
-            int start = 0, n = 0;
+            int start = 0, n = 0, len = 0;
             if (b < (int) p.c.B) {
                 start = seq_start(p.c, b);
                 n = max(0, seq_start(p.c, b + 1) - start);
+                len = p.c.len[b];
             }
-            const long long mine = ((long long) n * p.G + ROWS - 1) / ROWS * p.c.Hk;
+            const long long groups = ((long long) n * p.G + ROWS - 1) / ROWS, mine = groups * p.c.Hk;
             long long upto = mine;
 #pragma unroll
             for (int o = 1; o < 32; o <<= 1) {
@@ -96,10 +99,17 @@ paged_tiles_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant
             }
             const long long at = before + upto - mine;
             if (at <= gid && gid < at + mine) {
+                const unsigned u = (unsigned) (gid - at);
+                const int first = ((int) groups - 1 - (int) (u / p.c.Hk)) * ROWS, last = n * p.G - 1;
                 unit_of[0] = b;
                 unit_of[1] = start;
-                unit_of[2] = n;
-                unit_of[3] = (int) (gid - at);
+                unit_of[2] = (int) (u % p.c.Hk);
+                unit_of[3] = first;
+                unit_of[4] = min(ROWS, last + 1 - first);
+                unit_of[5] = len;
+                unit_of[6] = n;
+                unit_of[7] = min(last, first + 127) / p.G;
+                unit_of[8] = last < first + ROWS ? last / p.G : (first + ROWS - 1) / p.G;
             }
             before += __shfl_sync(~0u, upto, 31);
         }
@@ -114,24 +124,22 @@ paged_tiles_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant
         if (warp == 9) tmem_dealloc(tmem, L::TM);
         return;
     }
-    const int row0 = unit_of[1], fresh = unit_of[2], hk = unit_of[3] % (int) p.c.Hk;
-    const int all_rows = fresh * p.G;   // at most 2^30
-    const int r0 = ((all_rows + ROWS - 1) / ROWS - 1 - unit_of[3] / (int) p.c.Hk) * ROWS, R = min(ROWS, all_rows - r0);
-    const int len = p.c.len[b], n = cached(p, len), place0 = first_place(len, fresh);
-    // row t: token (r0 + t) / G, head (r0 + t) % G; keys lo .. hi - 1
-    auto place_of = [&](int t) { return place0 + (r0 + t) / p.G; };
-    auto hi_of = [&](int t) { return seen_to(p, place_of(t), n); };
-    auto lo_of = [&](int t) { return min(seen_from(p, place_of(t)), n); };
+    const int row0 = unit_of[1], hk = unit_of[2], r0 = unit_of[3], R = unit_of[4], len = unit_of[5], n = cached(p, len);
+    const int place0 = first_place(len, unit_of[6]), token0 = r0 / p.G;
+    // rows 0 .. 255 are (token, head of the group); a row at a place sees keys seen_from .. seen_to - 1
+    auto hi_at = [&](int token) { return seen_to(p, place0 + token, n); };
+    auto lo_at = [&](int token) { return min(seen_from(p, place0 + token), n); };
+    const int token127 = unit_of[7], token_last = unit_of[8], token128 = R > 128 ? (r0 + 128) / p.G : token_last;
     // tiles of keys that some row sees, this part of them
-    const int tile0 = lo_of(0) / KEYS, all_tiles = max(0, (hi_of(R - 1) + KEYS - 1) / KEYS - tile0);
+    const int least = hi_at(token0), latest = lo_at(token_last);   // before least and from latest on every row sees
+    const int tile0 = lo_at(token0) / KEYS, all_tiles = max(0, (hi_at(token_last) + KEYS - 1) / KEYS - tile0);
     const int per = (all_tiles + p.parts - 1) / p.parts;
     const int t0 = tile0 + min(all_tiles, (int) split * per), nt = fits ? tile0 + min(all_tiles, ((int) split + 1) * per) - t0 : 0;
-    const int least = hi_of(0), latest = lo_of(R - 1);   // before least and from latest on every row sees
     auto mixed = [&](int base) { return least < min(n, base + KEYS) || base < latest; };   // rows see different keys of the tile
-    auto unfit = [&](int base) { return base + KEYS > n || mixed(base); };                           // its values pass through warp 11
+    auto unfit = [&](int base) { return base + KEYS > n || mixed(base); };                 // its values pass through warp 11
     // the part's tiles that tile t of the rows sees: ja .. jb - 1
-    auto from_of = [&](int t) { return 128 * t < R ? min(nt, max(0, lo_of(128 * t) / KEYS - t0)) : 0; };
-    auto until_of = [&](int t) { return 128 * t < R ? max(from_of(t), min(nt, (hi_of(min(R, 128 * t + 128) - 1) + KEYS - 1) / KEYS - t0)) : 0; };
+    auto from_of = [&](int t) { return 128 * t < R ? min(nt, max(0, lo_at(t ? token128 : token0) / KEYS - t0)) : 0; };
+    auto until_of = [&](int t) { return 128 * t < R ? max(from_of(t), min(nt, (hi_at(t ? token_last : token127) + KEYS - 1) / KEYS - t0)) : 0; };
 
     if (warp >= 8) {
         if (warp == 8) {
@@ -186,22 +194,32 @@ paged_tiles_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant
                 __syncwarp();
                 uint32_t bad[4] = {0, 0, 0, 0};
                 if (mix) {
-                    constexpr int AT_ONCE = 32 / CH;   // rows of one step
-                    const int sub = lane / CH, ch = lane % CH;
-#pragma unroll
-                    for (int w = 0; w < 4; ++w) {
-#pragma unroll 4
-                        for (int y = 0; y < 32; y += AT_ONCE) {
-                            const int key = 32 * w + y + sub;
+                    // Mostly all are finite, and one look finds that out: with an exponent of ones, one more at the exponent's
+                    // lowest bit carries into the sign's place.
+                    constexpr uint32_t ONE = BF16 ? 0x00800080u : 0x04000400u;
+                    uint32_t any = 0;
+#pragma unroll 16
+                    for (int y = lane; y < L::TILE / 16; y += 32) {
+                        const uint4 o = *(const uint4 *) (v + y * 16);
+                        any |= ((o.x & 0x7fff7fffu) + ONE) | ((o.y & 0x7fff7fffu) + ONE) | ((o.z & 0x7fff7fffu) + ONE) | ((o.w & 0x7fff7fffu) + ONE);
+                    }
+                    if (__any_sync(~0u, any & 0x80008000u)) {
+                        constexpr int AT_ONCE = 32 / CH;   // rows of one step
+                        const int sub = lane / CH, ch = lane % CH;
+#pragma unroll 1
+                        for (int y = 0; y < KEYS; y += AT_ONCE) {
+                            const int key = y + sub;
                             uint4 * at = (uint4 *) (v + (ch >> 3) * L::BOX + key * 128 + (ch & 7) * 16);   // whichever piece lies there
                             const uint4 o = *at;
                             const uint4 f = make_uint4(finite_only<BF16>(o.x), finite_only<BF16>(o.y), finite_only<BF16>(o.z), finite_only<BF16>(o.w));
-                            if (o.x != f.x || o.y != f.y || o.z != f.z || o.w != f.w) {
-                                *at = f;
-                                bad[w] |= 1u << (key & 31);
-                            }
+                            const bool found = o.x != f.x || o.y != f.y || o.z != f.z || o.w != f.w;
+                            if (found) *at = f;
+#pragma unroll
+                            for (int w = 0; w < 4; ++w)
+                                if (found && key >> 5 == w) bad[w] |= 1u << (key & 31);
                         }
-                        bad[w] = __reduce_or_sync(~0u, bad[w]);
+#pragma unroll
+                        for (int w = 0; w < 4; ++w) bad[w] = __reduce_or_sync(~0u, bad[w]);
                     }
                 }
                 fence_proxy_async_smem();
@@ -280,35 +298,35 @@ paged_tiles_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant
         const int t = warp >> 2, row = tid & 127, ja = from_of(t), jb = until_of(t), mine = 128 * t + row;   // row of the unit
         const uint32_t lane0 = (uint32_t) ((warp & 3) * 32) << 16, ts = tmem + KEYS * t + lane0, to = TM_O + D * t + lane0;
         const bool there = mine < R;
+        const int token = (r0 + mine) / p.G;
+        row_of[mine] = (uint16_t) ((token - token0) << 7 | (r0 + mine - token * p.G));   // at most 256 tokens, 128 heads
+        bar_n(1 + t, 128);
         auto address = [&](const tsn_rows & x, int r) {   // of row r of the unit
-            const int u = r0 + r;
-            return (uint16_t *) x.p + (long long) (row0 + u / p.G) * x.sb + (long long) (hk * p.G + u % p.G) * x.st;
+            const int u = row_of[r];
+            return (uint16_t *) x.p + (long long) (row0 + token0 + (u >> 7)) * x.sb + (long long) (hk * p.G + (u & 127)) * x.st;
         };
         uint8_t * qs = smem + t * L::TILE;
         if (ja < jb) {   // Q into its swizzled boxes, rows past the last one as zeros
-            constexpr int AT_ONCE = 8;
+            uint4 q[CH];
+            const int ch = row % CH;
 #pragma unroll
-            for (int y0 = 0; y0 < CH; y0 += AT_ONCE) {
-                uint4 q[AT_ONCE];
+            for (int y = 0; y < CH; ++y) {
+                const int r = row / CH + 128 / CH * y;
+                q[y] = make_uint4(0, 0, 0, 0);
+                if (128 * t + r < R) q[y] = *(const uint4 *) (address(p.q, 128 * t + r) + ch * 8);
+            }
 #pragma unroll
-                for (int y = 0; y < AT_ONCE; ++y) {
-                    const int r = (row + 128 * (y0 + y)) / CH, ch = row % CH;
-                    q[y] = make_uint4(0, 0, 0, 0);
-                    if (128 * t + r < R) q[y] = *(const uint4 *) (address(p.q, 128 * t + r) + ch * 8);
-                }
-#pragma unroll
-                for (int y = 0; y < AT_ONCE; ++y) {
-                    const int r = (row + 128 * (y0 + y)) / CH, ch = row % CH;
-                    *(uint4 *) (qs + (ch >> 3) * L::BOX + r * 128 + (((ch & 7) ^ (r & 7)) << 4)) = q[y];
-                }
+            for (int y = 0; y < CH; ++y) {
+                const int r = row / CH + 128 / CH * y;
+                *(uint4 *) (qs + (ch >> 3) * L::BOX + r * 128 + (((ch & 7) ^ (r & 7)) << 4)) = q[y];
             }
             fence_proxy_async_smem();
             __syncwarp();
             if (lane == 0) mbar_arrive(&q_full[t]);
         }
-        const int hi = there ? hi_of(mine) : n, lo = there ? lo_of(mine) : 0;
+        const int hi = there ? hi_at(token) : n, lo = there ? lo_at(token) : 0;
         const int rows_end = min(R, 128 * t + 128);
-        const int sure_hi = ja < jb ? hi_of(128 * t) : 0, sure_lo = ja < jb ? lo_of(rows_end - 1) : 0;   // every row of the tile sees keys sure_lo .. sure_hi - 1
+        const int sure_hi = ja < jb ? hi_at(t ? token128 : token0) : 0, sure_lo = ja < jb ? lo_at(t ? token_last : token127) : 0;   // every row of the tile sees keys sure_lo .. sure_hi - 1
         float l = 0.0f, ref = -INFINITY;
         bool ok = true, poison = false;
         int fits_seen = 0;   // tiles of the part whose values passed through warp 11
@@ -331,10 +349,7 @@ paged_tiles_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant
             for (int w = 0; w < 4; ++w) tmem_landed32(x + 32 * w);
             if (masked)
 #pragma unroll
-                for (int w = 0; w < 4; ++w)
-#pragma unroll
-                    for (int e = 0; e < 32; ++e)
-                        if (!((vis[w] >> e) & 1u)) x[32 * w + e] = 0xff800000u;   // -inf
+                for (int w = 0; w < 4; ++w) hide(x + 32 * w, vis[w]);
             float mx[4];
 #pragma unroll
             for (int w = 0; w < 4; ++w) mx[w] = greatest(x + 32 * w);
@@ -424,10 +439,16 @@ paged_tiles_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant
 #pragma unroll
                 for (int e = 0; e < 32; ++e) o[e] = 0.0f;
             }
-            if (poison && there)
+            if (poison && there) {
+                float sums[32];   // a copy, as it goes through memory
+#pragma unroll
+                for (int e = 0; e < 32; ++e) sums[e] = o[e];
                 for (int j = ja; j < jb; ++j)
                     if (mixed((t0 + j) * KEYS))
-                        add_not_finite<BF16, 32>(p, b, hk, max(lo, (t0 + j) * KEYS), min(hi, (t0 + j + 1) * KEYS), x, o);
+                        add_not_finite<BF16, 32>(p, b, hk, max(lo, (t0 + j) * KEYS), min(hi, (t0 + j + 1) * KEYS), x, sums);
+#pragma unroll
+                for (int e = 0; e < 32; ++e) o[e] = sums[e];
+            }
         };
         if (p.parts > 1) {
             bar_n(3, 256);   // both tiles are done with the ring
@@ -555,16 +576,16 @@ cudaError_t configure_paged_tiles() {
 cudaError_t launch_paged_tiles(PagedArgs p, cudaStream_t s) {
     // units at most: a sequence has a last one that is not full
     const long long rows = (long long) p.c.N * p.G, units = std::min<long long>(p.c.N, rows / ROWS + p.c.B) * p.c.Hk;
-    // As many parts of a cluster as take the least time, in microseconds: start and end of a CTA 7, a tile 1.2, adding up the parts
-    // 3; clusters of one size run g_clusters[size] at a time. Four key tiles a part at least, eight parts at most (the largest portable
-    // cluster). The keys are what the tables have room for: lengths are on the device.
+    // As many parts of a cluster as take the least time, in microseconds: start and end of a CTA 6, a tile of 128-wide heads 2 and of
+    // 64-wide ones 1.7, adding up the parts 3; clusters of one size run g_clusters[size] at a time. Four key tiles a part at least, eight
+    // parts at most (the largest portable cluster). The keys are what the tables have room for: lengths are on the device.
     long long keys = (long long) p.c.M << p.page_log2;
     if (p.window) keys = std::min<long long>(keys, (long long) p.window + ROWS);
     const long long tiles = (keys + KEYS - 1) / KEYS;
     double least = 0.0;
     for (int parts = 1; parts <= 8 && (parts == 1 || parts * 4 <= tiles); ++parts) {
         const long long room = std::max(1, g_clusters[parts].load(std::memory_order_relaxed));
-        const double cost = (double) ((units + room - 1) / room) * (7.0 + (double) ((tiles + parts - 1) / parts) * 1.2) + (parts > 1 ? 3.0 : 0.0);
+        const double cost = (double) ((units + room - 1) / room) * (6.0 + (double) ((tiles + parts - 1) / parts) * (p.c.D == 64 ? 1.7 : 2.0)) + (parts > 1 ? 3.0 : 0.0);
         if (parts == 1 || cost < least) { least = cost; p.parts = parts; }
     }
     if (units * p.parts > 0x7fffffffLL) return cudaErrorInvalidValue;
