@@ -14,8 +14,10 @@
 // another in 64 bits. (Where more agree in 32 bits, the same goes on in 64.) The picks are written in the order of the pages.
 #include "kernels.h"
 #include "paged.h"
+#include "ptx.cuh"
 
 #include <cfloat>
+#include <type_traits>
 
 namespace tsn {
 
@@ -24,11 +26,23 @@ namespace {
 struct Select {
     tsn_sparse_attn_args a;
     int page_log2, G;
+    int parts;   // blocks of a cluster that share a token's pages
 };
 
-__device__ __forceinline__ double scaled(float v) {   // v * 2^-896
-    const uint32_t x = __float_as_uint(v);
-    return __hiloint2double((int) ((x & 0x80000000u) | ((x & 0x7fffffffu) >> 3)), (int) (x << 29));
+// Two 16-bit values of a word, each times 2^-896: the low words of such f64 are zero.
+template <class T>
+__device__ __forceinline__ void scaled(uint32_t w, double & a, double & b) {
+    int x, y;   // f32 bits
+    if constexpr (std::is_same<T, __nv_bfloat16>::value) {
+        x = (int) (w << 16);
+        y = (int) w;   // what lies below is cut off with the shifted bits
+    } else {
+        const float2 f = unpack2<T>(w);
+        x = __float_as_int(f.x);
+        y = __float_as_int(f.y);
+    }
+    a = __hiloint2double((x >> 3) & (int) 0x8fffffff, 0);
+    b = __hiloint2double((y >> 3) & (int) (std::is_same<T, __nv_bfloat16>::value ? 0x8fffe000 : 0x8fffffff), 0);
 }
 
 // A group of GT threads (whole warps) of a block, with a barrier of its own.
@@ -249,7 +263,8 @@ __global__ void __launch_bounds__(TOK * GT, 1) page_select_kernel(const __grid_c
     __shared__ __align__(16) double qs[TOK][D];
     __shared__ int seq[TOK], place[TOK];
     const tsn_sparse_attn_args & a = p.a;
-    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, row0 = (int) blockIdx.x * TOK, hk = (int) blockIdx.y;
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, parts = TOK > 1 ? 1 : p.parts, part = TOK > 1 ? 0 : (int) blockIdx.x % parts,
+              row0 = (int) blockIdx.x / parts * TOK, hk = (int) blockIdx.y;
     pdl_wait();
     if (warp < TOK) {
         const int row = row0 + warp, b = row < (int) a.c.N ? seq_of_row(a.c, row) : -1, pl = b < 0 ? 0 : place_of_row(a.c, b, row);
@@ -299,7 +314,7 @@ __global__ void __launch_bounds__(TOK * GT, 1) page_select_kernel(const __grid_c
 #pragma unroll
             for (int e = 0; e < 8; ++e) q[t][e] = qs[t][e0 + e];
         // lane (sub, l) reads its 8 elements of means j0 + sub * BATCH + y. No page: zeros
-        constexpr int STEP = THREADS / 32 * (BATCH * SIDE);
+        const int STEP = THREADS / 32 * (BATCH * SIDE) * parts;
         const int ahead = first + sub * BATCH + lane % BATCH;
         auto page_at = [&](int j) { return j + ahead < top ? table[j + ahead] : -1; };
         Words<T, 8> r[2][BATCH];
@@ -318,39 +333,50 @@ __global__ void __launch_bounds__(TOK * GT, 1) page_select_kernel(const __grid_c
         }
         auto sums = [&](int j0, int x) {
             const int mine = j0 + ahead;
+            double s[TOK][BATCH];
+#pragma unroll
+            for (int y = 0; y < BATCH; ++y) {
+                const uint32_t * w = (const uint32_t *) r[x][y].w;
+                double u[8];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) scaled<T>(w[e], u[2 * e], u[2 * e + 1]);
+#pragma unroll
+                for (int t = 0; t < TOK; ++t) {
+                    s[t][y] = q[t][0] * u[0];
+#pragma unroll
+                    for (int e = 1; e < 8; ++e) s[t][y] = fma(q[t][e], u[e], s[t][y]);
+                }
+            }
 #pragma unroll
             for (int t = 0; t < TOK; ++t) {
-                if (t < t0 || t >= t1) continue;
-                double s[BATCH];
-#pragma unroll
-                for (int y = 0; y < BATCH; ++y) {
-                    float u[8];
-                    to_floats<T, 8>(r[x][y], u);
-                    s[y] = 0.0;
-#pragma unroll
-                    for (int e = 0; e < 8; ++e) s[y] = fma(q[t][e], scaled(u[e]), s[y]);
-                }
                 // lane l of the mean's lanes ends with the sum of mean l % 8
                 if (LPH == 16)
 #pragma unroll
-                    for (int y = 0; y < BATCH; ++y) s[y] += __shfl_xor_sync(~0u, s[y], 8);
+                    for (int y = 0; y < BATCH; ++y) s[t][y] += __shfl_xor_sync(~0u, s[t][y], 8);
 #pragma unroll
                 for (int o = 4; o; o >>= 1)
 #pragma unroll
                     for (int y = 0; y < o; ++y) {
                         const bool up = (lane & o) != 0;
-                        const double give = up ? s[y] : s[y + o], keep = up ? s[y + o] : s[y];
-                        s[y] = keep + __shfl_xor_sync(~0u, give, o);
+                        const double give = up ? s[t][y] : s[t][y + o], keep = up ? s[t][y + o] : s[t][y];
+                        s[t][y] = keep + __shfl_xor_sync(~0u, give, o);
                     }
-                if (mine < top && (lane % LPH) < BATCH) {
+                if (mine < top && (lane % LPH) < BATCH && t >= t0 && t < t1) {
                     // numbers that bins can be made of: NaN and what exceeds 2^1000 (of queries that are not finite) at the ends
-                    const double v = (there[x] >> (lane % BATCH)) & 1u ? fmin(fmax(s[0], -0x1p1000), 0x1p1000) + 0.0 : 0.0;   // -0 becomes 0
-                    scores[t * a.c.M + mine - first] = v;
-                    rounded[t * a.c.M + mine - first] = fminf(fmaxf((float) v, -FLT_MAX), FLT_MAX);
+                    const double v = (there[x] >> (lane % BATCH)) & 1u ? fmin(fmax(s[t][0], -0x1p1000), 0x1p1000) + 0.0 : 0.0;   // -0 becomes 0
+                    const float f = fminf(fmaxf((float) v, -FLT_MAX), FLT_MAX);
+                    const int at = t * (int) a.c.M + mine - first;
+                    if (TOK > 1 || parts == 1) {
+                        scores[at] = v;
+                        rounded[at] = f;
+                    } else {   // the scores of a cluster's blocks meet in the first one
+                        asm volatile("st.shared::cluster.f64 [%0], %1;" ::"r"(dsmem_map(smem_u32(scores + at), 0)), "d"(v) : "memory");
+                        asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(dsmem_map(smem_u32(rounded + at), 0)), "f"(f) : "memory");
+                    }
                 }
             }
         };
-        int j0 = warp * (BATCH * SIDE), id = page_at(j0);
+        int j0 = (warp + part * (THREADS / 32)) * (BATCH * SIDE), id = page_at(j0);
         if (j0 < m) fetch(id, 0);
         id = page_at(j0 + STEP);
         while (j0 < m) {
@@ -365,7 +391,12 @@ __global__ void __launch_bounds__(TOK * GT, 1) page_select_kernel(const __grid_c
             j0 += STEP;
         }
     }
-    __syncthreads();
+    if (parts > 1) {
+        cluster_sync_all();
+        if (part) return;
+    } else {
+        __syncthreads();
+    }
     Group<GT> g;
     g.id = TOK == 1 ? 0 : tid / GT;
     g.tid = tid % GT;
@@ -390,13 +421,16 @@ cudaError_t launch(const Select & p, cudaStream_t s) {
     // Four tokens a block share the reads; single ones fill the GPU with fewer tokens, and hold the scores of more pages.
     if ((long long) p.a.c.N * p.a.c.Hk >= 2 * MANY * 148 && MANY * bytes <= MOST)
         return launch_cl(page_select_kernel<T, D, MANY, 64>, dim3((p.a.c.N + MANY - 1) / MANY, p.a.c.Hk), dim3(MANY * 64), MANY * bytes, s, dim3(1), p);
-    return launch_cl(page_select_kernel<T, D, 1, 512>, dim3(p.a.c.N, p.a.c.Hk), dim3(512), bytes, s, dim3(1), p);
+    // As many blocks for a token as there are SMs for, up to four, each with 512 pages or more.
+    Select one = p;
+    while (one.parts < 4 && (long long) p.a.c.N * p.a.c.Hk * one.parts * 2 <= 148 && p.a.c.M >= 1024u * one.parts) one.parts *= 2;
+    return launch_cl(page_select_kernel<T, D, 1, 512>, dim3(p.a.c.N * one.parts, p.a.c.Hk), dim3(512), bytes, s, dim3((unsigned) one.parts), one);
 }
 
 } // namespace
 
 cudaError_t launch_page_select(const tsn_sparse_attn_args & a, cudaStream_t s) {
-    const Select p{a, log2_of(a.c.page), (int) (a.H / a.c.Hk)};
+    const Select p{a, log2_of(a.c.page), (int) (a.H / a.c.Hk), 1};
     const bool bf = a.c.type == TSN_BF16;
     if (a.c.D == 64) return bf ? launch<__nv_bfloat16, 64>(p, s) : launch<__half, 64>(p, s);
     return bf ? launch<__nv_bfloat16, 128>(p, s) : launch<__half, 128>(p, s);
