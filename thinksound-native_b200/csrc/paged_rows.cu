@@ -6,7 +6,7 @@
 // side: S^T = K Q^T, O^T = V^T P^T; P^T is S^T's layout transposed in registers. Each warp streams 16-key slabs of its own by TMA,
 // a page holding whole slabs, through a ring of its own; the warps' sums meet in shared memory.
 // A unit is a kv head with up to 8 NT rows of a sequence, and its slabs. Lengths are on the device, so the device deals
-// them out: all units' slabs in a row, an equal share for each CTA, two of which fill an SM. A share may begin and end
+// them out: all units' slabs in a row, an equal share for each CTA; one of eight warps or two of four fill an SM. A share may begin and end
 // inside a unit; the CTA that is the last of a unit to arrive adds up its parts, in their order. Units of few slabs are not cut:
 // a trip through the workspace costs more.
 #include "kernels.h"
@@ -18,18 +18,24 @@ namespace tsn {
 
 namespace {
 
-constexpr int SLAB = 16, W = 4, CTAS = 2 * SMS;   // keys of a slab, warps
+constexpr int SLAB = 16;   // keys of a slab
 constexpr float LAZY = 8.0f;   // log2 units that a maximum may grow before o is rescaled
-// slabs of a share at least, slabs up to which a unit is not cut, parts of a unit at most (fewer slabs a part otherwise)
-constexpr int LEAST = 8, SHORT = 32, MOST_PARTS = 64;
+// Slabs of a share at least, slabs up to which a unit is not cut, parts of a unit at most (fewer slabs a part otherwise). One token, 8 kv
+// heads of 128, 2 x 1000 keys: with units of up to 32 slabs whole 15.7 us, 64: 12.1.
+constexpr int LEAST = 16, SHORT = 64, MOST_PARTS = 64;
+// Units up to which eight warps share one, a CTA an SM; above, two CTAs of four warps an SM, of which one loads while the
+// other adds up its unit's sums. us by eight / by four: 16 units of 704 keys 8.0/10.5, 8 of 1000 12.1/16.5, one of 32 768 15.7/21.7, 192 of
+// 8191 142/148, but 256 of 1000 29.4/27.1, 1024 of 300 45.5/38.2.
+constexpr long long FEW_UNITS = 200;
 
-template <int D, int NT>
+template <int D, int NT, int W>
 struct RowLay {
     static constexpr int BOX = SLAB * 128, HALF = SLAB * D * 2, STAGE = 2 * HALF, RING = D == 128 ? 3 : 6;   // a slab's keys, then its values
     static constexpr int ROWS = 8 * NT, ROW = D + 4;   // words of a row's sums: o, ref, l
     static constexpr int OFF_BAR = W * RING * STAGE, TOTAL = OFF_BAR + W * RING * 8 + 64;
     static_assert(ROWS * ROW * 4 <= RING * STAGE, "a warp's sums fit in its ring");
-    static_assert(2 * (TOTAL + 1024) <= 228 * 1024, "two CTAs fit on an SM");
+    static constexpr int CTAS = W == 4 ? 2 : 1;   // on an SM
+    static_assert(CTAS * (TOTAL + 2048) <= 228 * 1024, "they fit");
 };
 constexpr int part_words(int D, int rows) { return rows * (D + 4); }
 
@@ -55,10 +61,10 @@ __device__ __forceinline__ Seq sequence(const PagedArgs & p, int b) {
     return s;
 }
 
-template <int D, bool BF16, int NT, bool LIST>
-__global__ void __launch_bounds__(32 * W, 2)
+template <int D, bool BF16, int NT, bool LIST, int W>
+__global__ void __launch_bounds__(32 * W, W == 4 ? 2 : 1)
 paged_rows_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant__ CUtensorMap tv, const __grid_constant__ PagedArgs p) {
-    using L = RowLay<D, NT>;
+    using L = RowLay<D, NT, W>;
     constexpr int E = D / 32, RING = L::RING, ROWS = L::ROWS;
     extern __shared__ __align__(1024) uint8_t smem[];
     __shared__ int first_seq, first_off;
@@ -457,7 +463,7 @@ paged_rows_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant_
             if (flags[1]) {
                 // A row by one warp, or with fewer rows than warps by several, which take every `share`-th part and meet in shared memory.
                 const int share = R >= W ? 1 : W / R;
-                float * meet = (float *) smem;   // [W][D]
+                float * meet = (float *) smem;   // [warps][D]
                 for (int x = warp; x < (R * share + W - 1) / W * W && !flags[0]; x += W) {
                     const int r = x / share, mine_of = x % share;
                     float v[E] = {}, top = -INFINITY, sum = 0.0f;
@@ -537,48 +543,68 @@ paged_rows_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant_
     }
 }
 
-template <int D, bool BF16, int NT, bool LIST>
+template <int D, bool BF16, int NT, bool LIST, int W>
 cudaError_t launch(const PagedArgs & p, unsigned grid, cudaStream_t s) {
     CUtensorMap tk{}, tv{};
     if (!make_page_maps(p.c, SLAB, &tk, &tv)) return cudaErrorInvalidValue;
-    return launch_cl(paged_rows_kernel<D, BF16, NT, LIST>, dim3(grid), dim3(32 * W), RowLay<D, NT>::TOTAL, s, dim3(1), tk, tv, p);
+    return launch_cl(paged_rows_kernel<D, BF16, NT, LIST, W>, dim3(grid), dim3(32 * W), RowLay<D, NT, W>::TOTAL, s, dim3(1), tk, tv, p);
+}
+template <int D, bool BF16, int NT>
+cudaError_t launch(const PagedArgs & p, int warps, unsigned grid, cudaStream_t s) {
+    if (p.chosen) return warps == 8 ? launch<D, BF16, NT, true, 8>(p, grid, s) : launch<D, BF16, NT, true, 4>(p, grid, s);
+    return warps == 8 ? launch<D, BF16, NT, false, 8>(p, grid, s) : launch<D, BF16, NT, false, 4>(p, grid, s);
 }
 template <int D, bool BF16>
-cudaError_t launch(const PagedArgs & p, int nt, unsigned grid, cudaStream_t s) {
-    if (p.chosen) return nt == 1 ? launch<D, BF16, 1, true>(p, grid, s) : launch<D, BF16, 2, true>(p, grid, s);
-    return nt == 1 ? launch<D, BF16, 1, false>(p, grid, s) : launch<D, BF16, 2, false>(p, grid, s);
+cudaError_t launch(const PagedArgs & p, int nt, int warps, unsigned grid, cudaStream_t s) {
+    return nt == 1 ? launch<D, BF16, 1>(p, warps, grid, s) : launch<D, BF16, 2>(p, warps, grid, s);
 }
 
-int tiles_of(const PagedArgs & p, uint32_t most) { return (long long) p.G * (p.chosen ? 1 : most) > 8 ? 2 : 1; }
+// How a call's rows are grouped: eights of a group, units (at most), warps and CTAs.
+struct Plan {
+    int nt, warps;
+    long long units;
+    unsigned ctas;
+};
+Plan plan_of(const PagedArgs & p, uint32_t most) {
+    Plan r;
+    r.nt = (long long) p.G * (p.chosen ? 1 : most) > 8 ? 2 : 1;
+    const int rows = 8 * r.nt;
+    if (p.chosen || !p.c.q_start) r.units = (long long) p.c.N * ((p.G + rows - 1) / rows) * p.c.Hk;
+    else r.units = std::min((long long) p.c.N * ((p.G + rows - 1) / rows), (long long) p.c.N * p.G / rows + p.c.B) * p.c.Hk;
+    r.warps = r.units <= FEW_UNITS ? 8 : 4;
+    r.ctas = r.warps == 8 ? SMS : 2 * SMS;
+    return r;
+}
 
 } // namespace
 
 void plan_paged_rows(PagedArgs & p, uint32_t most, size_t * groups, size_t * bytes) {
-    const int nt = tiles_of(p, most), rows = 8 * nt;
+    const Plan r = plan_of(p, most);
     p.whole = 1;
     p.parts = 1;
     *groups = *bytes = 0;
-    unsigned ctas = CTAS;
+    unsigned ctas = r.ctas;
     if (p.chosen) {
-        const long long units = (long long) p.c.N * p.c.Hk * ((p.G + rows - 1) / rows), slabs = ((long long) p.picks << p.page_log2) / SLAB;
-        p.parts = (int) std::max(1ll, std::min({CTAS / units, slabs / (2 * LEAST), (long long) MOST_PARTS}));
-        ctas = (unsigned) (units * p.parts);
+        const long long slabs = ((long long) p.picks << p.page_log2) / SLAB;
+        p.parts = (int) std::max(1ll, std::min({r.ctas / r.units, slabs / LEAST, (long long) MOST_PARTS}));
+        if (slabs <= SHORT) p.parts = 1;
+        ctas = (unsigned) (r.units * p.parts);
         p.whole = p.parts == 1;
     } else {
         p.whole = (((long long) p.c.M << p.page_log2) + SLAB - 1) / SLAB <= SHORT;
     }
     if (!p.whole) {
         *groups = ctas;
-        *bytes = (size_t) ctas * 2 * part_words((int) p.c.D, rows) * 4;
+        *bytes = (size_t) ctas * 2 * part_words((int) p.c.D, 8 * r.nt) * 4;
     }
 }
 
 cudaError_t launch_paged_rows(const PagedArgs & p, uint32_t most, cudaStream_t s) {
-    const int nt = tiles_of(p, most);
-    const unsigned grid = p.chosen ? (unsigned) ((long long) p.c.N * p.c.Hk * ((p.G + 8 * nt - 1) / (8 * nt)) * p.parts) : CTAS;
+    const Plan r = plan_of(p, most);
+    const unsigned grid = p.chosen ? (unsigned) (r.units * p.parts) : r.ctas;
     const bool bf = p.c.type == TSN_BF16;
-    if (p.c.D == 64) return bf ? launch<64, true>(p, nt, grid, s) : launch<64, false>(p, nt, grid, s);
-    return bf ? launch<128, true>(p, nt, grid, s) : launch<128, false>(p, nt, grid, s);
+    if (p.c.D == 64) return bf ? launch<64, true>(p, r.nt, r.warps, grid, s) : launch<64, false>(p, r.nt, r.warps, grid, s);
+    return bf ? launch<128, true>(p, r.nt, r.warps, grid, s) : launch<128, false>(p, r.nt, r.warps, grid, s);
 }
 
 cudaError_t configure_paged_rows() {
@@ -586,11 +612,13 @@ cudaError_t configure_paged_rows() {
     auto set = [&](auto * k, int bytes) {
         if (e == cudaSuccess) e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
     };
-#define SET(D, B, NT) \
-    set(paged_rows_kernel<D, B, NT, false>, RowLay<D, NT>::TOTAL); \
-    set(paged_rows_kernel<D, B, NT, true>, RowLay<D, NT>::TOTAL);
-    SET(64, false, 1) SET(64, false, 2) SET(64, true, 1) SET(64, true, 2)
-    SET(128, false, 1) SET(128, false, 2) SET(128, true, 1) SET(128, true, 2)
+#define SET(D, B, NT, W) \
+    set(paged_rows_kernel<D, B, NT, false, W>, RowLay<D, NT, W>::TOTAL); \
+    set(paged_rows_kernel<D, B, NT, true, W>, RowLay<D, NT, W>::TOTAL);
+    SET(64, false, 1, 4) SET(64, false, 2, 4) SET(64, true, 1, 4) SET(64, true, 2, 4)
+    SET(128, false, 1, 4) SET(128, false, 2, 4) SET(128, true, 1, 4) SET(128, true, 2, 4)
+    SET(64, false, 1, 8) SET(64, false, 2, 8) SET(64, true, 1, 8) SET(64, true, 2, 8)
+    SET(128, false, 1, 8) SET(128, false, 2, 8) SET(128, true, 1, 8) SET(128, true, 2, 8)
 #undef SET
     return e;
 }
