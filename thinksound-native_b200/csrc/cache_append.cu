@@ -2,8 +2,8 @@
 //
 // Bound by HBM: q, k and v are read once, q_out and the pages written once. As in tsn_rope_axes a block takes a few whole
 // tokens, computes their cosines and sines once into shared memory (64-bit phases), and its warps run over the heads, 8 elements a
-// lane, loads one round ahead. What the cache adds is a chain of small reads for each token (its sequence, length and page), one
-// warp a token, while the heads' loads are on their way.
+// lane, loads some ahead. What the cache adds is a chain of small reads for each token (its sequence, length and page), a lane
+// a token, while the heads' loads are on their way.
 // The means of the pages are a second kernel, which reads the touched pages' keys after the first has written them.
 #include <algorithm>
 #include <type_traits>
@@ -25,16 +25,19 @@ enum { NEXT, LANES, SHARED };   // where the other element of a lane's pairs is:
 
 struct Append {
     tsn_cache_append_args a;
-    int page_log2, tok;   // tokens of a block
+    int page_log2, tok, span;   // tokens of a block, chunks of it
 };
 
-// Block (x, z): tokens x * tok .., chunks 8 z .. of 32 / LPH heads: the queries', then the keys', then the values'.
+// Block (x, y): tokens x * tok .., chunks y * span .. of 32 / LPH heads: the queries', then the keys', then the values'. A warp takes a
+// chunk through the block's tokens, so that a token costs its lanes a load, a store and the arithmetic (items that were each
+// worked out for themselves took as long as the memory traffic), loads AHEAD tokens before; then its next chunk.
 template <class TX, class T, int LPH, int PAIR>
 __global__ void __launch_bounds__(32 * WARPS, 4) cache_append_kernel(const __grid_constant__ tsn_rope_plan_t p, const __grid_constant__ Append n) {
-    constexpr int SIDE = 32 / LPH;
-    __shared__ __align__(16) float2 turn[MAX_TOK * TSN_ROPE_MAX_PAIRS + 8];
-    __shared__ float mate[PAIR == SHARED ? WARPS : 1][32 * 9];   // a lane's 8 elements, one word of padding between lanes
-    __shared__ int place[MAX_TOK], spot[MAX_TOK], slot[MAX_TOK];   // spot: the page, -1: none
+    constexpr int SIDE = 32 / LPH, AHEAD = sizeof(TX) == 4 ? 1 : 2;
+    constexpr bool SAME = std::is_same<TX, T>::value;
+    __shared__ __align__(16) float turn[MAX_TOK * 3 * TSN_ROPE_MAX_PAIRS];   // of a token's pairs: cosines, sines, sines with the other sign
+    __shared__ float mate[PAIR == SHARED ? WARPS : 1][32 * 9];               // a lane's 8 elements, one word of padding between lanes
+    __shared__ int place[MAX_TOK], spot[MAX_TOK], slot[MAX_TOK];             // spot: the page, -1: none
     pdl_wait();
     const tsn_cache_append_args & a = n.a;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -43,35 +46,38 @@ __global__ void __launch_bounds__(32 * WARPS, 4) cache_append_kernel(const __gri
     const int here = (int) min((long long) tok, a.c.N - s0);
     const int sub = lane / LPH, at = (lane & (LPH - 1)) * 8;
     const int q_chunks = (Hq + SIDE - 1) / SIDE, k_chunks = (Hk + SIDE - 1) / SIDE, chunks = q_chunks + 2 * k_chunks;
-    const int sharing = chunks < WARPS ? WARPS / chunks : 1;   // warps of a chunk
+    const int until = min(chunks, ((int) blockIdx.y + 1) * n.span);
     const float inv_D = 1.0f / (float) D;
-    const int row = (P + 1) & ~1;   // a token's pairs in the table, from a 16-byte boundary on
+    const int row = (P + 3) & ~3;   // a token's pairs in the table, from a 16-byte boundary on
 
-    const int chunk = sharing > 1 ? (warp < sharing * chunks ? warp % chunks : chunks) : (int) blockIdx.y * WARPS + warp;
-    const int what = chunk < q_chunks ? 0 : chunk < q_chunks + k_chunks ? 1 : 2;   // q, k, v
-    const tsn_rows & in = what == 0 ? a.q : what == 1 ? a.k : a.v;
-    const float * wp = what == 0 ? a.q_norm : what == 1 ? a.k_norm : nullptr;
-    const int head = (chunk - (what == 0 ? 0 : what == 1 ? q_chunks : q_chunks + k_chunks)) * SIDE + sub, from = sharing > 1 ? warp / chunks : 0;
-    const bool mine = chunk < chunks && at < D && head < (what == 0 ? Hq : Hk);
-    const TX * x = (const TX *) in.p + (s0 + from) * in.sb + head * in.st + at;
-    const long long dx = sharing * in.sb;
-    Words<TX, 8> raw, next;
-    auto fetch = [&](int k) {
-        if (mine && k < here) next = load_words<TX, 8>(x);
-        x += dx;
-    };
-    fetch(from);   // before the table: the loads are on their way
-    float2 w[4];
-    if (wp)
+    // the chunk: queries', keys' or values', the lane's head and its elements
+    int chunk = (int) blockIdx.y * n.span + warp, what = 0, head = 0;
+    bool mine = false;
+    const TX * x = nullptr;
+    long long dx = 0;
+    Words<TX, 8> ring[AHEAD];
+    auto begin = [&] {   // with the first tokens' loads
+        what = chunk < q_chunks ? 0 : chunk < q_chunks + k_chunks ? 1 : 2;
+        head = (chunk - (what == 0 ? 0 : what == 1 ? q_chunks : q_chunks + k_chunks)) * SIDE + sub;
+        mine = chunk < until && at < D && head < (what == 0 ? Hq : Hk);
+        const tsn_rows & in = what == 0 ? a.q : what == 1 ? a.k : a.v;
+        dx = in.sb;
+        x = (const TX *) in.p + s0 * dx + head * in.st + at;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) w[i] = mine ? make_float2(wp[at + 2 * i], wp[at + 2 * i + 1]) : make_float2(0.0f, 0.0f);
-    if (warp < here) {
-        const int i = (int) s0 + warp, b = seq_of_row(a.c, i);
-        const int at_place = b < 0 ? 0 : place_of_row(a.c, b, i);
-        if (lane == 0) {
-            place[warp] = at_place;
-            spot[warp] = b < 0 ? -2 : page_of(a.c, b, at_place >> n.page_log2);   // -2: a row of no sequence
-            slot[warp] = at_place & ((1 << n.page_log2) - 1);
+        for (int y = 0; y < AHEAD; ++y) {
+            if (mine && y < here) ring[y] = load_words<TX, 8>(x);
+            x += dx;
+        }
+    };
+    begin();   // before the table: the loads are on their way
+    if (warp == 0) {   // a lane a token; mostly all are of one sequence
+        const int b0 = seq_of_row(a.c, (int) s0), b1 = here > 1 ? seq_of_row(a.c, (int) s0 + here - 1) : b0;
+        if (lane < here) {
+            const int i = (int) s0 + lane, b = b0 == b1 ? b0 : seq_of_row_alone(a.c, i);
+            const int pl = b < 0 ? 0 : place_of_row(a.c, b, i);
+            place[lane] = pl;
+            spot[lane] = b < 0 ? -2 : page_of(a.c, b, pl >> n.page_log2);   // -2: a row of no sequence
+            slot[lane] = pl & ((1 << n.page_log2) - 1);
         }
     }
     __syncthreads();
@@ -80,85 +86,114 @@ __global__ void __launch_bounds__(32 * WARPS, 4) cache_append_kernel(const __gri
         const int pos = a.pos ? a.pos[(s0 + k) * a.pos_ss + p.axis[j]] : place[k];
         float sn, cs;
         sincospif(2.0f * phase(pos, p.turn[j]), &sn, &cs);
-        turn[k * row + j] = make_float2(cs, sn);
+        float * t = turn + k * 3 * row + j;
+        t[0] = cs;
+        t[row] = sn;
+        t[2 * row] = -sn;
     }
     __syncthreads();
-    if (chunk >= chunks) return;
 
-    for (int k = from; k < here; k += sharing) {
-        raw = next;
-        fetch(k + sharing);
-        float u[8];
-        to_floats<TX, 8>(raw, u);
-        if (wp) {
-            float2 q = make_float2(0.0f, 0.0f);
+    // halves: the lane's pairs, whether its elements are the first or the second ones, and the lane that holds the others
+    const bool low = at < P, turned = at < 2 * P;
+    const int other = PAIR == LANES && turned ? (low ? lane + P / 8 : lane - P / 8) : lane;
+    for (; chunk < until; chunk += WARPS) {
+        float2 w[4];
+        const float * wp = what == 0 ? a.q_norm : what == 1 ? a.k_norm : nullptr;
+        if (wp)
 #pragma unroll
-            for (int i = 0; i < 8; i += 2) q = fma2(make_float2(u[i], u[i + 1]), make_float2(u[i], u[i + 1]), q);
-            float ss = mine ? q.x + q.y : 0.0f;
+            for (int i = 0; i < 4; ++i) w[i] = mine ? make_float2(wp[at + 2 * i], wp[at + 2 * i + 1]) : make_float2(0.0f, 0.0f);
+        const tsn_heads & to = what == 1 ? a.c.k : a.c.v;
+        T * const out = what == 0 ? (T *) a.q_out.p + s0 * a.q_out.sb + head * a.q_out.st + at : (T *) to.p + head * to.sh + at;
+        auto target = [&](int k) {   // where token k goes; null: nowhere
+            if (what == 0) return spot[k] == -2 ? nullptr : out + k * a.q_out.sb;
+            return spot[k] < 0 ? nullptr : out + spot[k] * to.sb + slot[k] * to.ss;
+        };
+        for (int k0 = 0; k0 < here; k0 += AHEAD)
 #pragma unroll
-            for (int o = LPH >> 1; o; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
-            const float inv = rsqrtf(fmaf(ss, inv_D, a.eps));
-#pragma unroll
-            for (int i = 0; i < 8; i += 2) {
-                const float2 r = mul2(make_float2(u[i], u[i + 1]), mul2(w[i / 2], make_float2(inv, inv)));
-                u[i] = r.x;
-                u[i + 1] = r.y;
-            }
-        }
-        const float2 * tr = turn + k * row;
-        if (what == 2) {
-        } else if (PAIR == NEXT) {
-#pragma unroll
-            for (int i = 0; i < 8; i += 4) {
-                const int j = (at + i) >> 1;
-                const float4 cs = *(const float4 *) (tr + (j < row ? j : 0));
-                const float2 v = make_float2(u[i], u[i + 2]);
-                if (j < P) {
-                    u[i] = v.x * cs.x - u[i + 1] * cs.y;
-                    u[i + 1] = v.x * cs.y + u[i + 1] * cs.x;
+            for (int y = 0; y < AHEAD; ++y) {
+                const int k = k0 + y;
+                if (k >= here) break;
+                const Words<TX, 8> raw = ring[y];
+                if (mine && k + AHEAD < here) ring[y] = load_words<TX, 8>(x);
+                x += dx;
+                if (SAME && what == 2) {   // values go as they are
+                    T * const dst = target(k);
+                    if (mine && dst) *(uint4 *) dst = raw.w[0];
+                    continue;
                 }
-                if (j + 1 < P) {
-                    u[i + 2] = v.y * cs.z - u[i + 3] * cs.w;
-                    u[i + 3] = v.y * cs.w + u[i + 3] * cs.z;
-                }
-            }
-        } else if (PAIR == LANES) {
-            const bool low = at < P, turned = at < 2 * P;
-            const int other = turned ? (low ? lane + P / 8 : lane - P / 8) : lane;
-            const float4 * cs = (const float4 *) (tr + (turned ? (low ? at : at - P) : 0));
+                float u[8];
+                to_floats<TX, 8>(raw, u);
+                if (wp) {
+                    float2 q = make_float2(0.0f, 0.0f);
 #pragma unroll
-            for (int i = 0; i < 8; i += 2) {
-                const float4 c2 = cs[i / 2];
-                const float m0 = __shfl_sync(0xffffffffu, u[i], other), m1 = __shfl_sync(0xffffffffu, u[i + 1], other);
-                if (turned) {
-                    u[i] = fmaf(u[i], c2.x, low ? -m0 * c2.y : m0 * c2.y);
-                    u[i + 1] = fmaf(u[i + 1], c2.z, low ? -m1 * c2.w : m1 * c2.w);
-                }
-            }
-        } else {
-            float * m = mate[warp];
+                    for (int i = 0; i < 8; i += 2) q = fma2(make_float2(u[i], u[i + 1]), make_float2(u[i], u[i + 1]), q);
+                    float ss = mine ? q.x + q.y : 0.0f;
 #pragma unroll
-            for (int i = 0; i < 8; ++i) m[lane * 9 + i] = u[i];
-            __syncwarp();
-            const int base = lane & ~(LPH - 1);   // the head's first lane
+                    for (int o = LPH >> 1; o; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+                    const float inv = rsqrtf(fmaf(ss, inv_D, a.eps));
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                const int e = at + i;
-                if (e < 2 * P) {
-                    const int o = e < P ? e + P : e - P;
-                    const float v = m[(base + (o >> 3)) * 9 + (o & 7)];
-                    const float2 cs = tr[e < P ? e : e - P];
-                    u[i] = fmaf(u[i], cs.x, e < P ? -v * cs.y : v * cs.y);
+                    for (int i = 0; i < 8; i += 2) {
+                        const float2 r = mul2(make_float2(u[i], u[i + 1]), mul2(w[i / 2], make_float2(inv, inv)));
+                        u[i] = r.x;
+                        u[i + 1] = r.y;
+                    }
                 }
+                const float * tr = turn + k * 3 * row;
+                if (what == 2) {
+                } else if (PAIR == NEXT) {
+                    const int j = at >> 1;   // the lane's four pairs
+                    if (j < P) {
+                        const float4 c = *(const float4 *) (tr + j), s = *(const float4 *) (tr + row + j);
+                        const float cs[4] = {c.x, c.y, c.z, c.w}, sn[4] = {s.x, s.y, s.z, s.w};
+#pragma unroll
+                        for (int i = 0; i < 4; ++i)
+                            if (j + i < P) {
+                                const float v = u[2 * i];
+                                u[2 * i] = v * cs[i] - u[2 * i + 1] * sn[i];
+                                u[2 * i + 1] = v * sn[i] + u[2 * i + 1] * cs[i];
+                            }
+                    }
+                } else if (PAIR == LANES) {
+                    float m[8];
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) m[i] = __shfl_sync(0xffffffffu, u[i], other);
+                    if (turned) {
+                        const float * t = tr + (low ? at : at - P);
+                        const float * sines = t + (low ? 2 * row : row);
+#pragma unroll
+                        for (int i = 0; i < 8; i += 4) {
+                            const float4 c = *(const float4 *) (t + i), s = *(const float4 *) (sines + i);
+                            const float2 a0 = fma2(make_float2(m[i], m[i + 1]), make_float2(s.x, s.y), mul2(make_float2(u[i], u[i + 1]), make_float2(c.x, c.y)));
+                            const float2 a1 = fma2(make_float2(m[i + 2], m[i + 3]), make_float2(s.z, s.w), mul2(make_float2(u[i + 2], u[i + 3]), make_float2(c.z, c.w)));
+                            u[i] = a0.x;
+                            u[i + 1] = a0.y;
+                            u[i + 2] = a1.x;
+                            u[i + 3] = a1.y;
+                        }
+                    }
+                } else {
+                    float * m = mate[warp];
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) m[lane * 9 + i] = u[i];
+                    __syncwarp();
+                    const int base = lane & ~(LPH - 1);   // the head's first lane
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) {
+                        const int e = at + i;
+                        if (e < 2 * P) {
+                            const int o = e < P ? e + P : e - P, j = e < P ? e : e - P;
+                            u[i] = fmaf(m[(base + (o >> 3)) * 9 + (o & 7)], tr[(e < P ? 2 * row : row) + j], u[i] * tr[j]);
+                        }
+                    }
+                    __syncwarp();
+                }
+                T * const dst = target(k);
+                if (mine && dst) store_words<T, 8>(dst, u);
             }
-            __syncwarp();
-        }
-        if (!mine) continue;
-        if (what == 0) {
-            if (spot[k] != -2) store_words<T, 8>((T *) a.q_out.p + (s0 + k) * a.q_out.sb + head * a.q_out.st + at, u);
-        } else if (spot[k] >= 0) {
-            const tsn_heads & to = what == 1 ? a.c.k : a.c.v;
-            store_words<T, 8>((T *) to.p + spot[k] * to.sb + slot[k] * to.ss + head * to.sh + at, u);
+        if (chunk + WARPS < until) {
+            chunk += WARPS;
+            begin();
+            chunk -= WARPS;
         }
     }
 }
@@ -173,15 +208,19 @@ __global__ void __launch_bounds__(32 * WARPS) cache_means_kernel(const __grid_co
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, D = (int) a.c.D, Hk = (int) a.c.Hk;
     const int sub = lane / LPH, at = (lane & (LPH - 1)) * 8;
     const bool mine = at < D;
+    // a lane a token: whether it is its page's last, that page and the slot
     const long long s0 = (long long) blockIdx.x * n.tok;
-    const int here = (int) min((long long) n.tok, a.c.N - s0);
-    for (int k = 0; k < here; ++k) {
-        const int i = (int) s0 + k, b = seq_of_row(a.c, i);
-        if (b < 0) continue;
-        const int pl = place_of_row(a.c, b, i), slot = pl & ((1 << n.page_log2) - 1);
-        if (slot + 1 != (1 << n.page_log2) && i + 1 != seq_start(a.c, b + 1)) continue;
-        const int id = page_of(a.c, b, pl >> n.page_log2);
-        if (id < 0) continue;
+    int id_of = -1, slot_of = 0;
+    if (lane < n.tok && s0 + lane < a.c.N) {
+        const int i = (int) s0 + lane, b = seq_of_row_alone(a.c, i);
+        if (b >= 0) {
+            const int pl = place_of_row(a.c, b, i);
+            slot_of = pl & ((1 << n.page_log2) - 1);
+            if (slot_of + 1 == (1 << n.page_log2) || i + 1 == seq_start(a.c, b + 1)) id_of = page_of(a.c, b, pl >> n.page_log2);
+        }
+    }
+    for (uint32_t left = __ballot_sync(~0u, id_of >= 0); left; left &= left - 1) {
+        const int from = __ffs(left) - 1, id = __shfl_sync(~0u, id_of, from), slot = __shfl_sync(~0u, slot_of, from);
         for (int h = warp; h < Hk; h += WARPS) {
             const T * key = (const T *) a.c.k.p + id * a.c.k.sb + h * a.c.k.sh + at;
             float sum[8] = {};
@@ -218,9 +257,10 @@ cudaError_t launch(const tsn_rope_plan_t & p, Append & n, cudaStream_t s) {
     while (lph * 8 < (int) p.D) lph *= 2;
     const int side = 32 / lph, chunks = (int) ((a.Hq + side - 1) / side + 2 * ((a.c.Hk + side - 1) / side));
     const long long turns = (chunks + WARPS - 1) / WARPS;
-    // Tokens of a block: 8 share its start; fewer while four blocks per SM take them all.
-    n.tok = (int) std::min<long long>(MAX_TOK, ((long long) a.c.N * turns + 4 * 148 - 1) / (4 * 148));
-    const dim3 blocks((a.c.N + n.tok - 1) / n.tok, (unsigned) turns);
+    // Tokens of a block share its start; fewer while four blocks per SM take them all, and with few tokens their heads go to several.
+    n.span = (long long) a.c.N * turns <= 8 * 148 ? WARPS : chunks;
+    n.tok = (int) std::min<long long>(MAX_TOK, ((long long) a.c.N * (n.span == WARPS ? turns : 1) + 4 * 148 - 1) / (4 * 148));
+    const dim3 blocks((a.c.N + n.tok - 1) / n.tok, (unsigned) ((chunks + n.span - 1) / n.span));
     const int pair = p.layout == TSN_ROPE_INTERLEAVED ? NEXT : p.P % 8 == 0 ? LANES : SHARED;
     const int mean_tok = (int) std::max(1u, std::min(32u, a.c.N / 1024));
     cudaError_t e = cudaSuccess;
@@ -247,7 +287,7 @@ cudaError_t launch(const tsn_rope_plan_t & p, Append & n, cudaStream_t s) {
 
 int cache_append(DeviceCtx & c, const tsn_rope_plan_t & p, const tsn_cache_append_args & a) {
     if (a.c.N == 0 || a.c.B == 0) return TSN_OK;
-    Append n{a, log2_of(a.c.page), 1};
+    Append n{a, log2_of(a.c.page), 1, 1};
     if (!n.a.q.p) n.a.Hq = 0;
     const bool wide = a.xtype == TSN_F32;
     const cudaError_t e = a.c.type == TSN_F16 ? (wide ? launch<float, __half>(p, n, c.stream) : launch<__half, __half>(p, n, c.stream))

@@ -45,6 +45,19 @@ __device__ __forceinline__ int seq_of_row(const tsn_paged & c, int row) {
     return row < c.q_start[lo + 1] ? lo : -1;
 }
 
+// The same by a single thread.
+__device__ __forceinline__ int seq_of_row_alone(const tsn_paged & c, int row) {
+    if (!c.q_start) return row < (int) c.N ? row : -1;
+    if (c.q_start[0] > row) return -1;
+    int lo = 0, hi = (int) c.B;   // the last start that is not above the row lies in lo .. hi - 1
+    while (hi - lo > 1) {
+        const int mid = (lo + hi) >> 1;
+        if (c.q_start[mid] <= row) lo = mid;
+        else hi = mid;
+    }
+    return row < c.q_start[lo + 1] ? lo : -1;
+}
+
 // The place of a row of sequence b among its tokens: len - n + i, kept within 32 bits.
 __device__ __forceinline__ int place_of_row(const tsn_paged & c, int b, int row) {
     const long long p = (long long) c.len[b] - seq_start(c, b + 1) + row;
