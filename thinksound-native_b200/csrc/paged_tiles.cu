@@ -466,35 +466,54 @@ paged_tiles_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant
                 dst[D + 1] = l;
             }
             cluster_sync_all();
-            // this CTA's share of the rows, a warp a row, D / 32 columns a lane
-            constexpr int E = D / 32;
-            const int share = (R + p.parts - 1) / p.parts, from = (int) split * share, until = min(R, from + share);
-            for (int r = from + warp; r < until && !*abort_flag; r += 8) {
-                const uint32_t at = smem_u32(sums + r * L::SUM_ROW);
-                float f[8], top = -INFINITY, sum = 0.0f, o[E] = {}, v[8][4];
+            // this CTA's share of the rows: first each part's factors, 2^(ref - greatest) / l, in Q's place, then the parts' sums, a
+            // row by D / 4 lanes, four steps of rows at once
+            const int share = (R + p.parts - 1) / p.parts, from = (int) split * share, here = max(0, min(R - from, share));
+            const uint32_t at0 = smem_u32(sums + from * L::SUM_ROW);
+            float * fac = (float *) smem;   // [row][8 parts]
+            if (tid < here) {
+                float ref_of[8], top = -INFINITY, sum = 0.0f;
                 float4 st[8];
 #pragma unroll
                 for (int i = 0; i < 8; ++i)
                     if (i < p.parts) {
-                        st[i] = dsmem_ld4(dsmem_map(at + D * 4, (uint32_t) i));
-                        const float4 x = dsmem_ld4(dsmem_map(at + (E * lane / 4) * 16, (uint32_t) i));
-                        if (E == 4) { v[i][0] = x.x; v[i][1] = x.y; v[i][2] = x.z; v[i][3] = x.w; }
-                        else { v[i][0] = lane & 1 ? x.z : x.x; v[i][1] = lane & 1 ? x.w : x.y; }
+                        st[i] = dsmem_ld4(dsmem_map(at0 + (tid * L::SUM_ROW + D) * 4, (uint32_t) i));
                         top = fmaxf(top, st[i].x);
                     }
                 const float low = top == -INFINITY ? 0.0f : top;
 #pragma unroll
                 for (int i = 0; i < 8; ++i)
                     if (i < p.parts) {
-                        f[i] = ex2(st[i].x - low);
-                        sum += f[i] * st[i].y;
-#pragma unroll
-                        for (int e = 0; e < E; ++e) o[e] = fmaf(f[i], v[i][e], o[e]);
+                        ref_of[i] = ex2(st[i].x - low);
+                        sum += ref_of[i] * st[i].y;
                     }
                 const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
-                uint16_t * out = address(p.out, r) + E * lane;
-                if constexpr (E == 4) *(uint2 *) out = sum == 0.0f ? make_uint2(0, 0) : make_uint2(pack16<BF16>(o[0] * inv, o[1] * inv), pack16<BF16>(o[2] * inv, o[3] * inv));
-                else *(uint32_t *) out = sum == 0.0f ? 0u : pack16<BF16>(o[0] * inv, o[1] * inv);
+#pragma unroll
+                for (int i = 0; i < 8; ++i)
+                    if (i < p.parts) fac[tid * 8 + i] = ref_of[i] * inv;
+            }
+            bar_n(3, 256);
+            constexpr int LANES = D / 4, STEP = 8 * (32 / LANES), AT_ONCE = 4;   // lanes of a row; rows of a step of all warps
+            const int col = (lane % LANES) * 4;
+            for (int y0 = warp * (32 / LANES) + lane / LANES; y0 < here; y0 += STEP * AT_ONCE) {
+                float o[AT_ONCE][4] = {};
+                for (int i = 0; i < p.parts; ++i)
+#pragma unroll
+                    for (int y = 0; y < AT_ONCE; ++y) {
+                        const int r = y0 + y * STEP;
+                        if (r < here) {
+                            const float4 v = dsmem_ld4(dsmem_map(at0 + (r * L::SUM_ROW + col) * 4, (uint32_t) i));
+                            const float f = fac[r * 8 + i];
+                            o[y][0] = fmaf(f, v.x, o[y][0]); o[y][1] = fmaf(f, v.y, o[y][1]);
+                            o[y][2] = fmaf(f, v.z, o[y][2]); o[y][3] = fmaf(f, v.w, o[y][3]);
+                        }
+                    }
+#pragma unroll
+                for (int y = 0; y < AT_ONCE; ++y) {
+                    const int r = y0 + y * STEP;
+                    if (r < here && !*abort_flag)
+                        *(uint2 *) (address(p.out, from + r) + col) = make_uint2(pack16<BF16>(o[y][0], o[y][1]), pack16<BF16>(o[y][2], o[y][3]));
+                }
             }
             cluster_sync_all();   // nobody leaves while its sums are read
         } else {
@@ -576,16 +595,18 @@ cudaError_t configure_paged_tiles() {
 cudaError_t launch_paged_tiles(PagedArgs p, cudaStream_t s) {
     // units at most: a sequence has a last one that is not full
     const long long rows = (long long) p.c.N * p.G, units = std::min<long long>(p.c.N, rows / ROWS + p.c.B) * p.c.Hk;
-    // As many parts of a cluster as take the least time, in microseconds: start and end of a CTA 6, a tile of 128-wide heads 2 and of
-    // 64-wide ones 1.7, adding up the parts 3; clusters of one size run g_clusters[size] at a time. Four key tiles a part at least, eight
-    // parts at most (the largest portable cluster). The keys are what the tables have room for: lengths are on the device.
+    // As many parts of a cluster as take the least time, in microseconds: start and end of a CTA 5, a tile of 128-wide heads 2 and of
+    // 64-wide ones 1.7; with parts 4 to add them up and 5 for each wave of clusters; g_clusters[size] run at a time. Four
+    // key tiles a part at least, eight parts at most (the largest portable cluster). The keys are what the tables have room for: lengths
+    // are on the device. us in 1, 2, 4 and 8 parts: 64 tokens x 4 heads of 128 over 32 768 keys, 8 kv heads 448, 234, 125, 78; 4 x 517
+    // tokens x 3 heads of 64 with a window of 2000, 8 kv heads, 69, 85, 128, 235.
     long long keys = (long long) p.c.M << p.page_log2;
     if (p.window) keys = std::min<long long>(keys, (long long) p.window + ROWS);
     const long long tiles = (keys + KEYS - 1) / KEYS;
     double least = 0.0;
     for (int parts = 1; parts <= 8 && (parts == 1 || parts * 4 <= tiles); ++parts) {
         const long long room = std::max(1, g_clusters[parts].load(std::memory_order_relaxed));
-        const double cost = (double) ((units + room - 1) / room) * (6.0 + (double) ((tiles + parts - 1) / parts) * (p.c.D == 64 ? 1.7 : 2.0)) + (parts > 1 ? 3.0 : 0.0);
+        const double cost = (double) ((units + room - 1) / room) * (5.0 + (parts > 1 ? 5.0 : 0.0) + (double) ((tiles + parts - 1) / parts) * (p.c.D == 64 ? 1.7 : 2.0)) + (parts > 1 ? 4.0 : 0.0);
         if (parts == 1 || cost < least) { least = cost; p.parts = parts; }
     }
     if (units * p.parts > 0x7fffffffLL) return cudaErrorInvalidValue;
