@@ -245,3 +245,76 @@ def test_two_streams(dev):
             assert within(outs[i][r], *wants[i])
     for d in devs:
         d.close()
+
+
+def test_graphs_side_by_side(dev):
+    """Captured calls whose keys are split, replayed on two streams at once beside eager calls of this handle and of differential
+    attention, which share its workspace."""
+    batches = [Batch([1], [26000 - 7000 * i], page=64, D=128, Hk=1, seed=i) for i in range(3)]
+    qs = [b.rows(8) for b in batches]
+    wants = [attention(b, q) for b, q in zip(batches, qs)]
+    outs = [torch.empty_like(q) for q in qs]
+    op = tsn.PagedAttention(dev, 128)
+    call = lambda i: op(qs[i], batches[i].k, batches[i].v, batches[i].table, batches[i].lens, outs[i], q_start=batches[i].q_start, most=1)  # noqa: E731
+    lam = 0.1 * torch.ones(64, device="cuda")
+    diff = tsn.DiffAttention(dev, 64, lam, lam, lam, lam, lambda_init=0.3)
+    k = torch.randn(1, 20000, 2, 128, device="cuda").bfloat16()
+    dq, dout = torch.randn(1, 1, 8, 128, device="cuda").bfloat16(), torch.empty(1, 1, 8, 128, dtype=torch.bfloat16, device="cuda")
+    diff(dq, k, k, dout)
+    dev.commit()
+    dwant = dout.clone()
+    graphs, streams = [], [torch.cuda.Stream() for _ in range(2)]
+    for i in range(2):
+        tsn.check(tsn.lib().tsn_device_set_stream(dev.h, streams[i].cuda_stream))
+        graphs.append(torch.cuda.CUDAGraph())
+        with torch.cuda.graph(graphs[i], stream=streams[i]):
+            call(i)
+    tsn.check(tsn.lib().tsn_device_set_stream(dev.h, torch.cuda.current_stream().cuda_stream))
+    for o in outs + [dout]:
+        o.fill_(3.0)
+    torch.cuda.synchronize()
+    for _ in range(20):
+        for i in range(2):
+            with torch.cuda.stream(streams[i]):
+                graphs[i].replay()
+        call(2)
+        diff(dq, k, k, dout)
+    dev.commit()
+    torch.cuda.synchronize()
+    for i in range(3):
+        assert within(outs[i], *wants[i])
+    assert torch.equal(dout, dwant)
+
+
+def test_captured_twice_and_first_calls(dev):
+    """The first call of a handle may be a captured one; sequences without tokens and rows without a sequence stay as they are."""
+    stream = torch.cuda.Stream()
+    own = tsn.Device(0, stream=stream.cuda_stream)
+    batch = Batch([0, 3, 0], [50, 9000, 0], page=32, D=64, Hk=1, extra=2)
+    q = batch.rows(4)
+    out, op, graph = torch.full_like(q, 3.0), tsn.PagedAttention(own, 64), torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph, stream=stream):
+        op(q, batch.k, batch.v, batch.table, batch.lens, out, q_start=batch.q_start, most=3)
+        op(q, batch.k, batch.v, batch.table, batch.lens, out, q_start=batch.q_start, most=3)
+    graph.replay()
+    torch.cuda.synchronize()
+    want, bound = attention(batch, q)
+    assert within(out[:3], want[:3], bound[:3]) and bool((out[3:] == 3.0).all())
+    del graph
+    own.close()
+
+
+def test_starts_that_are_none(dev):
+    """Starts that do not ascend, or lie outside the rows, touch nothing outside the results; the other sequences are right."""
+    for n in (2, 60):
+        batch = Batch([n, n, n], [300, 200, 100], page=16, D=64, Hk=2)
+        q = batch.rows(4)
+        want, bound = attention(batch, q)
+        for starts in ([0, n, 2 * n, 2 ** 31 - 1], [-7, n, 2 * n, 3 * n + 1], [0, n, n - 1, n - 1]):
+            ids = torch.tensor(starts, dtype=torch.int32, device="cuda")
+            room = torch.full((3 * n + 8, 4, 64), 3.0, dtype=q.dtype, device="cuda")
+            tsn.PagedAttention(dev, 64)(q, batch.k, batch.v, batch.table, batch.lens, room[4:-4], q_start=ids, most=n)
+            dev.commit()
+            assert bool((room[:4] == 3.0).all()) and bool((room[-4:] == 3.0).all())
+            assert within(room[4:4 + n], want[:n], bound[:n])

@@ -530,8 +530,10 @@ paged_rows_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant_
             fence_proxy_async_smem();   // the sums were written where the next copies land
             if (++unit == s.units) {
                 unit = 0;
-                do s = sequence<ROWS>(p, ++b);
-                while (s.units == 0);
+                do {
+                    if (++b >= (int) p.c.B) return;   // (not reached while lengths and starts stay what they were)
+                    s = sequence<ROWS>(p, b);
+                } while (s.units == 0);
             }
             __syncthreads();
         }

@@ -2,8 +2,8 @@
 //
 //   o = sum_j p_j v_j / l,  l = sum_j p_j,  p_j = 2^(c q.k_j - ref)
 // in one pass over the keys; ref follows the row's running maximum and moves, with o and l rescaled, when that has grown by more than
-// 2^8. P is rounded to 16 bits, as the tensor cores take it, and l is the sum of the rounded ones, so that rounding cancels for a key
-// that dominates; scores, maxima, sums and o are f32.
+// 2^8. P is rounded to 16 bits, as the tensor cores take it; scores, maxima, sums and o are f32, and l is the sum before the rounding: the
+// rounded ones would take a mixed add a value instead of a packed one for two.
 // A unit is 256 query rows of a sequence and kv head, (token, head of the group), as two tiles of 128, so that heads of a group share
 // the keys; a CTA takes a unit or, where there are few, a part of its keys, the parts of a cluster adding up their sums. 384 threads:
 //   warps 0-3, 4-7  softmax of a tile, one row a thread: S from TMEM, mask, maximum, exponentials, P over S's columns
@@ -425,8 +425,6 @@ paged_tiles_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant
             tc_fence_after();
             tile(j);
         }
-        // no score above -inf: the FMA pipe's exponentials gave its keys 2^-126 each
-        if (ref == -INFINITY && l < INFINITY) l = 0.0f;
         if (ok && ja < jb) ok = mbar_wait_soon(&o_full[t], 0, abort_flag, p.err, DEV_TIMEOUT_TMEM);
         __syncwarp();
         tc_fence_after();
