@@ -6,7 +6,7 @@
 // side: S^T = K Q^T, O^T = V^T P^T; P^T is S^T's layout transposed in registers. Each warp streams 16-key slabs of its own by TMA,
 // a page holding whole slabs, through a ring of its own; the warps' sums meet in shared memory.
 // A unit is a kv head with up to 8 NT rows of a sequence, and its slabs. Lengths are on the device, so the device deals
-// them out: all units' slabs in a row, an equal share for each CTA; one of eight warps or two of four fill an SM. A share may begin and end
+// them out: all units' slabs in a row, an equal share for each CTA; one of eight warps or two or three of four fill an SM. A share may begin and end
 // inside a unit; the CTA that is the last of a unit to arrive adds up its parts, in their order. Units of few slabs are not cut:
 // a trip through the workspace costs more.
 #include "kernels.h"
@@ -23,18 +23,21 @@ constexpr float LAZY = 8.0f;   // log2 units that a maximum may grow before o is
 // Slabs of a share at least, slabs up to which a unit is not cut, parts of a unit at most (fewer slabs a part otherwise). One token, 8 kv
 // heads of 128, 2 x 1000 keys: with units of up to 32 slabs whole 15.7 us, 64: 12.1.
 constexpr int LEAST = 16, SHORT = 64, MOST_PARTS = 64;
-// Units up to which eight warps share one, a CTA an SM; above, two CTAs of four warps an SM, of which one loads while the
-// other adds up its unit's sums. us by eight / by four: 16 units of 704 keys 8.0/10.5, 8 of 1000 12.1/16.5, one of 32 768 15.7/21.7, 192 of
+// Units up to which eight warps share one, a CTA an SM; above, two or three CTAs of four warps an SM, of which one loads while
+// another adds up its unit's sums. us by eight / by four (two CTAs): 16 units of 704 keys 8.0/10.5, 8 of 1000 12.1/16.5, one of 32 768 15.7/21.7, 192 of
 // 8191 142/148, but 256 of 1000 29.4/27.1, 1024 of 300 45.5/38.2.
 constexpr long long FEW_UNITS = 200;
 
-template <int D, int NT, int W>
+template <int D, int NT, int W, bool LIST>
 struct RowLay {
-    static constexpr int BOX = SLAB * 128, HALF = SLAB * D * 2, STAGE = 2 * HALF, RING = D == 128 ? 3 : 6;   // a slab's keys, then its values
+    // CTAs of an SM: three with two slabs a ring start and end beside one another where two with three do so less (400 tokens x 4
+    // kv heads, 16 pages of 64: 71 and 97 us; 64 tokens over 1500 keys, 8 kv heads of 64, 46.8 and 55.5), but 16 rows do not fit in
+    // the registers of three (4 tokens over 1000 keys, 64 streams: 94.8 and 57.4).
+    static constexpr int CTAS = W == 8 ? 1 : LIST || NT == 1 ? 3 : 2;
+    static constexpr int BOX = SLAB * 128, HALF = SLAB * D * 2, STAGE = 2 * HALF, RING = (CTAS == 3 ? 2 : 3) * (128 / D);   // a slab's keys, then its values
     static constexpr int ROWS = 8 * NT, ROW = D + 4;   // words of a row's sums: o, ref, l
     static constexpr int OFF_BAR = W * RING * STAGE, TOTAL = OFF_BAR + W * RING * 8 + 64;
     static_assert(ROWS * ROW * 4 <= RING * STAGE, "a warp's sums fit in its ring");
-    static constexpr int CTAS = W == 4 ? 2 : 1;   // on an SM
     static_assert(CTAS * (TOTAL + 2048) <= 228 * 1024, "they fit");
 };
 constexpr int part_words(int D, int rows) { return rows * (D + 4); }
@@ -62,9 +65,9 @@ __device__ __forceinline__ Seq sequence(const PagedArgs & p, int b) {
 }
 
 template <int D, bool BF16, int NT, bool LIST, int W>
-__global__ void __launch_bounds__(32 * W, W == 4 ? 2 : 1)
+__global__ void __launch_bounds__(32 * W, RowLay<D, NT, W, LIST>::CTAS)
 paged_rows_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant__ CUtensorMap tv, const __grid_constant__ PagedArgs p) {
-    using L = RowLay<D, NT, W>;
+    using L = RowLay<D, NT, W, LIST>;
     constexpr int E = D / 32, RING = L::RING, ROWS = L::ROWS;
     extern __shared__ __align__(1024) uint8_t smem[];
     __shared__ int first_seq, first_off;
@@ -549,7 +552,7 @@ template <int D, bool BF16, int NT, bool LIST, int W>
 cudaError_t launch(const PagedArgs & p, unsigned grid, cudaStream_t s) {
     CUtensorMap tk{}, tv{};
     if (!make_page_maps(p.c, SLAB, &tk, &tv)) return cudaErrorInvalidValue;
-    return launch_cl(paged_rows_kernel<D, BF16, NT, LIST, W>, dim3(grid), dim3(32 * W), RowLay<D, NT, W>::TOTAL, s, dim3(1), tk, tv, p);
+    return launch_cl(paged_rows_kernel<D, BF16, NT, LIST, W>, dim3(grid), dim3(32 * W), RowLay<D, NT, W, LIST>::TOTAL, s, dim3(1), tk, tv, p);
 }
 template <int D, bool BF16, int NT>
 cudaError_t launch(const PagedArgs & p, int warps, unsigned grid, cudaStream_t s) {
@@ -574,7 +577,7 @@ Plan plan_of(const PagedArgs & p, uint32_t most) {
     if (p.chosen || !p.c.q_start) r.units = (long long) p.c.N * ((p.G + rows - 1) / rows) * p.c.Hk;
     else r.units = std::min((long long) p.c.N * ((p.G + rows - 1) / rows), (long long) p.c.N * p.G / rows + p.c.B) * p.c.Hk;
     r.warps = r.units <= FEW_UNITS ? 8 : 4;
-    r.ctas = r.warps == 8 ? SMS : 2 * SMS;
+    r.ctas = r.warps == 8 ? SMS : r.nt == 1 ? 3 * SMS : 2 * SMS;   // as the kernels' launch bounds have it
     return r;
 }
 
@@ -615,8 +618,8 @@ cudaError_t configure_paged_rows() {
         if (e == cudaSuccess) e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
     };
 #define SET(D, B, NT, W) \
-    set(paged_rows_kernel<D, B, NT, false, W>, RowLay<D, NT, W>::TOTAL); \
-    set(paged_rows_kernel<D, B, NT, true, W>, RowLay<D, NT, W>::TOTAL);
+    set(paged_rows_kernel<D, B, NT, false, W>, RowLay<D, NT, W, false>::TOTAL); \
+    set(paged_rows_kernel<D, B, NT, true, W>, RowLay<D, NT, W, true>::TOTAL);
     SET(64, false, 1, 4) SET(64, false, 2, 4) SET(64, true, 1, 4) SET(64, true, 2, 4)
     SET(128, false, 1, 4) SET(128, false, 2, 4) SET(128, true, 1, 4) SET(128, true, 2, 4)
     SET(64, false, 1, 8) SET(64, false, 2, 8) SET(64, true, 1, 8) SET(64, true, 2, 8)
