@@ -6,7 +6,7 @@
 // right by 3 into the high word, which is the value times 2^-896 exactly, subnormals and zero included (a conversion
 // instruction has a quarter of the FMAs' rate); q carries a factor of 2^880 against it. Factors that all scores share change no order.
 //
-// Scores: D / 8 lanes read a mean, a warp eight means a lane at once and the next eight ahead; partial sums are exchanged so that each
+// Scores: D / 8 lanes read a mean, a warp eight means a lane at once (four for four tokens) and the next ones ahead; partial sums are exchanged so that each
 // lane ends with whole ones. A block takes one token and kv head, or, where there are many tokens, four neighbouring ones,
 // which share the reads while they are of one sequence.
 // Picks: scores, rounded to f32, which keeps their order but for ties, are counted in bins of equal width between the least and the
@@ -49,7 +49,7 @@ __device__ __forceinline__ void scaled(uint32_t w, double & a, double & b) {
 template <int GT>
 struct Group {
     static constexpr int WARPS = GT / 32, BINS = 4 * GT, FEW = 64;   // FEW: scores that are ranked, each against the others
-    static constexpr int LOG_BINS = GT == 64 ? 8 : 11;
+    static constexpr int LOG_BINS = GT == 128 ? 9 : 11;
     static_assert(1 << LOG_BINS == BINS, "bins");
     int id, tid, lane, warp;
     struct Space {
@@ -257,10 +257,11 @@ struct Group {
 // TOK tokens of a block, GT threads for each in the end.
 template <class T, int D, int TOK, int GT>
 __global__ void __launch_bounds__(TOK * GT, 1) page_select_kernel(const __grid_constant__ Select p) {
-    constexpr int THREADS = TOK * GT, LPH = D / 8, SIDE = 32 / LPH, BATCH = 8;   // BATCH: means of a lane at once
+    constexpr int THREADS = TOK * GT, LPH = D / 8, SIDE = 32 / LPH, BATCH = TOK == 1 ? 8 : 4;   // BATCH: means of a lane at once
+    constexpr int SUMS = TOK * BATCH, KEPT = SUMS > LPH ? SUMS / LPH : 1, SAME = LPH > SUMS ? LPH / SUMS : 1;   // of a lane; in the end; lanes with the same
     extern __shared__ __align__(16) double scores[];   // [TOK][M], then the same in f32
     __shared__ typename Group<GT>::Space space[TOK];
-    __shared__ __align__(16) double qs[TOK][D];
+    __shared__ __align__(16) double qs[TOK][4][LPH][2];   // a lane's four pairs of elements, neighbouring lanes side by side
     __shared__ int seq[TOK], place[TOK];
     const tsn_sparse_attn_args & a = p.a;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, parts = TOK > 1 ? 1 : p.parts, part = TOK > 1 ? 0 : (int) blockIdx.x % parts,
@@ -286,7 +287,7 @@ __global__ void __launch_bounds__(TOK * GT, 1) page_select_kernel(const __grid_c
                 for (int y = 0; y < 4; ++y) s += (double) to_f32(v[y]);
             }
         }
-        qs[t][e] = s * 0x1p880;
+        qs[t][e / 2 % 4][e / 8][e % 2] = s * 0x1p880;
     }
     __syncthreads();
     pdl_trigger();
@@ -308,11 +309,6 @@ __global__ void __launch_bounds__(TOK * GT, 1) page_select_kernel(const __grid_c
             if (pages_of(t) > picks) top = max(top, pages_of(t) - (int) a.last);
         const int m = top - first;
         const int * table = a.c.table + b * a.c.table_sb;
-        double q[TOK][8];
-#pragma unroll
-        for (int t = 0; t < TOK; ++t)
-#pragma unroll
-            for (int e = 0; e < 8; ++e) q[t][e] = qs[t][e0 + e];
         // lane (sub, l) reads its 8 elements of means j0 + sub * BATCH + y. No page: zeros
         const int STEP = THREADS / 32 * (BATCH * SIDE) * parts;
         const int ahead = first + sub * BATCH + lane % BATCH;
@@ -332,38 +328,46 @@ __global__ void __launch_bounds__(TOK * GT, 1) page_select_kernel(const __grid_c
             continue;
         }
         auto sums = [&](int j0, int x) {
-            const int mine = j0 + ahead;
-            double s[TOK][BATCH];
+            double s[SUMS];   // token t, mean y at t * BATCH + y
 #pragma unroll
-            for (int y = 0; y < BATCH; ++y) {
-                const uint32_t * w = (const uint32_t *) r[x][y].w;
-                double u[8];
+            for (int i = 0; i < SUMS; ++i) s[i] = 0.0;
 #pragma unroll
-                for (int e = 0; e < 4; ++e) scaled<T>(w[e], u[2 * e], u[2 * e + 1]);
+            for (int e = 0; e < 4; ++e) {
+                double2 q[TOK];
 #pragma unroll
-                for (int t = 0; t < TOK; ++t) {
-                    s[t][y] = q[t][0] * u[0];
+                for (int t = 0; t < TOK; ++t) q[t] = *(const double2 *) qs[t][e][lane % LPH];
 #pragma unroll
-                    for (int e = 1; e < 8; ++e) s[t][y] = fma(q[t][e], u[e], s[t][y]);
+                for (int y = 0; y < BATCH; ++y) {
+                    double u, v;
+                    scaled<T>(((const uint32_t *) r[x][y].w)[e], u, v);
+#pragma unroll
+                    for (int t = 0; t < TOK; ++t) s[t * BATCH + y] = fma(q[t].y, v, fma(q[t].x, u, s[t * BATCH + y]));
+                }
+            }
+            // The lanes' parts of the sums are added up while each lane keeps half of them, then half of these: the lanes' bits, from the
+            // highest down, are the sums' that it ends with.
+            int n = SUMS;
+#pragma unroll
+            for (int o = LPH / 2; o; o >>= 1) {
+                const bool up = (lane & o) != 0;
+                if (n > 1) {
+                    n /= 2;
+#pragma unroll
+                    for (int i = 0; i < SUMS / 2; ++i)
+                        if (i < n) {
+                            const double give = up ? s[i] : s[i + n], keep = up ? s[i + n] : s[i];
+                            s[i] = keep + __shfl_xor_sync(~0u, give, o);
+                        }
+                } else {
+                    s[0] += __shfl_xor_sync(~0u, s[0], o);
                 }
             }
 #pragma unroll
-            for (int t = 0; t < TOK; ++t) {
-                // lane l of the mean's lanes ends with the sum of mean l % 8
-                if (LPH == 16)
-#pragma unroll
-                    for (int y = 0; y < BATCH; ++y) s[t][y] += __shfl_xor_sync(~0u, s[t][y], 8);
-#pragma unroll
-                for (int o = 4; o; o >>= 1)
-#pragma unroll
-                    for (int y = 0; y < o; ++y) {
-                        const bool up = (lane & o) != 0;
-                        const double give = up ? s[t][y] : s[t][y + o], keep = up ? s[t][y + o] : s[t][y];
-                        s[t][y] = keep + __shfl_xor_sync(~0u, give, o);
-                    }
-                if (mine < top && (lane % LPH) < BATCH && t >= t0 && t < t1) {
+            for (int k = 0; k < KEPT; ++k) {
+                const int i = lane % LPH / SAME * KEPT + k, t = i / BATCH, y = i % BATCH, mine = j0 + first + sub * BATCH + y;
+                if (mine < top && lane % SAME == 0 && t >= t0 && t < t1) {
                     // numbers that bins can be made of: NaN and what exceeds 2^1000 (of queries that are not finite) at the ends
-                    const double v = (there[x] >> (lane % BATCH)) & 1u ? fmin(fmax(s[t][0], -0x1p1000), 0x1p1000) + 0.0 : 0.0;   // -0 becomes 0
+                    const double v = (there[x] >> y) & 1u ? fmin(fmax(s[k], -0x1p1000), 0x1p1000) + 0.0 : 0.0;   // -0 becomes 0
                     const float f = fminf(fmaxf((float) v, -FLT_MAX), FLT_MAX);
                     const int at = t * (int) a.c.M + mine - first;
                     if (TOK > 1 || parts == 1) {
@@ -420,7 +424,7 @@ cudaError_t launch(const Select & p, cudaStream_t s) {
     const size_t bytes = (size_t) p.a.c.M * 12;
     // Four tokens a block share the reads; single ones fill the GPU with fewer tokens, and hold the scores of more pages.
     if ((long long) p.a.c.N * p.a.c.Hk >= 2 * MANY * 148 && MANY * bytes <= MOST)
-        return launch_cl(page_select_kernel<T, D, MANY, 64>, dim3((p.a.c.N + MANY - 1) / MANY, p.a.c.Hk), dim3(MANY * 64), MANY * bytes, s, dim3(1), p);
+        return launch_cl(page_select_kernel<T, D, MANY, 128>, dim3((p.a.c.N + MANY - 1) / MANY, p.a.c.Hk), dim3(MANY * 128), MANY * bytes, s, dim3(1), p);
     // As many blocks for a token as there are SMs for, up to four, each with 512 pages or more.
     Select one = p;
     while (one.parts < 4 && (long long) p.a.c.N * p.a.c.Hk * one.parts * 2 <= 148 && p.a.c.M >= 1024u * one.parts) one.parts *= 2;
@@ -445,10 +449,10 @@ cudaError_t configure_page_select() {
     set(page_select_kernel<__half, 128, 1, 512>);
     set(page_select_kernel<__nv_bfloat16, 64, 1, 512>);
     set(page_select_kernel<__nv_bfloat16, 128, 1, 512>);
-    set(page_select_kernel<__half, 64, MANY, 64>);
-    set(page_select_kernel<__half, 128, MANY, 64>);
-    set(page_select_kernel<__nv_bfloat16, 64, MANY, 64>);
-    set(page_select_kernel<__nv_bfloat16, 128, MANY, 64>);
+    set(page_select_kernel<__half, 64, MANY, 128>);
+    set(page_select_kernel<__half, 128, MANY, 128>);
+    set(page_select_kernel<__nv_bfloat16, 64, MANY, 128>);
+    set(page_select_kernel<__nv_bfloat16, 128, MANY, 128>);
     return e;
 }
 
