@@ -5,6 +5,10 @@
 // lane, loads some ahead. What the cache adds is a chain of small reads for each token (its sequence, length and page), a lane
 // a token, while the heads' loads are on their way.
 // The means of the pages are a second kernel, which reads the touched pages' keys after the first has written them.
+// 37 000 tokens x 48 heads of 128, bf16, with means take 215 us (986 MB, 4.6 TB/s, 0.70 of the measured copy), 191 of them the first
+// kernel: half reads, half writes, at 130 instructions a warp's 512 bytes and 64 registers; 3136 tokens from f32 12 to 16 us
+// (3.5 to 4.7 TB/s), 256 tokens with means 10 to 11 us, 4 tokens 4.9 us (the call).
+// Loads two tokens ahead: with four 254 us, with one 232; 8 tokens a block: with 16 218, with 4 227.
 #include <algorithm>
 #include <type_traits>
 

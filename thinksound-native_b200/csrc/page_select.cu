@@ -12,6 +12,9 @@
 // Picks: scores, rounded to f32, which keeps their order but for ties, are counted in bins of equal width between the least and the
 // greatest; the bin that the last pick falls into is taken apart again, by their bits, until few scores are left, and these are ranked against one
 // another in 64 bits. (Where more agree in 32 bits, the same goes on in 64.) The picks are written in the order of the pages.
+// 8 tokens x 8 kv heads over 2048 pages take 20 us (two blocks a token), 400 tokens x 4 over 600 pages 55 us: instructions, about
+// half of them FMAs' and conversions', the rest exchanges and the picks' small steps. Reads under branches took 2.4 times
+// as long, scores sorted by radix with a 64-bit compare 2 to 3 times.
 #include "kernels.h"
 #include "paged.h"
 #include "ptx.cuh"

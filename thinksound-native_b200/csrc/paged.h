@@ -28,7 +28,7 @@ __device__ __forceinline__ int seq_start(const tsn_paged & c, int b) {
     return c.q_start ? max(0, min(c.q_start[b], (int) c.N)) : b;
 }
 
-// The sequence of a row, by a whole warp; -1: none. 33 sequences a step.
+// The sequence of a row, by a whole warp; -1: none. A step leaves a 32nd of the sequences.
 __device__ __forceinline__ int seq_of_row(const tsn_paged & c, int row) {
     if (!c.q_start) return row < (int) c.N ? row : -1;
     const int lane = threadIdx.x & 31;

@@ -26,9 +26,6 @@ PagedArgs args_of(const DeviceCtx & c, const tsn_paged & cache, uint32_t H, floa
     return p;
 }
 
-// Rows of a kv head up to which groups of 8 or 16 are taken
-constexpr uint64_t FEW = 32;
-
 // The few-rows kernel with what it needs of the workspace.
 int few_rows(DeviceCtx & c, const char * name, PagedArgs & p, uint32_t most) {
     size_t groups = 0, bytes = 0;
@@ -83,7 +80,11 @@ int paged_attn(DeviceCtx & c, const tsn_paged_attn_args & a) {
     p.causal = a.causal != 0;
     p.window = (int) a.window;
     const uint32_t most = !a.c.q_start ? 1 : a.most ? std::min(a.most, a.c.N) : a.c.N;
-    if ((uint64_t) most * p.G <= FEW) return few_rows(c, "tsn_paged_attn", p, most);
+    // Up to eight rows of a kv head go to the kernel for few; beyond, the one that the estimates of both prefer: groups of rows read
+    // the keys anew, but go to every SM where a tile's keys have eight at most. us by groups / by tiles, heads of 128, bf16:
+    // 16 tokens x 4 heads, 8 kv heads over 8192 keys 37/24; 16 streams of 4 tokens over 4096 56/60, of 8 tokens 95/61; 64 streams of 4
+    // over 1000 57/78, of 8 164/79; one kv head over 32 768 keys, 64 rows 29/60, 128 rows 35/61.
+    if ((uint64_t) most * p.G <= 8 || paged_rows_cost(p, most) < plan_paged_tiles(p, most)) return few_rows(c, "tsn_paged_attn", p, most);
     const cudaError_t e = launch_paged_tiles(p, c.stream);
     if (e == cudaSuccess) return TSN_OK;
     cudaGetLastError();

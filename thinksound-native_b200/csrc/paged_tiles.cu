@@ -14,6 +14,15 @@
 // Values behind keys that are not there may be NaN, and 0 * NaN is NaN: those rows of V are cleared. Where rows differ in what they
 // see, values that are not finite are cleared too and added again to the rows that do see them.
 // Every wait is bounded; barriers of a whole block or cluster are on paths that all threads take.
+// What bounds it: 256 rows x 128 keys of 128 elements are 2048 cycles of the tensor cores (both products at 64 cycles an instruction of
+// 128 x 128 x 16, measured alone) and 1790 of the SFU (16 exponentials a cycle, one pair of eight on the FMA pipe). A tile's way is
+// 170 cycles for S to arrive, 280 for the maximum, 1220 for the exponentials, 150 to hand P over, then its products: the two tiles'
+// ways interleave at about 3800 cycles. 4096 tokens over 16 384 keys (32 heads over 8, bf16) take 815 to 840 us, 1.15 to 1.18
+// PFLOP/s, in short runs and 920 to 960 in long ones, where the power limit holds the clock; 64-wide heads 700 us (0.69).
+// Tried and worse: products under a branch that the compiler takes for divergent (100 cycles an instruction; 1245 us), both tiles'
+// products by one warp (880), side by side without turns (980), turns for the second half of P only (910), every fourth pair on
+// the FMA pipe (976) or none (845), exponentials before the maximum, done again where it moves (1370), spinning instead of suspended
+// waits (+1 to 3 %), registers moved to the softmax warps (+2 %).
 #include "kernels.h"
 #include "paged_attn.h"
 
@@ -590,9 +599,13 @@ cudaError_t configure_paged_tiles() {
     return e;
 }
 
-cudaError_t launch_paged_tiles(PagedArgs p, cudaStream_t s) {
-    // units at most: a sequence has a last one that is not full
-    const long long rows = (long long) p.c.N * p.G, units = std::min<long long>(p.c.N, rows / ROWS + p.c.B) * p.c.Hk;
+namespace {
+// units at most: a sequence has a last one that is not full
+long long units_of(const PagedArgs & p) { return std::min<long long>(p.c.N, (long long) p.c.N * p.G / ROWS + p.c.B) * p.c.Hk; }
+}
+
+double plan_paged_tiles(PagedArgs & p, uint32_t most) {
+    const long long units = std::min(units_of(p), (long long) p.c.B * (((long long) most * p.G + ROWS - 1) / ROWS) * p.c.Hk);
     // As many parts of a cluster as take the least time, in microseconds: start and end of a CTA 5, a tile of 128-wide heads 2 and of
     // 64-wide ones 1.7; with parts 4 to add them up and 5 for each wave of clusters; g_clusters[size] run at a time. Four
     // key tiles a part at least, eight parts at most (the largest portable cluster). The keys are what the tables have room for: lengths
@@ -607,6 +620,11 @@ cudaError_t launch_paged_tiles(PagedArgs p, cudaStream_t s) {
         const double cost = (double) ((units + room - 1) / room) * (5.0 + (parts > 1 ? 5.0 : 0.0) + (double) ((tiles + parts - 1) / parts) * (p.c.D == 64 ? 1.7 : 2.0)) + (parts > 1 ? 4.0 : 0.0);
         if (parts == 1 || cost < least) { least = cost; p.parts = parts; }
     }
+    return least;
+}
+
+cudaError_t launch_paged_tiles(const PagedArgs & p, cudaStream_t s) {
+    const long long units = units_of(p);
     if (units * p.parts > 0x7fffffffLL) return cudaErrorInvalidValue;
     const unsigned grid = (unsigned) (units * p.parts);
     const bool bf = p.c.type == TSN_BF16;
