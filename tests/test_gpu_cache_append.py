@@ -159,3 +159,33 @@ def test_nothing_to_do(dev):
     tsn.CacheAppend(dev, 64, (32,))(x, x, x, batch.k, batch.v, batch.table, batch.lens, q_start=batch.q_start)
     dev.commit()
     assert torch.equal(before.view(torch.int16), batch.k.view(torch.int16))
+
+
+def test_captured_and_replayed(dev):
+    """A captured call takes the lengths, tables and tokens that its buffers hold at each replay."""
+    batch = Batch([1, 4, 2], [90, 90, 90], D=64, Hk=2, page=16)
+    stream = torch.cuda.Stream()
+    own = tsn.Device(0, stream=stream.cuda_stream)
+    op = tsn.CacheAppend(own, 64, (32,), layout="half", eps=EPS)
+    q, k, v = batch.rows(4), batch.rows(2), batch.rows(2)
+    q_out, means = torch.empty_like(q), torch.zeros(batch.P, 2, 64, dtype=batch.dtype, device="cuda")
+    graph = torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph, stream=stream):
+        op(q, k, v, batch.k, batch.v, batch.table, batch.lens, q_out=q_out, q_start=batch.q_start, means=means)
+    for lens in ([90, 88, 60], [1, 4, 2], [33, 17, 90]):
+        batch.lens_ = lens
+        batch.lens.copy_(torch.tensor(lens, dtype=torch.int32))
+        for x in (q, k, v):
+            x.copy_(batch.normal(*x.shape))
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        for row, b, p in batch.tokens():
+            pos = torch.tensor([[p]], device="cuda")
+            id = batch.mapped(b, p)
+            for got, x in ((q_out[row], q[row]), (batch.k[id, p % 16], k[row])):
+                assert close(got, rotate(x[None], None, EPS, pos, (32,), "half")[0], x.abs().amax().double(), batch.dtype)
+            assert torch.equal(batch.v[id, p % 16], v[row])
+    del graph
+    own.close()

@@ -189,3 +189,37 @@ def test_a_stream_of_tokens(dev, chunks):
         assert within(out, *attention(step, q))
         assert torch.equal(chosen.cpu(), choose(step, q, means, picks, 1, 1))
         assert within(out2, *attention(step, q, pages=chosen))
+
+
+@pytest.mark.parametrize("D,dtype", [(64, torch.float16), (128, torch.bfloat16)])
+@pytest.mark.parametrize("last", [1, 3])
+def test_many_tokens(dev, D, dtype, last):
+    """Enough tokens that four share a block: of one sequence or of several, with rows of none behind."""
+    counts = [301, 1, 2, 0, 250, 3, 40]
+    lens = [n + 517 * b for b, n in enumerate(counts)]
+    check(dev, Batch(counts, lens, page=16, Hk=2, D=D, dtype=dtype, extra=3, layout="head"), 6, 7, 1, last)
+
+
+def test_many_single_tokens(dev):
+    B = 330
+    check(dev, Batch([1] * B, [1 + (97 * b) % 3000 for b in range(B)], page=32, Hk=4, D=128, one=True), 8, 6)
+    batch = Batch([1] * B, [1 + (97 * b) % 700 for b in range(B)], page=16, Hk=4, D=64, one=True)
+    g = torch.Generator(device="cuda")
+    g.manual_seed(2)
+    whole = lambda *s: torch.randint(-1, 2, s, generator=g, device="cuda").to(batch.dtype)  # noqa: E731
+    check(dev, batch, 4, 9, means=whole(batch.P, 4, 64), q=whole(B, 4, 64))   # ties
+
+
+def test_queries_and_means_that_are_not_finite(dev):
+    """The picks are of the pages that there are, in order; attention with the other tokens is not touched."""
+    batch = Batch([3, 2], [2000, 900], Hk=1, D=64)
+    q, means = batch.rows(2), batch.normal(batch.P, 1, 64).to(batch.dtype)
+    q[0, 0, 3], q[1, 1, 5], means[::7, 0, 9] = float("nan"), float("inf"), float("-inf")
+    out, chosen = torch.full_like(q, 3.0), torch.full((5, 1, 12), 77, dtype=torch.int32, device="cuda")
+    tsn.SparseAttention(dev, 64, 12)(q, batch.k, batch.v, means, batch.table, batch.lens, out, chosen, q_start=batch.q_start)
+    dev.commit()
+    for row, b, p in batch.tokens():
+        c = chosen[row, 0].tolist()
+        assert c == sorted(set(c)) and c[0] == 0 and c[-1] == p // 16
+    want, bound = attention(batch, q, pages=chosen)
+    assert within(out[2:], want[2:], bound[2:])
