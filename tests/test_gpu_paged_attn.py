@@ -157,6 +157,21 @@ def test_many_ragged_sequences(dev):
         check(dev, Batch(counts, [n + (13 * b) % 100 for b, n in enumerate(counts)], Hk=1, D=64, extra=7), 4)
 
 
+@pytest.mark.parametrize("n,G", [(1, 1), (3, 2), (3, 4)])
+@pytest.mark.parametrize("B", [1, 5, 60, 300])
+def test_short_caches(dev, B, n, G):
+    """Fewer keys than a share of the work holds: in units of their own, by the dozen a CTA, beside long ones, empty ones between."""
+    lens = [1 + (7 * b) % 40 for b in range(B)]
+    counts = [min(n, lens[b]) if b % 9 != 4 else 0 for b in range(B)]
+    check(dev, Batch(counts, lens, Hk=3, D=64), 3 * G)
+    lens[B // 2], counts[B // 2] = 2500, n
+    check(dev, Batch(counts, lens, Hk=3, D=64), 3 * G)
+    batch = Batch([1] * B, lens, Hk=3, D=128, one=True)
+    batch.lens_ = [0 if b % 3 == 1 else S for b, S in enumerate(lens)]
+    batch.lens = torch.tensor(batch.lens_, dtype=torch.int32, device="cuda")
+    check(dev, batch, 3 * G)
+
+
 def test_strides(dev):
     """Queries as columns of a wider product, results of padded heads, tables and lengths of a larger buffer, pages of another order."""
     for counts, lens in (([1, 1], [100, 300]), ([90, 200], [100, 300])):

@@ -27,6 +27,7 @@ constexpr float LAZY = 8.0f;   // log2 units that a maximum may grow before o is
 // Slabs of a share at least, slabs up to which a unit is not cut, parts of a unit at most (fewer slabs a part otherwise). One token, 8 kv
 // heads of 128, 2 x 1000 keys: with units of up to 32 slabs whole 15.7 us, 64: 12.1.
 constexpr int LEAST = 16, SHORT = 64, MOST_PARTS = 64;
+static_assert(LEAST <= SHORT, "what a unit counts as without its slabs is never cut");
 // Units up to which eight warps share one, a CTA an SM; above, two or three CTAs of four warps an SM, of which one loads while
 // another adds up its unit's sums. us by eight / by four (two CTAs): 16 units of 704 keys 8.0/10.5, 8 of 1000 12.1/16.5, one of 32 768 15.7/21.7, 192 of
 // 8191 142/148, but 256 of 1000 29.4/27.1, 1024 of 300 45.5/38.2.
@@ -46,11 +47,12 @@ struct RowLay {
 };
 constexpr int part_words(int D, int rows) { return rows * (D + 4); }
 
-// Sequence b of the batch: its rows and slabs. Every group of its rows takes the same slabs.
+// Sequence b of the batch: its rows and slabs. Every group of its rows takes the same slabs. A unit is dealt out as `weight` slabs: LEAST
+// of them at least, as even one of a single slab waits for its pages, keys and sums in turn, longer than 16 slabs stream (16 units of 16
+// and of 60 keys, 16 rows of 128: 8.3 and 8.8 us; 91 and 26.7 where a CTA took as many as hold LEAST slabs).
 struct Seq {
-    int start, n, place, len, from, slabs;   // first row, new tokens, the first one's place, cached keys; slabs from .. from + slabs - 1
+    int start, n, place, len, from, slabs, weight;   // first row, new tokens, the first one's place, cached keys; slabs from .. from + slabs - 1
     long long units;
-    bool empty;   // no key is seen: one slab that is not loaded, so that the rows are written
 };
 template <int ROWS>
 __device__ __forceinline__ Seq sequence(const PagedArgs & p, int b) {
@@ -63,8 +65,7 @@ __device__ __forceinline__ Seq sequence(const PagedArgs & p, int b) {
     s.from = min(seen_from(p, s.place), s.len) / SLAB;
     s.slabs = (s.len + SLAB - 1) / SLAB - s.from;
     s.units = ((long long) s.n * p.G + ROWS - 1) / ROWS * p.c.Hk;
-    s.empty = s.slabs == 0;
-    if (s.empty) s.slabs = 1;
+    s.weight = max(s.slabs, LEAST);
     return s;
 }
 
@@ -102,8 +103,8 @@ paged_rows_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant_
                 const int b = b0 + 32 * y + lane;
                 if (b < (int) p.c.B) {
                     const Seq s = sequence<ROWS>(p, b);
-                    total += s.units * s.slabs;
-                    if (s.units) longest = max(longest, s.slabs);
+                    total += s.units * s.weight;
+                    if (s.units) longest = max(longest, s.weight);
                 }
             }
         }
@@ -125,7 +126,7 @@ paged_rows_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant_
             const int b = b0 + lane;
             Seq s{};
             if (b < (int) p.c.B) s = sequence<ROWS>(p, b);
-            const long long mine = s.units * s.slabs;
+            const long long mine = s.units * s.weight;
             long long upto = mine;
 #pragma unroll
             for (int o = 1; o < 32; o <<= 1) {
@@ -134,15 +135,15 @@ paged_rows_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant_
             }
             const long long at = before + upto - mine;
             auto cut = [&](long long x) {   // x as an end of the share, at <= x < at + mine
-                const long long u = (x - at) / s.slabs;
-                return p.whole || s.slabs <= SHORT ? at + u * s.slabs : x;
+                const long long u = (x - at) / s.weight;
+                return p.whole || s.weight <= SHORT ? at + u * s.weight : x;
             };
             if (mine && at <= x0 && x0 < at + mine) {
-                const long long x = cut(x0), u = (x - at) / s.slabs;
+                const long long x = cut(x0), u = (x - at) / s.weight;
                 share_from = x;
                 first_seq = b;
                 first_unit = u;
-                first_off = (int) (x - at - u * s.slabs);
+                first_off = (int) (x - at - u * s.weight);
             }
             if (mine && at <= x1 && x1 < at + mine) share_to = cut(x1);
             before += __shfl_sync(~0u, upto, 31);
@@ -193,14 +194,14 @@ paged_rows_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant_
             row0 = s.start;
             n = s.len;
             place0 = s.place;
-            const int take = (int) min((long long) (s.slabs - off), to - at);
+            const int take = (int) min((long long) (s.weight - off), to - at);
             s0 = s.from + off;
-            s1 = s.empty ? s0 : s0 + take;
+            s1 = s.from + min(off + take, s.slabs);
             const long long begin = at - off;   // of the unit
-            if (take < s.slabs) {
+            if (take < s.weight) {
                 owner = (int) (begin / share_per);
                 part = (int) blockIdx.x - owner;
-                parts = (int) ((begin + s.slabs - 1) / share_per) - owner + 1;
+                parts = (int) ((begin + s.weight - 1) / share_per) - owner + 1;
             }
             at += take;
             off = 0;
