@@ -269,6 +269,7 @@ __global__ void __launch_bounds__(TOK * GT, 1) page_select_kernel(const __grid_c
     const tsn_sparse_attn_args & a = p.a;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, parts = TOK > 1 ? 1 : p.parts, part = TOK > 1 ? 0 : (int) blockIdx.x % parts,
               row0 = (int) blockIdx.x / parts * TOK, hk = (int) blockIdx.y;
+    if (TOK == 1 && parts > 1) cluster_arrive();
     pdl_wait();
     if (warp < TOK) {
         const int row = row0 + warp, b = row < (int) a.c.N ? seq_of_row(a.c, row) : -1, pl = b < 0 ? 0 : place_of_row(a.c, b, row);
@@ -293,6 +294,7 @@ __global__ void __launch_bounds__(TOK * GT, 1) page_select_kernel(const __grid_c
         qs[t][e / 2 % 4][e / 8][e % 2] = s * 0x1p880;
     }
     __syncthreads();
+    if (TOK == 1 && parts > 1) cluster_wait();   // the first block runs: scores may be stored into its shared memory
     pdl_trigger();
     const int picks = (int) a.picks, first = (int) a.first;
     float * rounded = (float *) (scores + TOK * a.c.M);
@@ -398,6 +400,7 @@ __global__ void __launch_bounds__(TOK * GT, 1) page_select_kernel(const __grid_c
             j0 += STEP;
         }
     }
+    __syncwarp();
     if (parts > 1) {
         cluster_sync_all();
         if (part) return;
