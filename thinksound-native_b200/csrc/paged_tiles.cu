@@ -2,8 +2,9 @@
 //
 //   o = sum_j p_j v_j / l,  l = sum_j p_j,  p_j = 2^(c q.k_j - ref)
 // in one pass over the keys; ref follows the row's running maximum and moves, with o and l rescaled, when that has grown by more than
-// 2^8. P is rounded to 16 bits, as the tensor cores take it; scores, maxima, sums and o are f32, and l is the sum before the rounding: the
-// rounded ones would take a mixed add a value instead of a packed one for two.
+// 2^8. P is rounded to 16 bits, as the tensor cores take it; scores, maxima, sums and o are f32, and l is the sum of the rounded ones, so
+// that rounding cancels where values are alike, and a NaN, which the FMA pipe's exponential only has after rounding (as an
+// infinity), reaches l. That takes a mixed add a value instead of a packed one for two: 795 -> 803 us for the 4096 tokens below, 702 -> 768 with 64-wide heads.
 // A unit is 256 query rows of a sequence and kv head, (token, head of the group), as two tiles of 128, so that heads of a group share
 // the keys; a CTA takes a unit or, where there are few, a part of its keys, the parts of a cluster adding up their sums. 384 threads:
 //   warps 0-3, 4-7  softmax of a tile, one row a thread: S from TMEM, mask, maximum, exponentials, P over S's columns
@@ -381,25 +382,23 @@ paged_tiles_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant
             }
             const float neg = ref == -INFINITY ? 0.0f : -ref;
             const uint64_t neg2 = f2_pack(neg, neg), c2 = f2_pack(p.scale, p.scale);
-            uint64_t sum[2] = {0, 0};
+            float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
                 uint32_t pk[32];
 #pragma unroll
                 for (int e = 0; e < 32; ++e) {
-                    uint64_t v = ffma2(f2_pack(__uint_as_float(x[64 * h + 2 * e]), __uint_as_float(x[64 * h + 2 * e + 1])), c2, neg2);
+                    const uint64_t v = ffma2(f2_pack(__uint_as_float(x[64 * h + 2 * e]), __uint_as_float(x[64 * h + 2 * e + 1])), c2, neg2);
                     float y, z;
                     if (e % L::EVERY == L::EVERY - 1) {
-                        v = ex2_fma<BF16, true>(v);
-                        f2_unpack(v, y, z);
+                        f2_unpack(ex2_fma<BF16, true>(v), y, z);
                     } else {
                         f2_unpack(v, y, z);
                         y = ex2(y);
                         z = ex2(z);
-                        v = f2_pack(y, z);
                     }
-                    sum[e & 1] = fadd2(sum[e & 1], v);
                     pk[e] = pack16<BF16>(y, z);
+                    add_rounded<BF16>(sum[2 * (e & 1)], sum[2 * (e & 1) + 1], pk[e]);
                 }
                 tmem_st32(ts + 32 * h, pk);
                 if (h == 0) {
@@ -409,12 +408,7 @@ paged_tiles_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant
                     if (lane == 0) mbar_arrive(&p_half[t]);
                 }
             }
-            {
-                float a, b, c, d;
-                f2_unpack(sum[0], a, b);
-                f2_unpack(sum[1], c, d);
-                l += (a + c) + (b + d);
-            }
+            l += (sum[0] + sum[2]) + (sum[1] + sum[3]);
             if (unfit(base)) {
                 if (mixed(base)) {
                     if (!mbar_wait_soon(&v_ready[fits_seen % STAGES], (fits_seen / STAGES) & 1, abort_flag, p.err, DEV_TIMEOUT_FULL)) ok = false;
