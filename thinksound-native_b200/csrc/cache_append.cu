@@ -77,7 +77,7 @@ __global__ void __launch_bounds__(32 * WARPS, 4) cache_append_kernel(const __gri
     if (warp == 0) {   // a lane a token; mostly all are of one sequence
         const int b0 = seq_of_row(a.c, (int) s0), b1 = here > 1 ? seq_of_row(a.c, (int) s0 + here - 1) : b0;
         if (lane < here) {
-            const int i = (int) s0 + lane, b = b0 == b1 ? b0 : seq_of_row_alone(a.c, i);
+            const int i = (int) s0 + lane, b = b0 == b1 && b0 >= 0 ? b0 : seq_of_row_alone(a.c, i);   // whole sequences may lie between rows of none
             const int pl = b < 0 ? 0 : place_of_row(a.c, b, i);
             place[lane] = pl;
             spot[lane] = b < 0 ? -2 : page_of(a.c, b, pl >> n.page_log2);   // -2: a row of no sequence
