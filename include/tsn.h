@@ -483,6 +483,10 @@ typedef struct tsn_paged_attn_args {
     tsn_rows q, out;
 } tsn_paged_attn_args;
 int tsn_paged_attn(tsn_device * dev, const tsn_paged_attn_args * a);
+/* A test hook for the failure path: the call by its kernel for few rows, in which the waits of block `block` for its first loads
+ * count as run out (nothing hangs, the loads land). Expected result: TSN_ERR_TIMEOUT where there is such a block with keys to read;
+ * out is undefined then, and later calls are not affected. Synchronises. */
+int tsn_selftest_paged_timeout(tsn_device * dev, const tsn_paged_attn_args * a, uint32_t block);
 
 /* Causal attention over `picks` pages of the cache, chosen for each new token and kv head by a cheap score: page x scores
  * (sum of the group's query heads) . means[x], in 64 bits. For a token at place p, with its own page o = p / page, the

@@ -350,6 +350,15 @@ int tsn_paged_attn(tsn_device * dev, const tsn_paged_attn_args * a) {
     if (int rc = refused([&] { return check_paged_attn(a); })) return rc;
     return guarded(dev, a, [&](DeviceCtx & c) { return paged_attn(c, *a); });
 }
+int tsn_selftest_paged_timeout(tsn_device * dev, const tsn_paged_attn_args * a, uint32_t block) {
+    if (int rc = refused([&] { return check_paged_attn(a); })) return rc;
+    if (block > 65535) return fail(TSN_ERR_ARG, "tsn_selftest_paged_timeout: at most 65535 blocks");
+    return guarded(dev, a, [&](DeviceCtx & c) {
+        if (int rc = c.sync()) return rc;   // a timeout reported below is this call's own
+        if (int rc = selftest_paged_timeout(c, *a, block)) return rc;
+        return c.sync();
+    });
+}
 int tsn_sparse_attn(tsn_device * dev, const tsn_sparse_attn_args * a) {
     if (int rc = refused([&] { return check_sparse_attn(a); })) return rc;
     return guarded(dev, a, [&](DeviceCtx & c) { return sparse_attn(c, *a); });

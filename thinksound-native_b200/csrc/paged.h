@@ -13,6 +13,7 @@ int check_sparse_attn(const tsn_sparse_attn_args * a);
 int cache_append(DeviceCtx & c, const tsn_rope_plan_t & plan, const tsn_cache_append_args & a);
 int paged_attn(DeviceCtx & c, const tsn_paged_attn_args & a);
 int sparse_attn(DeviceCtx & c, const tsn_sparse_attn_args & a);
+int selftest_paged_timeout(DeviceCtx & c, const tsn_paged_attn_args & a, uint32_t block);
 cudaError_t launch_page_select(const tsn_sparse_attn_args & a, cudaStream_t s);
 cudaError_t configure_paged();   // once per device, before the first launch
 

@@ -72,14 +72,31 @@ cudaError_t configure_paged() {
     return e;
 }
 
-int paged_attn(DeviceCtx & c, const tsn_paged_attn_args & a) {
-    if (a.c.N == 0 || a.c.B == 0) return TSN_OK;
+namespace {
+PagedArgs args_of(const DeviceCtx & c, const tsn_paged_attn_args & a, uint32_t & most) {
     PagedArgs p = args_of(c, a.c, a.H, a.scale);
     p.q = a.q;
     p.out = a.out;
     p.causal = a.causal != 0;
     p.window = (int) a.window;
-    const uint32_t most = !a.c.q_start ? 1 : a.most ? std::min(a.most, a.c.N) : a.c.N;
+    most = !a.c.q_start ? 1 : a.most ? std::min(a.most, a.c.N) : a.c.N;
+    return p;
+}
+} // namespace
+
+// The few-rows kernel whatever the rows are; what it reports is for the caller to fetch.
+int selftest_paged_timeout(DeviceCtx & c, const tsn_paged_attn_args & a, uint32_t block) {
+    if (a.c.N == 0 || a.c.B == 0) return TSN_OK;
+    uint32_t most;
+    PagedArgs p = args_of(c, a, most);
+    p.give_up = (int) block + 1;
+    return few_rows(c, "tsn_selftest_paged_timeout", p, most);
+}
+
+int paged_attn(DeviceCtx & c, const tsn_paged_attn_args & a) {
+    if (a.c.N == 0 || a.c.B == 0) return TSN_OK;
+    uint32_t most;
+    PagedArgs p = args_of(c, a, most);
     // Up to eight rows of a kv head go to the kernel for few; beyond, the one that the estimates of both prefer: groups of rows read
     // the keys anew, but go to every SM where a tile's keys have eight at most. us by groups / by tiles, heads of 128, bf16:
     // 16 tokens x 4 heads, 8 kv heads over 8192 keys 37/24; 16 streams of 4 tokens over 4096 56/60, of 8 tokens 95/61; 64 streams of 4

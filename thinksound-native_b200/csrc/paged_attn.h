@@ -22,6 +22,7 @@ struct PagedArgs {
     float * part;
     unsigned int * count;
     int * err;
+    int give_up;          // a test of the failure path: the block (from 1) whose first unit's waits count as run out
 };
 
 // {D, page, Hk, P} views of keys and values with {64, tokens, 1, 1} boxes

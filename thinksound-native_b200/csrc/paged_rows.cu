@@ -213,7 +213,9 @@ paged_rows_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant_
         auto hi_of = [&](int r) { return r < R ? seen_to(p, place_of(r), n) : n; };
         auto lo_of = [&](int r) { return r < R ? seen_from(p, place_of(r)) : 0; };
         const int least = hi_of(0), latest = lo_of(R - 1);   // before least and from latest on every row sees
-        const int mine = s1 - s0 > warp ? (s1 - s0 - warp + W - 1) / W : 0;
+        // After a wait that gave up nothing is loaded any more, but the share is walked to its end: every part arrives, so that the
+        // counters are zero after the call whatever became of it.
+        const int mine = !flags[0] && s1 - s0 > warp ? (s1 - s0 - warp + W - 1) / W : 0;
 
         // pages of the warp's slabs, 32 at once, and which of them are none
         auto load_ids = [&](int i) {
@@ -248,6 +250,11 @@ paged_rows_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant_
             }
         };
         for (int i = 0; i < RING && i < mine; ++i) request(i);
+        const bool give_up = p.give_up == (int) blockIdx.x + 1;
+        if (give_up && tid == 0) {
+            flags[0] = 1;
+            if (p.err) atomicCAS(p.err, 0, DEV_TIMEOUT_FULL);
+        }
 
         // Q^T as B operands: row g0 of each eight, rows past the last one as zeros
         uint32_t qb[NT][D / 16][2];
@@ -278,7 +285,7 @@ paged_rows_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant_
         }
         uint32_t to_mend = 0;   // rows that see a value which is not finite, among those with rows that do not
         int bases = LIST ? load_base(0) : 0;
-        for (int i = 0; i < mine; ++i) {
+        for (int i = 0; i < mine && !give_up; ++i) {
             if (LIST && i && (i & 31) == 0) bases = load_base(i);
             const int base = LIST ? __shfl_sync(~0u, bases, i & 31) : (s0 + warp + i * W) * SLAB;
             const unsigned st = (turn + i) % RING;
@@ -534,7 +541,6 @@ paged_rows_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant_
         if (at < to) {
             __syncthreads();   // the rings are free again
             if (tid == 0) flags[2] = 0;
-            if (flags[0]) break;
             fence_proxy_async_smem();   // the sums were written where the next copies land
             if (++unit == s.units) {
                 unit = 0;

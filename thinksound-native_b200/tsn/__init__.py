@@ -217,6 +217,7 @@ _SIGS = [
     ("tsn_diff_attn", C.c_int, [C.c_void_p, C.POINTER(DiffAttnArgs)]),
     ("tsn_cache_append", C.c_int, [C.c_void_p, C.POINTER(RopePlan), C.POINTER(CacheAppendArgs)]),
     ("tsn_paged_attn", C.c_int, [C.c_void_p, C.POINTER(PagedAttnArgs)]),
+    ("tsn_selftest_paged_timeout", C.c_int, [C.c_void_p, C.POINTER(PagedAttnArgs), C.c_uint32]),
     ("tsn_sparse_attn", C.c_int, [C.c_void_p, C.POINTER(SparseAttnArgs)]),
     ("tsn_gguf_write_synthetic", C.c_int, [C.c_char_p, C.POINTER(Geom), C.c_uint64, C.c_int]),
     ("tsn_gguf_write_synthetic_vae", C.c_int, [C.c_char_p, C.c_uint32, C.c_uint32, C.c_uint32, C.c_uint64]),
@@ -321,6 +322,11 @@ class Device:
         """Run the bounded-wait self-test (a wait nothing completes); raises TsnError (TSN_ERR_TIMEOUT
         expected) unless the wait somehow completed."""
         check(lib().tsn_selftest_device_timeout(self.h, limit_us))
+
+    def selftest_paged_timeout(self, args, block: int):
+        """Paged attention (args: PagedAttnArgs) in which the waits of one block count as run out; raises TsnError
+        (TSN_ERR_TIMEOUT expected) where there is such a block with keys to read."""
+        check(lib().tsn_selftest_paged_timeout(self.h, C.byref(args), block))
 
     def selftest_gemm_lo8(self, W, X, Y, bias, M, N, K, wexp, mode, bn, reps=1) -> float:
         """Experimental GEMM with an e4m3 low-order product (mode 0) or the split f16 GEMM (mode 1);
