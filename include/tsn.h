@@ -471,7 +471,8 @@ int tsn_cache_append(tsn_device * dev, const tsn_rope_plan_t * plan, const tsn_c
  * with causal j <= p; and with window > 0 (causal only) j > p - window. A row that sees no key is zero.
  * What unseen keys and values hold has no effect, NaN and infinities included; what seen ones hold enters as the arithmetic has
  * it (a row with a score of NaN or +infinity is NaN, a key whose score is -infinity has no share).
- * The probabilities are rounded to `type` before the product with v, as the tensor cores take them.
+ * The probabilities are rounded to `type` before the product with v, as the tensor cores take them, and the sum that divides is of the
+ * rounded ones. In f16, keys whose share is below 2^-21 of the greatest one's lose bits of it: each is off by at most 2^-32 of that.
  * most: new tokens of a sequence at most, as far as the caller knows (0: not known); it decides which kernel
  * runs, never the result's extent. Split keys meet in a workspace, as those of tsn_diff_attn do. */
 typedef struct tsn_paged_attn_args {

@@ -1,7 +1,7 @@
 // paged_rows.cu — attention over the paged cache for a few query rows of a kv head: single tokens, drafts, picked pages.
 //
-//   o = sum_j p_j v_j / l,  l = sum_j p_j,  p_j = 2^(c q.k_j - ref);  ref follows the row's running maximum and moves when that has grown
-//   by more than 2^8, with o and l rescaled. P is rounded to 16 bits, as the tensor cores take it; l is the sum of the rounded ones.
+//   o = sum_j p_j v_j / l,  l = sum_j p_j,  p_j = 2^(c q.k_j - ref + ABOVE);  ref follows the row's running maximum and moves when that has
+//   grown by more than LAZY (struct Reference), with o and l rescaled. P is rounded to 16 bits, as the tensor cores take it; l is the sum of the rounded ones.
 // Bound by reading K and V. mma.sync takes 8 rows (NT times) with the keys, and for the product with V the columns, on its 16-row
 // side: S^T = K Q^T, O^T = V^T P^T; P^T is S^T's layout transposed in registers. Each warp streams 16-key slabs of its own by TMA,
 // a page holding whole slabs, through a ring of its own; the warps' sums meet in shared memory.
@@ -23,7 +23,6 @@ namespace tsn {
 namespace {
 
 constexpr int SLAB = 16;   // keys of a slab
-constexpr float LAZY = 8.0f;   // log2 units that a maximum may grow before o is rescaled
 // Slabs of a share at least, slabs up to which a unit is not cut, parts of a unit at most (fewer slabs a part otherwise). One token, 8 kv
 // heads of 128, 2 x 1000 keys: with units of up to 32 slabs whole 15.7 us, 64: 12.1.
 constexpr int LEAST = 16, SHORT = 64, MOST_PARTS = 64;
@@ -74,6 +73,7 @@ __global__ void __launch_bounds__(32 * W, RowLay<D, NT, W, LIST>::CTAS)
 paged_rows_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant__ CUtensorMap tv, const __grid_constant__ PagedArgs p) {
     using L = RowLay<D, NT, W, LIST>;
     constexpr int E = D / 32, RING = L::RING, ROWS = L::ROWS;
+    constexpr float LAZY = Reference<BF16>::LAZY, ABOVE = Reference<BF16>::ABOVE;
     extern __shared__ __align__(1024) uint8_t smem[];
     __shared__ int first_seq, first_off;
     __shared__ long long first_unit, share_from, share_to, share_per;
@@ -348,7 +348,7 @@ paged_rows_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant_
             uint32_t pb[NT][2];
 #pragma unroll
             for (int t = 0; t < NT; ++t) {
-                const float n0 = ref[t][0] == -INFINITY ? 0.0f : -ref[t][0], n1 = ref[t][1] == -INFINITY ? 0.0f : -ref[t][1];
+                const float n0 = ref[t][0] == -INFINITY ? 0.0f : ABOVE - ref[t][0], n1 = ref[t][1] == -INFINITY ? 0.0f : ABOVE - ref[t][1];
                 const uint32_t p0 = pack16<BF16>(ex2(fmaf(sc[t][0], p.scale, n0)), ex2(fmaf(sc[t][1], p.scale, n1)));
                 const uint32_t p1 = pack16<BF16>(ex2(fmaf(sc[t][2], p.scale, n0)), ex2(fmaf(sc[t][3], p.scale, n1)));
                 add_rounded<BF16>(l[t][0], l[t][1], p0);   // the sums are of what the product takes

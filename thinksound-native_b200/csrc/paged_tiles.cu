@@ -1,8 +1,8 @@
 // paged_tiles.cu — attention over the paged cache for many query rows of a kv head, on the tcgen05 tensor cores.
 //
-//   o = sum_j p_j v_j / l,  l = sum_j p_j,  p_j = 2^(c q.k_j - ref)
+//   o = sum_j p_j v_j / l,  l = sum_j p_j,  p_j = 2^(c q.k_j - ref + ABOVE)
 // in one pass over the keys; ref follows the row's running maximum and moves, with o and l rescaled, when that has grown by more than
-// 2^8. P is rounded to 16 bits, as the tensor cores take it; scores, maxima, sums and o are f32, and l is the sum of the rounded ones, so
+// LAZY (struct Reference). P is rounded to 16 bits, as the tensor cores take it; scores, maxima, sums and o are f32, and l is the sum of the rounded ones, so
 // that rounding cancels where values are alike, and a NaN, which the FMA pipe's exponential only has after rounding (as an
 // infinity), reaches l. That takes a mixed add a value instead of a packed one for two: 795 -> 803 us for the 4096 tokens below, 702 -> 768 with 64-wide heads.
 // A unit is 256 query rows of a sequence and kv head, (token, head of the group), as two tiles of 128, so that heads of a group share
@@ -35,7 +35,6 @@ namespace tsn {
 namespace {
 
 constexpr int ROWS = 256, KEYS = 128, THREADS = 384;
-constexpr float LAZY = 8.0f;   // log2 units that a maximum may grow before o is rescaled
 
 template <int D>
 struct Lay {
@@ -58,6 +57,7 @@ __global__ void __launch_bounds__(THREADS, 1)
 paged_tiles_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant__ CUtensorMap tv, const __grid_constant__ PagedArgs p) {
     using L = Lay<D>;
     constexpr int CH = D / 8, STAGES = L::STAGES;   // CH: 16-byte pieces of a head
+    constexpr float LAZY = Reference<BF16>::LAZY, ABOVE = Reference<BF16>::ABOVE;
     extern __shared__ __align__(1024) uint8_t smem[];
     // sequence, its first row, kv head, first query row, query rows, length, new tokens, tokens of rows 127 and the last; (token, head) of the rows
     __shared__ int unit_of[9];
@@ -380,7 +380,7 @@ paged_tiles_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant
                     }
                 }
             }
-            const float neg = ref == -INFINITY ? 0.0f : -ref;
+            const float neg = ref == -INFINITY ? 0.0f : ABOVE - ref;
             const uint64_t neg2 = f2_pack(neg, neg), c2 = f2_pack(p.scale, p.scale);
             float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
