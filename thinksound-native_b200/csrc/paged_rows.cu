@@ -306,6 +306,10 @@ paged_rows_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant_
 #pragma unroll
                 for (int t = 0; t < NT; ++t) mma16816<BF16>(sc[t], f, qb[t][k][0], qb[t][k][1]);
             }
+#pragma unroll
+            for (int t = 0; t < NT; ++t)
+#pragma unroll
+                for (int k = 0; k < 4; ++k) sc[t][k] = __fmul_rn(sc[t][k], p.scale);   // rounded by itself, so that the greatest one less itself is zero however large
             const bool gone = there != 0xffffu, mixed = least < min(n, base + SLAB) || base < latest;
             uint32_t vis[NT][2];
 #pragma unroll
@@ -325,8 +329,8 @@ paged_rows_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant_
             for (int t = 0; t < NT; ++t)
 #pragma unroll
                 for (int h = 0; h < 2; ++h) {
-                    top[t][h] = fmaxf(sc[t][h], sc[t][2 + h]) * p.scale;
-                    move |= top[t][h] > ref[t][h] + LAZY;
+                    top[t][h] = fmaxf(sc[t][h], sc[t][2 + h]);
+                    move |= top[t][h] - ref[t][h] > LAZY;
                 }
             if (__any_sync(~0u, move)) {
 #pragma unroll
@@ -336,7 +340,7 @@ paged_rows_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant_
                         float m = top[t][h];
 #pragma unroll
                         for (int x = 4; x < 32; x <<= 1) m = fmaxf(m, __shfl_xor_sync(~0u, m, x));
-                        if (m > ref[t][h] + LAZY) {   // a row moves its reference by itself
+                        if (m - ref[t][h] > LAZY) {   // a row moves its reference by itself
                             const float f = ex2(ref[t][h] - m);
                             ref[t][h] = m;
                             l[t][h] *= f;
@@ -348,9 +352,9 @@ paged_rows_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant_
             uint32_t pb[NT][2];
 #pragma unroll
             for (int t = 0; t < NT; ++t) {
-                const float n0 = ref[t][0] == -INFINITY ? 0.0f : ABOVE - ref[t][0], n1 = ref[t][1] == -INFINITY ? 0.0f : ABOVE - ref[t][1];
-                const uint32_t p0 = pack16<BF16>(ex2(fmaf(sc[t][0], p.scale, n0)), ex2(fmaf(sc[t][1], p.scale, n1)));
-                const uint32_t p1 = pack16<BF16>(ex2(fmaf(sc[t][2], p.scale, n0)), ex2(fmaf(sc[t][3], p.scale, n1)));
+                const float r0 = ref[t][0] == -INFINITY ? 0.0f : ref[t][0], r1 = ref[t][1] == -INFINITY ? 0.0f : ref[t][1];
+                const uint32_t p0 = pack16<BF16>(ex2(sc[t][0] - r0 + ABOVE), ex2(sc[t][1] - r1 + ABOVE));
+                const uint32_t p1 = pack16<BF16>(ex2(sc[t][2] - r0 + ABOVE), ex2(sc[t][3] - r1 + ABOVE));
                 add_rounded<BF16>(l[t][0], l[t][1], p0);   // the sums are of what the product takes
                 add_rounded<BF16>(l[t][0], l[t][1], p1);
                 pb[t][0] = movmatrix(p0);

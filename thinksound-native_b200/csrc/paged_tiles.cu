@@ -337,7 +337,7 @@ paged_tiles_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant
         const int hi = there ? hi_at(token) : n, lo = there ? lo_at(token) : 0;
         const int rows_end = min(R, 128 * t + 128);
         const int sure_hi = ja < jb ? hi_at(t ? token128 : token0) : 0, sure_lo = ja < jb ? lo_at(t ? token_last : token127) : 0;   // every row of the tile sees keys sure_lo .. sure_hi - 1
-        float l = 0.0f, ref = -INFINITY;
+        float l = 0.0f, raw = -INFINITY;   // raw: the score that the reference is of
         bool ok = true, poison = false;
         int fits_seen = 0;   // tiles of the part whose values passed through warp 11
         for (int j = 0; j < ja; ++j) fits_seen += unfit((t0 + j) * KEYS);
@@ -363,12 +363,12 @@ paged_tiles_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant
             float mx[4];
 #pragma unroll
             for (int w = 0; w < 4; ++w) mx[w] = greatest(x + 32 * w);
-            const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * p.scale;
-            const bool move = top > ref + LAZY;
+            const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
+            const bool move = (top - raw) * p.scale > LAZY;
             if (__any_sync(~0u, move)) {
                 // a row moves its reference by itself, so its result does not depend on its neighbours
-                const float f = move ? ex2(ref - top) : 1.0f;
-                if (move) { ref = top; l *= f; }
+                const float f = move ? ex2(__fmul_ru(raw, p.scale) - __fmul_ru(top, p.scale)) : 1.0f;
+                if (move) { raw = top; l *= f; }
                 if (j > ja) {   // O holds the tiles before: their products were issued before these scores'
 #pragma unroll 1
                     for (int y = 0; y < D; y += 16) {
@@ -380,8 +380,15 @@ paged_tiles_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant
                     }
                 }
             }
-            const float neg = ref == -INFINITY ? 0.0f : ABOVE - ref;
-            const uint64_t neg2 = f2_pack(neg, neg), c2 = f2_pack(p.scale, p.scale);
+            // c s - ref in one rounding: ref is c raw rounded up and ABOVE - ref down, so that no probability exceeds 2^15 however large
+            // the scores are. The greatest one falls below 2^ABOVE by the steps of numbers this size: from 2^26 on, where neighbouring f32
+            // scores are 4 log2 units and more apart, c becomes a power of two, whose products are exact. (With c raw rounded to nearest
+            // rows of scores of 2^36 were NaN or zero. Scores scaled and subtracted one after the other where a row needs it: 7 % more time.)
+            const float high = __fmul_ru(raw, p.scale);
+            const bool far = fabsf(high) >= 0x1p26f;
+            const float c = far ? __uint_as_float(__float_as_uint(p.scale) & 0x7f800000u) : p.scale;
+            const float neg = raw == -INFINITY ? 0.0f : __fadd_rd(ABOVE, far ? -(raw * c) : -high);
+            const uint64_t neg2 = f2_pack(neg, neg), c2 = f2_pack(c, c);
             float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
@@ -463,7 +470,7 @@ paged_tiles_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant
 #pragma unroll
                     for (int e = 0; e < 32; e += 4) *(float4 *) (dst + x + e) = make_float4(o[e], o[e + 1], o[e + 2], o[e + 3]);
                 }
-                dst[D] = ref;
+                dst[D] = __fmul_ru(raw, p.scale);   // the reference
                 dst[D + 1] = l;
             }
             cluster_sync_all();
