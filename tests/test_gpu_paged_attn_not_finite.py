@@ -88,3 +88,19 @@ def test_picked_pages(dev):
         op(q, batch.k, batch.v, means, batch.table, batch.lens, out, chosen, q_start=batch.q_start)
         dev.commit()
         assert bool(out.isnan().all())
+
+
+@pytest.mark.parametrize("dtype,D", [(torch.bfloat16, 64), (torch.float16, 128)], ids=["bf16-64", "f16-128"])
+@pytest.mark.parametrize("n,S,Hk,G", SHAPES)
+@pytest.mark.parametrize("bad", [INF, -INF, float("nan")])
+def test_rows_without_a_score_are_zero(dev, n, S, Hk, G, dtype, D, bad):
+    """All seen scores are -infinity: whatever the values hold, on every path."""
+    batch, q = case(n, S, Hk, G, dtype, D)
+    j = torch.arange(S, device="cuda")
+    batch.k[batch.table[0].long()[j // 64], j % 64, :, 3] = -INF
+    for places in ([0], [S - n], [3, S // 2, S - 1]):
+        v = batch.v.clone()
+        for place in places:
+            batch.v[batch.table[0, place // 64].long(), place % 64, :, 7] = bad
+        assert bool((run(dev, batch, q, n) == 0).all())
+        batch.v.copy_(v)

@@ -498,7 +498,7 @@ paged_tiles_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant
                 const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
 #pragma unroll
                 for (int i = 0; i < 8; ++i)
-                    if (i < p.parts) fac[tid * 8 + i] = ref_of[i] * inv;
+                    if (i < p.parts) fac[tid * 8 + i] = sum == 0.0f ? -1.0f : ref_of[i] * inv;   // -1: no key has a share, and no sum of values counts
             }
             bar_n(3, 256);
             constexpr int LANES = D / 4, STEP = 8 * (32 / LANES), AT_ONCE = 4;   // lanes of a row; rows of a step of all warps
@@ -520,7 +520,7 @@ paged_tiles_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant
                 for (int y = 0; y < AT_ONCE; ++y) {
                     const int r = y0 + y * STEP;
                     if (r < here && !*abort_flag)
-                        *(uint2 *) (address(p.out, from + r) + col) = make_uint2(pack16<BF16>(o[y][0], o[y][1]), pack16<BF16>(o[y][2], o[y][3]));
+                        *(uint2 *) (address(p.out, from + r) + col) = fac[r * 8] < 0.0f ? make_uint2(0u, 0u) : make_uint2(pack16<BF16>(o[y][0], o[y][1]), pack16<BF16>(o[y][2], o[y][3]));
                 }
             }
             cluster_sync_all();   // nobody leaves while its sums are read
