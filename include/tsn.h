@@ -469,8 +469,10 @@ int tsn_cache_append(tsn_device * dev, const tsn_rope_plan_t * plan, const tsn_c
  * q and out [N, H, D] of c.type, row i, head h at element i * sb + h * st; query head h reads kv head h / (H / Hk), H / Hk at
  * most 128; D is 64 or 128. scale 0 means 1 / sqrt(D). A token at place p sees place j of its sequence where j < len[b];
  * with causal j <= p; and with window > 0 (causal only) j > p - window. A row that sees no key is zero.
- * What unseen keys and values hold has no effect, NaN and infinities included; what seen ones hold enters as the arithmetic has
- * it (a row with a score of NaN or +infinity is NaN, a key whose score is -infinity has no share).
+ * What unseen keys and values hold has no effect, NaN and infinities included. Of seen ones: a row with a score of NaN or +infinity is
+ * NaN; a key whose score is -infinity has no share, and a row that sees no others is zero; a value that is not finite makes its
+ * column of the row so, NaN or an infinity, however small its key's share (which of them is left open: 0 times infinity is NaN where the
+ * product takes it, but where the rows of a tile see different keys such values are added apart).
  * The probabilities are rounded to `type` before the product with v, as the tensor cores take them, and the sum that divides is of the
  * rounded ones. In f16, keys whose share is below 2^-21 of the greatest one's lose bits of it: each is off by at most 2^-32 of that.
  * most: new tokens of a sequence at most, as far as the caller knows (0: not known); it decides which kernel

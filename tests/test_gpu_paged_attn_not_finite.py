@@ -104,3 +104,28 @@ def test_rows_without_a_score_are_zero(dev, n, S, Hk, G, dtype, D, bad):
             batch.v[batch.table[0, place // 64].long(), place % 64, :, 7] = bad
         assert bool((run(dev, batch, q, n) == 0).all())
         batch.v.copy_(v)
+
+
+@pytest.mark.parametrize("dtype,D", [(torch.bfloat16, 64), (torch.float16, 64), (torch.float16, 128)], ids=["bf16-64", "f16-64", "f16-128"])
+@pytest.mark.parametrize("n,S,Hk,G", SHAPES)
+@pytest.mark.parametrize("bad", [INF, -INF, float("nan")])
+def test_values_of_keys_without_weight(dev, n, S, Hk, G, dtype, D, bad):
+    """A seen value that is not finite leaves its column so, however small its key's share is (it rounds to zero here), and touches
+    neither the other columns nor the rows that do not see it."""
+    batch, q = case(n, S, Hk, G, dtype, D)
+    j = torch.arange(S, device="cuda")
+    batch.k[batch.table[0].long()[j // 64], j % 64, :, 3] = 0.0
+    for place in {1, S // 2, S - 1 - n // 2, S - 1}:
+        k, v = batch.k.clone(), batch.v.clone()
+        at = (batch.table[0, place // 64].long(), place % 64)
+        batch.k[at][:, 3] = -2000.0   # 250 nats and 177 below the others
+        clean, (_, bound) = run(dev, batch, q, n), attention(batch, q)
+        batch.v[at][0, 7] = bad
+        out = run(dev, batch, q, n)
+        first = max(0, place - (S - n))
+        assert not bool(out[first:, :G, 7].isfinite().any()), place
+        out[first:, :G, 7] = clean[first:, :G, 7]
+        batch.k.copy_(k)
+        batch.v.copy_(v)
+        assert torch.equal(out[:first], clean[:first])
+        assert bool(((out.double() - clean.double()).abs() <= 2 * bound).all())   # either is within the bound of the exact one

@@ -52,7 +52,8 @@ __device__ __forceinline__ int cached(const PagedArgs & p, int len) {
 __device__ __forceinline__ int first_place(int len, int n) { return (int) max(-0x40000000ll, (long long) len - n); }
 
 // The values of keys from .. until - 1 that are not finite, added to E columns of a row: where rows see different keys of a
-// tile, the product took zeros in their place. Rare, one key after another.
+// tile, the product took zeros in their place. They are added whatever the keys' probabilities: the column is not finite either way, as
+// it is where the product takes them (p times infinity, or NaN where p is 0). Rare, one key after another.
 template <bool BF16, int E>
 __device__ __noinline__ void add_not_finite(const PagedArgs & p, int b, int hk, int from, int until, int col, float * o) {
     using T = typename std::conditional<BF16, __nv_bfloat16, __half>::type;
