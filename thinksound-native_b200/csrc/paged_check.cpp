@@ -24,7 +24,7 @@ int check_cache(const char * name, const tsn_paged & c) {
     if (!c.q_start && c.N != c.B) return refuse(name, "without q_start, N must be B");
     if (!c.len || (c.M && !c.table) || (c.P && (!c.k.p || !c.v.p))) return refuse(name, "null cache, table or len");
     if ((((uintptr_t) c.len | (uintptr_t) c.table | (uintptr_t) c.q_start) & 3)) return refuse(name, "an address that is no multiple of its element's size");
-    if (c.B > 1 && c.M > 1 && c.table_sb < 0) return refuse(name, "a negative stride of the table");
+    if (c.B > 1 && c.M && c.table_sb < 0) return refuse(name, "a negative stride of the table");
     for (const tsn_heads * t : {&c.k, &c.v})
         if (((uintptr_t) t->p & 15) || !stride_ok(c.P, t->sb, 8) || !stride_ok(c.page, t->ss, 8) || !stride_ok(c.Hk, t->sh, 8))
             return refuse(name, "base addresses and strides of k and v must be multiples of 16 bytes, strides positive");
