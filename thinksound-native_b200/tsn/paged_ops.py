@@ -61,6 +61,22 @@ def _paged(args):
     return (C.addressof(args.c.k), C.addressof(args.c.v), at + Paged.table.offset, at + Paged.len.offset, at + Paged.q_start.offset)
 
 
+def _scale(scale):
+    """The factor on the scores as the arguments have it, where 0 stands for the default; the rest the library checks."""
+    if scale is None:
+        return 0.0
+    if scale == 0:
+        raise ValueError("scale must be positive")
+    return scale
+
+
+def _count(name, n):
+    """A whole number that the arguments' 32 bits hold: what exceeds them would arrive as another number."""
+    if not 0 <= n < 2 ** 32:
+        raise ValueError(f"{name} must be a whole number of 32 bits, got {n}")
+    return n
+
+
 class _Op:
     def _ready(self, args, call, *places):
         self._a, self._ref, self._call = args, C.byref(args), call
@@ -152,7 +168,7 @@ class PagedAttention(_Op):
     def __init__(self, dev, head_dim: int, scale: float | None = None):
         self.dev, self.D = dev, head_dim
         a = PagedAttnArgs()
-        a.scale = 0.0 if scale is None else scale
+        a.scale = _scale(scale)
         self._ready(a, lib().tsn_paged_attn, C.addressof(a.q), C.addressof(a.out), *_paged(a))
 
     def __call__(self, q, k_pages, v_pages, table, lens, out, q_start=None, causal: bool = True, window: int = 0, most: int = 0):
@@ -160,7 +176,7 @@ class PagedAttention(_Op):
         the last `window` of them. most: new tokens of a sequence at most, where the caller knows it; 0: unknown."""
         a = self._a
         self._take((q, out, k_pages, v_pages, table, lens, q_start))
-        a.causal, a.window, a.most = 1 if causal else 0, window, most
+        a.causal, a.window, a.most = 1 if causal else 0, _count("window", window), _count("most", most)
         rc = self._call(self.dev.h, self._ref)
         if rc:
             check(rc)
@@ -184,7 +200,7 @@ class SparseAttention(_Op):
     def __init__(self, dev, head_dim: int, picks: int, first: int = 1, last: int = 1, scale: float | None = None):
         self.dev, self.D, self.picks = dev, head_dim, picks
         a = SparseAttnArgs()
-        a.picks, a.first, a.last, a.scale = picks, first, last, 0.0 if scale is None else scale
+        a.picks, a.first, a.last, a.scale = _count("picks", picks), _count("first", first), _count("last", last), _scale(scale)
         self._ready(a, lib().tsn_sparse_attn, C.addressof(a.q), C.addressof(a.out), C.addressof(a.means),
                     C.addressof(a) + SparseAttnArgs.chosen.offset, *_paged(a))
 
