@@ -9,9 +9,9 @@
 // them out: all units' slabs in a row, an equal share for each CTA; one of eight warps or two or three of four fill an SM. A share may begin and end
 // inside a unit; the CTA that is the last of a unit to arrive adds up its parts, in their order. Units of few slabs are not cut:
 // a trip through the workspace costs more.
-// 16 tokens over caches of 16 384 to 32 768 keys (32 heads over 8 of 128, bf16) take 261 us: 1.64 GB, 6.3 TB/s, 0.96 of the
+// 16 tokens over caches of 16 384 to 32 768 keys (32 heads over 8 of 128, bf16) take 260 us: 1.64 GB, 6.3 TB/s, 0.96 of the
 // measured copy; 24 x 4 tokens over up to 8191 112 us (5.5 TB/s; 16 rows take twice the products and the registers of a second CTA);
-// two tokens over 704 keys 7.9 us, from the launch through lengths, pages and keys to the warps' sums one after another.
+// two tokens over 704 keys 8.1 us, from the launch through lengths, pages and keys to the warps' sums one after another.
 // Where pages are chosen, a CTA takes a unit (a token's rows of a kv head) or a part of it; lists of many tokens come from L2, at 8 to 12 TB/s.
 #include "kernels.h"
 #include "paged_attn.h"
@@ -35,8 +35,9 @@ constexpr long long FEW_UNITS = 200;
 template <int D, int NT, int W, bool LIST>
 struct RowLay {
     // CTAs of an SM: three with two slabs a ring start and end beside one another where two with three do so less (400 tokens x 4
-    // kv heads, 16 pages of 64: 71 and 97 us; 64 tokens over 1500 keys, 8 kv heads of 64, 46.8 and 55.5), but 16 rows do not fit in
-    // the registers of three (4 tokens over 1000 keys, 64 streams: 94.8 and 57.4).
+    // kv heads, 16 pages of 64: 71 and 97 us; 64 tokens over 1500 keys, 8 kv heads of 64, 46.8 and 55.5), but 16 rows without
+    // picked pages do not fit in the registers of three (4 tokens over 1000 keys, 64 streams: 94.8 and 57.4). With picked pages they do, one
+    // word of 128-wide heads spilled.
     static constexpr int CTAS = W == 8 ? 1 : LIST || NT == 1 ? 3 : 2;
     static constexpr int BOX = SLAB * 128, HALF = SLAB * D * 2, STAGE = 2 * HALF, RING = (CTAS == 3 ? 2 : 3) * (128 / D);   // a slab's keys, then its values
     static constexpr int ROWS = 8 * NT, ROW = D + 4;   // words of a row's sums: o, ref, l
@@ -592,7 +593,8 @@ Plan plan_of(const PagedArgs & p, uint32_t most) {
     if (p.chosen || !p.c.q_start) r.units = (long long) p.c.N * ((p.G + rows - 1) / rows) * p.c.Hk;
     else r.units = std::min((long long) p.c.B * (((long long) most * p.G + rows - 1) / rows), (long long) p.c.N * p.G / rows + p.c.B) * p.c.Hk;
     r.warps = r.units <= FEW_UNITS ? 8 : 4;
-    r.ctas = r.warps == 8 ? SMS : r.nt == 1 ? 3 * SMS : 2 * SMS;   // as the kernels' launch bounds have it
+    // As many as run at once; picked pages with 16 rows, of which three would, are cut into parts for two.
+    r.ctas = r.warps == 8 ? SMS : r.nt == 1 ? 3 * SMS : 2 * SMS;
     return r;
 }
 

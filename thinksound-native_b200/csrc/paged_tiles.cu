@@ -18,9 +18,9 @@
 // What bounds it: 256 rows x 128 keys of 128 elements are 2048 cycles of the tensor cores (both products at 64 cycles an instruction of
 // 128 x 128 x 16, measured alone) and 1790 of the SFU (16 exponentials a cycle, one pair of eight on the FMA pipe). A tile's way is
 // 170 cycles for S to arrive, 280 for the maximum, 1220 for the exponentials, 150 to hand P over, then its products: the two tiles'
-// ways interleave at about 3800 cycles. 4096 tokens over 16 384 keys (32 heads over 8, bf16) take 815 to 840 us, 1.15 to 1.18
-// PFLOP/s, in short runs and 920 to 960 in long ones, where the power limit holds the clock; 64-wide heads 700 us (0.69).
-// Tried and worse: products under a branch that the compiler takes for divergent (100 cycles an instruction; 1245 us), both tiles'
+// ways interleave at about 3800 cycles. 4096 tokens over 16 384 keys (32 heads over 8, bf16) take 810 us, 1.19
+// PFLOP/s, in short runs and 940 to 950 in long ones, where the power limit holds the clock; 64-wide heads 768 us (0.63).
+// Tried and worse, against the 816 us of an earlier step: products under a branch that the compiler takes for divergent (100 cycles an instruction; 1245 us), both tiles'
 // products by one warp (880), side by side without turns (980), turns for the second half of P only (910), every fourth pair on
 // the FMA pipe (976) or none (845), exponentials before the maximum, done again where it moves (1370), spinning instead of suspended
 // waits (+1 to 3 %), registers moved to the softmax warps (+2 %).
@@ -610,8 +610,8 @@ double plan_paged_tiles(PagedArgs & p, uint32_t most) {
     // As many parts of a cluster as take the least time, in microseconds: start and end of a CTA 5, a tile of 128-wide heads 2 and of
     // 64-wide ones 1.7; with parts 4 to add them up and 5 for each wave of clusters; g_clusters[size] run at a time. Four
     // key tiles a part at least, eight parts at most (the largest portable cluster). The keys are what the tables have room for: lengths
-    // are on the device. us in 1, 2, 4 and 8 parts: 64 tokens x 4 heads of 128 over 32 768 keys, 8 kv heads 448, 234, 125, 78; 4 x 517
-    // tokens x 3 heads of 64 with a window of 2000, 8 kv heads, 69, 85, 128, 235.
+    // are on the device. us in 1, 2, 4 and 8 parts: 64 tokens x 4 heads of 128 over 32 768 keys, 8 kv heads 448, 234, 125, 80; 4 x 517
+    // tokens x 3 heads of 64 with a window of 2000, 8 kv heads, 76, 85, 128, 235 (but for 80 and 76 of an earlier step).
     long long keys = (long long) p.c.M << p.page_log2;
     if (p.window) keys = std::min<long long>(keys, (long long) p.window + ROWS);
     const long long tiles = (keys + KEYS - 1) / KEYS;
