@@ -39,3 +39,18 @@ def test_the_greatest_take_the_row(dev, dtype, D, exponents, n, S, Hk, G):
             dev.commit()
             want, bound = attention(batch, q, scale=0.125)
             assert bool(((out.double() - want).abs() <= bound).all()), (eq, ek, factor)
+
+
+@pytest.mark.parametrize("scale", [1e-30, 1.2e-38, 1e-39, 1e-45])
+@pytest.mark.parametrize("n,S,Hk,G", [(1, 90, 1, 2), (300, 700, 8, 4)])
+def test_scales_of_almost_nothing(dev, scale, n, S, Hk, G):
+    """Down to subnormal ones: seen keys share the row evenly, and rows that see nothing of a tile take nothing of it."""
+    for causal, window in ((False, 0), (True, 0), (True, 20)):
+        batch = Batch([n], [S], page=64, Hk=Hk, D=64)
+        q = batch.rows(Hk * G)
+        out = torch.full_like(q, 3.0)
+        tsn.PagedAttention(dev, 64, scale=scale)(q, batch.k, batch.v, batch.table, batch.lens, out, q_start=batch.q_start, causal=causal,
+                                                 window=window, most=n)
+        dev.commit()
+        want, bound = attention(batch, q, causal, window, scale=scale)
+        assert bool(((out.double() - want).abs() <= bound).all()), (causal, window)

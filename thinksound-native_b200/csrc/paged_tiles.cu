@@ -20,7 +20,7 @@
 // 170 cycles for S to arrive, 280 for the maximum, 1220 for the exponentials, 150 to hand P over, then its products: the two tiles'
 // ways interleave at about 3800 cycles. 4096 tokens over 16 384 keys (32 heads over 8, bf16) take 810 us, 1.19
 // PFLOP/s, in short runs and 940 to 950 in long ones, where the power limit holds the clock; 64-wide heads 768 us (0.63).
-// Tried and worse, against the 816 us of an earlier step: products under a branch that the compiler takes for divergent (100 cycles an instruction; 1245 us), both tiles'
+// Tried and worse, when the kernel took 816 us: products under a branch that the compiler takes for divergent (100 cycles an instruction; 1245 us), both tiles'
 // products by one warp (880), side by side without turns (980), turns for the second half of P only (910), every fourth pair on
 // the FMA pipe (976) or none (845), exponentials before the maximum, done again where it moves (1370), spinning instead of suspended
 // waits (+1 to 3 %), registers moved to the softmax warps (+2 %).
@@ -385,7 +385,7 @@ paged_tiles_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant
             // scores are 4 log2 units and more apart, c becomes a power of two, whose products are exact. (With c raw rounded to nearest
             // rows of scores of 2^36 were NaN or zero. Scores scaled and subtracted one after the other where a row needs it: 7 % more time.)
             const float high = __fmul_ru(raw, p.scale);
-            const bool far = fabsf(high) >= 0x1p26f;
+            const bool far = fabsf(high) >= 0x1p26f && raw != -INFINITY;
             const float c = far ? __uint_as_float(__float_as_uint(p.scale) & 0x7f800000u) : p.scale;
             const float neg = raw == -INFINITY ? 0.0f : __fadd_rd(ABOVE, far ? -(raw * c) : -high);
             const uint64_t neg2 = f2_pack(neg, neg), c2 = f2_pack(c, c);
@@ -611,7 +611,7 @@ double plan_paged_tiles(PagedArgs & p, uint32_t most) {
     // 64-wide ones 1.7; with parts 4 to add them up and 5 for each wave of clusters; g_clusters[size] run at a time. Four
     // key tiles a part at least, eight parts at most (the largest portable cluster). The keys are what the tables have room for: lengths
     // are on the device. us in 1, 2, 4 and 8 parts: 64 tokens x 4 heads of 128 over 32 768 keys, 8 kv heads 448, 234, 125, 80; 4 x 517
-    // tokens x 3 heads of 64 with a window of 2000, 8 kv heads, 76, 85, 128, 235 (but for 80 and 76 of an earlier step).
+    // tokens x 3 heads of 64 with a window of 2000, 8 kv heads, 76, 85, 128, 235 (the others measured when these were 78 and 69).
     long long keys = (long long) p.c.M << p.page_log2;
     if (p.window) keys = std::min<long long>(keys, (long long) p.window + ROWS);
     const long long tiles = (keys + KEYS - 1) / KEYS;
